@@ -380,6 +380,156 @@ NRN_API nrn_status_t nrn_cuda_bsr_spikes(uint64_t seed, int64_t step, float p, i
                                          uint16_t* tiles, nrn_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Sequence memory over recorded activity                                   */
+/* ------------------------------------------------------------------------ */
+
+/* The operators of a memory layer that reads sequences of recorded activity
+ * (libnrn_b200/readout.py puts them together): a fast Hebbian projection with
+ * forgetting, products in 8 bits for its projections, and the norms around
+ * it.  No counterpart in the reference, whose only learning rule is pair
+ * STDP (src/plasticity/stdp.cpp:43-141).  All of them enqueue on `stream`;
+ * arrays are the caller's, strides count elements, and the innermost stride
+ * is 1. */
+enum { NRN_BF16 = 0, NRN_FP16 = 1, NRN_FP32 = 2 };
+
+/* Linear attention with a decay for each head.  With lam = exp(log_decay[h])
+ * and the state S [dk][dv] of each sequence and head in fp32:
+ *     S_t = lam S_{t-1} + k_t v_t^T        o_t = scale S_t^T q_t
+ * Token arrays are [seq][token][head][d] by their strides; heads may share
+ * key and value heads (head h reads h / (heads / kv_heads)).  Packed
+ * sequences (cu_seqlens, seqs + 1 starts on the device, the first 0): the
+ * sequence stride is not used and `tokens` counts all of them.  log_decay
+ * is at most 0; -inf drops the state at every token.  Sequences may be
+ * empty: their state passes through. */
+typedef struct {
+    int32_t dtype;             /* of q, k, v, o and their gradients          */
+    int32_t seqs;
+    int32_t heads, kv_heads;
+    int32_t dk, dv;            /* 1 .. 256                                   */
+    int64_t tokens;            /* of each sequence, or of all packed ones    */
+    const int32_t* cu_seqlens; /* [seqs + 1], or NULL                        */
+    const float* log_decay;    /* [heads]                                    */
+    float scale;               /* finite, not 0                              */
+    int32_t pad;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* o;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];   /* seq, token, head */
+    const float* state_in;     /* [seqs][heads][dk][dv], or NULL: zero       */
+    float* state_out;          /* the same, or NULL                          */
+    void* workspace;           /* nrn_cuda_linattn_workspace bytes           */
+    int64_t workspace_bytes;
+} nrn_linattn_t;
+
+/* The gradients of a forward pass with the same q, k, v and state_in (o and
+ * state_out are not read).  d_o and dstate_out come in, the others go out. */
+typedef struct {
+    const void* d_o;
+    const float* dstate_out;   /* [seqs][heads][dk][dv], or NULL: zero       */
+    void* dq;
+    void* dk;
+    void* dv;
+    float* dstate_in;          /* [seqs][heads][dk][dv], or NULL             */
+    int64_t d_o_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} nrn_linattn_grad_t;
+
+/* Bytes of device workspace of a call with these sizes (0 where none is
+ * needed); its contents are not kept from call to call. */
+NRN_API nrn_status_t nrn_cuda_linattn_workspace(const nrn_linattn_t* a, int32_t backward, int64_t* bytes);
+NRN_API nrn_status_t nrn_cuda_linattn_forward(const nrn_linattn_t* a, nrn_stream_t stream);
+NRN_API nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const nrn_linattn_grad_t* g,
+                                               nrn_stream_t stream);
+/* One token for each sequence (tokens = 1; the token strides are not used),
+ * updating the states where they are: sequence s uses state slots[s] of
+ * n_slots (slots NULL: state s), each [heads][dk][dv], slot_stride elements
+ * apart.  A slot may appear once.  A negative slot is padding: its output is
+ * 0 and no state is touched; a slot past the last gives NaN outputs. */
+NRN_API nrn_status_t nrn_cuda_linattn_step(const nrn_linattn_t* a, float* state, int64_t slot_stride,
+                                           int32_t n_slots, const int32_t* slots, nrn_stream_t stream);
+
+/* A matrix in 8 bits: element (r, c) is values[r][c] (e4m3) times
+ * scales[r / row_block][c / 128].  The calls that fill one may write a row's
+ * storage up to the next multiple of 16 columns.  row_block is 1 (a scale for each row and
+ * 128 columns: activations and gradients) or 128 (weights). */
+typedef struct {
+    uint8_t* values;           /* 16-byte aligned                            */
+    float* scales;
+    int64_t rows, cols;
+    int64_t value_stride;      /* bytes from row to row, a multiple of 16    */
+    int64_t scale_stride[2];   /* along rows / row_block, along columns / 128 */
+    int32_t row_block;
+    int32_t pad;
+} nrn_scaled_t;
+
+/* Quantises x [rows][cols] (row stride in elements): a block's scale is
+ * max(|x|, 2^-64) times 1/448 in fp32, its values x * (1 / scale) rounded to
+ * the nearest (ties to even).  An infinity or NaN makes its whole block NaN.  With
+ * `transpose`, out is x^T ([cols][rows], row_block 1). */
+NRN_API nrn_status_t nrn_cuda_scaled_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols,
+                                              int64_t row_stride, int32_t transpose, const nrn_scaled_t* out,
+                                              nrn_stream_t stream);
+/* values of out = values of in transposed, for a row_block of 128, whose
+ * scales are the same ones with their strides exchanged. */
+NRN_API nrn_status_t nrn_cuda_scaled_transpose(const nrn_scaled_t* in, const nrn_scaled_t* out, nrn_stream_t stream);
+/* out [a.rows][b.rows] = a b^T: products of 8-bit values summed in fp32 over
+ * each block of 128 columns, times both scales, summed in fp32.  Work split
+ * over the columns leaves partial sums in the workspace
+ * (nrn_cuda_scaled_workspace bytes, zeroed once before its first use and
+ * left zeroed where it has to be; not shared by calls that run at once). */
+NRN_API nrn_status_t nrn_cuda_scaled_workspace(const nrn_scaled_t* a, const nrn_scaled_t* b, int64_t* bytes);
+NRN_API nrn_status_t nrn_cuda_scaled_product(const nrn_scaled_t* a, const nrn_scaled_t* b, void* out, int32_t dtype,
+                                             int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                                             int32_t* err, nrn_stream_t stream);
+
+/* The norms before and after a block with its gate and residual scale, for
+ * rows of d elements, norm(x) = x / sqrt(mean(x^2) + eps):
+ *     y = residual + alpha * act(gate) * norm(h) * w_post
+ *     z = norm(y) * w_pre
+ * in fp32, each output rounded once.  h NULL: y is the residual (not
+ * written); gate, alpha, w_post, w_pre NULL: 1. */
+enum { NRN_ACT_SILU = 0, NRN_ACT_SIGMOID = 1 };
+typedef struct {
+    int32_t dtype;             /* of residual, h, gate, y, z and their gradients */
+    int32_t act;
+    int64_t rows;
+    int32_t d;                 /* 1 .. 16384                                 */
+    float eps;
+    const void* residual;
+    const void* h;
+    const void* gate;
+    int64_t residual_stride, h_stride, gate_stride;
+    const float* alpha;        /* [d] each                                   */
+    const float* w_post;
+    const float* w_pre;
+    void* y;                   /* NULL: not written                          */
+    void* z;                   /* NULL: not written                          */
+    int64_t y_stride, z_stride;
+    const nrn_scaled_t* z_scaled;   /* z in 8 bits (row_block 1) instead, or NULL */
+} nrn_gatednorm_t;
+
+/* Gradients; dy and dz come in (NULL: zero), the others go out (NULL: not
+ * wanted).  y, z and z_scaled of the forward arguments are not read. */
+typedef struct {
+    const void* dy;
+    const void* dz;
+    void* dresidual;
+    void* dh;
+    void* dgate;
+    float* dalpha;             /* [d] each, sums over the rows in a fixed order */
+    float* dw_post;
+    float* dw_pre;
+    int64_t dy_stride, dz_stride, dresidual_stride, dh_stride, dgate_stride;
+    void* workspace;           /* nrn_cuda_gatednorm_workspace bytes         */
+    int64_t workspace_bytes;
+} nrn_gatednorm_grad_t;
+
+NRN_API nrn_status_t nrn_cuda_gatednorm_forward(const nrn_gatednorm_t* a, nrn_stream_t stream);
+NRN_API nrn_status_t nrn_cuda_gatednorm_workspace(const nrn_gatednorm_t* a, int64_t* bytes);
+NRN_API nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* a, const nrn_gatednorm_grad_t* g,
+                                                 nrn_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Engine: a network resident on one GPU                                   */
 /* ------------------------------------------------------------------------ */
 

@@ -41,6 +41,9 @@ EXPORTS = [
     "nrn_engine_spike_stats_reset", "nrn_engine_set_comm_timeout", "nrn_comm_bounded_wait",
     "nrn_comm_fake_async_error", "nrn_engine_profile_kernels", "nrn_engine_add_synapse_channel",
     "nrn_engine_set_deterministic", "nrn_engine_add_probe", "nrn_engine_clear_probes",
+    "nrn_cuda_linattn_workspace", "nrn_cuda_linattn_forward", "nrn_cuda_linattn_backward", "nrn_cuda_linattn_step",
+    "nrn_cuda_scaled_quantize", "nrn_cuda_scaled_transpose", "nrn_cuda_scaled_workspace", "nrn_cuda_scaled_product",
+    "nrn_cuda_gatednorm_forward", "nrn_cuda_gatednorm_workspace", "nrn_cuda_gatednorm_backward",
 ]
 
 
@@ -111,6 +114,51 @@ class Bsr(C.Structure):
     _fields_ = [
         ("n_post_blocks", C.c_int32), ("n_pre_blocks", C.c_int32), ("n_blocks", C.c_int64),
         ("row_ptr", C.c_void_p), ("col_idx", C.c_void_p), ("tiles", C.c_void_p),
+    ]
+
+
+class LinAttn(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("seqs", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+        ("dk", C.c_int32), ("dv", C.c_int32), ("tokens", C.c_int64), ("cu_seqlens", C.c_void_p),
+        ("log_decay", C.c_void_p), ("scale", C.c_float), ("pad", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p),
+        ("v", C.c_void_p), ("o", C.c_void_p), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+        ("v_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3), ("state_in", C.c_void_p),
+        ("state_out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class LinAttnGrad(C.Structure):
+    _fields_ = [
+        ("d_o", C.c_void_p), ("dstate_out", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("dstate_in", C.c_void_p), ("d_o_stride", C.c_int64 * 3), ("dq_stride", C.c_int64 * 3),
+        ("dk_stride", C.c_int64 * 3), ("dv_stride", C.c_int64 * 3),
+    ]
+
+
+class Scaled(C.Structure):
+    _fields_ = [
+        ("values", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64),
+        ("value_stride", C.c_int64), ("scale_stride", C.c_int64 * 2), ("row_block", C.c_int32), ("pad", C.c_int32),
+    ]
+
+
+class GatedNorm(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("act", C.c_int32), ("rows", C.c_int64), ("d", C.c_int32), ("eps", C.c_float),
+        ("residual", C.c_void_p), ("h", C.c_void_p), ("gate", C.c_void_p), ("residual_stride", C.c_int64),
+        ("h_stride", C.c_int64), ("gate_stride", C.c_int64), ("alpha", C.c_void_p), ("w_post", C.c_void_p),
+        ("w_pre", C.c_void_p), ("y", C.c_void_p), ("z", C.c_void_p), ("y_stride", C.c_int64),
+        ("z_stride", C.c_int64), ("z_scaled", C.POINTER(Scaled)),
+    ]
+
+
+class GatedNormGrad(C.Structure):
+    _fields_ = [
+        ("dy", C.c_void_p), ("dz", C.c_void_p), ("dresidual", C.c_void_p), ("dh", C.c_void_p), ("dgate", C.c_void_p),
+        ("dalpha", C.c_void_p), ("dw_post", C.c_void_p), ("dw_pre", C.c_void_p), ("dy_stride", C.c_int64),
+        ("dz_stride", C.c_int64), ("dresidual_stride", C.c_int64), ("dh_stride", C.c_int64),
+        ("dgate_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
     ]
 
 
@@ -207,6 +255,17 @@ def lib() -> C.CDLL:
             "nrn_engine_profile_kernels": [vp, i64, C.POINTER(C.c_double), C.POINTER(i64)],
             "nrn_engine_info": [vp, C.POINTER(EngineInfo)],
             "nrn_engine_prepare": [vp, i64, i64, i32],
+            "nrn_cuda_linattn_workspace": [C.POINTER(LinAttn), i32, C.POINTER(i64)],
+            "nrn_cuda_linattn_forward": [C.POINTER(LinAttn), vp],
+            "nrn_cuda_linattn_backward": [C.POINTER(LinAttn), C.POINTER(LinAttnGrad), vp],
+            "nrn_cuda_linattn_step": [C.POINTER(LinAttn), vp, i64, i32, vp, vp],
+            "nrn_cuda_scaled_quantize": [vp, i32, i64, i64, i64, i32, C.POINTER(Scaled), vp],
+            "nrn_cuda_scaled_transpose": [C.POINTER(Scaled), C.POINTER(Scaled), vp],
+            "nrn_cuda_scaled_workspace": [C.POINTER(Scaled), C.POINTER(Scaled), C.POINTER(i64)],
+            "nrn_cuda_scaled_product": [C.POINTER(Scaled), C.POINTER(Scaled), vp, i32, i64, vp, i64, vp, vp],
+            "nrn_cuda_gatednorm_forward": [C.POINTER(GatedNorm), vp],
+            "nrn_cuda_gatednorm_workspace": [C.POINTER(GatedNorm), C.POINTER(i64)],
+            "nrn_cuda_gatednorm_backward": [C.POINTER(GatedNorm), C.POINTER(GatedNormGrad), vp],
         }
         for name, args in sig.items():
             f = getattr(L, name)

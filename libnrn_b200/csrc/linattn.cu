@@ -1,0 +1,675 @@
+// linattn.cu -- linear attention with a decay for each head: a fast Hebbian
+// projection with forgetting, read by queries.
+//
+// For each sequence and head, with lam = exp(log_decay[head]):
+//     S_t = lam S_{t-1} + k_t v_t^T            (S: dk x dv, fp32)
+//     o_t = scale S_t^T q_t
+// The rate form of the exponentially decaying traces of the pair STDP rule
+// (src/plasticity/stdp.cpp:89-141): presynaptic key times postsynaptic value,
+// summed with forgetting.
+//
+// One scan serves the forward pass and, with the roles of its operands
+// exchanged, all gradients.  In general form, over tokens p = 0, 1, ..
+//     o_p = out_mul (lam^(p+off) X0^T a_p + sum_{j<=p} lam^(p-j) (a_p . b_j) c_j)
+//   forward:  a, b, c = q, k, v            off = 1, X0 = S_0
+//   dq:       a, b, c = do, v, k           off = 1, X0 = S_0^T
+//   dk:       a, b, c = v, do, q reversed  off = 0, X0 = dS^T / scale
+//   dv:       a, b, c = k, q, do reversed  off = 0, X0 = dS / scale
+// (dS: gradient of the final state; the state the reversed scan ends with,
+// times scale, is the gradient of S_0).  `off` says whether the state that
+// enters a token decays before it is read.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "internal.h"
+#include "vecio.cuh"
+
+namespace nrn {
+namespace {
+
+constexpr int kMaxDim = 256;       // largest key or value dimension
+
+struct Strided {
+    const void* p;
+    int64_t seq, tok, head;        // strides in elements
+    int32_t share;                 // heads of the scan that read one head here
+    int32_t d;                     // innermost extent (stride 1)
+};
+
+struct ScanArgs {
+    Strided a, b, c;
+    void* o;
+    int64_t o_seq, o_tok, o_head;
+    int32_t o_f32;                 // o is fp32 whatever the inputs' type (partial sums of shared heads)
+    int32_t vec;                   // rows of a, b, c start on 16-byte boundaries
+    int32_t heads;
+    int32_t seqs;
+    int64_t tokens;                // per sequence, or of all packed sequences
+    const int32_t* cu;             // [seqs + 1] starts of packed sequences, or null
+    const float* log_decay;
+    float out_mul, in_mul, end_mul;
+    int32_t off, reverse;
+    const float* s_in;             // [seqs][heads] states, element (i of b, j of c) at i*s_i + j*s_j; or null
+    float* s_out;                  // the same layout, or null
+    int64_t s_i, s_j;
+    float* seg;                    // [units][heads][b.d][c.d]: states of segments, or null
+    int64_t seg_len;               // tokens of a segment (a multiple of the chunk)
+    int32_t units;
+};
+
+// ------------------------------------------------------------------ units
+//
+// A unit is one segment of one sequence.  Units of sequence s start at
+// first(s) = floor(start of s / seg_len) + s: a place that needs no sum over
+// the sequences before it and leaves room for ceil(length / seg_len)
+// segments; a unit past its sequence's last segment is empty.
+struct Unit {
+    int64_t row0;                  // first token of the sequence in packed arrays (0 otherwise)
+    int64_t len;                   // tokens of the sequence
+    int64_t begin, end;            // this segment's tokens
+    int32_t seq;
+    bool last;                     // it ends the sequence
+    bool any;
+};
+
+__device__ __forceinline__ int64_t clamp_start(const ScanArgs& p, int s) {
+    const int64_t x = p.cu[s];
+    return x < 0 ? 0 : (x > p.tokens ? p.tokens : x);
+}
+
+__device__ __forceinline__ Unit unit_of(const ScanArgs& p, int u) {
+    Unit r;
+    int64_t seg;
+    if (p.cu == nullptr) {
+        const int64_t per = p.tokens > 0 ? (p.tokens + p.seg_len - 1) / p.seg_len : 1;
+        r.seq = static_cast<int32_t>(u / per);
+        seg = u - r.seq * per;
+        r.row0 = 0;
+        r.len = p.tokens;
+    } else {
+        int lo = 0, hi = p.seqs - 1;          // the last sequence whose first unit is <= u
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (clamp_start(p, mid) / p.seg_len + mid <= u) lo = mid;
+            else hi = mid - 1;
+        }
+        r.seq = lo;
+        r.row0 = clamp_start(p, lo);
+        const int64_t next = clamp_start(p, lo + 1);
+        r.len = next > r.row0 ? next - r.row0 : 0;
+        seg = u - (r.row0 / p.seg_len + lo);
+    }
+    r.begin = seg * p.seg_len;
+    r.end = r.begin + p.seg_len < r.len ? r.begin + p.seg_len : r.len;
+    r.any = seg >= 0 && (r.begin < r.len || (r.len == 0 && seg == 0));
+    r.last = r.end == r.len;
+    return r;
+}
+
+// lam^n: n = 0 is 1 whatever the decay (log_decay may be -inf: the state is
+// dropped at every token).  In double, so that a power is off by its rounding
+// to fp32 alone: it is applied once for every chunk of a long memory.
+__device__ __forceinline__ float decay_power(float log_decay, int64_t n) {
+    return n == 0 ? 1.0f : static_cast<float>(exp(static_cast<double>(log_decay) * static_cast<double>(n)));
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_ptr(const Strided& m, const Unit& u, int64_t t, int head) {
+    return static_cast<const T*>(m.p) + (u.row0 + t) * m.tok + static_cast<int64_t>(u.seq) * m.seq +
+           static_cast<int64_t>(head / m.share) * m.head;
+}
+
+// ------------------------------------------------------- token by token
+//
+// The recurrence itself, for every type and dimension.  A block has 32
+// columns (c) of one state: 8 lanes share a column, each with every eighth
+// group of four rows in registers, so a token costs each thread
+// 3 * b.d / 8 operations and three shuffles; 16 tokens at a time are staged
+// in shared memory as fp32.  Bound by the fp32 pipe: 3 b.d c.d operations a
+// token and head.
+//
+// lam in fp32 is off by up to 3e-8, which over a memory of thousands of
+// tokens would show; the error of its powers is taken out of the state after
+// every 16 tokens.
+constexpr int kSerialThreads = 256;
+constexpr int kSerialCols = 32;
+constexpr int kSerialTokens = 16;
+
+template <typename T, int G>   // G groups of 4 rows a thread: b.d <= 32 G
+__global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __grid_constant__ ScanArgs p, int state_only) {
+    __shared__ __align__(16) float sa[kSerialTokens][32 * G];
+    __shared__ __align__(16) float sb[kSerialTokens][32 * G];
+    __shared__ float sc[kSerialTokens][kSerialCols];
+    const int db = p.b.d, dc = p.c.d;
+    const int tiles = (dc + kSerialCols - 1) / kSerialCols;
+    const int tile = blockIdx.x % tiles;
+    const int head = (blockIdx.x / tiles) % p.heads;
+    const int unit = blockIdx.x / tiles / p.heads;
+    const Unit u = unit_of(p, unit);
+    if (!u.any) return;
+    const int part = threadIdx.x & 7, col_l = threadIdx.x >> 3, col = tile * kSerialCols + col_l;
+    const float lam = decay_power(p.log_decay[head], 1);
+    // lam^16 / (fp32 lam)^16 - 1; where lam^16 vanishes there is nothing to mend
+    double l2 = static_cast<double>(lam) * lam, l4 = l2 * l2, l16 = l4 * l4 * (l4 * l4);
+    const float mend = l16 > 1e-30 ? static_cast<float>(exp(16.0 * static_cast<double>(p.log_decay[head])) / l16 - 1.0) : 0.0f;
+
+    float s[4 * G];
+#pragma unroll
+    for (int g = 0; g < 4 * G; ++g) s[g] = 0.0f;
+    const int64_t sh = (static_cast<int64_t>(u.seq) * p.heads + head) * db * dc;
+    const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
+    if (!state_only && col < dc && (p.seg != nullptr || p.s_in != nullptr)) {
+#pragma unroll
+        for (int g = 0; g < 4 * G; ++g) {
+            const int i = ((g >> 2) * 8 + part) * 4 + (g & 3);
+            if (i < db)
+                s[g] = p.seg ? p.seg[gh + static_cast<int64_t>(i) * dc + col] : p.s_in[sh + i * p.s_i + col * p.s_j] * p.in_mul;
+        }
+    }
+    for (int64_t t0 = u.begin; t0 < u.end; t0 += kSerialTokens) {
+        const int n = static_cast<int>(u.end - t0 < kSerialTokens ? u.end - t0 : kSerialTokens);
+        __syncthreads();
+        for (int e = threadIdx.x; e < kSerialTokens * 32 * G; e += kSerialThreads) {
+            const int t = e / (32 * G), i = e - t * 32 * G;
+            float x = 0.0f, y = 0.0f;
+            if (t < n && i < db) {
+                const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
+                y = to_f32(row_ptr<T>(p.b, u, tok, head)[i]);
+                if (!state_only) x = to_f32(row_ptr<T>(p.a, u, tok, head)[i]);
+            }
+            sa[t][i] = x;
+            sb[t][i] = y;
+        }
+        for (int e = threadIdx.x; e < kSerialTokens * kSerialCols; e += kSerialThreads) {
+            const int t = e / kSerialCols, j = tile * kSerialCols + e % kSerialCols;
+            float x = 0.0f;
+            if (t < n && j < dc) {
+                const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
+                x = to_f32(row_ptr<T>(p.c, u, tok, head)[j]);
+            }
+            sc[t][e % kSerialCols] = x;
+        }
+        __syncthreads();
+        for (int t = 0; t < n; ++t) {
+            const float c = sc[t][col_l];
+            float o = 0.0f;
+            // off = 1: decay, add, read.  off = 0: add, read, decay.
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float4 b = *reinterpret_cast<const float4*>(&sb[t][(g * 8 + part) * 4]);
+                const float4 a = *reinterpret_cast<const float4*>(&sa[t][(g * 8 + part) * 4]);
+                if (p.off) {
+                    s[4 * g + 0] = fmaf(b.x, c, lam * s[4 * g + 0]);
+                    s[4 * g + 1] = fmaf(b.y, c, lam * s[4 * g + 1]);
+                    s[4 * g + 2] = fmaf(b.z, c, lam * s[4 * g + 2]);
+                    s[4 * g + 3] = fmaf(b.w, c, lam * s[4 * g + 3]);
+                } else {
+                    s[4 * g + 0] = fmaf(b.x, c, s[4 * g + 0]);
+                    s[4 * g + 1] = fmaf(b.y, c, s[4 * g + 1]);
+                    s[4 * g + 2] = fmaf(b.z, c, s[4 * g + 2]);
+                    s[4 * g + 3] = fmaf(b.w, c, s[4 * g + 3]);
+                }
+                o = fmaf(a.x, s[4 * g + 0], o);
+                o = fmaf(a.y, s[4 * g + 1], o);
+                o = fmaf(a.z, s[4 * g + 2], o);
+                o = fmaf(a.w, s[4 * g + 3], o);
+                if (!p.off) {
+                    s[4 * g + 0] *= lam;
+                    s[4 * g + 1] *= lam;
+                    s[4 * g + 2] *= lam;
+                    s[4 * g + 3] *= lam;
+                }
+            }
+            if (state_only) continue;
+            o += __shfl_xor_sync(0xffffffffu, o, 1);
+            o += __shfl_xor_sync(0xffffffffu, o, 2);
+            o += __shfl_xor_sync(0xffffffffu, o, 4);
+            if (part == 0 && col < dc) {
+                const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
+                const int64_t at = (u.row0 + tok) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + col;
+                if (p.o_f32) static_cast<float*>(p.o)[at] = o * p.out_mul;
+                else static_cast<T*>(p.o)[at] = from_f32<T>(o * p.out_mul);
+            }
+        }
+        if (n == kSerialTokens) {
+#pragma unroll
+            for (int g = 0; g < 4 * G; ++g) s[g] = fmaf(s[g], mend, s[g]);
+        }
+    }
+    if (col >= dc) return;
+    if (state_only) {
+#pragma unroll
+        for (int g = 0; g < 4 * G; ++g) {
+            const int i = ((g >> 2) * 8 + part) * 4 + (g & 3);
+            if (i < db) p.seg[gh + static_cast<int64_t>(i) * dc + col] = s[g];
+        }
+    } else if (u.last && p.s_out != nullptr && p.seg == nullptr) {
+#pragma unroll
+        for (int g = 0; g < 4 * G; ++g) {
+            const int i = ((g >> 2) * 8 + part) * 4 + (g & 3);
+            if (i < db) p.s_out[sh + i * p.s_i + col * p.s_j] = s[g] * p.end_mul;
+        }
+    }
+}
+
+// ---------------------------------------------------------- segment states
+//
+// The segments' own end states (from zero) become the states that enter
+// them: X_{g+1} = lam^len(g) X_g + E_g with X_0 the given state; the state
+// after the last segment is the final one.  One thread an element.
+__global__ void scan_join_kernel(const __grid_constant__ ScanArgs p) {
+    const int64_t n = static_cast<int64_t>(p.b.d) * p.c.d;
+    const int head = blockIdx.y % p.heads, seq = blockIdx.y / p.heads;
+    int64_t len = p.tokens, first;
+    if (p.cu == nullptr) {
+        first = static_cast<int64_t>(seq) * (p.tokens > 0 ? (p.tokens + p.seg_len - 1) / p.seg_len : 1);
+    } else {
+        const int64_t a = clamp_start(p, seq), b = clamp_start(p, seq + 1);
+        len = b > a ? b - a : 0;
+        first = a / p.seg_len + seq;
+    }
+    const float whole = decay_power(p.log_decay[head], p.seg_len);
+    const int64_t segs = (len + p.seg_len - 1) / p.seg_len;
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n;
+         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t i = e / p.c.d, j = e - i * p.c.d;
+        const int64_t sh = (static_cast<int64_t>(seq) * p.heads + head) * n;
+        float x = p.s_in ? p.s_in[sh + i * p.s_i + j * p.s_j] * p.in_mul : 0.0f;
+        for (int64_t g = 0; g < segs; ++g) {
+            float* at = p.seg + ((first + g) * p.heads + head) * n + e;
+            const float own = *at;
+            *at = x;
+            const int64_t m = len - g * p.seg_len;
+            x = fmaf(m < p.seg_len ? decay_power(p.log_decay[head], m) : whole, x, own);
+        }
+        if (p.s_out) p.s_out[sh + i * p.s_i + j * p.s_j] = x * p.end_mul;
+    }
+}
+
+// Sums the partial gradients of `share` heads that read one key or value
+// head, in the heads' order: out[token][kv][d] = sum_h part[token][kv*share + h][d].
+template <typename T>
+__global__ void sum_heads_kernel(const float* part, int64_t tokens, int kv, int share, int d, T* out, int64_t o_seq,
+                                 int64_t o_tok, int64_t o_head, int64_t per_seq) {
+    const int64_t total = tokens * kv * d;
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < total;
+         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t t = e / (static_cast<int64_t>(kv) * d);
+        const int rem = static_cast<int>(e - t * kv * d), h = rem / d, i = rem - h * d;
+        const float* at = part + (t * kv + h) * share * d + i;
+        float x = 0.0f;
+        for (int g = 0; g < share; ++g) x += at[static_cast<int64_t>(g) * d];
+        const int64_t s = t / per_seq;
+        out[s * o_seq + (t - s * per_seq) * o_tok + h * o_head + i] = from_f32<T>(x);
+    }
+}
+
+// -------------------------------------------------------------- one token
+//
+// One token for each sequence: the state is read, updated and written once,
+// 8 bytes an element, which is all that counts.  A block has 32 columns of
+// one state (8 lanes of float4 a row, 32 rows at a time): every load of a
+// thread is in flight at once and small batches still spread over the GPU.
+constexpr int kStepThreads = 256;
+
+struct StepArgs {
+    const void *q, *k, *v;
+    void* o;
+    int64_t q_seq, q_head, k_seq, k_head, v_seq, v_head, o_seq, o_head;
+    float* state;
+    int64_t s_slot;                // elements from slot to slot
+    const int32_t* slots;          // [seqs] or null
+    int32_t n_slots;
+    int32_t heads, share, dk, dv;
+    const float* log_decay;
+    float scale;
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constant__ StepArgs p) {
+    __shared__ float part[8][8 * V];
+    const int tiles = (p.dv + 8 * V - 1) / (8 * V);
+    const int tile = blockIdx.x % tiles;
+    const int head = (blockIdx.x / tiles) % p.heads;
+    const int seq = blockIdx.x / tiles / p.heads;
+    const int slot = p.slots ? p.slots[seq] : seq;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int cl = (threadIdx.x & 7) * V, col = tile * 8 * V + cl, r0 = threadIdx.x >> 3;
+    T* o = static_cast<T*>(p.o) + seq * p.o_seq + head * p.o_head;
+    if (slot < 0 || slot >= p.n_slots) {
+        // a negative slot is padding; one past the cache is a caller's error that must not go unseen
+        if (threadIdx.x < 8 * V && tile * 8 * V + static_cast<int>(threadIdx.x) < p.dv)
+            o[tile * 8 * V + threadIdx.x] = from_f32<T>(slot < 0 ? 0.0f : __int_as_float(0x7fc00000));
+        return;
+    }
+    const T* q = static_cast<const T*>(p.q) + seq * p.q_seq + head * p.q_head;
+    const T* k = static_cast<const T*>(p.k) + seq * p.k_seq + (head / p.share) * p.k_head;
+    const T* v = static_cast<const T*>(p.v) + seq * p.v_seq + (head / p.share) * p.v_head;
+    float* s = p.state + slot * p.s_slot + static_cast<int64_t>(head) * p.dk * p.dv;
+    // lam to 48 bits: a long run of steps applies it thousands of times
+    const double whole = exp(static_cast<double>(p.log_decay[head]));
+    const float lam = static_cast<float>(whole), lam_lo = static_cast<float>(whole - lam);
+    const bool in = col < p.dv;
+    float vv[V], acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        vv[e] = in ? to_f32(v[col + e]) : 0.0f;
+        acc[e] = 0.0f;
+    }
+#pragma unroll
+    for (int g = 0; g < kMaxDim / 32; g += 4) {
+        if (32 * g >= p.dk) break;
+        float x[4][V];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + 32 * (g + i);
+            if (in && r < p.dk) {
+                if constexpr (V == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(s + static_cast<int64_t>(r) * p.dv + col);
+                    x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+                } else {
+                    x[i][0] = s[static_cast<int64_t>(r) * p.dv + col];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + 32 * (g + i);
+            if (in && r < p.dk) {
+                const float kk = to_f32(k[r]), qq = to_f32(q[r]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[i][e] = fmaf(lam, x[i][e], fmaf(lam_lo, x[i][e], kk * vv[e]));
+                    acc[e] = fmaf(qq, x[i][e], acc[e]);
+                }
+                if constexpr (V == 4)
+                    *reinterpret_cast<float4*>(s + static_cast<int64_t>(r) * p.dv + col) =
+                        make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+                else
+                    s[static_cast<int64_t>(r) * p.dv + col] = x[i][0];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 8);
+        acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
+        if (lane < 8) part[warp][cl + e] = acc[e];
+    }
+    __syncthreads();
+    if (threadIdx.x < 8 * V) {
+        const int j = tile * 8 * V + threadIdx.x;
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) x += part[w][threadIdx.x];
+        if (j < p.dv) o[j] = from_f32<T>(x * p.scale);
+    }
+}
+
+// ---------------------------------------------------------------- launches
+
+template <typename T>
+cudaError_t launch_serial(const ScanArgs& p, bool state_only, cudaStream_t s) {
+    const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kSerialCols - 1) / kSerialCols);
+    const unsigned g = static_cast<unsigned>(blocks);
+    if (p.b.d <= 64) scan_serial_kernel<T, 2><<<g, kSerialThreads, 0, s>>>(p, state_only);
+    else if (p.b.d <= 128) scan_serial_kernel<T, 4><<<g, kSerialThreads, 0, s>>>(p, state_only);
+    else scan_serial_kernel<T, 8><<<g, kSerialThreads, 0, s>>>(p, state_only);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, cudaStream_t s) {
+    if (dtype == NRN_BF16) return launch_serial<__nv_bfloat16>(p, state_only, s);
+    if (dtype == NRN_FP16) return launch_serial<__half>(p, state_only, s);
+    return launch_serial<float>(p, state_only, s);
+}
+
+int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
+
+constexpr int64_t kChunk = 64;
+
+// Tokens of a segment.  A scan is serial in time, so its parallelism is
+// sequences x heads x 64-column tiles; where that leaves most SMs idle the
+// sequences are split.
+int64_t segment_length(const nrn_linattn_t* a, int dc) {
+    const int64_t tiles = (dc + 63) / 64;
+    const int64_t want = 2LL * sm_count_current();                    // blocks that fill the GPU
+    const int64_t rows = static_cast<int64_t>(a->heads) * tiles;
+    const int64_t all = a->cu_seqlens ? a->tokens : a->tokens * a->seqs;
+    if (all == 0) return kChunk;
+    const int64_t units = std::max<int64_t>(1, want / rows);          // segments of all sequences together
+    const bool whole = a->cu_seqlens == nullptr && a->seqs * 2 >= units;
+    if (whole) return std::max<int64_t>(kChunk, (a->tokens + kChunk - 1) / kChunk * kChunk);
+    const int64_t len = std::max<int64_t>(8 * kChunk, ((all + units - 1) / units + kChunk - 1) / kChunk * kChunk);
+    return len;
+}
+
+int64_t unit_count(const nrn_linattn_t* a, int64_t seg_len) {
+    if (a->cu_seqlens) return a->tokens / seg_len + a->seqs;
+    return a->seqs * std::max<int64_t>(1, (a->tokens + seg_len - 1) / seg_len);
+}
+
+bool is_split(const nrn_linattn_t* a, int64_t seg_len) {
+    return a->cu_seqlens ? a->tokens > seg_len : a->tokens > seg_len;
+}
+
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+int64_t seg_bytes(const nrn_linattn_t* a) {
+    int64_t most = 0;
+    for (int dc : {a->dv, a->dk}) {
+        const int64_t l = segment_length(a, dc);
+        if (is_split(a, l)) most = std::max(most, unit_count(a, l));
+    }
+    return align256(most * a->heads * a->dk * a->dv * 4);
+}
+
+int64_t all_tokens(const nrn_linattn_t* a) { return a->cu_seqlens ? a->tokens : a->tokens * a->seqs; }
+
+int64_t workspace_need(const nrn_linattn_t* a, bool backward) {
+    int64_t n = seg_bytes(a);
+    if (backward && a->kv_heads != a->heads) n += align256(all_tokens(a) * a->heads * std::max(a->dk, a->dv) * 4);
+    return n;
+}
+
+nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, cudaStream_t s) {
+    if (p.cu) p.a.seq = p.b.seq = p.c.seq = p.o_seq = 0;      // packed: a token's row counts from the arrays' start
+    p.seg_len = segment_length(a, p.c.d);
+    const int64_t units = unit_count(a, p.seg_len);
+    NRN_CHECK_ARG(units * p.heads * ((p.c.d + 31) / 32) < (int64_t(1) << 31), "nrn_cuda_linattn: too many sequences, heads and segments for one launch");
+    NRN_CHECK_ARG(static_cast<int64_t>(p.seqs) * p.heads < 65536 || !is_split(a, p.seg_len),
+                  "nrn_cuda_linattn: at most 65,535 sequences times heads when sequences are split");
+    p.units = static_cast<int32_t>(units);
+    if (is_split(a, p.seg_len)) {
+        p.seg = static_cast<float*>(a->workspace);
+        NRN_CUDA_TRY(launch_scan(p, a->dtype, true, s));
+        const int64_t n = static_cast<int64_t>(p.b.d) * p.c.d;
+        const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 64)), static_cast<unsigned>(p.seqs * p.heads));
+        scan_join_kernel<<<grid, 256, 0, s>>>(p);
+        NRN_CUDA_TRY(cudaGetLastError());
+    }
+    NRN_CUDA_TRY(launch_scan(p, a->dtype, false, s));
+    return NRN_OK;
+}
+
+Strided strided(const void* p, const int64_t* st, int share, int d) {
+    Strided r;
+    r.p = p;
+    r.seq = st[0], r.tok = st[1], r.head = st[2];
+    r.share = share;
+    r.d = d;
+    return r;
+}
+
+bool rows_aligned(const Strided& m, int dtype) {
+    const int64_t n = 16 / elem_size(dtype);
+    return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.seq % n == 0 && m.tok % n == 0 && m.head % n == 0 && m.d % n == 0;
+}
+
+nrn_status_t check_common(const nrn_linattn_t* a, const char* who) {
+    const std::string w(who);
+    NRN_CHECK_ARG(a != nullptr, w + ": null arguments");
+    NRN_CHECK_ARG(a->dtype == NRN_BF16 || a->dtype == NRN_FP16 || a->dtype == NRN_FP32, w + ": unknown type");
+    NRN_CHECK_ARG(a->seqs >= 0 && a->tokens >= 0, w + ": negative sizes");
+    NRN_CHECK_ARG(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0,
+                  w + ": heads must be a multiple of kv_heads");
+    NRN_CHECK_ARG(a->dk >= 1 && a->dk <= kMaxDim && a->dv >= 1 && a->dv <= kMaxDim, w + ": key and value dimensions are 1 to 256");
+    NRN_CHECK_ARG(std::isfinite(a->scale) && a->scale != 0.0f, w + ": scale must be finite and not 0");
+    NRN_CHECK_ARG(a->log_decay != nullptr, w + ": null log_decay");
+    return NRN_OK;
+}
+
+ScanArgs scan_args(const nrn_linattn_t* a) {
+    ScanArgs p{};
+    p.heads = a->heads;
+    p.seqs = a->seqs;
+    p.tokens = a->tokens;
+    p.cu = a->cu_seqlens;
+    p.log_decay = a->log_decay;
+    p.out_mul = a->scale;
+    p.in_mul = p.end_mul = 1.0f;
+    p.off = 1;
+    return p;
+}
+
+template <typename T>
+void launch_step(const StepArgs& p, int seqs, bool vec, cudaStream_t s) {
+    if (vec) {
+        const int64_t n = static_cast<int64_t>(seqs) * p.heads * ((p.dv + 31) / 32);
+        step_kernel<T, 4><<<static_cast<unsigned>(n), kStepThreads, 0, s>>>(p);
+    } else {
+        const int64_t n = static_cast<int64_t>(seqs) * p.heads * ((p.dv + 7) / 8);
+        step_kernel<T, 1><<<static_cast<unsigned>(n), kStepThreads, 0, s>>>(p);
+    }
+}
+
+}  // namespace
+}  // namespace nrn
+
+using namespace nrn;
+
+extern "C" nrn_status_t nrn_cuda_linattn_workspace(const nrn_linattn_t* a, int32_t backward, int64_t* bytes) {
+    NRN_TRY(check_common(a, "nrn_cuda_linattn_workspace"));
+    NRN_CHECK_ARG(bytes != nullptr, "nrn_cuda_linattn_workspace: null result");
+    *bytes = workspace_need(a, backward != 0);
+    return NRN_OK;
+}
+
+extern "C" nrn_status_t nrn_cuda_linattn_forward(const nrn_linattn_t* a, nrn_stream_t stream) {
+    NRN_TRY(check_common(a, "nrn_cuda_linattn_forward"));
+    if (a->seqs == 0) return NRN_OK;
+    NRN_CHECK_ARG(all_tokens(a) == 0 || (a->q && a->k && a->v && a->o), "nrn_cuda_linattn_forward: null array");
+    const int64_t need = workspace_need(a, false);
+    NRN_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need), "nrn_cuda_linattn_forward: workspace too small");
+    ScanArgs p = scan_args(a);
+    const int share = a->heads / a->kv_heads;
+    p.a = strided(a->q, a->q_stride, 1, a->dk);
+    p.b = strided(a->k, a->k_stride, share, a->dk);
+    p.c = strided(a->v, a->v_stride, share, a->dv);
+    p.vec = rows_aligned(p.a, a->dtype) && rows_aligned(p.b, a->dtype) && rows_aligned(p.c, a->dtype);
+    p.o = a->o;
+    p.o_seq = a->o_stride[0], p.o_tok = a->o_stride[1], p.o_head = a->o_stride[2];
+    p.s_in = a->state_in, p.s_out = a->state_out;
+    p.s_i = a->dv, p.s_j = 1;
+    return run_scan(p, a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const nrn_linattn_grad_t* g, nrn_stream_t stream) {
+    NRN_TRY(check_common(a, "nrn_cuda_linattn_backward"));
+    NRN_CHECK_ARG(g != nullptr, "nrn_cuda_linattn_backward: null gradients");
+    if (a->seqs == 0) return NRN_OK;
+    NRN_CHECK_ARG(all_tokens(a) == 0 || (a->q && a->k && a->v && g->d_o && g->dq && g->dk && g->dv),
+                  "nrn_cuda_linattn_backward: null array");
+    const int64_t need = workspace_need(a, true);
+    NRN_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need), "nrn_cuda_linattn_backward: workspace too small");
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const int share = a->heads / a->kv_heads;
+    const Strided q = strided(a->q, a->q_stride, 1, a->dk), k = strided(a->k, a->k_stride, share, a->dk);
+    const Strided v = strided(a->v, a->v_stride, share, a->dv), d = strided(g->d_o, g->d_o_stride, 1, a->dv);
+    const int vec = rows_aligned(q, a->dtype) && rows_aligned(k, a->dtype) && rows_aligned(v, a->dtype) && rows_aligned(d, a->dtype);
+
+    ScanArgs p = scan_args(a);
+    p.vec = vec;
+    p.a = d, p.b = v, p.c = k;
+    p.o = g->dq;
+    p.o_seq = g->dq_stride[0], p.o_tok = g->dq_stride[1], p.o_head = g->dq_stride[2];
+    p.s_in = a->state_in;
+    p.s_i = 1, p.s_j = a->dv;
+    NRN_TRY(run_scan(p, a, s));
+
+    // the gradients of keys and values run backwards in time; heads that
+    // share one key or value head leave fp32 parts, summed in a fixed order
+    p.reverse = 1;
+    p.off = 0;
+    p.in_mul = 1.0f / a->scale;
+    p.end_mul = a->scale;
+    p.s_in = g->dstate_out;
+    float* part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + seg_bytes(a));
+    for (int which = 0; which < 2; ++which) {
+        p.a = which ? k : v, p.b = which ? q : d, p.c = which ? d : q;
+        const int dd = which ? a->dv : a->dk;
+        const int64_t* st = which ? g->dv_stride : g->dk_stride;
+        void* out = which ? g->dv : g->dk;
+        p.s_i = which ? a->dv : 1, p.s_j = which ? 1 : a->dv;
+        p.s_out = which ? g->dstate_in : nullptr;
+        if (share == 1) {
+            p.o = out;
+            p.o_seq = st[0], p.o_tok = st[1], p.o_head = st[2];
+        } else {
+            p.o = part;
+            p.o_f32 = 1;
+            p.o_head = dd;
+            p.o_tok = static_cast<int64_t>(a->heads) * dd;
+            p.o_seq = a->cu_seqlens ? 0 : p.o_tok * a->tokens;
+        }
+        NRN_TRY(run_scan(p, a, s));
+        const int64_t n = all_tokens(a);
+        if (share == 1 || n == 0) continue;
+        const int64_t total = n * a->kv_heads * dd, per = a->cu_seqlens ? n : a->tokens;
+        const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 16LL * sm_count_current()));
+        if (a->dtype == NRN_BF16)
+            sum_heads_kernel<<<blocks, 256, 0, s>>>(part, n, a->kv_heads, share, dd, static_cast<__nv_bfloat16*>(out), st[0], st[1], st[2], per);
+        else if (a->dtype == NRN_FP16)
+            sum_heads_kernel<<<blocks, 256, 0, s>>>(part, n, a->kv_heads, share, dd, static_cast<__half*>(out), st[0], st[1], st[2], per);
+        else
+            sum_heads_kernel<<<blocks, 256, 0, s>>>(part, n, a->kv_heads, share, dd, static_cast<float*>(out), st[0], st[1], st[2], per);
+        NRN_CUDA_TRY(cudaGetLastError());
+    }
+    return NRN_OK;
+}
+
+extern "C" nrn_status_t nrn_cuda_linattn_step(const nrn_linattn_t* a, float* state, int64_t slot_stride, int32_t n_slots,
+                                              const int32_t* slots, nrn_stream_t stream) {
+    NRN_TRY(check_common(a, "nrn_cuda_linattn_step"));
+    NRN_CHECK_ARG(a->tokens == 1 && a->cu_seqlens == nullptr, "nrn_cuda_linattn_step: one token for each sequence");
+    NRN_CHECK_ARG(n_slots >= 0 && (slots || n_slots >= a->seqs), "nrn_cuda_linattn_step: fewer states than sequences");
+    if (a->seqs == 0) return NRN_OK;
+    NRN_CHECK_ARG(a->q && a->k && a->v && a->o && state, "nrn_cuda_linattn_step: null array");
+    NRN_CHECK_ARG(static_cast<int64_t>(a->seqs) * a->heads * ((a->dv + 7) / 8) < (int64_t(1) << 31),
+                  "nrn_cuda_linattn_step: too many sequences and heads for one launch");
+    StepArgs p{};
+    p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->o;
+    p.q_seq = a->q_stride[0], p.q_head = a->q_stride[2];
+    p.k_seq = a->k_stride[0], p.k_head = a->k_stride[2];
+    p.v_seq = a->v_stride[0], p.v_head = a->v_stride[2];
+    p.o_seq = a->o_stride[0], p.o_head = a->o_stride[2];
+    p.state = state;
+    p.s_slot = slot_stride;
+    p.slots = slots;
+    p.n_slots = n_slots;
+    p.heads = a->heads;
+    p.share = a->heads / a->kv_heads;
+    p.dk = a->dk, p.dv = a->dv;
+    p.log_decay = a->log_decay;
+    p.scale = a->scale;
+    const bool vec = a->dv % 4 == 0 && slot_stride % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (a->dtype == NRN_BF16) launch_step<__nv_bfloat16>(p, a->seqs, vec, s);
+    else if (a->dtype == NRN_FP16) launch_step<__half>(p, a->seqs, vec, s);
+    else launch_step<float>(p, a->seqs, vec, s);
+    NRN_CUDA_TRY(cudaGetLastError());
+    return NRN_OK;
+}

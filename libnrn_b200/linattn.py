@@ -1,0 +1,153 @@
+"""Linear attention with a decay for each head: a fast Hebbian projection
+with forgetting, for sequences (``forward``, ``backward``) and one token at a
+time (``step``).  For each sequence and head, with lam = exp(log_decay[head]):
+
+    S_t = lam S_{t-1} + k_t v_t^T          o_t = scale * S_t^T q_t
+
+Tokens are [batch, tokens, heads, d] tensors with any strides but the last,
+which is 1; bf16, fp16 or fp32.  k and v may have fewer heads (a divisor of
+q's), each read by as many heads of q.  States are fp32
+[batch, heads, dk, dv].  With ``cu_seqlens`` (int32 starts of packed
+sequences, [sequences + 1], on the device, from 0 to the number of tokens) the
+batch dimension is 1 and states have one entry for each sequence.  dk and dv
+are at most 256; ``log_decay`` (fp32 [heads]) is at most 0, -inf forgets
+everything at each token.  The decays are time constants, not learned: they
+have no gradient.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _native as N
+from ._tensors import DTYPE, check_rows, check_state, check_tensor, check_vector, on, ptr, require
+
+
+def _strides(t):
+    return t.stride(0), t.stride(1), t.stride(2)
+
+
+def _describe(q, k, v, log_decay, scale, cu_seqlens):
+    require(isinstance(q, torch.Tensor) and q.is_cuda, "q: a CUDA tensor is needed")
+    require(q.dtype in DTYPE, f"q: must be bfloat16, float16 or float32, is {q.dtype}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        require(isinstance(t, torch.Tensor) and t.dim() == 4, f"{name}: must be [batch, tokens, heads, d]")
+    b, t, h, dk = q.shape
+    hk, dv = k.shape[2], v.shape[3]
+    require(h >= 1 and hk >= 1 and h % hk == 0, f"heads: {h} of q are no multiple of {hk} of k")
+    check_rows(q, "q", q.dtype, q.device, (b, t, h, dk))
+    check_rows(k, "k", q.dtype, q.device, (b, t, hk, dk))
+    check_rows(v, "v", q.dtype, q.device, (b, t, hk, dv))
+    check_vector(log_decay, "log_decay", h, q.device)
+    a = N.LinAttn()
+    a.dtype, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[q.dtype], h, hk, dk, dv, t
+    if cu_seqlens is None:
+        a.seqs = b
+    else:
+        require(b == 1, "cu_seqlens: packed sequences have a batch dimension of 1")
+        check_tensor(cu_seqlens, "cu_seqlens", torch.int32, q.device)
+        require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and cu_seqlens.is_contiguous(),
+                "cu_seqlens: must be a contiguous vector of sequences + 1 starts")
+        a.seqs, a.cu_seqlens = cu_seqlens.numel() - 1, cu_seqlens.data_ptr()
+    a.log_decay = log_decay.data_ptr()
+    a.scale = dk ** -0.5 if scale is None else float(scale)
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
+    return a
+
+
+def _workspace(a, backward: bool, device):
+    n = C.c_int64()
+    N.check(N.lib().nrn_cuda_linattn_workspace(C.byref(a), int(backward), C.byref(n)), "nrn_cuda_linattn_workspace")
+    if n.value == 0:
+        return None
+    w = torch.empty(n.value, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = w.data_ptr(), n.value
+    return w
+
+
+def forward(q, k, v, log_decay, *, scale=None, state=None, cu_seqlens=None, out=None, stream=None):
+    """(o, final states) of whole sequences that go on from ``state`` (default: zero states).
+    o is like q with v's last dimension; ``scale`` defaults to dk ** -0.5."""
+    a = _describe(q, k, v, log_decay, scale, cu_seqlens)
+    b, t, h, _ = q.shape
+    with on(q.device, stream) as st:
+        if out is None:
+            out = torch.empty(b, t, h, a.dv, dtype=q.dtype, device=q.device)
+        else:
+            check_rows(out, "out", q.dtype, q.device, (b, t, h, a.dv))
+        if state is not None:
+            check_state(state, "state", q.device, (a.seqs, h, a.dk, a.dv))
+        end = torch.empty(a.seqs, h, a.dk, a.dv, dtype=torch.float32, device=q.device)
+        a.o, a.state_in, a.state_out = out.data_ptr(), ptr(state), end.data_ptr()
+        a.o_stride[:] = _strides(out)
+        w = _workspace(a, False, q.device)   # noqa: F841  (kept until the launches are enqueued)
+        N.check(N.lib().nrn_cuda_linattn_forward(C.byref(a), st), "nrn_cuda_linattn_forward")
+    return out, end
+
+
+def backward(do, q, k, v, log_decay, *, scale=None, state=None, dstate=None, cu_seqlens=None, stream=None):
+    """(dq, dk, dv, dstate) of a ``forward`` call with these arguments, given the gradients of o (``do``) and of the final
+    states (``dstate``, default: zero); the last result is the gradient of the states it started from."""
+    a = _describe(q, k, v, log_decay, scale, cu_seqlens)
+    b, t, h, _ = q.shape
+    check_rows(do, "do", q.dtype, q.device, (b, t, h, a.dv))
+    shape = (a.seqs, h, a.dk, a.dv)
+    for name, x in (("state", state), ("dstate", dstate)):
+        if x is not None:
+            check_state(x, name, q.device, shape)
+    with on(q.device, stream) as st:
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+        ds = torch.empty(shape, dtype=torch.float32, device=q.device)
+        a.state_in = ptr(state)
+        g = N.LinAttnGrad()
+        g.d_o, g.dstate_out, g.dstate_in = do.data_ptr(), ptr(dstate), ds.data_ptr()
+        g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        g.d_o_stride[:], g.dq_stride[:] = _strides(do), _strides(dq)
+        g.dk_stride[:], g.dv_stride[:] = _strides(dk), _strides(dv)
+        w = _workspace(a, True, q.device)    # noqa: F841
+        N.check(N.lib().nrn_cuda_linattn_backward(C.byref(a), C.byref(g), st), "nrn_cuda_linattn_backward")
+    return dq, dk, dv, ds
+
+
+def step(q, k, v, log_decay, state, *, scale=None, slots=None, out=None, stream=None):
+    """o of one token for each sequence ([batch, heads, d] tensors), updating ``state`` in place.  Sequence i uses
+    ``state[slots[i]]`` (int32, default: state[i]); a slot appears at most once in a call, a negative one is padding whose
+    output is 0, and one past the states gives NaN."""
+    require(isinstance(q, torch.Tensor) and q.is_cuda, "q: a CUDA tensor is needed")
+    require(q.dtype in DTYPE, f"q: must be bfloat16, float16 or float32, is {q.dtype}")
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        require(isinstance(x, torch.Tensor) and x.dim() == 3, f"{name}: must be [batch, heads, d]")
+    b, h, dk = q.shape
+    hk, dv = k.shape[1], v.shape[2]
+    require(h >= 1 and hk >= 1 and h % hk == 0, f"heads: {h} of q are no multiple of {hk} of k")
+    dev = q.device
+    check_rows(q, "q", q.dtype, dev, (b, h, dk))
+    check_rows(k, "k", q.dtype, dev, (b, hk, dk))
+    check_rows(v, "v", q.dtype, dev, (b, hk, dv))
+    check_vector(log_decay, "log_decay", h, dev)
+    require(isinstance(state, torch.Tensor) and state.dim() == 4, "state: must be [states, heads, dk, dv]")
+    check_tensor(state, "state", torch.float32, dev, (state.shape[0], h, dk, dv))
+    require(state.shape[0] <= 1 or state.stride()[1:] == (dk * dv, dv, 1) or state[0].is_contiguous(),
+            "state: each state must be contiguous")
+    if slots is not None:
+        check_tensor(slots, "slots", torch.int32, dev, (b,))
+        require(slots.is_contiguous(), "slots: must be contiguous")
+    else:
+        require(state.shape[0] >= b, f"state: {state.shape[0]} states for {b} sequences")
+    with on(dev, stream) as st:
+        if out is None:
+            out = torch.empty(b, h, dv, dtype=q.dtype, device=dev)
+        else:
+            check_rows(out, "out", q.dtype, dev, (b, h, dv))
+        a = N.LinAttn()
+        a.dtype, a.seqs, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[q.dtype], b, h, hk, dk, dv, 1
+        a.log_decay = log_decay.data_ptr()
+        a.scale = dk ** -0.5 if scale is None else float(scale)
+        a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        for f, x in ((a.q_stride, q), (a.k_stride, k), (a.v_stride, v), (a.o_stride, out)):
+            f[0], f[2] = x.stride(0), x.stride(1)
+        N.check(N.lib().nrn_cuda_linattn_step(C.byref(a), state.data_ptr(), state.stride(0), state.shape[0], ptr(slots), st),
+                "nrn_cuda_linattn_step")
+    return out

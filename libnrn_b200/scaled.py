@@ -1,0 +1,164 @@
+"""Matrix products in 8-bit floating point (e4m3) with a scale for each block
+of 128 columns.
+
+A ``Scaled`` matrix stands for values[r, c] * scales[r // row_block, c // 128].
+Activations and gradients have a scale for each row (row_block 1), weights one
+for each 128 x 128 block (row_block 128).  ``product`` is a @ b^T: 8-bit
+products summed in fp32 within a block, scaled, and summed in fp32.
+
+    w = scaled.quantize(weights, row_block=128)          # once
+    y = scaled.product(scaled.quantize(x), w)            # x @ weights^T, bf16
+    dx, dw = scaled.product_backward(dy, x, w)
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _native as N
+from ._tensors import DTYPE, check_tensor, on, require
+
+BLOCK = 128
+
+
+class Scaled:
+    """``values`` (float8_e4m3fn [rows, cols], rows 16-byte aligned) and their ``scales`` (fp32
+    [ceil(rows / row_block), ceil(cols / 128)], any strides).  ``quantize`` makes one; values and scales of a checkpoint
+    can be given as they are."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, row_block: int = 1):
+        require(row_block in (1, BLOCK), f"row_block: must be 1 or {BLOCK}, is {row_block}")
+        require(isinstance(values, torch.Tensor) and values.is_cuda and values.dim() == 2, "values: a CUDA matrix is needed")
+        check_tensor(values, "values", torch.float8_e4m3fn, values.device)
+        rows, cols = values.shape
+        check_tensor(scales, "scales", torch.float32, values.device, (-(-rows // row_block), -(-cols // BLOCK)))
+        require(cols <= 1 or values.stride(1) == 1, "values: the last dimension must have stride 1")
+        stride = values.stride(0)
+        if rows <= 1 or cols == 0:           # the stride of a single row or of empty ones says nothing
+            stride = -(-max(cols, 1) // 16) * 16
+        require(values.data_ptr() % 16 == 0 and stride % 16 == 0 and stride >= cols,
+                "values: rows must start on 16-byte boundaries (Scaled.empty allocates them so)")
+        self.values, self.scales, self.row_block = values, scales, row_block
+        self.desc = N.Scaled()
+        d = self.desc
+        d.values, d.scales, d.rows, d.cols = values.data_ptr(), scales.data_ptr(), rows, cols
+        d.value_stride, d.row_block = stride, row_block
+        d.scale_stride[0], d.scale_stride[1] = scales.stride(0), scales.stride(1)
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def device(self):
+        return self.values.device
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, device, row_block: int = 1) -> "Scaled":
+        pitch = -(-cols // 16) * 16
+        values = torch.empty(rows, pitch, dtype=torch.float8_e4m3fn, device=device)
+        # scales of neighbouring rows next to each other: as the product's threads read them
+        scales = torch.empty(-(-cols // BLOCK), -(-rows // row_block), dtype=torch.float32, device=device).t()
+        return cls(values[:, :cols] if pitch != cols else values, scales, row_block)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """What the matrix stands for, by torch operations (for checks and export)."""
+        rows, cols = self.shape
+        s = self.scales.repeat_interleave(self.row_block, 0)[:rows] if self.row_block > 1 else self.scales
+        return (self.values.float() * s.repeat_interleave(BLOCK, 1)[:, :cols]).to(dtype)
+
+
+def quantize(x: torch.Tensor, *, row_block: int = 1, transpose: bool = False, stream=None) -> Scaled:
+    """x (bf16, fp16 or fp32 [rows, cols], last stride 1) in 8 bits.  A block's scale is its largest magnitude / 448; an
+    infinity or NaN makes its whole block NaN.  ``transpose`` gives x^T with a scale for each of its rows (row_block 1)."""
+    require(isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2, "x: a CUDA matrix is needed")
+    require(x.dtype in DTYPE, f"x: must be bfloat16, float16 or float32, is {x.dtype}")
+    rows, cols = x.shape
+    require(cols <= 1 or x.stride(1) == 1, f"x: the last dimension must have stride 1, has {x.stride(1)}")
+    require(rows <= 1 or x.stride(0) >= cols, "x: rows overlap")
+    require(not transpose or row_block == 1, "transpose: only with a scale for each row")
+    with on(x.device, stream) as st:
+        out = Scaled.empty(cols, rows, x.device) if transpose else Scaled.empty(rows, cols, x.device, row_block)
+        N.check(N.lib().nrn_cuda_scaled_quantize(x.data_ptr(), DTYPE[x.dtype], rows, cols, x.stride(0) if rows > 1 else max(cols, 1),
+                                                 int(transpose), C.byref(out.desc), st), "nrn_cuda_scaled_quantize")
+    return out
+
+
+def transpose(w: Scaled, *, stream=None) -> Scaled:
+    """w^T of weights (row_block 128): the same values and scales."""
+    require(isinstance(w, Scaled) and w.row_block == BLOCK, "w: must be Scaled with a row_block of 128")
+    rows, cols = w.shape
+    with on(w.device, stream) as st:
+        pitch = -(-rows // 16) * 16
+        values = torch.empty(cols, pitch, dtype=torch.float8_e4m3fn, device=w.device)
+        out = Scaled(values[:, :rows], w.scales.t(), BLOCK)
+        N.check(N.lib().nrn_cuda_scaled_transpose(C.byref(w.desc), C.byref(out.desc), st), "nrn_cuda_scaled_transpose")
+    return out
+
+
+# Split products' workspaces, one for each stream (calls on one stream follow one another), and error flags.
+_workspaces: dict = {}
+_errors: dict = {}
+
+
+def _error_flag(device) -> torch.Tensor:
+    if device.index not in _errors:
+        _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+    return _errors[device.index]
+
+
+def _workspace(n: int, device, st) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(n, dtype=torch.uint8, device=device)      # belongs to the graph, zeroed by it
+    key = (device.index, st.value)
+    w = _workspaces.get(key)
+    if w is None or w.numel() < n:
+        w = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=device)
+    return w
+
+
+def check(device=None) -> None:
+    """Raises if a device-side wait of an earlier product on `device` (default: the current one) timed out."""
+    i = torch.cuda.current_device() if device is None else torch.device(device).index
+    if i in _errors and int(_errors[i].item()) != 0:
+        raise N.NrnError(7, f"nrn_cuda_scaled_product: device wait timed out (code {int(_errors[i].item())})")
+
+
+def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None) -> torch.Tensor:
+    """a @ b^T, [a rows, b rows], in ``dtype`` (bf16, fp16 or fp32)."""
+    require(isinstance(a, Scaled) and isinstance(b, Scaled), "a, b: must be Scaled (scaled.quantize)")
+    require(a.device == b.device, f"b: must be on {a.device}, is on {b.device}")
+    m, n = a.shape[0], b.shape[0]
+    require(a.shape[1] == b.shape[1], f"b: has {b.shape[1]} columns, a has {a.shape[1]}")
+    dev = a.device
+    with on(dev, stream) as st:
+        if out is None:
+            require(dtype in DTYPE, f"dtype: must be bfloat16, float16 or float32, is {dtype}")
+            out = torch.empty(m, n, dtype=dtype, device=dev)
+        else:
+            require(isinstance(out, torch.Tensor) and out.dtype in DTYPE, "out: must be bfloat16, float16 or float32")
+            check_tensor(out, "out", out.dtype, dev, (m, n))
+            require(n <= 1 or out.stride(1) == 1, "out: the last dimension must have stride 1")
+            require(m <= 1 or out.stride(0) >= n, "out: rows overlap")
+        need = C.c_int64()
+        L = N.lib()
+        N.check(L.nrn_cuda_scaled_workspace(C.byref(a.desc), C.byref(b.desc), C.byref(need)), "nrn_cuda_scaled_workspace")
+        w = _workspace(need.value, dev, st) if need.value else None
+        N.check(L.nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), DTYPE[out.dtype],
+                                          out.stride(0) if m > 1 else max(n, 1), None if w is None else w.data_ptr(), need.value,
+                                          _error_flag(dev).data_ptr(), st), "nrn_cuda_scaled_product")
+    return out
+
+
+def product_backward(dy: torch.Tensor, x: torch.Tensor, w: Scaled, *, dx_dtype=None, dw_dtype=torch.float32, stream=None):
+    """(dx, dw) of y = x @ w^T: dx = dy @ w and dw = dy^T @ x, with dy and x quantised along the axis that each of the two
+    sums over (dy's rows for dx; the columns of dy and x for dw)."""
+    require(isinstance(w, Scaled) and w.row_block == BLOCK, "w: must be Scaled with a row_block of 128")
+    for name, t, cols in (("dy", dy, w.shape[0]), ("x", x, w.shape[1])):
+        require(isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[1] == cols, f"{name}: must be [rows, {cols}]")
+    require(dy.shape[0] == x.shape[0], f"dy: has {dy.shape[0]} rows, x has {x.shape[0]}")
+    dx = product(quantize(dy, stream=stream), transpose(w, stream=stream), dtype=dx_dtype or dy.dtype, stream=stream)
+    dw = product(quantize(dy, transpose=True, stream=stream), quantize(x, transpose=True, stream=stream), dtype=dw_dtype,
+                 stream=stream)
+    return dx, dw
