@@ -31,6 +31,7 @@ namespace nrn {
 namespace {
 
 constexpr int kMaxDim = 256;       // largest key or value dimension
+constexpr int kChunk = 64;         // tokens of a chunk
 
 struct Strided {
     const void* p;
@@ -45,6 +46,7 @@ struct ScanArgs {
     int64_t o_seq, o_tok, o_head;
     int32_t o_f32;                 // o is fp32 whatever the inputs' type (partial sums of shared heads)
     int32_t vec;                   // rows of a, b, c start on 16-byte boundaries
+    int32_t o_vec;                 // rows of o do
     int32_t heads;
     int32_t seqs;
     int64_t tokens;                // per sequence, or of all packed sequences
@@ -255,6 +257,314 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
     }
 }
 
+// ------------------------------------------------------- chunks of 64 tokens
+//
+// bf16 inputs, b.d <= 128.  For a chunk of tokens p with entering state X:
+//     o_p = lam^(p+off) X^T a_p + sum_{j<=p} lam^(p-j) (a_p . b_j) c_j
+//     X'  = lam^n X + sum_j lam^(n-off-j) b_j c_j^T
+// A block holds 64 columns (c) of one state, a warp 16 of them: X^T as
+// 16 x b.d fp32 accumulators in registers for the whole scan, which are, cast
+// to bf16, the left operand of X^T a^T as they lie.  All products are 16x8x16
+// tensor-core instructions:
+//     P    = decayed a b^T, lower triangle only, once for the block (shared)
+//     o^T  = c^T P^T + (X^T a^T) lam^(p+off), written through shared memory
+//     X'^T = lam^n X^T + (w c)^T b
+// Roundings: P and the copy of X that is read are bf16, as the result is
+// (each at most 2^-9, sums fp32).  The state itself keeps fp32: the decayed
+// values w c are split into bf16 terms (TERMS = 3: all 24 bits; 2 where the
+// state that comes out is made elsewhere: 16 bits, below the results' 8).
+//
+// A token that is no number must not reach earlier tokens of its chunk
+// through the zeros of P (0 * inf): where the product with P has an element
+// that is not finite, the warp sums it again over j <= p alone.
+constexpr int kMmaThreads = 128;
+constexpr int kMmaCols = 64;
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+}
+__device__ __forceinline__ void stsm4t(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(p))),
+                 "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two fp32 as bf16, the first in the low half.
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float low_f32(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high_f32(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// Rows [t0, t0 + 64) of one operand as 64 x COLS bf16 in shared memory; zeros past the tokens and past m.d.
+template <int COLS>
+__device__ __forceinline__ void load_rows(__nv_bfloat16* dst, const Strided& m, const ScanArgs& p, const Unit& u, int64_t t0, int n, int head, int col0) {
+    constexpr int kPitch = COLS + 8;
+#pragma unroll
+    for (int e = threadIdx.x; e < kChunk * COLS / 8; e += kMmaThreads) {
+        const int t = e / (COLS / 8), c = (e % (COLS / 8)) * 8;
+        const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
+        const bool in = t < n && col0 + c < m.d;
+        const __nv_bfloat16* src = in ? row_ptr<__nv_bfloat16>(m, u, tok, head) + col0 + c : static_cast<const __nv_bfloat16*>(m.p);
+        __nv_bfloat16* d = dst + t * kPitch + c;
+        if (p.vec) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(d))), "l"(src),
+                         "r"(in ? 16 : 0)
+                         : "memory");
+        } else {
+            const Raw8<__nv_bfloat16> r = load8(src, in ? m.d - col0 - c : 0, false);
+            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(&r);
+        }
+    }
+}
+
+template <int DK>
+struct MmaSmem {
+    __nv_bfloat16 a[2][kChunk][DK + 8];
+    __nv_bfloat16 b[2][kChunk][DK + 8];
+    __nv_bfloat16 c[2][kChunk][kMmaCols + 8];
+    __nv_bfloat16 prob[kChunk][kChunk + 8];
+    __nv_bfloat16 out[4][32][24];
+    float pw[kChunk + 4];              // lam^0 .. lam^64
+};
+
+template <int DK, int TERMS, bool STATE_ONLY>
+__global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel(const __grid_constant__ ScanArgs p) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    MmaSmem<DK>& M = *reinterpret_cast<MmaSmem<DK>*>(smem_raw);
+    const int dc = p.c.d, db = p.b.d;
+    const int tiles = (dc + kMmaCols - 1) / kMmaCols;
+    const int tile = blockIdx.x % tiles;
+    const int head = (blockIdx.x / tiles) % p.heads;
+    const int unit = blockIdx.x / tiles / p.heads;
+    const Unit u = unit_of(p, unit);
+    if (!u.any) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, q = lane & 3;                  // row and column group of a fragment
+    const int l7 = lane & 7, l8 = (lane >> 3) & 1, l16 = lane >> 4;
+    const int col0 = tile * kMmaCols, wcol = col0 + warp * 16;
+    for (int i = threadIdx.x; i <= kChunk; i += kMmaThreads) M.pw[i] = decay_power(p.log_decay[head], i);
+
+    // X^T: element (wcol + g + 8 (e >> 1), 8 nt + 2 q + (e & 1)) in s[nt][e]
+    float s[DK / 8][4];
+    const int64_t sh = (static_cast<int64_t>(u.seq) * p.heads + head) * db * dc;
+    const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
+    const bool given = !STATE_ONLY && (p.seg != nullptr || p.s_in != nullptr);
+#pragma unroll
+    for (int nt = 0; nt < DK / 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = nt * 8 + 2 * q + (e & 1), j = wcol + g + 8 * (e >> 1);
+            s[nt][e] = 0.0f;
+            if (given && i < db && j < dc)
+                s[nt][e] = p.seg ? p.seg[gh + static_cast<int64_t>(i) * dc + j] : p.s_in[sh + i * p.s_i + j * p.s_j] * p.in_mul;
+        }
+
+    auto fetch = [&](int64_t t0, int stage) {
+        const int n = static_cast<int>(u.end - t0 < kChunk ? u.end - t0 : kChunk);
+        load_rows<DK>(&M.b[stage][0][0], p.b, p, u, t0, n, head, 0);
+        load_rows<kMmaCols>(&M.c[stage][0][0], p.c, p, u, t0, n, head, col0);
+        if (!STATE_ONLY) load_rows<DK>(&M.a[stage][0][0], p.a, p, u, t0, n, head, 0);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (u.begin < u.end) fetch(u.begin, 0);
+
+    int stage = 0;
+    for (int64_t t0 = u.begin; t0 < u.end; t0 += kChunk, stage ^= 1) {
+        const int n = static_cast<int>(u.end - t0 < kChunk ? u.end - t0 : kChunk);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();                 // this chunk is here, and everybody is done with the last one
+        if (t0 + kChunk < u.end) fetch(t0 + kChunk, stage ^ 1);
+        const auto& A = M.a[stage];
+        const auto& B = M.b[stage];
+        const auto& C = M.c[stage];
+
+        if constexpr (!STATE_ONLY) {
+            // P: the ten 16 x 16 tiles of the lower triangle, in turn over the warps
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+                const int id = warp + 4 * t;
+                if (id >= 10) break;
+                const int r = id < 1 ? 0 : (id < 3 ? 1 : (id < 6 ? 2 : 3)), c = id - r * (r + 1) / 2;
+                float acc[2][2][4] = {};
+#pragma unroll
+                for (int kk = 0; kk < DK / 16; ++kk) {
+                    uint32_t fa[4], fb[4];
+                    ldsm4(fa, &A[r * 16 + l7 + 8 * l8][kk * 16 + 8 * l16]);
+                    ldsm4(fb, &B[c * 16 + l7 + 8 * l16][kk * 16 + 8 * l8]);
+                    mma16816(acc[kk & 1][0], fa, fb[0], fb[1]);
+                    mma16816(acc[kk & 1][1], fa, fb[2], fb[3]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int i = r * 16 + g + 8 * h, j = c * 16 + nt * 8 + 2 * q;
+                        const float x = acc[0][nt][2 * h] + acc[1][nt][2 * h], y = acc[0][nt][2 * h + 1] + acc[1][nt][2 * h + 1];
+                        *reinterpret_cast<uint32_t*>(&M.prob[i][j]) =
+                            bf16x2(j <= i ? x * M.pw[i - j] : 0.0f, j + 1 <= i ? y * M.pw[i - j - 1] : 0.0f);
+                    }
+            }
+            __syncthreads();
+
+            // o^T: element (wcol + g + 8 (e >> 1), token 8 nt + 2 q + (e & 1))
+            float o[8][4] = {};
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                uint32_t fc[4];
+                ldsm4t(fc, &C[kk * 16 + l7 + 8 * l16][warp * 16 + 8 * l8]);
+#pragma unroll
+                for (int np = kk; np < 4; ++np) {
+                    uint32_t fp[4];
+                    ldsm4(fp, &M.prob[np * 16 + l7 + 8 * l16][kk * 16 + 8 * l8]);
+                    mma16816(o[2 * np], fc, fp[0], fp[1]);
+                    mma16816(o[2 * np + 1], fc, fp[2], fp[3]);
+                }
+            }
+            bool bad = false;
+#pragma unroll
+            for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[nt][e]) <= 3.4028234e38f);
+            if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = nt * 8 + 2 * q + (e & 1);
+                        float x = 0.0f;
+                        for (int j = 0; j <= i; ++j)
+                            x = fmaf(to_f32(M.prob[i][j]), to_f32(C[j][warp * 16 + g + 8 * (e >> 1)]), x);
+                        o[nt][e] = x;
+                    }
+            }
+            {
+                float x[8][4] = {};
+#pragma unroll
+                for (int kk = 0; kk < DK / 16; ++kk) {
+                    const uint32_t fs[4] = {bf16x2(s[2 * kk][0], s[2 * kk][1]), bf16x2(s[2 * kk][2], s[2 * kk][3]),
+                                            bf16x2(s[2 * kk + 1][0], s[2 * kk + 1][1]), bf16x2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+                    for (int np = 0; np < 4; ++np) {
+                        uint32_t fa[4];
+                        ldsm4(fa, &A[np * 16 + l7 + 8 * l16][kk * 16 + 8 * l8]);
+                        mma16816(x[2 * np], fs, fa[0], fa[1]);
+                        mma16816(x[2 * np + 1], fs, fa[2], fa[3]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[nt][e] = p.out_mul * fmaf(M.pw[nt * 8 + 2 * q + (e & 1) + p.off], x[nt][e], o[nt][e]);
+            }
+            if (p.o_f32) {
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int t = nt * 8 + 2 * q + (e & 1), j = wcol + g + 8 * (e >> 1);
+                        const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
+                        if (t < n && j < dc)
+                            static_cast<float*>(p.o)[(u.row0 + tok) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + j] = o[nt][e];
+                    }
+            } else {
+                // 32 tokens at a time through the warp's own 32 x 16 elements: 32 bytes a token
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int nt = half * 4 + 2 * k;
+                        stsm4t(&M.out[warp][k * 16 + l7 + 8 * l16][8 * l8], bf16x2(o[nt][0], o[nt][1]), bf16x2(o[nt][2], o[nt][3]),
+                               bf16x2(o[nt + 1][0], o[nt + 1][1]), bf16x2(o[nt + 1][2], o[nt + 1][3]));
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int r = k * 16 + (lane >> 1), t = half * 32 + r, j = wcol + 8 * (lane & 1);
+                        const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
+                        if (t >= n || j >= dc) continue;
+                        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.o) + (u.row0 + tok) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq +
+                                             head * p.o_head + j;
+                        const __nv_bfloat16* src = &M.out[warp][r][8 * (lane & 1)];
+                        if (p.o_vec) {
+                            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+                        } else {
+                            for (int e = 0; e < 8 && j + e < dc; ++e) dst[e] = src[e];
+                        }
+                    }
+                }
+            }
+        }
+
+        // the state
+        const float whole = M.pw[n];
+#pragma unroll
+        for (int nt = 0; nt < DK / 8; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][e] *= whole;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            if (kk * 16 >= n) break;
+            uint32_t fc[4], term[3][4];
+            ldsm4t(fc, &C[kk * 16 + l7 + 8 * l16][warp * 16 + 8 * l8]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {           // tokens 2 q and 2 q + 1 of the first and second eight
+                const int j = kk * 16 + 8 * h + 2 * q;
+                const float w0 = j < n ? M.pw[n - p.off - j] : 0.0f, w1 = j + 1 < n ? M.pw[n - p.off - j - 1] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float x = low_f32(fc[2 * h + r]) * w0, y = high_f32(fc[2 * h + r]) * w1;
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        const uint32_t z = bf16x2(x, y);
+                        term[k][2 * h + r] = z;
+                        x -= low_f32(z);
+                        y -= high_f32(z);
+                    }
+                }
+            }
+#pragma unroll
+            for (int np = 0; np < DK / 16; ++np) {
+                uint32_t fb[4];
+                ldsm4t(fb, &B[kk * 16 + l7 + 8 * l8][np * 16 + 8 * l16]);
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k) {
+                    mma16816(s[2 * np], term[k], fb[0], fb[1]);
+                    mma16816(s[2 * np + 1], term[k], fb[2], fb[3]);
+                }
+            }
+        }
+    }
+
+    float* to = STATE_ONLY ? p.seg : (u.last && p.seg == nullptr ? p.s_out : nullptr);
+    if (to == nullptr) return;
+#pragma unroll
+    for (int nt = 0; nt < DK / 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = nt * 8 + 2 * q + (e & 1), j = wcol + g + 8 * (e >> 1);
+            if (i >= db || j >= dc) continue;
+            if (STATE_ONLY) to[gh + static_cast<int64_t>(i) * dc + j] = s[nt][e];
+            else to[sh + i * p.s_i + j * p.s_j] = s[nt][e] * p.end_mul;
+        }
+}
+
 // ---------------------------------------------------------- segment states
 //
 // The segments' own end states (from zero) become the states that enter
@@ -421,15 +731,32 @@ cudaError_t launch_serial(const ScanArgs& p, bool state_only, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+template <int DK, int TERMS, bool STATE_ONLY>
+cudaError_t launch_mma(const ScanArgs& p, cudaStream_t s) {
+    const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kMmaCols - 1) / kMmaCols);
+    constexpr int bytes = sizeof(MmaSmem<DK>);
+    const cudaError_t e = cudaFuncSetAttribute(scan_mma_kernel<DK, TERMS, STATE_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    scan_mma_kernel<DK, TERMS, STATE_ONLY><<<static_cast<unsigned>(blocks), kMmaThreads, bytes, s>>>(p);
+    return cudaGetLastError();
+}
+
+template <int DK>
+cudaError_t launch_mma_any(const ScanArgs& p, bool state_only, cudaStream_t s) {
+    if (state_only) return launch_mma<DK, 3, true>(p, s);
+    // the final state comes out of this scan only where sequences are whole
+    return p.seg == nullptr && p.s_out != nullptr ? launch_mma<DK, 3, false>(p, s) : launch_mma<DK, 2, false>(p, s);
+}
+
 cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, cudaStream_t s) {
+    if (dtype == NRN_BF16 && p.b.d <= 64) return launch_mma_any<64>(p, state_only, s);
+    if (dtype == NRN_BF16 && p.b.d <= 128) return launch_mma_any<128>(p, state_only, s);
     if (dtype == NRN_BF16) return launch_serial<__nv_bfloat16>(p, state_only, s);
     if (dtype == NRN_FP16) return launch_serial<__half>(p, state_only, s);
     return launch_serial<float>(p, state_only, s);
 }
 
 int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
-
-constexpr int64_t kChunk = 64;
 
 // Tokens of a segment.  A scan is serial in time, so its parallelism is
 // sequences x heads x 64-column tiles; where that leaves most SMs idle the
@@ -476,6 +803,8 @@ int64_t workspace_need(const nrn_linattn_t* a, bool backward) {
 }
 
 nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, cudaStream_t s) {
+    const int per16 = 16 / elem_size(a->dtype);
+    p.o_vec = reinterpret_cast<uintptr_t>(p.o) % 16 == 0 && p.o_seq % per16 == 0 && p.o_tok % per16 == 0 && p.o_head % per16 == 0 && p.c.d % per16 == 0;
     if (p.cu) p.a.seq = p.b.seq = p.c.seq = p.o_seq = 0;      // packed: a token's row counts from the arrays' start
     p.seg_len = segment_length(a, p.c.d);
     const int64_t units = unit_count(a, p.seg_len);
