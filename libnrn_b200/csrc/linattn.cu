@@ -279,6 +279,10 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
 // that is not finite, the warp sums it again over j <= p alone.
 constexpr int kMmaThreads = 128;
 constexpr int kMmaCols = 64;
+#ifndef KMMA
+#define KMMA 32
+#endif
+constexpr int kMmaChunk = KMMA;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -297,7 +301,7 @@ __device__ __forceinline__ void stsm4t(void* p, uint32_t a, uint32_t b, uint32_t
                  : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -310,42 +314,58 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
 __device__ __forceinline__ float low_f32(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_f32(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
-// Rows [t0, t0 + 64) of one operand as 64 x COLS bf16 in shared memory; zeros past the tokens and past m.d.
-template <int COLS>
-__device__ __forceinline__ void load_rows(__nv_bfloat16* dst, const Strided& m, const ScanArgs& p, const Unit& u, int64_t t0, int n, int head, int col0) {
-    constexpr int kPitch = COLS + 8;
+// One operand's rows of CH tokens as CH x COLS bf16 in shared memory, zeros
+// past the tokens and past the operand's columns.  A thread has one place in
+// every kRows-th row; its address moves on by additions alone.
+template <int CH, int COLS>
+struct RowLoader {
+    static constexpr int kPitch = COLS + 8, kRows = kMmaThreads / (COLS / 8), kLoads = CH / kRows;
+    const __nv_bfloat16* src;
+    int64_t step;                  // kRows tokens on
+    int t, left;                   // first row; columns of the operand from this place on
+    uint32_t place;                // bytes from the start of the rows
+
+    __device__ __forceinline__ RowLoader(const Strided& m, const ScanArgs& p, const Unit& u, int head, int col0) {
+        t = threadIdx.x / (COLS / 8);
+        const int c = (threadIdx.x % (COLS / 8)) * 8;
+        left = m.d - col0 - c;
+        const int64_t first = p.reverse ? u.len - 1 - (u.begin + t) : u.begin + t;
+        src = row_ptr<__nv_bfloat16>(m, u, 0, head) + first * m.tok + col0 + c;
+        step = (p.reverse ? -m.tok : m.tok) * kRows;
+        place = static_cast<uint32_t>((t * kPitch + c) * 2);
+    }
+    // the next CH tokens, n of which there are
+    __device__ __forceinline__ void load(void* dst, const void* safe, int n, bool vec) {
+        const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst)) + place;
 #pragma unroll
-    for (int e = threadIdx.x; e < kChunk * COLS / 8; e += kMmaThreads) {
-        const int t = e / (COLS / 8), c = (e % (COLS / 8)) * 8;
-        const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
-        const bool in = t < n && col0 + c < m.d;
-        const __nv_bfloat16* src = in ? row_ptr<__nv_bfloat16>(m, u, tok, head) + col0 + c : static_cast<const __nv_bfloat16*>(m.p);
-        __nv_bfloat16* d = dst + t * kPitch + c;
-        if (p.vec) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(d))), "l"(src),
-                         "r"(in ? 16 : 0)
-                         : "memory");
-        } else {
-            const Raw8<__nv_bfloat16> r = load8(src, in ? m.d - col0 - c : 0, false);
-            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(&r);
+        for (int i = 0; i < kLoads; ++i, src += step) {
+            const bool in = t + i * kRows < n && left > 0;
+            if (vec) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + i * kRows * kPitch * 2), "l"(in ? static_cast<const void*>(src) : safe),
+                             "r"(in ? 16 : 0)
+                             : "memory");
+            } else {
+                const Raw8<__nv_bfloat16> r = load8(src, in ? left : 0, false);
+                *reinterpret_cast<uint4*>(static_cast<char*>(dst) + place + i * kRows * kPitch * 2) = *reinterpret_cast<const uint4*>(&r);
+            }
         }
     }
-}
-
-template <int DK>
-struct MmaSmem {
-    __nv_bfloat16 a[2][kChunk][DK + 8];
-    __nv_bfloat16 b[2][kChunk][DK + 8];
-    __nv_bfloat16 c[2][kChunk][kMmaCols + 8];
-    __nv_bfloat16 prob[kChunk][kChunk + 8];
-    __nv_bfloat16 out[4][32][24];
-    float pw[kChunk + 4];              // lam^0 .. lam^64
 };
 
-template <int DK, int TERMS, bool STATE_ONLY>
-__global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel(const __grid_constant__ ScanArgs p) {
+template <int DK, int CH>
+struct MmaSmem {
+    __nv_bfloat16 a[2][CH][DK + 8];
+    __nv_bfloat16 b[2][CH][DK + 8];
+    __nv_bfloat16 c[2][CH][kMmaCols + 8];
+    __nv_bfloat16 prob[CH][CH + 8];
+    __nv_bfloat16 out[4][32][24];
+    float pw[CH + 4];                  // lam^0 .. lam^CH
+};
+
+template <int DK, int CH, int TERMS, bool STATE_ONLY>
+__global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel(const __grid_constant__ ScanArgs p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    MmaSmem<DK>& M = *reinterpret_cast<MmaSmem<DK>*>(smem_raw);
+    MmaSmem<DK, CH>& M = *reinterpret_cast<MmaSmem<DK, CH>*>(smem_raw);
     const int dc = p.c.d, db = p.b.d;
     const int tiles = (dc + kMmaCols - 1) / kMmaCols;
     const int tile = blockIdx.x % tiles;
@@ -355,9 +375,10 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
     if (!u.any) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, q = lane & 3;                  // row and column group of a fragment
+    constexpr int kTiles = (CH / 16) * (CH / 16 + 1) / 2;
     const int l7 = lane & 7, l8 = (lane >> 3) & 1, l16 = lane >> 4;
     const int col0 = tile * kMmaCols, wcol = col0 + warp * 16;
-    for (int i = threadIdx.x; i <= kChunk; i += kMmaThreads) M.pw[i] = decay_power(p.log_decay[head], i);
+    for (int i = threadIdx.x; i <= CH; i += kMmaThreads) M.pw[i] = decay_power(p.log_decay[head], i);
 
     // X^T: element (wcol + g + 8 (e >> 1), 8 nt + 2 q + (e & 1)) in s[nt][e]
     float s[DK / 8][4];
@@ -374,31 +395,38 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
                 s[nt][e] = p.seg ? p.seg[gh + static_cast<int64_t>(i) * dc + j] : p.s_in[sh + i * p.s_i + j * p.s_j] * p.in_mul;
         }
 
+    RowLoader<CH, DK> la(p.a, p, u, head, 0), lb(p.b, p, u, head, 0);
+    RowLoader<CH, kMmaCols> lc(p.c, p, u, head, col0);
+    const bool vec = p.vec != 0;
+    // the results' place of this lane: token begin + lane / 2, eight of the warp's columns
+    const int oj = wcol + 8 * (lane & 1);
+    const int64_t ofirst = u.begin + (lane >> 1), ostep = p.reverse ? -p.o_tok : p.o_tok;
+    int64_t oat = (u.row0 + (p.reverse ? u.len - 1 - ofirst : ofirst)) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + oj;
     auto fetch = [&](int64_t t0, int stage) {
-        const int n = static_cast<int>(u.end - t0 < kChunk ? u.end - t0 : kChunk);
-        load_rows<DK>(&M.b[stage][0][0], p.b, p, u, t0, n, head, 0);
-        load_rows<kMmaCols>(&M.c[stage][0][0], p.c, p, u, t0, n, head, col0);
-        if (!STATE_ONLY) load_rows<DK>(&M.a[stage][0][0], p.a, p, u, t0, n, head, 0);
+        const int n = static_cast<int>(u.end - t0 < CH ? u.end - t0 : CH);
+        lb.load(&M.b[stage][0][0], p.b.p, n, vec);
+        lc.load(&M.c[stage][0][0], p.c.p, n, vec);
+        if (!STATE_ONLY) la.load(&M.a[stage][0][0], p.a.p, n, vec);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (u.begin < u.end) fetch(u.begin, 0);
 
     int stage = 0;
-    for (int64_t t0 = u.begin; t0 < u.end; t0 += kChunk, stage ^= 1) {
-        const int n = static_cast<int>(u.end - t0 < kChunk ? u.end - t0 : kChunk);
+    for (int64_t t0 = u.begin; t0 < u.end; t0 += CH, stage ^= 1) {
+        const int n = static_cast<int>(u.end - t0 < CH ? u.end - t0 : CH);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();                 // this chunk is here, and everybody is done with the last one
-        if (t0 + kChunk < u.end) fetch(t0 + kChunk, stage ^ 1);
+        if (t0 + CH < u.end) fetch(t0 + CH, stage ^ 1);
         const auto& A = M.a[stage];
         const auto& B = M.b[stage];
         const auto& C = M.c[stage];
 
         if constexpr (!STATE_ONLY) {
-            // P: the ten 16 x 16 tiles of the lower triangle, in turn over the warps
+            // P: the 16 x 16 tiles of the lower triangle, in turn over the warps
 #pragma unroll
-            for (int t = 0; t < 3; ++t) {
+            for (int t = 0; t < (kTiles + 3) / 4; ++t) {
                 const int id = warp + 4 * t;
-                if (id >= 10) break;
+                if (id >= kTiles) break;
                 const int r = id < 1 ? 0 : (id < 3 ? 1 : (id < 6 ? 2 : 3)), c = id - r * (r + 1) / 2;
                 float acc[2][2][4] = {};
 #pragma unroll
@@ -422,13 +450,13 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
             __syncthreads();
 
             // o^T: element (wcol + g + 8 (e >> 1), token 8 nt + 2 q + (e & 1))
-            float o[8][4] = {};
+            float o[CH / 8][4] = {};
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
+            for (int kk = 0; kk < CH / 16; ++kk) {
                 uint32_t fc[4];
                 ldsm4t(fc, &C[kk * 16 + l7 + 8 * l16][warp * 16 + 8 * l8]);
 #pragma unroll
-                for (int np = kk; np < 4; ++np) {
+                for (int np = kk; np < CH / 16; ++np) {
                     uint32_t fp[4];
                     ldsm4(fp, &M.prob[np * 16 + l7 + 8 * l16][kk * 16 + 8 * l8]);
                     mma16816(o[2 * np], fc, fp[0], fp[1]);
@@ -437,12 +465,12 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
             }
             bool bad = false;
 #pragma unroll
-            for (int nt = 0; nt < 8; ++nt)
+            for (int nt = 0; nt < CH / 8; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[nt][e]) <= 3.4028234e38f);
             if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll
-                for (int nt = 0; nt < 8; ++nt)
+                for (int nt = 0; nt < CH / 8; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = nt * 8 + 2 * q + (e & 1);
@@ -453,13 +481,13 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
                     }
             }
             {
-                float x[8][4] = {};
+                float x[CH / 8][4] = {};
 #pragma unroll
                 for (int kk = 0; kk < DK / 16; ++kk) {
                     const uint32_t fs[4] = {bf16x2(s[2 * kk][0], s[2 * kk][1]), bf16x2(s[2 * kk][2], s[2 * kk][3]),
                                             bf16x2(s[2 * kk + 1][0], s[2 * kk + 1][1]), bf16x2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
 #pragma unroll
-                    for (int np = 0; np < 4; ++np) {
+                    for (int np = 0; np < CH / 16; ++np) {
                         uint32_t fa[4];
                         ldsm4(fa, &A[np * 16 + l7 + 8 * l16][kk * 16 + 8 * l8]);
                         mma16816(x[2 * np], fs, fa[0], fa[1]);
@@ -467,14 +495,14 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
                     }
                 }
 #pragma unroll
-                for (int nt = 0; nt < 8; ++nt)
+                for (int nt = 0; nt < CH / 8; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         o[nt][e] = p.out_mul * fmaf(M.pw[nt * 8 + 2 * q + (e & 1) + p.off], x[nt][e], o[nt][e]);
             }
             if (p.o_f32) {
 #pragma unroll
-                for (int nt = 0; nt < 8; ++nt)
+                for (int nt = 0; nt < CH / 8; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int t = nt * 8 + 2 * q + (e & 1), j = wcol + g + 8 * (e >> 1);
@@ -485,7 +513,7 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
             } else {
                 // 32 tokens at a time through the warp's own 32 x 16 elements: 32 bytes a token
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int half = 0; half < CH / 32; ++half) {
                     __syncwarp();
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
@@ -496,16 +524,15 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
                     __syncwarp();
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const int r = k * 16 + (lane >> 1), t = half * 32 + r, j = wcol + 8 * (lane & 1);
-                        const int64_t tok = p.reverse ? u.len - 1 - (t0 + t) : t0 + t;
-                        if (t >= n || j >= dc) continue;
-                        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.o) + (u.row0 + tok) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq +
-                                             head * p.o_head + j;
+                        const int r = k * 16 + (lane >> 1), t = half * 32 + r;
+                        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.o) + oat;
+                        oat += 16 * ostep;
+                        if (t >= n || oj >= dc) continue;
                         const __nv_bfloat16* src = &M.out[warp][r][8 * (lane & 1)];
                         if (p.o_vec) {
                             *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
                         } else {
-                            for (int e = 0; e < 8 && j + e < dc; ++e) dst[e] = src[e];
+                            for (int e = 0; e < 8 && oj + e < dc; ++e) dst[e] = src[e];
                         }
                     }
                 }
@@ -519,7 +546,7 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[nt][e] *= whole;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
+        for (int kk = 0; kk < CH / 16; ++kk) {
             if (kk * 16 >= n) break;
             uint32_t fc[4], term[3][4];
             ldsm4t(fc, &C[kk * 16 + l7 + 8 * l16][warp * 16 + 8 * l8]);
@@ -540,14 +567,17 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 3 : 2) scan_mma_kernel
                 }
             }
 #pragma unroll
-            for (int np = 0; np < DK / 16; ++np) {
-                uint32_t fb[4];
-                ldsm4t(fb, &B[kk * 16 + l7 + 8 * l8][np * 16 + 8 * l16]);
+            for (int n4 = 0; n4 < DK / 16; n4 += 4) {   // eight accumulators between the terms of one
+                uint32_t fb[4][4];
 #pragma unroll
-                for (int k = 0; k < TERMS; ++k) {
-                    mma16816(s[2 * np], term[k], fb[0], fb[1]);
-                    mma16816(s[2 * np + 1], term[k], fb[2], fb[3]);
-                }
+                for (int i = 0; i < 4; ++i) ldsm4t(fb[i], &B[kk * 16 + l7 + 8 * l8][(n4 + i) * 16 + 8 * l16]);
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mma16816(s[2 * (n4 + i)], term[k], fb[i][0], fb[i][1]);
+                        mma16816(s[2 * (n4 + i) + 1], term[k], fb[i][2], fb[i][3]);
+                    }
             }
         }
     }
@@ -731,21 +761,21 @@ cudaError_t launch_serial(const ScanArgs& p, bool state_only, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-template <int DK, int TERMS, bool STATE_ONLY>
+template <int DK, int CH, int TERMS, bool STATE_ONLY>
 cudaError_t launch_mma(const ScanArgs& p, cudaStream_t s) {
     const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kMmaCols - 1) / kMmaCols);
-    constexpr int bytes = sizeof(MmaSmem<DK>);
-    const cudaError_t e = cudaFuncSetAttribute(scan_mma_kernel<DK, TERMS, STATE_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    constexpr int bytes = sizeof(MmaSmem<DK, CH>);
+    const cudaError_t e = cudaFuncSetAttribute(scan_mma_kernel<DK, CH, TERMS, STATE_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    scan_mma_kernel<DK, TERMS, STATE_ONLY><<<static_cast<unsigned>(blocks), kMmaThreads, bytes, s>>>(p);
+    scan_mma_kernel<DK, CH, TERMS, STATE_ONLY><<<static_cast<unsigned>(blocks), kMmaThreads, bytes, s>>>(p);
     return cudaGetLastError();
 }
 
 template <int DK>
 cudaError_t launch_mma_any(const ScanArgs& p, bool state_only, cudaStream_t s) {
-    if (state_only) return launch_mma<DK, 3, true>(p, s);
+    if (state_only) return launch_mma<DK, kMmaChunk, 3, true>(p, s);
     // the final state comes out of this scan only where sequences are whole
-    return p.seg == nullptr && p.s_out != nullptr ? launch_mma<DK, 3, false>(p, s) : launch_mma<DK, 2, false>(p, s);
+    return p.seg == nullptr && p.s_out != nullptr ? launch_mma<DK, kMmaChunk, 3, false>(p, s) : launch_mma<DK, kMmaChunk, 2, false>(p, s);
 }
 
 cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, cudaStream_t s) {
