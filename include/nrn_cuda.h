@@ -420,6 +420,7 @@ typedef struct {
     float* state_out;          /* the same, or NULL                          */
     void* workspace;           /* nrn_cuda_linattn_workspace bytes           */
     int64_t workspace_bytes;
+    int32_t* err;              /* device flag, set to 5 when a device-side wait gives up, or NULL */
 } nrn_linattn_t;
 
 /* The gradients of a forward pass with the same q, k, v and state_in (o and

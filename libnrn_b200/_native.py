@@ -124,7 +124,7 @@ class LinAttn(C.Structure):
         ("log_decay", C.c_void_p), ("scale", C.c_float), ("pad", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p),
         ("v", C.c_void_p), ("o", C.c_void_p), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
         ("v_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3), ("state_in", C.c_void_p),
-        ("state_out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("state_out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("err", C.c_void_p),
     ]
 
 

@@ -74,3 +74,23 @@ def on(device, stream=None):
     if stream is None and torch.cuda.current_device() == device.index:
         return _CURRENT
     return _switched(device, stream)
+
+
+# A flag on each device that kernels set when one of their bounded waits gives up.
+_errors: dict = {}
+
+
+def error_flag(device) -> int:
+    """Address of the device's flag."""
+    t = _errors.get(device.index)
+    if t is None:
+        t = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+    return t.data_ptr()
+
+
+def check_waits(device=None) -> None:
+    """Raises if a device-side wait of an earlier call on `device` (default: the current one) gave up.  Waits for the GPU."""
+    i = torch.cuda.current_device() if device is None else torch.device(device).index
+    t = _errors.get(i)
+    if t is not None and int(t.item()) != 0:
+        raise N.NrnError(7, f"a device-side wait timed out (code {int(t.item())})")

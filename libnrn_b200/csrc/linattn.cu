@@ -18,6 +18,7 @@
 // (dS: gradient of the final state; the state the reversed scan ends with,
 // times scale, is the gradient of S_0).  `off` says whether the state that
 // enters a token decays before it is read.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -25,6 +26,8 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "tc.cuh"
+#include "tensor_map.h"
 #include "vecio.cuh"
 
 namespace nrn {
@@ -60,6 +63,7 @@ struct ScanArgs {
     float* seg;                    // [units][heads][b.d][c.d]: states of segments, or null
     int64_t seg_len;               // tokens of a segment (a multiple of the chunk)
     int32_t units;
+    int32_t* err;                  // set when a device-side wait gives up, or null
 };
 
 // ------------------------------------------------------------------ units
@@ -595,6 +599,479 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
         }
 }
 
+// -------------------------------------------------- the same on tcgen05
+//
+// bf16 rows on 16-byte boundaries, b.d <= 128: chunks of 64 tokens, 128
+// columns (c) of one state a block, products on tcgen05 with fp32
+// accumulators in TMEM, in the transposed form (TMEM lane = column of c):
+//     P     [64 x 64]   = a b^T                 lanes: tokens i
+//     inter [128 x 64]  = X16^T a^T             X16: the entering state in bf16
+//     U     [128 x b.d] = sum over terms of (w c)^T b
+//     intra [128 x 64]  = c^T P^T
+// Ten warps, one block an SM:
+//   warp 0    copies: a, b and c of a chunk by TMA into one of two stages;
+//   warp 1    issues the MMAs (one thread);
+//   warps 2-9 everything else, in the order that keeps the tensor cores busy
+//             behind them: (1) c^T, its decayed terms and b^T through
+//             ldmatrix/stmatrix into K-major tiles, while P and inter run;
+//             (2) P out of TMEM, decay and mask, bf16, while U runs; (3) the
+//             fp32 state, kept in registers (64 a thread): lam^n X + U, and
+//             its bf16 copy, while intra runs; (4) the results.
+// About 70 warp instructions a token and head against 270 with mma.sync
+// (whose operands pass through registers in every warp).
+constexpr int kTcThreads = 320;
+constexpr int kTcCols = 128;
+enum { ERR_LINATTN_TIMEOUT = 5 };
+
+using namespace tc;
+
+template <int DK, int TERMS, bool STATE_ONLY>
+struct TcSmem {
+    static constexpr int kTile = kChunk * 128;                        // 64 rows of 64 bf16: 8 KB
+    static constexpr int kTilesA = STATE_ONLY ? 0 : DK / 64, kTilesB = DK / 64, kTilesC = 2;
+    static constexpr int kStage = (kTilesA + kTilesB + kTilesC) * kTile;
+    static constexpr int kHead = 2048;
+    static constexpr int kCt = kHead + 2 * kStage;                    // c^T [128][64]
+    static constexpr int kWt = kCt + (STATE_ONLY ? 0 : 128 * 128);    // its terms
+    static constexpr int kBt = kWt + TERMS * 128 * 128;               // b^T [DK][64]
+    static constexpr int kX16 = kBt + DK * 128;                       // [128][DK]
+    static constexpr int kProb = kX16 + (STATE_ONLY ? 0 : 128 * DK * 2);   // [64][64]
+    static constexpr int kBytes = kProb + (STATE_ONLY ? 0 : kTile);
+};
+static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
+
+struct TcHead {
+    uint64_t full[2], empty[2], pready, psm, x16, vk, uready, oready, drain;
+    uint32_t tmem;
+    int abort;
+    float lag[128];                // factor of P at token i - token j, from -63 on
+    float w[kChunk];               // decay of each token to the chunk's end
+    float out[kChunk];             // and of the entering state to each token, times out_mul
+};
+static_assert(sizeof(TcHead) <= 2048, "barriers and factors");
+
+// No swizzle: rows of 16 bytes, eight rows to a core matrix, core matrices of
+// one row group 128 bytes apart, row groups `group` bytes apart.
+__device__ __forceinline__ uint64_t desc_plain(uint32_t addr, uint32_t group) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128 >> 4) << 16) |
+           (static_cast<uint64_t>(group >> 4) << 32) | (1ull << 46);
+}
+// 128-byte swizzle as TMA writes it.
+__device__ __forceinline__ uint64_t desc_swizzled(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+template <int MM, int NN>
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, bool accumulate) {
+    constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NN >> 3) << 17) | (static_cast<uint32_t>(MM >> 4) << 24);
+    const uint32_t zero = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(zero)
+        : "memory");
+}
+__device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void ldsm4t_at(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+// 16 lanes x 32 columns as the fragments of four 16x8 accumulators.
+__device__ __forceinline__ void tc_ld_frag(uint32_t taddr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld32(uint32_t* v) {
+    tc_wait_ld16(v);
+    tc_wait_ld16(v + 16);
+}
+
+template <int DK, int TERMS, bool STATE_ONLY>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    scan_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                   const __grid_constant__ CUtensorMap cmap, const __grid_constant__ ScanArgs p) {
+    using L = TcSmem<DK, TERMS, STATE_ONLY>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    TcHead& M = *reinterpret_cast<TcHead*>(smem);
+    const uint32_t base = smem_u32(smem);
+    volatile int* abort = &M.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int db = p.b.d, dc = p.c.d;
+    const int tiles = (dc + kTcCols - 1) / kTcCols;
+    const int tile = blockIdx.x % tiles;
+    const int head = (blockIdx.x / tiles) % p.heads;
+    const int unit = blockIdx.x / tiles / p.heads;
+    const Unit u = unit_of(p, unit);
+    if (!u.any) return;
+    const int chunks = static_cast<int>((u.end - u.begin + kChunk - 1) / kChunk);
+    constexpr uint32_t kP = 0, kU = 64, kIntra = 192, kInter = 256;      // TMEM columns
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&M.full[i], 1);
+            mbar_init(&M.empty[i], 1);
+        }
+        mbar_init(&M.pready, 1);
+        mbar_init(&M.uready, 1);
+        mbar_init(&M.oready, 1);
+        mbar_init(&M.drain, 1);
+        mbar_init(&M.psm, 8);
+        mbar_init(&M.x16, 8);
+        mbar_init(&M.vk, 8);
+        M.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&M.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = M.tmem;
+    auto fail = [&]() {
+        *abort = 1;
+        if (p.err) atomicCAS(p.err, 0, ERR_LINATTN_TIMEOUT);
+    };
+    // tokens of chunk c, and the first of them in memory order
+    auto tokens = [&](int c) { return static_cast<int>(u.end - u.begin - static_cast<int64_t>(c) * kChunk < kChunk ? u.end - u.begin - static_cast<int64_t>(c) * kChunk : kChunk); };
+    auto first = [&](int c) {
+        const int64_t t = u.begin + static_cast<int64_t>(c) * kChunk;
+        return p.reverse ? u.len - t - tokens(c) : t;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int c = 0;
+            for (; c < chunks; ++c) {
+                const int st = c & 1;
+                if (!mbar_wait(&M.empty[st], ((c >> 1) & 1) ^ 1u, abort)) {
+                    fail();
+                    break;
+                }
+                const uint32_t dst = base + L::kHead + st * L::kStage;
+                const int tok = static_cast<int>(u.row0 + first(c)), seq = p.cu ? 0 : u.seq;
+                mbar_expect_tx(&M.full[st], L::kStage);
+                for (int i = 0; i < L::kTilesA; ++i)
+                    tma_load_4d(dst + i * L::kTile, &amap, 64 * i, head / p.a.share, tok, seq, &M.full[st]);
+                for (int i = 0; i < L::kTilesB; ++i)
+                    tma_load_4d(dst + (L::kTilesA + i) * L::kTile, &bmap, 64 * i, head / p.b.share, tok, seq, &M.full[st]);
+                for (int i = 0; i < L::kTilesC; ++i)
+                    tma_load_4d(dst + (L::kTilesA + L::kTilesB + i) * L::kTile, &cmap, tile * kTcCols + 64 * i, head / p.c.share, tok, seq, &M.full[st]);
+            }
+            // the copies still in flight land before the block ends
+            for (int q = c - 1; q >= 0 && q >= c - 2; --q) mbar_wait(&M.full[q & 1], (q >> 1) & 1, nullptr);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int c = 0; c < chunks && ok; ++c) {
+                const int st = c & 1;
+                const uint32_t ph = c & 1;
+                const uint32_t sa = base + L::kHead + st * L::kStage, sb = sa + L::kTilesA * L::kTile;
+                ok = mbar_wait(&M.full[st], (c >> 1) & 1, abort);
+                if (!ok) break;
+                tc_fence_after();
+                if constexpr (!STATE_ONLY) {
+                    // P: the last chunk's was read before psm of that chunk, on which intra waited
+#pragma unroll
+                    for (int kk = 0; kk < DK / 16; ++kk)
+                        mma_bf16<64, 64>(tmem + kP, desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32),
+                                         desc_swizzled(sb + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
+                    tc_commit(&M.pready);
+                    ok = mbar_wait(&M.x16, ph, abort);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < DK / 16; ++kk)
+                        mma_bf16<128, 64>(tmem + kInter + 64 * st, desc_plain(base + L::kX16 + kk * 256, DK * 16),
+                                          desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
+                }
+                ok = mbar_wait(&M.vk, ph, abort);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_bf16<128, DK>(tmem + kU, desc_plain(base + L::kWt + t * 128 * 128 + kk * 256, 1024),
+                                          desc_plain(base + L::kBt + kk * 256, 1024), t + kk > 0);
+                tc_commit(&M.uready);
+                if constexpr (!STATE_ONLY) {
+                    ok = mbar_wait(&M.psm, ph, abort);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_bf16<128, 64>(tmem + kIntra, desc_plain(base + L::kCt + kk * 256, 1024),
+                                          desc_plain(base + L::kProb + kk * 256, 1024), kk > 0);
+                    tc_commit(&M.oready);
+                }
+                tc_commit(&M.empty[st]);
+            }
+            if (!ok) fail();
+            // every MMA issued has completed before the accumulators are freed
+            tc_commit(&M.drain);
+            mbar_wait(&M.drain, 0, nullptr);
+        }
+    } else {
+        const int ew = warp - 2, sub = warp & 3, half = ew >> 2;      // TMEM lanes 32 sub ..; this warp's half of the columns
+        const int et = threadIdx.x - 64;
+        const int l7 = lane & 7, l8 = (lane >> 3) & 1, l16 = lane >> 4, q = lane & 3, g8 = lane >> 2;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * sub) << 16);
+        const float g = p.log_decay[head];
+        const int row = tile * kTcCols + 32 * sub + lane;             // column of c
+        const int64_t sh = (static_cast<int64_t>(u.seq) * p.heads + head) * db * dc;
+        const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
+        constexpr int kX = DK / 2;
+        const int x0 = half * kX;                                     // first row of b's dimension of this thread
+        float x[kX];
+        const bool given = !STATE_ONLY && (p.seg != nullptr || p.s_in != nullptr) && row < dc;
+#pragma unroll
+        for (int i = 0; i < kX; ++i) {
+            x[i] = 0.0f;
+            if (given && x0 + i < db)
+                x[i] = p.seg ? p.seg[gh + static_cast<int64_t>(x0 + i) * dc + row] : p.s_in[sh + (x0 + i) * p.s_i + row * p.s_j] * p.in_mul;
+        }
+        // the bf16 copy of this thread's part of the state: 16-byte rows of core matrices
+        auto copy_state = [&]() {
+            const uint32_t at = base + L::kX16 + ((32 * sub + lane) >> 3) * (DK * 16) + (lane & 7) * 16 + (x0 / 8) * 128;
+#pragma unroll
+            for (int i = 0; i < kX; i += 8)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 16), "r"(bf16x2(x[i], x[i + 1])),
+                             "r"(bf16x2(x[i + 2], x[i + 3])), "r"(bf16x2(x[i + 4], x[i + 5])), "r"(bf16x2(x[i + 6], x[i + 7]))
+                             : "memory");
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&M.x16);
+        };
+        if (!STATE_ONLY && chunks > 0) copy_state();
+        if (et < 127) M.lag[et] = p.out_mul * ((p.reverse ? et <= 63 : et >= 63) ? decay_power(g, p.reverse ? 63 - et : et - 63) : 0.0f);
+        float whole = 0.0f;
+        bool ok = true;
+        for (int c = 0; c < chunks; ++c) {
+            const int st = c & 1, n = tokens(c);
+            const uint32_t ph = c & 1;
+            const uint32_t sb = base + L::kHead + st * L::kStage + L::kTilesA * L::kTile, sc = sb + L::kTilesB * L::kTile;
+            // everybody is done with the last chunk's tiles and factors
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (c == 0 || n < kChunk) {
+                if (et < kChunk) {
+                    const int pos = p.reverse ? n - 1 - et : et;
+                    M.w[et] = et < n ? decay_power(g, n - p.off - pos) : 0.0f;
+                    M.out[et] = et < n ? p.out_mul * decay_power(g, pos + p.off) : 0.0f;
+                }
+                whole = decay_power(g, n);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            }
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
+            if (ok) {
+                // (1) c^T, its terms and b^T: this warp's 16 columns of each, 16 tokens at a time
+                const uint32_t to = (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
+                const uint32_t from = (ew >> 2) * L::kTile + (l7 + 8 * l16) * 128 + (((2 * (ew & 3) + l8) ^ l7) << 4);
+                uint32_t fc[4][4], fb[4][4];
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) ldsm4t_at(fc[kk], sc + from + kk * 2048);
+                if (ew < DK / 16)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) ldsm4t_at(fb[kk], sb + from + kk * 2048);
+                if (n < kChunk) {
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const int j = kk * 16 + (h >> 1) * 8 + 2 * q;
+                            const uint32_t keep = j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
+                            fc[kk][h] &= keep;
+                            fb[kk][h] &= keep;
+                        }
+                }
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    uint32_t term[TERMS][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 w = *reinterpret_cast<const float2*>(&M.w[kk * 16 + 8 * h + 2 * q]);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float y = low_f32(fc[kk][2 * h + r]) * w.x, z = high_f32(fc[kk][2 * h + r]) * w.y;
+#pragma unroll
+                            for (int k = 0; k < TERMS; ++k) {
+                                const uint32_t b2 = bf16x2(y, z);
+                                term[k][2 * h + r] = b2;
+                                if (k + 1 < TERMS) {
+                                    y -= low_f32(b2);
+                                    z -= high_f32(b2);
+                                }
+                            }
+                        }
+                    }
+                    if (!STATE_ONLY) stsm4(base + L::kCt + to + kk * 256, fc[kk][0], fc[kk][1], fc[kk][2], fc[kk][3]);
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k)
+                        stsm4(base + L::kWt + k * 128 * 128 + to + kk * 256, term[k][0], term[k][1], term[k][2], term[k][3]);
+                    if (ew < DK / 16) stsm4(base + L::kBt + to + kk * 256, fb[kk][0], fb[kk][1], fb[kk][2], fb[kk][3]);
+                }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&M.vk);
+            }
+            if constexpr (!STATE_ONLY) {
+                // (2) P
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.pready, ph, abort));
+                if (ok) {
+                    tc_fence_after();
+                    // rows i = 16 sub + g and + 8, columns j = 32 half + 8 nt + 2 q and + 1: v[4 nt ..]
+                    uint32_t v[16];
+                    tc_ld_frag(lanes + kP + 32 * half, v);
+                    tc_wait_ld16(v);
+                    const int i = 16 * sub + g8, j0 = 32 * half + 2 * q, jn = n - j0;
+                    const float* lag = &M.lag[63 + i - j0];
+                    const int d = i - j0;
+                    uint32_t r[8];
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int e = 8 * nt - 8 * h;                // token j - token i is e - d
+                            // in reverse the tokens past the sequence's end come before: they are masked here
+                            const bool s0 = p.reverse ? d <= e && 8 * nt < jn : d >= e, s1 = p.reverse ? d <= e + 1 && 8 * nt + 1 < jn : d >= e + 1;
+                            r[2 * nt + h] = bf16x2(s0 ? __uint_as_float(v[4 * nt + 2 * h]) * lag[-e] : 0.0f,
+                                                   s1 ? __uint_as_float(v[4 * nt + 2 * h + 1]) * lag[-e - 1] : 0.0f);
+                        }
+                    // matrices (rows 0-7, 8-15) x (columns 8 nt, 8 nt + 8)
+                    const uint32_t at = base + L::kProb + (2 * sub + l8) * 1024 + (4 * half + l16) * 128 + l7 * 16;
+                    stsm4(at, r[0], r[1], r[2], r[3]);
+                    stsm4(at + 256, r[4], r[5], r[6], r[7]);
+                    tc_fence_before();
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&M.psm);
+                }
+            }
+            // (3) the state
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph, abort));
+            bool bad = false;
+            if (ok) {
+                tc_fence_after();
+#pragma unroll
+                for (int i0 = 0; i0 < kX; i0 += 32) {
+                    uint32_t v[32];
+                    tc_ld32(lanes + kU + x0 + i0, v);
+                    tc_wait_ld32(v);
+                    // a column of c with a value that is no number shows in every element of its row of U
+                    if (i0 == 0) bad = !(fabsf(__uint_as_float(v[0])) <= 3.4028234e38f);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i0 + i] = fmaf(whole, x[i0 + i], __uint_as_float(v[i]));
+                }
+                tc_fence_before();
+                if (!STATE_ONLY && c + 1 < chunks) copy_state();
+            }
+            if constexpr (!STATE_ONLY) {
+                // (4) the results: 32 tokens of this lane's column
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.oready, ph, abort));
+                if (ok) {
+                    tc_fence_after();
+                    const int m = n - 32 * half;         // tokens of this half
+                    // bf16 results pass through 2 KB of this warp's own (the terms were read when U was done)
+                    unsigned char* own = smem + L::kWt + ew * 2048;
+#pragma unroll
+                    for (int t0 = 0; t0 < 32; t0 += 16) {
+                        uint32_t a[16], b[16];
+                        tc_ld16(lanes + kIntra + 32 * half + t0, a);
+                        tc_ld16(lanes + kInter + 64 * st + 32 * half + t0, b);
+                        tc_wait_ld16(a);
+                        tc_wait_ld16(b);
+                        if (__any_sync(0xffffffffu, bad)) {
+                            // sum over the tokens that count, alone
+#pragma unroll
+                            for (int t = 0; t < 16; ++t) {
+                                const int i = 32 * half + t0 + t;
+                                const unsigned char* pp = smem + L::kProb + (i >> 3) * 1024 + (i & 7) * 16;
+                                const unsigned char* cc = smem + L::kCt + (4 * sub + (lane >> 3)) * 1024 + l7 * 16;
+                                float y = 0.0f;
+                                for (int j = p.reverse ? i : 0; j < (p.reverse ? n : i + 1); ++j)
+                                    y = fmaf(to_f32(*reinterpret_cast<const __nv_bfloat16*>(pp + (j >> 3) * 128 + (j & 7) * 2)),
+                                             to_f32(*reinterpret_cast<const __nv_bfloat16*>(cc + (j >> 3) * 128 + (j & 7) * 2)), y);
+                                a[t] = __float_as_uint(y);
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < 16; t += 4) {
+                            const float4 w = *reinterpret_cast<const float4*>(&M.out[32 * half + t0 + t]);
+                            a[t] = __float_as_uint(fmaf(w.x, __uint_as_float(b[t]), __uint_as_float(a[t])));
+                            a[t + 1] = __float_as_uint(fmaf(w.y, __uint_as_float(b[t + 1]), __uint_as_float(a[t + 1])));
+                            a[t + 2] = __float_as_uint(fmaf(w.z, __uint_as_float(b[t + 2]), __uint_as_float(a[t + 2])));
+                            a[t + 3] = __float_as_uint(fmaf(w.w, __uint_as_float(b[t + 3]), __uint_as_float(a[t + 3])));
+                        }
+                        if (p.o_f32) {
+                            float* to = static_cast<float*>(p.o) + (u.row0 + first(c) + 32 * half + t0) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + row;
+#pragma unroll
+                            for (int t = 0; t < 16; ++t, to += p.o_tok)
+                                if (t0 + t < m && row < dc) *to = __uint_as_float(a[t]);
+                        } else {
+#pragma unroll
+                            for (int t = 0; t < 16; t += 2) {
+                                const uint32_t two = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
+                                *reinterpret_cast<uint16_t*>(own + (t0 + t) * 64 + lane * 2) = static_cast<uint16_t>(two);
+                                *reinterpret_cast<uint16_t*>(own + (t0 + t + 1) * 64 + lane * 2) = static_cast<uint16_t>(two >> 16);
+                            }
+                        }
+                    }
+                    if (!p.o_f32) {
+                        __syncwarp();
+                        // 64 bytes a token, eight tokens at a time
+                        const int t = lane >> 2, j = tile * kTcCols + 32 * sub + 8 * q;
+                        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + (u.row0 + first(c) + 32 * half + t) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + j;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k, to += 8 * p.o_tok) {
+                            const uint4 r = *reinterpret_cast<const uint4*>(own + (8 * k + t) * 64 + q * 16);
+                            if (8 * k + t >= m || j >= dc) continue;
+                            if (p.o_vec) {
+                                *reinterpret_cast<uint4*>(to) = r;
+                            } else {
+                                const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&r);
+#pragma unroll
+                                for (int x8 = 0; x8 < 8; ++x8)
+                                    if (j + x8 < dc) to[x8] = e[x8];
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                }
+            }
+        }
+        float* to = STATE_ONLY ? p.seg : (u.last && p.seg == nullptr ? p.s_out : nullptr);
+        if (to != nullptr && row < dc && ok) {
+#pragma unroll
+            for (int i = 0; i < kX; ++i) {
+                if (x0 + i >= db) continue;
+                if (STATE_ONLY) to[gh + static_cast<int64_t>(x0 + i) * dc + row] = x[i];
+                else to[sh + (x0 + i) * p.s_i + row * p.s_j] = x[i] * p.end_mul;
+            }
+        }
+        if (!ok && lane == 0) fail();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
 // ---------------------------------------------------------- segment states
 //
 // The segments' own end states (from zero) become the states that enter
@@ -778,7 +1255,42 @@ cudaError_t launch_mma_any(const ScanArgs& p, bool state_only, cudaStream_t s) {
     return p.seg == nullptr && p.s_out != nullptr ? launch_mma<DK, kMmaChunk, 3, false>(p, s) : launch_mma<DK, kMmaChunk, 2, false>(p, s);
 }
 
+// Tensor map of one operand: d, head, token, sequence; boxes of 64 elements of 64 tokens.
+bool make_scan_map(const Strided& m, const ScanArgs& p, CUtensorMap* map) {
+    const TensorMapEncode fn = tensor_map_encode();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(m.d), static_cast<cuuint64_t>(p.heads / m.share), static_cast<cuuint64_t>(p.tokens),
+                                static_cast<cuuint64_t>(p.cu ? 1 : p.seqs)};
+    // the stride of a dimension of one says nothing, and may be anything
+    const cuuint64_t strides[3] = {dims[1] > 1 ? static_cast<cuuint64_t>(m.head) * 2 : 16, dims[2] > 1 ? static_cast<cuuint64_t>(m.tok) * 2 : 16,
+                                   dims[3] > 1 ? static_cast<cuuint64_t>(m.seq) * 2 : 16};
+    const cuuint32_t box[4] = {64, 1, kChunk, 1}, one[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(m.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DK, int TERMS, bool STATE_ONLY>
+cudaError_t launch_tc(const ScanArgs& p, const CUtensorMap* maps, cudaStream_t s) {
+    const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kTcCols - 1) / kTcCols);
+    constexpr int bytes = TcSmem<DK, TERMS, STATE_ONLY>::kBytes;
+    const cudaError_t e = cudaFuncSetAttribute(scan_tc_kernel<DK, TERMS, STATE_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    scan_tc_kernel<DK, TERMS, STATE_ONLY><<<static_cast<unsigned>(blocks), kTcThreads, bytes, s>>>(maps[0], maps[1], maps[2], p);
+    return cudaGetLastError();
+}
+
+template <int DK>
+cudaError_t launch_tc_any(const ScanArgs& p, const CUtensorMap* maps, bool state_only, cudaStream_t s) {
+    if (state_only) return launch_tc<DK, 3, true>(p, maps, s);
+    return p.seg == nullptr && p.s_out != nullptr ? launch_tc<DK, 3, false>(p, maps, s) : launch_tc<DK, 2, false>(p, maps, s);
+}
+
 cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, cudaStream_t s) {
+    if (dtype == NRN_BF16 && p.b.d <= 128 && p.vec && p.tokens > 0 && p.tokens < (int64_t(1) << 31) - kChunk) {
+        CUtensorMap maps[3];
+        if (make_scan_map(p.a, p, &maps[0]) && make_scan_map(p.b, p, &maps[1]) && make_scan_map(p.c, p, &maps[2]))
+            return p.b.d <= 64 ? launch_tc_any<64>(p, maps, state_only, s) : launch_tc_any<128>(p, maps, state_only, s);
+    }
     if (dtype == NRN_BF16 && p.b.d <= 64) return launch_mma_any<64>(p, state_only, s);
     if (dtype == NRN_BF16 && p.b.d <= 128) return launch_mma_any<128>(p, state_only, s);
     if (dtype == NRN_BF16) return launch_serial<__nv_bfloat16>(p, state_only, s);
@@ -792,8 +1304,8 @@ int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
 // sequences x heads x 64-column tiles; where that leaves most SMs idle the
 // sequences are split.
 int64_t segment_length(const nrn_linattn_t* a, int dc) {
-    const int64_t tiles = (dc + 63) / 64;
-    const int64_t want = 2LL * sm_count_current();                    // blocks that fill the GPU
+    const int64_t tiles = (dc + kTcCols - 1) / kTcCols;
+    const int64_t want = sm_count_current();                          // blocks that fill the GPU
     const int64_t rows = static_cast<int64_t>(a->heads) * tiles;
     const int64_t all = a->cu_seqlens ? a->tokens : a->tokens * a->seqs;
     if (all == 0) return kChunk;
@@ -888,6 +1400,7 @@ ScanArgs scan_args(const nrn_linattn_t* a) {
     p.tokens = a->tokens;
     p.cu = a->cu_seqlens;
     p.log_decay = a->log_decay;
+    p.err = a->err;
     p.out_mul = a->scale;
     p.in_mul = p.end_mul = 1.0f;
     p.off = 1;

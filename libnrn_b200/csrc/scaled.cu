@@ -37,6 +37,7 @@
 #include "internal.h"
 #include "scaled.cuh"
 #include "tc.cuh"
+#include "tensor_map.h"
 #include "vecio.cuh"
 
 namespace nrn {
@@ -556,25 +557,8 @@ __global__ void __launch_bounds__(kQuantThreads)
 
 // --------------------------------------------------------------- launches
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-    static std::once_flag once;
-    static EncodeFn fn = nullptr;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeFn>(p);
-    });
-    return fn;
-}
-
 nrn_status_t make_map(const nrn_scaled_t* m, int box_rows, CUtensorMap* map) {
-    EncodeFn fn = encode_fn();
+    const TensorMapEncode fn = tensor_map_encode();
     if (!fn) return fail(NRN_ERR_UNSUPPORTED, "nrn_cuda_scaled_product: the driver has no cuTensorMapEncodeTiled");
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(m->cols), static_cast<cuuint64_t>(m->rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(m->value_stride)};
@@ -695,6 +679,20 @@ nrn_status_t quantize(const void* x, int64_t rows, int64_t cols, int64_t stride,
 }
 
 }  // namespace
+
+TensorMapEncode tensor_map_encode() {
+    static std::once_flag once;
+    static TensorMapEncode fn = nullptr;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<TensorMapEncode>(p);
+    });
+    return fn;
+}
+
 }  // namespace nrn
 
 using namespace nrn;

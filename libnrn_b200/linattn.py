@@ -21,7 +21,10 @@ import ctypes as C
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, check_rows, check_state, check_tensor, check_vector, on, ptr, require
+from ._tensors import DTYPE, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, on, ptr, require
+
+
+check = check_waits
 
 
 def _strides(t):
@@ -82,6 +85,7 @@ def forward(q, k, v, log_decay, *, scale=None, state=None, cu_seqlens=None, out=
         end = torch.empty(a.seqs, h, a.dk, a.dv, dtype=torch.float32, device=q.device)
         a.o, a.state_in, a.state_out = out.data_ptr(), ptr(state), end.data_ptr()
         a.o_stride[:] = _strides(out)
+        a.err = error_flag(q.device)
         w = _workspace(a, False, q.device)   # noqa: F841  (kept until the launches are enqueued)
         N.check(N.lib().nrn_cuda_linattn_forward(C.byref(a), st), "nrn_cuda_linattn_forward")
     return out, end
@@ -100,7 +104,7 @@ def backward(do, q, k, v, log_decay, *, scale=None, state=None, dstate=None, cu_
     with on(q.device, stream) as st:
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
         ds = torch.empty(shape, dtype=torch.float32, device=q.device)
-        a.state_in = ptr(state)
+        a.state_in, a.err = ptr(state), error_flag(q.device)
         g = N.LinAttnGrad()
         g.d_o, g.dstate_out, g.dstate_in = do.data_ptr(), ptr(dstate), ds.data_ptr()
         g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()

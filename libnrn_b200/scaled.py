@@ -17,7 +17,7 @@ import ctypes as C
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, check_tensor, on, require
+from ._tensors import DTYPE, check_tensor, check_waits, error_flag, on, require
 
 BLOCK = 128
 
@@ -97,15 +97,8 @@ def transpose(w: Scaled, *, stream=None) -> Scaled:
     return out
 
 
-# Split products' workspaces, one for each stream (calls on one stream follow one another), and error flags.
+# Split products' workspaces, one for each stream (calls on one stream follow one another).
 _workspaces: dict = {}
-_errors: dict = {}
-
-
-def _error_flag(device) -> torch.Tensor:
-    if device.index not in _errors:
-        _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-    return _errors[device.index]
 
 
 def _workspace(n: int, device, st) -> torch.Tensor:
@@ -118,11 +111,7 @@ def _workspace(n: int, device, st) -> torch.Tensor:
     return w
 
 
-def check(device=None) -> None:
-    """Raises if a device-side wait of an earlier product on `device` (default: the current one) timed out."""
-    i = torch.cuda.current_device() if device is None else torch.device(device).index
-    if i in _errors and int(_errors[i].item()) != 0:
-        raise N.NrnError(7, f"nrn_cuda_scaled_product: device wait timed out (code {int(_errors[i].item())})")
+check = check_waits
 
 
 def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None) -> torch.Tensor:
@@ -147,7 +136,7 @@ def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None
         w = _workspace(need.value, dev, st) if need.value else None
         N.check(L.nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), DTYPE[out.dtype],
                                           out.stride(0) if m > 1 else max(n, 1), None if w is None else w.data_ptr(), need.value,
-                                          _error_flag(dev).data_ptr(), st), "nrn_cuda_scaled_product")
+                                          error_flag(dev), st), "nrn_cuda_scaled_product")
     return out
 
 
