@@ -608,18 +608,19 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
 //     inter [128 x 64]  = X16^T a^T             X16: the entering state in bf16
 //     U     [128 x b.d] = sum over terms of (w c)^T b
 //     intra [128 x 64]  = c^T P^T
-// Ten warps, one block an SM:
+// 18 warps, one block an SM:
 //   warp 0    copies: a, b and c of a chunk by TMA into one of two stages;
 //   warp 1    issues the MMAs (one thread);
-//   warps 2-9 everything else, in the order that keeps the tensor cores busy
+//   warps 2-  everything else, in the order that keeps the tensor cores busy
 //             behind them: (1) c^T, its decayed terms and b^T through
 //             ldmatrix/stmatrix into K-major tiles, while P and inter run;
 //             (2) P out of TMEM, decay and mask, bf16, while U runs; (3) the
-//             fp32 state, kept in registers (64 a thread): lam^n X + U, and
+//             fp32 state, kept in registers (32 a thread): lam^n X + U, and
 //             its bf16 copy, while intra runs; (4) the results.
 // About 70 warp instructions a token and head against 270 with mma.sync
 // (whose operands pass through registers in every warp).
-constexpr int kTcThreads = 320;
+constexpr int kTcWarps = 16;            // that are not copying or issuing
+constexpr int kTcThreads = 64 + 32 * kTcWarps;
 constexpr int kTcCols = 128;
 enum { ERR_LINATTN_TIMEOUT = 5 };
 
@@ -686,13 +687,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
         : "memory");
 }
-// 16 lanes x 32 columns as the fragments of four 16x8 accumulators.
+// 16 lanes x 16 columns as the fragments of two 16x8 accumulators.
 __device__ __forceinline__ void tc_ld_frag(uint32_t taddr, uint32_t* v) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr));
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tc_ld1(uint32_t taddr, uint32_t& v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v)::"memory");
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld32(uint32_t* v) {
@@ -729,9 +732,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_init(&M.uready, 1);
         mbar_init(&M.oready, 1);
         mbar_init(&M.drain, 1);
-        mbar_init(&M.psm, 8);
-        mbar_init(&M.x16, 8);
-        mbar_init(&M.vk, 8);
+        mbar_init(&M.psm, kTcWarps);
+        mbar_init(&M.x16, kTcWarps);
+        mbar_init(&M.vk, kTcWarps);
         M.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -829,7 +832,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_wait(&M.drain, 0, nullptr);
         }
     } else {
-        const int ew = warp - 2, sub = warp & 3, half = ew >> 2;      // TMEM lanes 32 sub ..; this warp's half of the columns
+        const int ew = warp - 2, sub = warp & 3, part = ew >> 2;      // TMEM lanes 32 sub ..; this warp's fourth of the columns
         const int et = threadIdx.x - 64;
         const int l7 = lane & 7, l8 = (lane >> 3) & 1, l16 = lane >> 4, q = lane & 3, g8 = lane >> 2;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * sub) << 16);
@@ -837,8 +840,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int row = tile * kTcCols + 32 * sub + lane;             // column of c
         const int64_t sh = (static_cast<int64_t>(u.seq) * p.heads + head) * db * dc;
         const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
-        constexpr int kX = DK / 2;
-        const int x0 = half * kX;                                     // first row of b's dimension of this thread
+        constexpr int kX = DK / 4;
+        const int x0 = part * kX;                                     // first row of b's dimension of this thread
         float x[kX];
         const bool given = !STATE_ONLY && (p.seg != nullptr || p.s_in != nullptr) && row < dc;
 #pragma unroll
@@ -868,7 +871,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t ph = c & 1;
             const uint32_t sb = base + L::kHead + st * L::kStage + L::kTilesA * L::kTile, sc = sb + L::kTilesB * L::kTile;
             // everybody is done with the last chunk's tiles and factors
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 1, 512;" ::: "memory");
             if (c == 0 || n < kChunk) {
                 if (et < kChunk) {
                     const int pos = p.reverse ? n - 1 - et : et;
@@ -876,39 +879,44 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     M.out[et] = et < n ? p.out_mul * decay_power(g, pos + p.off) : 0.0f;
                 }
                 whole = decay_power(g, n);
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 1, 512;" ::: "memory");
             }
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
             if (ok) {
-                // (1) c^T, its terms and b^T: this warp's 16 columns of each, 16 tokens at a time
-                const uint32_t to = (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
-                const uint32_t from = (ew >> 2) * L::kTile + (l7 + 8 * l16) * 128 + (((2 * (ew & 3) + l8) ^ l7) << 4);
-                uint32_t fc[4][4], fb[4][4];
+                // (1) c^T, its terms and b^T, in blocks of 16 columns by 16 tokens: two of c and two (DK = 64: one) of b a warp
+                constexpr int kCb = 2, kBb = DK / 64;
+                const int ccol = ew & 7, ckk = kCb * (ew >> 3), bcol = DK == 128 ? ew & 7 : ew & 3, bkk = DK == 128 ? 2 * (ew >> 3) : ew >> 2;
+                const uint32_t lrow = (l7 + 8 * l16) * 128, trow = l8 * 1024 + l16 * 128 + l7 * 16;
+                const uint32_t cfrom = sc + (ccol >> 2) * L::kTile + lrow + (((2 * (ccol & 3) + l8) ^ l7) << 4) + ckk * 2048;
+                const uint32_t bfrom = sb + (bcol >> 2) * L::kTile + lrow + (((2 * (bcol & 3) + l8) ^ l7) << 4) + bkk * 2048;
+                const uint32_t cto = 2 * ccol * 1024 + trow + ckk * 256, bto = 2 * bcol * 1024 + trow + bkk * 256;
+                uint32_t fc[kCb][4], fb[kBb][4];
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) ldsm4t_at(fc[kk], sc + from + kk * 2048);
-                if (ew < DK / 16)
+                for (int i = 0; i < kCb; ++i) ldsm4t_at(fc[i], cfrom + i * 2048);
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) ldsm4t_at(fb[kk], sb + from + kk * 2048);
+                for (int i = 0; i < kBb; ++i) ldsm4t_at(fb[i], bfrom + i * 2048);
                 if (n < kChunk) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
+                    for (int h = 0; h < 4; ++h) {
+                        auto keep = [&](int kk) {
                             const int j = kk * 16 + (h >> 1) * 8 + 2 * q;
-                            const uint32_t keep = j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
-                            fc[kk][h] &= keep;
-                            fb[kk][h] &= keep;
-                        }
+                            return j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
+                        };
+#pragma unroll
+                        for (int i = 0; i < kCb; ++i) fc[i][h] &= keep(ckk + i);
+#pragma unroll
+                        for (int i = 0; i < kBb; ++i) fb[i][h] &= keep(bkk + i);
+                    }
                 }
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
+                for (int i = 0; i < kCb; ++i) {
                     uint32_t term[TERMS][4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float2 w = *reinterpret_cast<const float2*>(&M.w[kk * 16 + 8 * h + 2 * q]);
+                        const float2 w = *reinterpret_cast<const float2*>(&M.w[(ckk + i) * 16 + 8 * h + 2 * q]);
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            float y = low_f32(fc[kk][2 * h + r]) * w.x, z = high_f32(fc[kk][2 * h + r]) * w.y;
+                            float y = low_f32(fc[i][2 * h + r]) * w.x, z = high_f32(fc[i][2 * h + r]) * w.y;
 #pragma unroll
                             for (int k = 0; k < TERMS; ++k) {
                                 const uint32_t b2 = bf16x2(y, z);
@@ -920,12 +928,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             }
                         }
                     }
-                    if (!STATE_ONLY) stsm4(base + L::kCt + to + kk * 256, fc[kk][0], fc[kk][1], fc[kk][2], fc[kk][3]);
+                    if (!STATE_ONLY) stsm4(base + L::kCt + cto + i * 256, fc[i][0], fc[i][1], fc[i][2], fc[i][3]);
 #pragma unroll
                     for (int k = 0; k < TERMS; ++k)
-                        stsm4(base + L::kWt + k * 128 * 128 + to + kk * 256, term[k][0], term[k][1], term[k][2], term[k][3]);
-                    if (ew < DK / 16) stsm4(base + L::kBt + to + kk * 256, fb[kk][0], fb[kk][1], fb[kk][2], fb[kk][3]);
+                        stsm4(base + L::kWt + k * 128 * 128 + cto + i * 256, term[k][0], term[k][1], term[k][2], term[k][3]);
                 }
+#pragma unroll
+                for (int i = 0; i < kBb; ++i) stsm4(base + L::kBt + bto + i * 256, fb[i][0], fb[i][1], fb[i][2], fb[i][3]);
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&M.vk);
@@ -935,16 +944,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.pready, ph, abort));
                 if (ok) {
                     tc_fence_after();
-                    // rows i = 16 sub + g and + 8, columns j = 32 half + 8 nt + 2 q and + 1: v[4 nt ..]
-                    uint32_t v[16];
-                    tc_ld_frag(lanes + kP + 32 * half, v);
-                    tc_wait_ld16(v);
-                    const int i = 16 * sub + g8, j0 = 32 * half + 2 * q, jn = n - j0;
+                    // rows i = 16 sub + g and + 8, columns j = 16 part + 8 nt + 2 q and + 1: v[4 nt ..]
+                    uint32_t v[8];
+                    tc_ld_frag(lanes + kP + 16 * part, v);
+                    tc_wait_ld8(v);
+                    const int i = 16 * sub + g8, j0 = 16 * part + 2 * q, jn = n - j0;
                     const float* lag = &M.lag[63 + i - j0];
                     const int d = i - j0;
-                    uint32_t r[8];
+                    uint32_t r[4];
 #pragma unroll
-                    for (int nt = 0; nt < 4; ++nt)
+                    for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int e = 8 * nt - 8 * h;                // token j - token i is e - d
@@ -953,10 +962,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             r[2 * nt + h] = bf16x2(s0 ? __uint_as_float(v[4 * nt + 2 * h]) * lag[-e] : 0.0f,
                                                    s1 ? __uint_as_float(v[4 * nt + 2 * h + 1]) * lag[-e - 1] : 0.0f);
                         }
-                    // matrices (rows 0-7, 8-15) x (columns 8 nt, 8 nt + 8)
-                    const uint32_t at = base + L::kProb + (2 * sub + l8) * 1024 + (4 * half + l16) * 128 + l7 * 16;
-                    stsm4(at, r[0], r[1], r[2], r[3]);
-                    stsm4(at + 256, r[4], r[5], r[6], r[7]);
+                    // matrices (rows 0-7, 8-15) x (columns 0-7, 8-15)
+                    stsm4(base + L::kProb + (2 * sub + l8) * 1024 + (2 * part + l16) * 128 + l7 * 16, r[0], r[1], r[2], r[3]);
                     tc_fence_before();
                     proxy_fence();
                     __syncwarp();
@@ -968,77 +975,82 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             bool bad = false;
             if (ok) {
                 tc_fence_after();
-#pragma unroll
-                for (int i0 = 0; i0 < kX; i0 += 32) {
-                    uint32_t v[32];
-                    tc_ld32(lanes + kU + x0 + i0, v);
-                    tc_wait_ld32(v);
-                    // a column of c with a value that is no number shows in every element of its row of U
-                    if (i0 == 0) bad = !(fabsf(__uint_as_float(v[0])) <= 3.4028234e38f);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i0 + i] = fmaf(whole, x[i0 + i], __uint_as_float(v[i]));
+                uint32_t v[kX];
+                tc_ld16(lanes + kU + x0, v);
+                if constexpr (kX == 32) {
+                    tc_ld16(lanes + kU + x0 + 16, v + 16);
+                    tc_wait_ld16(v + 16);
                 }
+                tc_wait_ld16(v);
+                // a column of c with a value that is no number shows in every element of its row of U
+                bad = !(fabsf(__uint_as_float(v[0])) <= 3.4028234e38f);
+#pragma unroll
+                for (int i = 0; i < kX; ++i) x[i] = fmaf(whole, x[i], __uint_as_float(v[i]));
                 tc_fence_before();
                 if (!STATE_ONLY && c + 1 < chunks) copy_state();
             }
             if constexpr (!STATE_ONLY) {
-                // (4) the results: 32 tokens of this lane's column
+                // (4) the results: 16 tokens of this lane's column
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.oready, ph, abort));
                 if (ok) {
                     tc_fence_after();
-                    const int m = n - 32 * half;         // tokens of this half
-                    // bf16 results pass through 2 KB of this warp's own (the terms were read when U was done)
-                    unsigned char* own = smem + L::kWt + ew * 2048;
+                    const int m = n - 16 * part;         // tokens of this part
+                    uint32_t a[16], b[16];
+                    tc_ld16(lanes + kIntra + 16 * part, a);
+                    tc_ld16(lanes + kInter + 64 * st + 16 * part, b);
+                    tc_wait_ld16(a);
+                    tc_wait_ld16(b);
 #pragma unroll
-                    for (int t0 = 0; t0 < 32; t0 += 16) {
-                        uint32_t a[16], b[16];
-                        tc_ld16(lanes + kIntra + 32 * half + t0, a);
-                        tc_ld16(lanes + kInter + 64 * st + 32 * half + t0, b);
-                        tc_wait_ld16(a);
-                        tc_wait_ld16(b);
-                        if (__any_sync(0xffffffffu, bad)) {
-                            // sum over the tokens that count, alone
+                    for (int t = 0; t < 16; t += 4) {
+                        const float4 w = *reinterpret_cast<const float4*>(&M.out[16 * part + t]);
+                        a[t] = __float_as_uint(fmaf(w.x, __uint_as_float(b[t]), __uint_as_float(a[t])));
+                        a[t + 1] = __float_as_uint(fmaf(w.y, __uint_as_float(b[t + 1]), __uint_as_float(a[t + 1])));
+                        a[t + 2] = __float_as_uint(fmaf(w.z, __uint_as_float(b[t + 2]), __uint_as_float(a[t + 2])));
+                        a[t + 3] = __float_as_uint(fmaf(w.w, __uint_as_float(b[t + 3]), __uint_as_float(a[t + 3])));
+                    }
+                    const int64_t at = (u.row0 + first(c) + 16 * part) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head;
+                    // bf16 results pass through 1 KB of this warp's own (the terms were read when U was done)
+                    unsigned char* own = smem + L::kWt + ew * 1024;
+                    if (p.o_f32) {
+                        float* to = static_cast<float*>(p.o) + at + row;
 #pragma unroll
-                            for (int t = 0; t < 16; ++t) {
-                                const int i = 32 * half + t0 + t;
-                                const unsigned char* pp = smem + L::kProb + (i >> 3) * 1024 + (i & 7) * 16;
-                                const unsigned char* cc = smem + L::kCt + (4 * sub + (lane >> 3)) * 1024 + l7 * 16;
-                                float y = 0.0f;
-                                for (int j = p.reverse ? i : 0; j < (p.reverse ? n : i + 1); ++j)
-                                    y = fmaf(to_f32(*reinterpret_cast<const __nv_bfloat16*>(pp + (j >> 3) * 128 + (j & 7) * 2)),
-                                             to_f32(*reinterpret_cast<const __nv_bfloat16*>(cc + (j >> 3) * 128 + (j & 7) * 2)), y);
-                                a[t] = __float_as_uint(y);
-                            }
-                        }
+                        for (int t = 0; t < 16; ++t, to += p.o_tok)
+                            if (t < m && row < dc) *to = __uint_as_float(a[t]);
+                    } else {
 #pragma unroll
-                        for (int t = 0; t < 16; t += 4) {
-                            const float4 w = *reinterpret_cast<const float4*>(&M.out[32 * half + t0 + t]);
-                            a[t] = __float_as_uint(fmaf(w.x, __uint_as_float(b[t]), __uint_as_float(a[t])));
-                            a[t + 1] = __float_as_uint(fmaf(w.y, __uint_as_float(b[t + 1]), __uint_as_float(a[t + 1])));
-                            a[t + 2] = __float_as_uint(fmaf(w.z, __uint_as_float(b[t + 2]), __uint_as_float(a[t + 2])));
-                            a[t + 3] = __float_as_uint(fmaf(w.w, __uint_as_float(b[t + 3]), __uint_as_float(a[t + 3])));
-                        }
-                        if (p.o_f32) {
-                            float* to = static_cast<float*>(p.o) + (u.row0 + first(c) + 32 * half + t0) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + row;
-#pragma unroll
-                            for (int t = 0; t < 16; ++t, to += p.o_tok)
-                                if (t0 + t < m && row < dc) *to = __uint_as_float(a[t]);
-                        } else {
-#pragma unroll
-                            for (int t = 0; t < 16; t += 2) {
-                                const uint32_t two = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
-                                *reinterpret_cast<uint16_t*>(own + (t0 + t) * 64 + lane * 2) = static_cast<uint16_t>(two);
-                                *reinterpret_cast<uint16_t*>(own + (t0 + t + 1) * 64 + lane * 2) = static_cast<uint16_t>(two >> 16);
-                            }
+                        for (int t = 0; t < 16; t += 2) {
+                            const uint32_t two = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
+                            *reinterpret_cast<uint16_t*>(own + t * 64 + lane * 2) = static_cast<uint16_t>(two);
+                            *reinterpret_cast<uint16_t*>(own + (t + 1) * 64 + lane * 2) = static_cast<uint16_t>(two >> 16);
                         }
                     }
+                    if (__any_sync(0xffffffffu, bad)) {
+                        // sum again over the tokens that count alone
+#pragma unroll 1
+                        for (int t = 0; t < 16; ++t) {
+                            const int i = 16 * part + t;
+                            const unsigned char* pp = smem + L::kProb + (i >> 3) * 1024 + (i & 7) * 16;
+                            const unsigned char* cc = smem + L::kCt + (4 * sub + (lane >> 3)) * 1024 + l7 * 16;
+                            uint32_t entering;
+                            tc_ld1(lanes + kInter + 64 * st + i, entering);
+                            float y = 0.0f;
+#pragma unroll 1
+                            for (int j = p.reverse ? i : 0; j < (p.reverse ? n : i + 1); ++j)
+                                y = fmaf(to_f32(*reinterpret_cast<const __nv_bfloat16*>(pp + (j >> 3) * 128 + (j & 7) * 2)),
+                                         to_f32(*reinterpret_cast<const __nv_bfloat16*>(cc + (j >> 3) * 128 + (j & 7) * 2)), y);
+                            y = fmaf(M.out[i], __uint_as_float(entering), y);
+                            if (!p.o_f32) *reinterpret_cast<__nv_bfloat16*>(own + t * 64 + lane * 2) = __float2bfloat16_rn(y);
+                            else if (t < m && row < dc) static_cast<float*>(p.o)[at + t * p.o_tok + row] = y;
+                        }
+                    }
+                    tc_fence_before();
                     if (!p.o_f32) {
                         __syncwarp();
                         // 64 bytes a token, eight tokens at a time
                         const int t = lane >> 2, j = tile * kTcCols + 32 * sub + 8 * q;
-                        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + (u.row0 + first(c) + 32 * half + t) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + j;
+                        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + at + t * p.o_tok + j;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k, to += 8 * p.o_tok) {
+                        for (int k = 0; k < 2; ++k, to += 8 * p.o_tok) {
                             const uint4 r = *reinterpret_cast<const uint4*>(own + (8 * k + t) * 64 + q * 16);
                             if (8 * k + t >= m || j >= dc) continue;
                             if (p.o_vec) {
@@ -1051,7 +1063,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             }
                         }
                     }
-                    tc_fence_before();
                 }
             }
         }
