@@ -1,9 +1,13 @@
 """What the tensor operators (linattn, scaled, gatednorm) share: types, the
-checks of their tensor arguments, and the device and stream of a call."""
+checks of their tensor arguments, and the device and stream of a call.
+
+A call's checks depend on its arguments' layouts alone (shapes, strides,
+types, devices), so each operator keeps the outcome by layout: a later call
+with the same layouts fills a copy of the checked argument block with its
+pointers (``Layouts``)."""
 from __future__ import annotations
 
 import contextlib
-import ctypes as C
 
 import torch
 
@@ -46,33 +50,63 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def layout(t):
+    """All of a tensor argument that its checks look at (None and anything else stand for themselves)."""
+    return (t.shape, t.stride(), t.dtype, t.device) if isinstance(t, torch.Tensor) else (t if t is None else type(t))
+
+
+class Layouts:
+    """Checked argument blocks by the layouts they were checked for."""
+
+    def __init__(self, build, most: int = 4096):
+        self.build, self.most, self.known = build, most, {}
+
+    def get(self, key, *args):
+        """What ``build(*args)`` gives for these layouts; it raises where they are refused."""
+        got = self.known.get(key)
+        if got is None:
+            got = self.build(*args)
+            if len(self.known) >= self.most:
+                self.known.clear()
+            self.known[key] = got
+        return got
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 @contextlib.contextmanager
 def _switched(device, stream):
     with torch.cuda.device(device):
         if stream is None:
-            yield C.c_void_p(torch.cuda.current_stream().cuda_stream)
+            yield _raw_stream(device.index)
         else:
             with torch.cuda.stream(stream):
-                yield C.c_void_p(stream.cuda_stream)
+                yield stream.cuda_stream
 
 
 class _Current:
     """The context of a call on the current device and stream: nothing to switch."""
 
+    __slots__ = ("stream",)
+
+    def __init__(self, stream):
+        self.stream = stream
+
     def __enter__(self):
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        return self.stream
 
     def __exit__(self, *exc):
         return False
 
 
-_CURRENT = _Current()
-
-
 def on(device, stream=None):
-    """Context of a call on `device`: its kernels, results and workspaces belong to `stream` (default: the current one)."""
-    if stream is None and torch.cuda.current_device() == device.index:
-        return _CURRENT
+    """Context of a call on `device`: its kernels, results and workspaces belong to `stream` (default: the current one),
+    whose handle it gives."""
+    i = device.index
+    if stream is None and _current_device() == i:
+        return _Current(_raw_stream(i))
     return _switched(device, stream)
 
 

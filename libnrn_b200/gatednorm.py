@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, check_rows, check_vector, on, ptr, require
+from ._tensors import DTYPE, Layouts, check_rows, check_vector, layout, on, ptr, require
 from .scaled import Scaled
 
 ACTIVATION = {"silu": 0, "sigmoid": 1}
@@ -36,14 +36,15 @@ def _stride(t):
     return 0 if t is None else t.stride(0)
 
 
-def _describe(residual, h, gate, alpha, w_post, w_pre, eps, activation):
-    require(isinstance(residual, torch.Tensor) and residual.is_cuda and residual.dim() == 2, "residual: a CUDA matrix is needed")
+def _describe(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
+    """The checked argument block of a call (its pointers are set by each call), and the bytes of its backward's workspace."""
+    require(residual.dim() == 2, "residual: must be [rows, d]")
     require(residual.dtype in DTYPE, f"residual: must be bfloat16, float16 or float32, is {residual.dtype}")
     require(activation in ACTIVATION, f"activation: must be one of {sorted(ACTIVATION)}, is {activation!r}")
     rows, d = residual.shape
     dev, dt = residual.device, residual.dtype
     check_rows(residual, "residual", dt, dev, (rows, d))
-    for name, t in (("h", h), ("gate", gate)):
+    for name, t in (("h", h), ("gate", gate), ("dy", dy), ("dz", dz)):
         if t is not None:
             check_rows(t, name, dt, dev, (rows, d))
     require(h is not None or (gate is None and alpha is None and w_post is None),
@@ -53,28 +54,42 @@ def _describe(residual, h, gate, alpha, w_post, w_pre, eps, activation):
             check_vector(t, name, d, dev)
     a = N.GatedNorm()
     a.dtype, a.act, a.rows, a.d, a.eps = DTYPE[dt], ACTIVATION[activation], rows, d, float(eps)
-    a.residual, a.h, a.gate = residual.data_ptr(), ptr(h), ptr(gate)
     a.residual_stride, a.h_stride, a.gate_stride = residual.stride(0), _stride(h), _stride(gate)
+    n = C.c_int64()
+    N.check(N.lib().nrn_cuda_gatednorm_workspace(C.byref(a), C.byref(n)), "nrn_cuda_gatednorm_workspace")
+    return bytes(a), max(n.value, 16)
+
+
+_layouts = Layouts(_describe)
+
+
+def _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
+    require(isinstance(residual, torch.Tensor) and residual.is_cuda, "residual: a CUDA tensor is needed")
+    key = (layout(residual), layout(h), layout(gate), layout(alpha), layout(w_post), layout(w_pre), eps, activation, layout(dy), layout(dz))
+    block, need = _layouts.get(key, residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz)
+    a = N.GatedNorm.from_buffer_copy(block)
+    a.residual, a.h, a.gate = residual.data_ptr(), ptr(h), ptr(gate)
     a.alpha, a.w_post, a.w_pre = ptr(alpha), ptr(w_post), ptr(w_pre)
-    return a
+    return a, need
 
 
 def forward(residual, h=None, gate=None, *, alpha=None, w_post=None, w_pre=None, eps=1e-6, activation="silu",
             scaled=False, want_z=True, stream=None):
     """(y, z) of [rows, d] tensors (bf16, fp16 or fp32; last stride 1).  z is None without ``want_z``, and a ``Scaled``
     matrix with ``scaled``: the next block's 8-bit input.  Without h, y is ``residual`` itself."""
-    a = _describe(residual, h, gate, alpha, w_post, w_pre, eps, activation)
+    a, _ = _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, None, None)
     rows, d = residual.shape
+    dev = residual.device
     y, z = residual, None
-    with on(residual.device, stream) as st:
+    with on(dev, stream) as st:
         if h is not None:
-            y = torch.empty(rows, d, dtype=residual.dtype, device=residual.device)
+            y = torch.empty((rows, d), dtype=residual.dtype, device=dev)
             a.y, a.y_stride = y.data_ptr(), d
         if want_z and scaled:
-            z = Scaled.empty(rows, d, residual.device)
+            z = Scaled.empty(rows, d, dev)
             a.z_scaled = C.pointer(z.desc)
         elif want_z:
-            z = torch.empty(rows, d, dtype=residual.dtype, device=residual.device)
+            z = torch.empty((rows, d), dtype=residual.dtype, device=dev)
             a.z, a.z_stride = z.data_ptr(), d
         N.check(N.lib().nrn_cuda_gatednorm_forward(C.byref(a), st), "nrn_cuda_gatednorm_forward")
     return y, z
@@ -84,25 +99,19 @@ def backward(dy, dz, residual, h=None, gate=None, *, alpha=None, w_post=None, w_
              stream=None) -> Gradients:
     """Gradients of a ``forward`` call with these arguments, given those of y and z (None: zero).  Those of alpha, w_post
     and w_pre are fp32 sums over the rows, added in a fixed order."""
-    a = _describe(residual, h, gate, alpha, w_post, w_pre, eps, activation)
+    a, need = _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz)
     rows, d = residual.shape
     dev, dt = residual.device, residual.dtype
-    for name, t in (("dy", dy), ("dz", dz)):
-        if t is not None:
-            check_rows(t, name, dt, dev, (rows, d))
     with on(dev, stream) as st:
         g = N.GatedNormGrad()
         g.dy, g.dz, g.dy_stride, g.dz_stride = ptr(dy), ptr(dz), _stride(dy), _stride(dz)
-        like = [torch.empty(rows, d, dtype=dt, device=dev) if want else None for want in (True, h is not None, gate is not None)]
+        like = [torch.empty((rows, d), dtype=dt, device=dev) if want else None for want in (True, h is not None, gate is not None)]
         sums = [torch.empty(d, dtype=torch.float32, device=dev) if t is not None else None for t in (alpha, w_post, w_pre)]
         g.dresidual, g.dh, g.dgate = (ptr(t) for t in like)
         g.dresidual_stride = g.dh_stride = g.dgate_stride = d
         g.dalpha, g.dw_post, g.dw_pre = (ptr(t) for t in sums)
-        L = N.lib()
         if any(t is not None for t in sums):
-            n = C.c_int64()
-            N.check(L.nrn_cuda_gatednorm_workspace(C.byref(a), C.byref(n)), "nrn_cuda_gatednorm_workspace")
-            w = torch.empty(max(n.value, 16), dtype=torch.uint8, device=dev)
-            g.workspace, g.workspace_bytes = w.data_ptr(), n.value
-        N.check(L.nrn_cuda_gatednorm_backward(C.byref(a), C.byref(g), st), "nrn_cuda_gatednorm_backward")
+            w = torch.empty(need, dtype=torch.uint8, device=dev)
+            g.workspace, g.workspace_bytes = w.data_ptr(), need
+        N.check(N.lib().nrn_cuda_gatednorm_backward(C.byref(a), C.byref(g), st), "nrn_cuda_gatednorm_backward")
     return Gradients(*like, *sums)

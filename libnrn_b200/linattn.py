@@ -21,8 +21,8 @@ import ctypes as C
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, on, ptr, require
-
+from ._tensors import (DTYPE, Layouts, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, layout, on,
+                       ptr, require)
 
 check = check_waits
 
@@ -31,62 +31,80 @@ def _strides(t):
     return t.stride(0), t.stride(1), t.stride(2)
 
 
-def _describe(q, k, v, log_decay, scale, cu_seqlens):
+def _check_q(q):
     require(isinstance(q, torch.Tensor) and q.is_cuda, "q: a CUDA tensor is needed")
     require(q.dtype in DTYPE, f"q: must be bfloat16, float16 or float32, is {q.dtype}")
+
+
+def _describe(q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out):
+    """The checked argument block of a forward or backward call (its pointers are set by each call), and its workspace."""
+    _check_q(q)
     for name, t in (("q", q), ("k", k), ("v", v)):
         require(isinstance(t, torch.Tensor) and t.dim() == 4, f"{name}: must be [batch, tokens, heads, d]")
     b, t, h, dk = q.shape
     hk, dv = k.shape[2], v.shape[3]
     require(h >= 1 and hk >= 1 and h % hk == 0, f"heads: {h} of q are no multiple of {hk} of k")
-    check_rows(q, "q", q.dtype, q.device, (b, t, h, dk))
-    check_rows(k, "k", q.dtype, q.device, (b, t, hk, dk))
-    check_rows(v, "v", q.dtype, q.device, (b, t, hk, dv))
-    check_vector(log_decay, "log_decay", h, q.device)
+    dev, dt = q.device, q.dtype
+    check_rows(q, "q", dt, dev, (b, t, h, dk))
+    check_rows(k, "k", dt, dev, (b, t, hk, dk))
+    check_rows(v, "v", dt, dev, (b, t, hk, dv))
+    check_vector(log_decay, "log_decay", h, dev)
     a = N.LinAttn()
-    a.dtype, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[q.dtype], h, hk, dk, dv, t
+    a.dtype, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[dt], h, hk, dk, dv, t
     if cu_seqlens is None:
         a.seqs = b
     else:
         require(b == 1, "cu_seqlens: packed sequences have a batch dimension of 1")
-        check_tensor(cu_seqlens, "cu_seqlens", torch.int32, q.device)
+        check_tensor(cu_seqlens, "cu_seqlens", torch.int32, dev)
         require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and cu_seqlens.is_contiguous(),
                 "cu_seqlens: must be a contiguous vector of sequences + 1 starts")
         a.seqs, a.cu_seqlens = cu_seqlens.numel() - 1, cu_seqlens.data_ptr()
+    shape = (a.seqs, h, dk, dv)
+    for name, x in (("state", state), ("dstate", dstate)):
+        if x is not None:
+            check_state(x, name, dev, shape)
+    for name, x in (("do", do), ("out", out)):
+        if x is not None:
+            check_rows(x, name, dt, dev, (b, t, h, dv))
     a.log_decay = log_decay.data_ptr()
     a.scale = dk ** -0.5 if scale is None else float(scale)
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
-    return a
-
-
-def _workspace(a, backward: bool, device):
+    if out is not None:
+        a.o_stride[:] = _strides(out)
+    elif do is None:
+        a.o_stride[:] = (t * h * dv, h * dv, dv)
     n = C.c_int64()
-    N.check(N.lib().nrn_cuda_linattn_workspace(C.byref(a), int(backward), C.byref(n)), "nrn_cuda_linattn_workspace")
-    if n.value == 0:
-        return None
-    w = torch.empty(n.value, dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = w.data_ptr(), n.value
-    return w
+    N.check(N.lib().nrn_cuda_linattn_workspace(C.byref(a), int(do is not None), C.byref(n)), "nrn_cuda_linattn_workspace")
+    return bytes(a), n.value, shape
+
+
+_sequences = Layouts(_describe)
+
+
+def _call(q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out):
+    """(argument block with the inputs' pointers, workspace bytes, shape of the states)."""
+    key = (layout(q), layout(k), layout(v), layout(log_decay), scale, layout(cu_seqlens), layout(state), layout(dstate), layout(do),
+           layout(out))
+    block, need, shape = _sequences.get(key, q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out)
+    a = N.LinAttn.from_buffer_copy(block)
+    a.q, a.k, a.v, a.log_decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr()
+    a.cu_seqlens, a.state_in, a.err = ptr(cu_seqlens), ptr(state), error_flag(q.device)
+    return a, need, shape
 
 
 def forward(q, k, v, log_decay, *, scale=None, state=None, cu_seqlens=None, out=None, stream=None):
     """(o, final states) of whole sequences that go on from ``state`` (default: zero states).
     o is like q with v's last dimension; ``scale`` defaults to dk ** -0.5."""
-    a = _describe(q, k, v, log_decay, scale, cu_seqlens)
-    b, t, h, _ = q.shape
+    _check_q(q)
     with on(q.device, stream) as st:
+        a, need, shape = _call(q, k, v, log_decay, scale, cu_seqlens, state, None, None, out)
         if out is None:
-            out = torch.empty(b, t, h, a.dv, dtype=q.dtype, device=q.device)
-        else:
-            check_rows(out, "out", q.dtype, q.device, (b, t, h, a.dv))
-        if state is not None:
-            check_state(state, "state", q.device, (a.seqs, h, a.dk, a.dv))
-        end = torch.empty(a.seqs, h, a.dk, a.dv, dtype=torch.float32, device=q.device)
-        a.o, a.state_in, a.state_out = out.data_ptr(), ptr(state), end.data_ptr()
-        a.o_stride[:] = _strides(out)
-        a.err = error_flag(q.device)
-        w = _workspace(a, False, q.device)   # noqa: F841  (kept until the launches are enqueued)
+            out = torch.empty((*q.shape[:3], a.dv), dtype=q.dtype, device=q.device)
+        end = torch.empty(shape, dtype=torch.float32, device=q.device)
+        a.o, a.state_out = out.data_ptr(), end.data_ptr()
+        if need:
+            w = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = w.data_ptr(), need
         N.check(N.lib().nrn_cuda_linattn_forward(C.byref(a), st), "nrn_cuda_linattn_forward")
     return out, end
 
@@ -94,33 +112,25 @@ def forward(q, k, v, log_decay, *, scale=None, state=None, cu_seqlens=None, out=
 def backward(do, q, k, v, log_decay, *, scale=None, state=None, dstate=None, cu_seqlens=None, stream=None):
     """(dq, dk, dv, dstate) of a ``forward`` call with these arguments, given the gradients of o (``do``) and of the final
     states (``dstate``, default: zero); the last result is the gradient of the states it started from."""
-    a = _describe(q, k, v, log_decay, scale, cu_seqlens)
-    b, t, h, _ = q.shape
-    check_rows(do, "do", q.dtype, q.device, (b, t, h, a.dv))
-    shape = (a.seqs, h, a.dk, a.dv)
-    for name, x in (("state", state), ("dstate", dstate)):
-        if x is not None:
-            check_state(x, name, q.device, shape)
+    _check_q(q)
+    require(do is not None, "do: a tensor is needed")
     with on(q.device, stream) as st:
+        a, need, shape = _call(q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, None)
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
         ds = torch.empty(shape, dtype=torch.float32, device=q.device)
-        a.state_in, a.err = ptr(state), error_flag(q.device)
         g = N.LinAttnGrad()
         g.d_o, g.dstate_out, g.dstate_in = do.data_ptr(), ptr(dstate), ds.data_ptr()
         g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         g.d_o_stride[:], g.dq_stride[:] = _strides(do), _strides(dq)
         g.dk_stride[:], g.dv_stride[:] = _strides(dk), _strides(dv)
-        w = _workspace(a, True, q.device)    # noqa: F841
+        if need:
+            w = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = w.data_ptr(), need
         N.check(N.lib().nrn_cuda_linattn_backward(C.byref(a), C.byref(g), st), "nrn_cuda_linattn_backward")
     return dq, dk, dv, ds
 
 
-def step(q, k, v, log_decay, state, *, scale=None, slots=None, out=None, stream=None):
-    """o of one token for each sequence ([batch, heads, d] tensors), updating ``state`` in place.  Sequence i uses
-    ``state[slots[i]]`` (int32, default: state[i]); a slot appears at most once in a call, a negative one is padding whose
-    output is 0, and one past the states gives NaN."""
-    require(isinstance(q, torch.Tensor) and q.is_cuda, "q: a CUDA tensor is needed")
-    require(q.dtype in DTYPE, f"q: must be bfloat16, float16 or float32, is {q.dtype}")
+def _describe_step(q, k, v, log_decay, state, scale, slots, out):
     for name, x in (("q", q), ("k", k), ("v", v)):
         require(isinstance(x, torch.Tensor) and x.dim() == 3, f"{name}: must be [batch, heads, d]")
     b, h, dk = q.shape
@@ -133,25 +143,37 @@ def step(q, k, v, log_decay, state, *, scale=None, slots=None, out=None, stream=
     check_vector(log_decay, "log_decay", h, dev)
     require(isinstance(state, torch.Tensor) and state.dim() == 4, "state: must be [states, heads, dk, dv]")
     check_tensor(state, "state", torch.float32, dev, (state.shape[0], h, dk, dv))
-    require(state.shape[0] <= 1 or state.stride()[1:] == (dk * dv, dv, 1) or state[0].is_contiguous(),
-            "state: each state must be contiguous")
+    require(state.shape[0] == 0 or state[0].is_contiguous(), "state: each state must be contiguous")
     if slots is not None:
         check_tensor(slots, "slots", torch.int32, dev, (b,))
         require(slots.is_contiguous(), "slots: must be contiguous")
     else:
         require(state.shape[0] >= b, f"state: {state.shape[0]} states for {b} sequences")
-    with on(dev, stream) as st:
+    if out is not None:
+        check_rows(out, "out", q.dtype, dev, (b, h, dv))
+    a = N.LinAttn()
+    a.dtype, a.seqs, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[q.dtype], b, h, hk, dk, dv, 1
+    a.scale = dk ** -0.5 if scale is None else float(scale)
+    for f, x in ((a.q_stride, q), (a.k_stride, k), (a.v_stride, v)):
+        f[0], f[2] = x.stride(0), x.stride(1)
+    a.o_stride[0], a.o_stride[2] = (out.stride(0), out.stride(1)) if out is not None else (h * dv, dv)
+    return bytes(a), (b, h, dv), state.stride(0), state.shape[0]
+
+
+_steps = Layouts(_describe_step)
+
+
+def step(q, k, v, log_decay, state, *, scale=None, slots=None, out=None, stream=None):
+    """o of one token for each sequence ([batch, heads, d] tensors), updating ``state`` in place.  Sequence i uses
+    ``state[slots[i]]`` (int32, default: state[i]); a slot appears at most once in a call, a negative one is padding whose
+    output is 0, and one past the states gives NaN."""
+    _check_q(q)
+    key = (layout(q), layout(k), layout(v), layout(log_decay), layout(state), scale, layout(slots), layout(out))
+    block, shape, stride, count = _steps.get(key, q, k, v, log_decay, state, scale, slots, out)
+    with on(q.device, stream) as st:
         if out is None:
-            out = torch.empty(b, h, dv, dtype=q.dtype, device=dev)
-        else:
-            check_rows(out, "out", q.dtype, dev, (b, h, dv))
-        a = N.LinAttn()
-        a.dtype, a.seqs, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[q.dtype], b, h, hk, dk, dv, 1
-        a.log_decay = log_decay.data_ptr()
-        a.scale = dk ** -0.5 if scale is None else float(scale)
-        a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-        for f, x in ((a.q_stride, q), (a.k_stride, k), (a.v_stride, v), (a.o_stride, out)):
-            f[0], f[2] = x.stride(0), x.stride(1)
-        N.check(N.lib().nrn_cuda_linattn_step(C.byref(a), state.data_ptr(), state.stride(0), state.shape[0], ptr(slots), st),
-                "nrn_cuda_linattn_step")
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        a = N.LinAttn.from_buffer_copy(block)
+        a.q, a.k, a.v, a.o, a.log_decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr()
+        N.check(N.lib().nrn_cuda_linattn_step(C.byref(a), state.data_ptr(), stride, count, ptr(slots), st), "nrn_cuda_linattn_step")
     return out

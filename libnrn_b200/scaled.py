@@ -17,9 +17,30 @@ import ctypes as C
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, check_tensor, check_waits, error_flag, on, require
+from ._tensors import DTYPE, Layouts, check_tensor, check_waits, error_flag, layout, on, require
 
 BLOCK = 128
+
+
+def _describe(values, scales, row_block):
+    """The checked description of a matrix, without its pointers."""
+    require(row_block in (1, BLOCK), f"row_block: must be 1 or {BLOCK}, is {row_block}")
+    require(values.dim() == 2, "values: must be a matrix")
+    check_tensor(values, "values", torch.float8_e4m3fn, values.device)
+    rows, cols = values.shape
+    check_tensor(scales, "scales", torch.float32, values.device, (-(-rows // row_block), -(-cols // BLOCK)))
+    require(cols <= 1 or values.stride(1) == 1, "values: the last dimension must have stride 1")
+    stride = values.stride(0)
+    if rows <= 1 or cols == 0:           # the stride of a single row or of empty ones says nothing
+        stride = -(-max(cols, 1) // 16) * 16
+    require(stride % 16 == 0 and stride >= cols, "values: rows must start on 16-byte boundaries (Scaled.empty allocates them so)")
+    d = N.Scaled()
+    d.rows, d.cols, d.value_stride, d.row_block = rows, cols, stride, row_block
+    d.scale_stride[0], d.scale_stride[1] = scales.stride(0), scales.stride(1)
+    return bytes(d)
+
+
+_matrices = Layouts(_describe)
 
 
 class Scaled:
@@ -27,24 +48,16 @@ class Scaled:
     [ceil(rows / row_block), ceil(cols / 128)], any strides).  ``quantize`` makes one; values and scales of a checkpoint
     can be given as they are."""
 
+    __slots__ = ("values", "scales", "row_block", "desc")
+
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, row_block: int = 1):
-        require(row_block in (1, BLOCK), f"row_block: must be 1 or {BLOCK}, is {row_block}")
-        require(isinstance(values, torch.Tensor) and values.is_cuda and values.dim() == 2, "values: a CUDA matrix is needed")
-        check_tensor(values, "values", torch.float8_e4m3fn, values.device)
-        rows, cols = values.shape
-        check_tensor(scales, "scales", torch.float32, values.device, (-(-rows // row_block), -(-cols // BLOCK)))
-        require(cols <= 1 or values.stride(1) == 1, "values: the last dimension must have stride 1")
-        stride = values.stride(0)
-        if rows <= 1 or cols == 0:           # the stride of a single row or of empty ones says nothing
-            stride = -(-max(cols, 1) // 16) * 16
-        require(values.data_ptr() % 16 == 0 and stride % 16 == 0 and stride >= cols,
-                "values: rows must start on 16-byte boundaries (Scaled.empty allocates them so)")
+        require(isinstance(values, torch.Tensor) and values.is_cuda, "values: a CUDA matrix is needed")
+        block = _matrices.get((layout(values), layout(scales), row_block), values, scales, row_block)
         self.values, self.scales, self.row_block = values, scales, row_block
-        self.desc = N.Scaled()
-        d = self.desc
-        d.values, d.scales, d.rows, d.cols = values.data_ptr(), scales.data_ptr(), rows, cols
-        d.value_stride, d.row_block = stride, row_block
-        d.scale_stride[0], d.scale_stride[1] = scales.stride(0), scales.stride(1)
+        self.desc = N.Scaled.from_buffer_copy(block)
+        self.desc.values, self.desc.scales = values.data_ptr(), scales.data_ptr()
+        require(self.desc.values is None or self.desc.values % 16 == 0,
+                "values: rows must start on 16-byte boundaries (Scaled.empty allocates them so)")
 
     @property
     def shape(self):
@@ -57,9 +70,9 @@ class Scaled:
     @classmethod
     def empty(cls, rows: int, cols: int, device, row_block: int = 1) -> "Scaled":
         pitch = -(-cols // 16) * 16
-        values = torch.empty(rows, pitch, dtype=torch.float8_e4m3fn, device=device)
+        values = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=device)
         # scales of neighbouring rows next to each other: as the product's threads read them
-        scales = torch.empty(-(-cols // BLOCK), -(-rows // row_block), dtype=torch.float32, device=device).t()
+        scales = torch.empty((-(-cols // BLOCK), -(-rows // row_block)), dtype=torch.float32, device=device).t()
         return cls(values[:, :cols] if pitch != cols else values, scales, row_block)
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
@@ -69,19 +82,30 @@ class Scaled:
         return (self.values.float() * s.repeat_interleave(BLOCK, 1)[:, :cols]).to(dtype)
 
 
-def quantize(x: torch.Tensor, *, row_block: int = 1, transpose: bool = False, stream=None) -> Scaled:
-    """x (bf16, fp16 or fp32 [rows, cols], last stride 1) in 8 bits.  A block's scale is its largest magnitude / 448; an
-    infinity or NaN makes its whole block NaN.  ``transpose`` gives x^T with a scale for each of its rows (row_block 1)."""
-    require(isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2, "x: a CUDA matrix is needed")
+def _describe_quantize(x, row_block, transpose):
+    require(x.dim() == 2, "x: must be a matrix")
     require(x.dtype in DTYPE, f"x: must be bfloat16, float16 or float32, is {x.dtype}")
+    require(row_block in (1, BLOCK), f"row_block: must be 1 or {BLOCK}, is {row_block}")
     rows, cols = x.shape
     require(cols <= 1 or x.stride(1) == 1, f"x: the last dimension must have stride 1, has {x.stride(1)}")
     require(rows <= 1 or x.stride(0) >= cols, "x: rows overlap")
     require(not transpose or row_block == 1, "transpose: only with a scale for each row")
-    with on(x.device, stream) as st:
-        out = Scaled.empty(cols, rows, x.device) if transpose else Scaled.empty(rows, cols, x.device, row_block)
-        N.check(N.lib().nrn_cuda_scaled_quantize(x.data_ptr(), DTYPE[x.dtype], rows, cols, x.stride(0) if rows > 1 else max(cols, 1),
-                                                 int(transpose), C.byref(out.desc), st), "nrn_cuda_scaled_quantize")
+    return DTYPE[x.dtype], rows, cols, x.stride(0) if rows > 1 else max(cols, 1)
+
+
+_quantized = Layouts(_describe_quantize)
+
+
+def quantize(x: torch.Tensor, *, row_block: int = 1, transpose: bool = False, stream=None) -> Scaled:
+    """x (bf16, fp16 or fp32 [rows, cols], last stride 1) in 8 bits.  A block's scale is its largest magnitude / 448; an
+    infinity or NaN makes its whole block NaN.  ``transpose`` gives x^T with a scale for each of its rows (row_block 1)."""
+    require(isinstance(x, torch.Tensor) and x.is_cuda, "x: a CUDA tensor is needed")
+    dtype, rows, cols, stride = _quantized.get((layout(x), row_block, transpose), x, row_block, transpose)
+    dev = x.device
+    with on(dev, stream) as st:
+        out = Scaled.empty(cols, rows, dev) if transpose else Scaled.empty(rows, cols, dev, row_block)
+        N.check(N.lib().nrn_cuda_scaled_quantize(x.data_ptr(), dtype, rows, cols, stride, int(transpose), C.byref(out.desc), st),
+                "nrn_cuda_scaled_quantize")
     return out
 
 
@@ -101,10 +125,10 @@ def transpose(w: Scaled, *, stream=None) -> Scaled:
 _workspaces: dict = {}
 
 
-def _workspace(n: int, device, st) -> torch.Tensor:
+def _workspace(n: int, device, stream: int) -> torch.Tensor:
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(n, dtype=torch.uint8, device=device)      # belongs to the graph, zeroed by it
-    key = (device.index, st.value)
+    key = (device.index, stream)
     w = _workspaces.get(key)
     if w is None or w.numel() < n:
         w = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=device)
@@ -114,29 +138,38 @@ def _workspace(n: int, device, st) -> torch.Tensor:
 check = check_waits
 
 
+def _describe_product(a, b, dtype, out):
+    """(type, row stride of the result, bytes of workspace)."""
+    m, n = a.shape[0], b.shape[0]
+    require(a.device == b.device, f"b: must be on {a.device}, is on {b.device}")
+    require(a.shape[1] == b.shape[1], f"b: has {b.shape[1]} columns, a has {a.shape[1]}")
+    if out is not None:
+        require(isinstance(out, torch.Tensor) and out.dtype in DTYPE, "out: must be bfloat16, float16 or float32")
+        check_tensor(out, "out", out.dtype, a.device, (m, n))
+        require(n <= 1 or out.stride(1) == 1, "out: the last dimension must have stride 1")
+        require(m <= 1 or out.stride(0) >= n, "out: rows overlap")
+        dtype = out.dtype
+    require(dtype in DTYPE, f"dtype: must be bfloat16, float16 or float32, is {dtype}")
+    need = C.c_int64()
+    N.check(N.lib().nrn_cuda_scaled_workspace(C.byref(a.desc), C.byref(b.desc), C.byref(need)), "nrn_cuda_scaled_workspace")
+    return DTYPE[dtype], out.stride(0) if out is not None and m > 1 else max(n, 1), need.value
+
+
+_products = Layouts(_describe_product)
+
+
 def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None) -> torch.Tensor:
     """a @ b^T, [a rows, b rows], in ``dtype`` (bf16, fp16 or fp32)."""
     require(isinstance(a, Scaled) and isinstance(b, Scaled), "a, b: must be Scaled (scaled.quantize)")
-    require(a.device == b.device, f"b: must be on {a.device}, is on {b.device}")
-    m, n = a.shape[0], b.shape[0]
-    require(a.shape[1] == b.shape[1], f"b: has {b.shape[1]} columns, a has {a.shape[1]}")
     dev = a.device
+    key = (a.shape, b.shape, dev, b.device, dtype, layout(out))
+    kind, stride, need = _products.get(key, a, b, dtype, out)
     with on(dev, stream) as st:
         if out is None:
-            require(dtype in DTYPE, f"dtype: must be bfloat16, float16 or float32, is {dtype}")
-            out = torch.empty(m, n, dtype=dtype, device=dev)
-        else:
-            require(isinstance(out, torch.Tensor) and out.dtype in DTYPE, "out: must be bfloat16, float16 or float32")
-            check_tensor(out, "out", out.dtype, dev, (m, n))
-            require(n <= 1 or out.stride(1) == 1, "out: the last dimension must have stride 1")
-            require(m <= 1 or out.stride(0) >= n, "out: rows overlap")
-        need = C.c_int64()
-        L = N.lib()
-        N.check(L.nrn_cuda_scaled_workspace(C.byref(a.desc), C.byref(b.desc), C.byref(need)), "nrn_cuda_scaled_workspace")
-        w = _workspace(need.value, dev, st) if need.value else None
-        N.check(L.nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), DTYPE[out.dtype],
-                                          out.stride(0) if m > 1 else max(n, 1), None if w is None else w.data_ptr(), need.value,
-                                          error_flag(dev), st), "nrn_cuda_scaled_product")
+            out = torch.empty((a.shape[0], b.shape[0]), dtype=dtype, device=dev)
+        w = _workspace(need, dev, st).data_ptr() if need else None
+        N.check(N.lib().nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), kind, stride, w, need, error_flag(dev), st),
+                "nrn_cuda_scaled_product")
     return out
 
 
