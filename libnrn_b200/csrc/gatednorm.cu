@@ -8,10 +8,14 @@
 // rounded.  z may go out as e4m3 with a scale for each row and 128 columns,
 // ready for the 8-bit product.
 //
-// Bound by HBM: three rows in, two out (six and three backward), a few dozen
-// operations an element.  A row is held in registers, eight elements a thread
-// and vector (16 bytes of bf16): 32 threads a row where the row is short, else
-// a block a row.
+// Bound by HBM: three rows in, two out (five and three backward), if the
+// operations an element stay near 30: the sigmoid is two special-function
+// operations (its error, about 2^-22 where the gate is not small, is below
+// every output's rounding), alpha and w_post are one factor, and a block keeps
+// its columns' factors in registers over all the rows it takes in turn.  A row
+// is held in registers, eight elements a thread and vector (16 bytes of bf16):
+// 32 threads a row where the row is short, else a block a row; the next row's
+// loads are in flight while a row is worked on.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -38,11 +42,11 @@ struct NormArgs {
 struct GradArgs {
     nrn_gatednorm_t f;
     nrn_gatednorm_grad_t g;
-    float* part;                       // [blocks][3][d]: dalpha, dw_post, dw_pre
+    float* part;                       // [parts][2][d]: sums over rows
     int32_t vec;
 };
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
 // N sums over the threads of a row; every thread gets them.  Rows of one
 // warp need no barrier; else `red` is [2][N][32] floats used in turn.
@@ -84,272 +88,281 @@ __device__ __forceinline__ void load_param(const float* p, int c, int n, float* 
     }
 }
 
-// TPR threads a row, VPT vectors of eight a thread; ROWS rows a block.
+// Blocks of one SM that the kernels' registers leave room for.
+template <int TPR, int VPT, int REGS>
+constexpr int blocks_per_sm() {
+    constexpr int regs = REGS * VPT * (TPR == 32 ? 128 : TPR);
+    return 65536 / regs < 1 ? 1 : 65536 / regs;
+}
+constexpr int kForwardRegs = 64, kBackwardRegs = 102;
+
+// What a row's forward and backward passes read.
+template <typename T, int VPT>
+struct Row {
+    Raw8<T> r[VPT], h[VPT], gate[VPT];
+};
+
 template <typename T, int TPR, int VPT>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_kernel(const __grid_constant__ NormArgs a) {
-    __shared__ float red[128];
-    const nrn_gatednorm_t& f = a.f;
-    const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int rows_per = TPR == 32 ? 4 : 1;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per + (TPR == 32 ? threadIdx.x >> 5 : 0);
-    if (row >= f.rows) return;
-    const bool vec = a.vec != 0;
-    const float inv_d = 1.0f / static_cast<float>(f.d);
-    int turn = 0;
-    Raw8<T> rr[VPT], rh[VPT], rg[VPT];
-    auto left = [&](int v) { return f.d - (tid + v * TPR) * 8; };
+__device__ __forceinline__ void load_row(Row<T, VPT>& x, const nrn_gatednorm_t& f, int64_t row, int tid, bool vec) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-        const int n = left(v);
-        const int64_t c = n > 0 ? (tid + v * TPR) * 8 : 0;
-        rr[v] = load8(static_cast<const T*>(f.residual) + row * f.residual_stride + c, n, vec);
-        if (f.h) rh[v] = load8(static_cast<const T*>(f.h) + row * f.h_stride + c, n, vec);
-        if (f.gate) rg[v] = load8(static_cast<const T*>(f.gate) + row * f.gate_stride + c, n, vec);
-    }
-    float y[VPT][8];
-    if (f.h) {
-        float s[1] = {0.0f};
-#pragma unroll
-        for (int v = 0; v < VPT; ++v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = to_f32(rh[v].e[e]);
-                s[0] = fmaf(x, x, s[0]);
-            }
-        row_sum<1, TPR>(s, red, turn);
-        const float inv = rsqrtf(s[0] * inv_d + f.eps);
-#pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            const int n = left(v), c = (tid + v * TPR) * 8;
-            float w[8], al[8];
-            load_param(f.w_post, n > 0 ? c : 0, n, w);
-            load_param(f.alpha, n > 0 ? c : 0, n, al);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float u = to_f32(rh[v].e[e]) * inv * w[e] * al[e];
-                if (f.gate) {
-                    const float g = to_f32(rg[v].e[e]), sg = sigmoid(g);
-                    u *= f.act == NRN_ACT_SILU ? g * sg : sg;
-                }
-                y[v][e] = to_f32(rr[v].e[e]) + u;
-            }
-            if (f.y && n > 0) store8(static_cast<T*>(f.y) + row * f.y_stride + c, y[v], n, vec);
-        }
-    } else {
-#pragma unroll
-        for (int v = 0; v < VPT; ++v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[v][e] = to_f32(rr[v].e[e]);
-    }
-    if (f.z == nullptr && a.zv == nullptr) return;
-    float s[1] = {0.0f};
-#pragma unroll
-    for (int v = 0; v < VPT; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < left(v)) s[0] = fmaf(y[v][e], y[v][e], s[0]);
-    row_sum<1, TPR>(s, red, turn);
-    const float inv = rsqrtf(s[0] * inv_d + f.eps);
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        const int n = left(v), c = (tid + v * TPR) * 8;
-        float w[8];
-        load_param(f.w_pre, n > 0 ? c : 0, n, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[v][e] = e < n ? y[v][e] * inv * w[e] : 0.0f;
-        if (a.zv == nullptr) {
-            if (n > 0) store8(static_cast<T*>(f.z) + row * f.z_stride + c, y[v], n, vec);
-            continue;
-        }
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, abs_bits(y[v][e]));
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));   // 16 lanes: 128 columns
-        if (n <= 0) continue;
-        const float sc = block_scale(m), q = 1.0f / sc;
-        if ((tid & 15) == 0) a.zs[row * a.zs_row + (c / 128) * a.zs_col] = sc;
-        *reinterpret_cast<uint2*>(a.zv + row * a.zv_stride + c) =
-            make_uint2(e4m3x4(y[v][0] * q, y[v][1] * q, y[v][2] * q, y[v][3] * q),
-                       e4m3x4(y[v][4] * q, y[v][5] * q, y[v][6] * q, y[v][7] * q));
+        const int c = (tid + v * TPR) * 8, n = f.d - c;
+        x.r[v] = load8(static_cast<const T*>(f.residual) + row * f.residual_stride + (n > 0 ? c : 0), n, vec);
+        if (f.h) x.h[v] = load8(static_cast<const T*>(f.h) + row * f.h_stride + (n > 0 ? c : 0), n, vec);
+        if (f.gate) x.gate[v] = load8(static_cast<const T*>(f.gate) + row * f.gate_stride + (n > 0 ? c : 0), n, vec);
     }
 }
 
-// Backward.  With hh = norm(h), u = hh w_post, a = act(gate), yh = norm(y):
-//     dzw = dz w_pre;   dy' = dy + inv_y (dzw - yh mean(dzw yh))      = dresidual
-//     dgate = dy' alpha u act'(gate);  dalpha += dy' a u
-//     dhh = dy' alpha a w_post;  dh = inv_h (dhh - hh mean(dhh hh))
-//     dw_post += dy' alpha a hh;  dw_pre += dz yh
-// y is computed again from h, gate and r: reading it would cost a fourth of
-// the reads and its rounding.  Blocks take rows in turn and keep their part of
-// the three sums over rows in registers; a second kernel adds the parts.
+// TPR threads a row, VPT vectors of eight a thread.  Elements past the row's
+// end are loaded as 0 and stay 0: they add nothing to the sums.
 template <typename T, int TPR, int VPT>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_grad_kernel(const __grid_constant__ GradArgs a) {
-    __shared__ float red[256];
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT, kForwardRegs>())
+    norm_kernel(const __grid_constant__ NormArgs a) {
+    __shared__ float red[128];
     const nrn_gatednorm_t& f = a.f;
-    const nrn_gatednorm_grad_t& g = a.g;
     const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int rows_per = TPR == 32 ? 4 : 1;
-    const int slot = blockIdx.x * rows_per + (TPR == 32 ? threadIdx.x >> 5 : 0);
-    const int64_t step = static_cast<int64_t>(gridDim.x) * rows_per;
-    const bool vec = a.vec != 0;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 4 : 1);
+    int64_t row = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= f.rows) return;
+    const bool vec = a.vec != 0, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
     const float inv_d = 1.0f / static_cast<float>(f.d);
     int turn = 0;
-    float sal[VPT][8], spo[VPT][8], spr[VPT][8];
+    float aw[VPT][8], wp[VPT][8];
 #pragma unroll
-    for (int v = 0; v < VPT; ++v)
+    for (int v = 0; v < VPT; ++v) {
+        const int c = (tid + v * TPR) * 8, n = f.d - c;
+        float al[8];
+        load_param(f.w_post, n > 0 ? c : 0, n, aw[v]);
+        load_param(f.alpha, n > 0 ? c : 0, n, al);
+        load_param(f.w_pre, n > 0 ? c : 0, n, wp[v]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sal[v][e] = spo[v][e] = spr[v][e] = 0.0f;
-    auto left = [&](int v) { return f.d - (tid + v * TPR) * 8; };
-
-    for (int64_t row = slot; row < f.rows; row += step) {
-        Raw8<T> rr[VPT], rh[VPT], rg[VPT], ry[VPT], rz[VPT];
-#pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            const int n = left(v);
-            const int64_t c = n > 0 ? (tid + v * TPR) * 8 : 0;
-            rr[v] = load8(static_cast<const T*>(f.residual) + row * f.residual_stride + c, n, vec);
-            if (f.h) rh[v] = load8(static_cast<const T*>(f.h) + row * f.h_stride + c, n, vec);
-            if (f.gate) rg[v] = load8(static_cast<const T*>(f.gate) + row * f.gate_stride + c, n, vec);
-            if (g.dy) ry[v] = load8(static_cast<const T*>(g.dy) + row * g.dy_stride + c, n, vec);
-            if (g.dz) rz[v] = load8(static_cast<const T*>(g.dz) + row * g.dz_stride + c, n, vec);
-        }
-        float inv_h = 0.0f;
+        for (int e = 0; e < 8; ++e) aw[v][e] *= al[e];
+    }
+    Row<T, VPT> x;
+    load_row<T, TPR, VPT>(x, f, row, tid, vec);
+    for (; row < f.rows; row += step) {
+        float y[VPT][8];
         if (f.h) {
             float s[1] = {0.0f};
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float x = to_f32(rh[v].e[e]);
-                    s[0] = fmaf(x, x, s[0]);
+                    y[v][e] = to_f32(x.h[v].e[e]);
+                    s[0] = fmaf(y[v][e], y[v][e], s[0]);
                 }
             row_sum<1, TPR>(s, red, turn);
-            inv_h = rsqrtf(s[0] * inv_d + f.eps);
-        }
-        // y, and the two sums its norm's gradient needs
-        float y[VPT][8];
-        float s2[2] = {0.0f, 0.0f};
+            const float inv = rsqrtf(fmaf(s[0], inv_d, f.eps));
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            const int n = left(v), c = n > 0 ? (tid + v * TPR) * 8 : 0;
-            float w[8], al[8], wp[8];
-            load_param(f.w_post, c, n, w);
-            load_param(f.alpha, c, n, al);
-            load_param(f.w_pre, c, n, wp);
+            for (int v = 0; v < VPT; ++v)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                y[v][e] = to_f32(rr[v].e[e]);
-                if (f.h) {
-                    float u = to_f32(rh[v].e[e]) * inv_h * w[e] * al[e];
-                    if (f.gate) {
-                        const float x = to_f32(rg[v].e[e]), sg = sigmoid(x);
-                        u *= f.act == NRN_ACT_SILU ? x * sg : sg;
+                for (int e = 0; e < 8; ++e) {
+                    float u = y[v][e] * inv * aw[v][e];
+                    if (gated) {
+                        const float g = to_f32(x.gate[v].e[e]), sg = sigmoid(g);
+                        u *= silu ? g * sg : sg;
                     }
-                    y[v][e] += u;
+                    y[v][e] = to_f32(x.r[v].e[e]) + u;
                 }
-                if (e < n) {
-                    s2[0] = fmaf(y[v][e], y[v][e], s2[0]);
-                    if (g.dz) s2[1] = fmaf(to_f32(rz[v].e[e]) * wp[e], y[v][e], s2[1]);
-                }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[v][e] = to_f32(x.r[v].e[e]);
+        }
+        if (row + step < f.rows) load_row<T, TPR, VPT>(x, f, row + step, tid, vec);
+        if (f.y) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = (tid + v * TPR) * 8, n = f.d - c;
+                if (n > 0) store8(static_cast<T*>(f.y) + row * f.y_stride + c, y[v], n, vec);
             }
         }
+        if (f.z == nullptr && a.zv == nullptr) continue;
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[0] = fmaf(y[v][e], y[v][e], s[0]);
+        row_sum<1, TPR>(s, red, turn);
+        const float inv = rsqrtf(fmaf(s[0], inv_d, f.eps));
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = (tid + v * TPR) * 8, n = f.d - c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[v][e] = y[v][e] * inv * wp[v][e];
+            if (a.zv == nullptr) {
+                if (n > 0) store8(static_cast<T*>(f.z) + row * f.z_stride + c, y[v], n, vec);
+                continue;
+            }
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = max(m, abs_bits(y[v][e]));
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));   // 16 lanes: 128 columns
+            if (n <= 0) continue;
+            const float sc = block_scale(m), q = 1.0f / sc;
+            if ((tid & 15) == 0) a.zs[row * a.zs_row + (c / 128) * a.zs_col] = sc;
+            *reinterpret_cast<uint2*>(a.zv + row * a.zv_stride + c) =
+                make_uint2(e4m3x4(y[v][0] * q, y[v][1] * q, y[v][2] * q, y[v][3] * q),
+                           e4m3x4(y[v][4] * q, y[v][5] * q, y[v][6] * q, y[v][7] * q));
+        }
+    }
+}
+
+// Backward.  With hh = norm(h), a = act(gate), f = alpha w_post, yh = norm(y):
+//     d  = dy + inv_y (dz w_pre - yh mean(dz w_pre yh))            = dresidual
+//     dgate = d f hh act'(gate);   t = d f a;   dh = inv_h (t - hh mean(t hh))
+//     s1 = sum over rows of d a hh: dalpha = s1 w_post, dw_post = s1 alpha
+//     s2 = sum over rows of dz yh = dw_pre
+// y is computed again from h, gate and r: reading it would cost a fifth of
+// the reads and its rounding.  Blocks take rows in turn and keep their part of
+// the two sums in registers; a second kernel adds the parts.
+template <typename T, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT, kBackwardRegs>())
+    norm_grad_kernel(const __grid_constant__ GradArgs a) {
+    __shared__ float red[128];
+    const nrn_gatednorm_t& f = a.f;
+    const nrn_gatednorm_grad_t& g = a.g;
+    const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
+    const int slot = TPR == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 4 : 1);
+    const bool vec = a.vec != 0, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
+    const float inv_d = 1.0f / static_cast<float>(f.d);
+    int turn = 0;
+    float s1[VPT][8], s2[VPT][8], aw[VPT][8], wp[VPT][8];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int c = (tid + v * TPR) * 8, n = f.d - c;
+        float al[8];
+        load_param(f.w_post, n > 0 ? c : 0, n, aw[v]);
+        load_param(f.alpha, n > 0 ? c : 0, n, al);
+        load_param(f.w_pre, n > 0 ? c : 0, n, wp[v]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            aw[v][e] *= al[e];
+            s1[v][e] = s2[v][e] = 0.0f;
+        }
+    }
+    for (int64_t row = slot; row < f.rows; row += step) {
+        Row<T, VPT> x;
+        Raw8<T> ry[VPT], rz[VPT];
+        load_row<T, TPR, VPT>(x, f, row, tid, vec);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = (tid + v * TPR) * 8, n = f.d - c;
+            if (g.dy) ry[v] = load8(static_cast<const T*>(g.dy) + row * g.dy_stride + (n > 0 ? c : 0), n, vec);
+            if (g.dz) rz[v] = load8(static_cast<const T*>(g.dz) + row * g.dz_stride + (n > 0 ? c : 0), n, vec);
+        }
+        float hh[VPT][8], y[VPT][8], act[VPT][8], dact[VPT][8], inv_h = 0.0f;
+        if (f.h) {
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    hh[v][e] = to_f32(x.h[v].e[e]);
+                    s[0] = fmaf(hh[v][e], hh[v][e], s[0]);
+                }
+            row_sum<1, TPR>(s, red, turn);
+            inv_h = rsqrtf(fmaf(s[0], inv_d, f.eps));
+        }
+        float sy[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[v][e] = to_f32(x.r[v].e[e]);
+                if (f.h) {
+                    hh[v][e] *= inv_h;
+                    act[v][e] = 1.0f;
+                    dact[v][e] = 0.0f;
+                    if (gated) {
+                        const float t = to_f32(x.gate[v].e[e]), sg = sigmoid(t), ts = t * sg;
+                        act[v][e] = silu ? ts : sg;
+                        dact[v][e] = silu ? fmaf(ts, 1.0f - sg, sg) : sg * (1.0f - sg);
+                    }
+                    y[v][e] = fmaf(hh[v][e] * aw[v][e], act[v][e], y[v][e]);
+                }
+                sy[0] = fmaf(y[v][e], y[v][e], sy[0]);
+                if (g.dz) sy[1] = fmaf(to_f32(rz[v].e[e]) * wp[v][e], y[v][e], sy[1]);
+            }
         float inv_y = 0.0f, my = 0.0f;
         if (g.dz) {
-            row_sum<2, TPR>(s2, red, turn);
-            inv_y = rsqrtf(s2[0] * inv_d + f.eps);
-            my = inv_y * inv_y * s2[1] * inv_d;      // mean(dzw yh) inv_y
+            row_sum<2, TPR>(sy, red, turn);
+            inv_y = rsqrtf(fmaf(sy[0], inv_d, f.eps));
+            my = inv_y * inv_y * sy[1] * inv_d;      // mean(dz w_pre yh) inv_y
         }
-        // dy' into y; dgate out; mean(dhh hh)
-        float s3[1] = {0.0f};
+        float st[1] = {0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int n = left(v), c = n > 0 ? (tid + v * TPR) * 8 : 0;
-            float w[8], al[8], wp[8], dg[8];
-            load_param(f.w_post, c, n, w);
-            load_param(f.alpha, c, n, al);
-            load_param(f.w_pre, c, n, wp);
+            const int c = (tid + v * TPR) * 8, n = f.d - c;
+            float d[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float d = g.dy ? to_f32(ry[v].e[e]) : 0.0f;
+                d[e] = g.dy ? to_f32(ry[v].e[e]) : 0.0f;
                 if (g.dz) {
                     const float z = to_f32(rz[v].e[e]);
-                    spr[v][e] = fmaf(z, y[v][e] * inv_y, spr[v][e]);
-                    d += inv_y * (z * wp[e] - y[v][e] * my);
-                }
-                y[v][e] = d;
-                if (f.h) {
-                    const float hh = to_f32(rh[v].e[e]) * inv_h;
-                    float act = 1.0f, dact = 0.0f;
-                    if (f.gate) {
-                        const float x = to_f32(rg[v].e[e]), sg = sigmoid(x);
-                        act = f.act == NRN_ACT_SILU ? x * sg : sg;
-                        dact = f.act == NRN_ACT_SILU ? sg * fmaf(x, 1.0f - sg, 1.0f) : sg * (1.0f - sg);
-                    }
-                    const float u = hh * w[e];
-                    sal[v][e] = fmaf(d * act, u, sal[v][e]);
-                    const float da = d * al[e];
-                    dg[e] = da * u * dact;
-                    spo[v][e] = fmaf(da * act, hh, spo[v][e]);
-                    s3[0] = fmaf(da * act * w[e], hh, s3[0]);
+                    s2[v][e] = fmaf(z, y[v][e] * inv_y, s2[v][e]);
+                    d[e] = fmaf(inv_y, z * wp[v][e] - y[v][e] * my, d[e]);
                 }
             }
-            if (n > 0) {
-                if (g.dresidual) store8(static_cast<T*>(g.dresidual) + row * g.dresidual_stride + c, y[v], n, vec);
-                if (g.dgate && f.h && f.gate) store8(static_cast<T*>(g.dgate) + row * g.dgate_stride + c, dg, n, vec);
+            if (n > 0 && g.dresidual) store8(static_cast<T*>(g.dresidual) + row * g.dresidual_stride + c, d, n, vec);
+            if (f.h) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    s1[v][e] = fmaf(d[e] * act[v][e], hh[v][e], s1[v][e]);
+                    const float da = d[e] * aw[v][e];
+                    dact[v][e] *= da * hh[v][e];
+                    y[v][e] = da * act[v][e];
+                    st[0] = fmaf(y[v][e], hh[v][e], st[0]);
+                }
+                if (n > 0 && g.dgate && gated) store8(static_cast<T*>(g.dgate) + row * g.dgate_stride + c, dact[v], n, vec);
             }
         }
         if (f.h && g.dh) {
-            row_sum<1, TPR>(s3, red, turn);
-            const float mh = s3[0] * inv_d;
+            row_sum<1, TPR>(st, red, turn);
+            const float mh = st[0] * inv_d;
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const int n = left(v), c = n > 0 ? (tid + v * TPR) * 8 : 0;
-                float w[8], al[8], dh[8];
-                load_param(f.w_post, c, n, w);
-                load_param(f.alpha, c, n, al);
+                const int c = (tid + v * TPR) * 8, n = f.d - c;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float act = 1.0f;
-                    if (f.gate) {
-                        const float x = to_f32(rg[v].e[e]), sg = sigmoid(x);
-                        act = f.act == NRN_ACT_SILU ? x * sg : sg;
-                    }
-                    dh[e] = inv_h * (y[v][e] * al[e] * act * w[e] - to_f32(rh[v].e[e]) * inv_h * mh);
-                }
-                if (n > 0) store8(static_cast<T*>(g.dh) + row * g.dh_stride + c, dh, n, vec);
+                for (int e = 0; e < 8; ++e) y[v][e] = inv_h * (y[v][e] - hh[v][e] * mh);
+                if (n > 0) store8(static_cast<T*>(g.dh) + row * g.dh_stride + c, y[v], n, vec);
             }
         }
     }
     if (a.part == nullptr) return;
-    float* at = a.part + static_cast<int64_t>(slot) * 3 * f.d;
+    float* at = a.part + static_cast<int64_t>(slot) * 2 * f.d;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-        const int n = left(v), c = (tid + v * TPR) * 8;
+        const int c = (tid + v * TPR) * 8, n = f.d - c;
         if (n <= 0) continue;
-        store8(at + c, sal[v], n, false);
-        store8(at + f.d + c, spo[v], n, false);
-        store8(at + 2 * f.d + c, spr[v], n, false);
+        store8(at + c, s1[v], n, f.d % 4 == 0);
+        store8(at + f.d + c, s2[v], n, f.d % 4 == 0);
     }
 }
 
-// Adds the parts of one of the three sums, in their order: 32 columns a
-// block, eight runs of parts at once.
-__global__ void __launch_bounds__(256) norm_parts_kernel(const float* part, int parts, int d, float* dalpha, float* dw_post,
-                                                         float* dw_pre) {
-    __shared__ float sum[8][32];
-    float* out = blockIdx.y == 0 ? dalpha : (blockIdx.y == 1 ? dw_post : dw_pre);
-    if (out == nullptr) return;
+// Adds the blocks' parts of one of the two sums, in their order: 32 columns a
+// block, 32 runs of parts at once.
+__global__ void __launch_bounds__(1024) norm_parts_kernel(const float* part, int parts, int d, const float* alpha, const float* w_post,
+                                                          float* dalpha, float* dw_post, float* dw_pre) {
+    __shared__ float sum[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5;
     float s = 0.0f;
     if (c < d)
-        for (int p = run; p < parts; p += 8) s += part[(static_cast<int64_t>(p) * 3 + blockIdx.y) * d + c];
+#pragma unroll 4
+        for (int p = run; p < parts; p += 32) s += part[(static_cast<int64_t>(p) * 2 + blockIdx.y) * d + c];
     sum[run][threadIdx.x & 31] = s;
     __syncthreads();
-    if (run == 0 && c < d) {
+    if (run != 0 || c >= d) return;
 #pragma unroll
-        for (int r = 1; r < 8; ++r) s += sum[r][threadIdx.x];
-        out[c] = s;
+    for (int r = 1; r < 32; ++r) s += sum[r][threadIdx.x];
+    if (blockIdx.y == 1) {
+        if (dw_pre) dw_pre[c] = s;
+    } else {
+        if (dalpha) dalpha[c] = w_post ? s * w_post[c] : s;
+        if (dw_post) dw_post[c] = alpha ? s * alpha[c] : s;
     }
 }
 
@@ -360,45 +373,55 @@ struct Shape {
 Shape shape_of(int d) {
     const int vecs = (d + 7) / 8;
     if (vecs <= 32) return {32, 1};
-    if (vecs <= 64) return {32, 2};
+    if (vecs <= 64) return {64, 1};
     if (vecs <= 128) return {128, 1};
     if (vecs <= 256) return {256, 1};
     if (vecs <= 320) return {320, 1};
     if (vecs <= 512) return {512, 1};
-    if (vecs <= 1024) return {1024, 1};
+    if (vecs <= 1024) return {512, 2};
     return {1024, 2};
+}
+
+// Blocks that take the rows in turn: as many as are on the GPU at once.
+template <int TPR, int VPT, int REGS>
+unsigned blocks_for(int64_t rows) {
+    constexpr int rows_per = TPR == 32 ? 4 : 1;
+    return static_cast<unsigned>(std::min<int64_t>((rows + rows_per - 1) / rows_per,
+                                                   static_cast<int64_t>(blocks_per_sm<TPR, VPT, REGS>()) * sm_count_current()));
 }
 
 template <typename T, int TPR, int VPT>
 void run_forward(const NormArgs& a, cudaStream_t s) {
-    const int rows_per = TPR == 32 ? 4 : 1;
-    norm_kernel<T, TPR, VPT><<<static_cast<unsigned>((a.f.rows + rows_per - 1) / rows_per), TPR == 32 ? 128 : TPR, 0, s>>>(a);
+    norm_kernel<T, TPR, VPT><<<blocks_for<TPR, VPT, kForwardRegs>(a.f.rows), TPR == 32 ? 128 : TPR, 0, s>>>(a);
 }
-
-// Blocks of the backward kernel: enough threads for every SM, but a part of
-// the sums for each, which the second kernel reads.
-int grad_blocks(int64_t rows, int tpr) {
-    const int threads = tpr == 32 ? 128 : tpr, per = std::max(1, 1024 / threads), rows_per = tpr == 32 ? 4 : 1;
-    return static_cast<int>(std::min<int64_t>((rows + rows_per - 1) / rows_per, static_cast<int64_t>(per) * sm_count_current()));
-}
-int grad_parts(int64_t rows, int tpr) { return grad_blocks(rows, tpr) * (tpr == 32 ? 4 : 1); }
 
 template <typename T, int TPR, int VPT>
 void run_backward(const GradArgs& a, cudaStream_t s) {
-    norm_grad_kernel<T, TPR, VPT><<<grad_blocks(a.f.rows, TPR), TPR == 32 ? 128 : TPR, 0, s>>>(a);
+    norm_grad_kernel<T, TPR, VPT><<<blocks_for<TPR, VPT, kBackwardRegs>(a.f.rows), TPR == 32 ? 128 : TPR, 0, s>>>(a);
+}
+
+// Parts of the sums over rows that the backward kernel leaves: one for each block, or warp where a warp has a row.
+int grad_parts(int64_t rows, int tpr, int vpt) {
+    if (tpr == 32) return 4 * static_cast<int>(blocks_for<32, 1, kBackwardRegs>(rows));
+    if (tpr == 64) return static_cast<int>(blocks_for<64, 1, kBackwardRegs>(rows));
+    if (tpr == 128) return static_cast<int>(blocks_for<128, 1, kBackwardRegs>(rows));
+    if (tpr == 256) return static_cast<int>(blocks_for<256, 1, kBackwardRegs>(rows));
+    if (tpr == 320) return static_cast<int>(blocks_for<320, 1, kBackwardRegs>(rows));
+    if (tpr == 1024) return static_cast<int>(blocks_for<1024, 2, kBackwardRegs>(rows));
+    return static_cast<int>(vpt == 1 ? blocks_for<512, 1, kBackwardRegs>(rows) : blocks_for<512, 2, kBackwardRegs>(rows));
 }
 
 #define NRN_NORM_SHAPES(T, CALL)                                \
     do {                                                        \
         const Shape sh = shape_of(a.f.d);                       \
-        if (sh.tpr == 32 && sh.vpt == 1) CALL<T, 32, 1>(a, s);  \
-        else if (sh.tpr == 32) CALL<T, 32, 2>(a, s);            \
+        if (sh.tpr == 32) CALL<T, 32, 1>(a, s);                 \
+        else if (sh.tpr == 64) CALL<T, 64, 1>(a, s);            \
         else if (sh.tpr == 128) CALL<T, 128, 1>(a, s);          \
         else if (sh.tpr == 256) CALL<T, 256, 1>(a, s);          \
         else if (sh.tpr == 320) CALL<T, 320, 1>(a, s);          \
-        else if (sh.tpr == 512) CALL<T, 512, 1>(a, s);          \
-        else if (sh.vpt == 1) CALL<T, 1024, 1>(a, s);           \
-        else CALL<T, 1024, 2>(a, s);                            \
+        else if (sh.tpr == 1024) CALL<T, 1024, 2>(a, s);        \
+        else if (sh.vpt == 1) CALL<T, 512, 1>(a, s);            \
+        else CALL<T, 512, 2>(a, s);                             \
     } while (0)
 
 bool row_ok(const void* p, int64_t stride, int size) {
@@ -453,7 +476,8 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_forward(const nrn_gatednorm_t* in, nr
 extern "C" nrn_status_t nrn_cuda_gatednorm_workspace(const nrn_gatednorm_t* a, int64_t* bytes) {
     NRN_CHECK_ARG(a && bytes, "nrn_cuda_gatednorm_workspace: null argument");
     NRN_CHECK_ARG(a->rows >= 0 && a->d >= 1 && a->d <= kMaxD, "nrn_cuda_gatednorm_workspace: sizes out of range");
-    *bytes = static_cast<int64_t>(grad_parts(a->rows, shape_of(a->d).tpr)) * 3 * a->d * 4;
+    const Shape sh = shape_of(a->d);
+    *bytes = static_cast<int64_t>(grad_parts(a->rows, sh.tpr, sh.vpt)) * 2 * a->d * 4;
     return NRN_OK;
 }
 
@@ -472,10 +496,11 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* in, c
     GradArgs a{};
     a.f = *in;
     a.g = *g;
-    const int size = in->dtype == NRN_FP32 ? 4 : 2, tpr = shape_of(in->d).tpr;
-    const int parts = grad_parts(in->rows, tpr);
+    const int size = in->dtype == NRN_FP32 ? 4 : 2;
+    const Shape sh = shape_of(in->d);
+    const int parts = grad_parts(in->rows, sh.tpr, sh.vpt);
     if (sums) {
-        NRN_CHECK_ARG(g->workspace && g->workspace_bytes >= static_cast<int64_t>(parts) * 3 * in->d * 4, who + ": workspace too small");
+        NRN_CHECK_ARG(g->workspace && g->workspace_bytes >= static_cast<int64_t>(parts) * 2 * in->d * 4, who + ": workspace too small");
         a.part = static_cast<float*>(g->workspace);
     }
     a.vec = row_ok(in->residual, in->residual_stride, size) && row_ok(in->h, in->h_stride, size) &&
@@ -486,7 +511,8 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* in, c
     else NRN_NORM_SHAPES(float, run_backward);
     NRN_CUDA_TRY(cudaGetLastError());
     if (sums) {
-        norm_parts_kernel<<<dim3(static_cast<unsigned>((in->d + 31) / 32), 3), 256, 0, s>>>(a.part, parts, in->d, g->dalpha, g->dw_post, g->dw_pre);
+        norm_parts_kernel<<<dim3(static_cast<unsigned>((in->d + 31) / 32), 2), 1024, 0, s>>>(a.part, parts, in->d, in->alpha, in->w_post, g->dalpha, g->dw_post,
+                                                                                          g->dw_pre);
         NRN_CUDA_TRY(cudaGetLastError());
     }
     return NRN_OK;
