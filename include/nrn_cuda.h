@@ -507,6 +507,7 @@ typedef struct {
     void* z;                   /* NULL: not written                          */
     int64_t y_stride, z_stride;
     const nrn_scaled_t* z_scaled;   /* z in 8 bits (row_block 1) instead, or NULL */
+    int32_t* err;              /* device flag, set to 5 when a device-side wait gives up, or NULL */
 } nrn_gatednorm_t;
 
 /* Gradients; dy and dz come in (NULL: zero), the others go out (NULL: not

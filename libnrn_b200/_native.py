@@ -149,7 +149,7 @@ class GatedNorm(C.Structure):
         ("residual", C.c_void_p), ("h", C.c_void_p), ("gate", C.c_void_p), ("residual_stride", C.c_int64),
         ("h_stride", C.c_int64), ("gate_stride", C.c_int64), ("alpha", C.c_void_p), ("w_post", C.c_void_p),
         ("w_pre", C.c_void_p), ("y", C.c_void_p), ("z", C.c_void_p), ("y_stride", C.c_int64),
-        ("z_stride", C.c_int64), ("z_scaled", C.POINTER(Scaled)),
+        ("z_stride", C.c_int64), ("z_scaled", C.POINTER(Scaled)), ("err", C.c_void_p),
     ]
 
 

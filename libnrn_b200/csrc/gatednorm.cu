@@ -14,8 +14,10 @@
 // every output's rounding), alpha and w_post are one factor, and a block keeps
 // its columns' factors in registers over all the rows it takes in turn.  A row
 // is held in registers, eight elements a thread and vector (16 bytes of bf16):
-// 32 threads a row where the row is short, else a block a row; the next row's
-// loads are in flight while a row is worked on.
+// 32 threads a row where the row is short, else a block a row.  The reductions
+// over a row are barriers that a block waits at, so its next rows must be on
+// their way meanwhile: rows on 16-byte boundaries come by bulk copies into a
+// ring of two to four in shared memory.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -24,6 +26,7 @@
 #include "common.cuh"
 #include "internal.h"
 #include "scaled.cuh"
+#include "tc.cuh"
 #include "vecio.cuh"
 
 namespace nrn {
@@ -37,6 +40,7 @@ struct NormArgs {
     float* zs;
     int64_t zv_stride, zs_row, zs_col;
     int32_t vec;                       // every row starts on a 16-byte boundary
+    int32_t stages;                    // rows of the ring
 };
 
 struct GradArgs {
@@ -44,9 +48,15 @@ struct GradArgs {
     nrn_gatednorm_grad_t g;
     float* part;                       // [parts][2][d]: sums over rows
     int32_t vec;
+    int32_t stages;
 };
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float sigmoid(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
 
 // N sums over the threads of a row; every thread gets them.  Rows of one
 // warp need no barrier; else `red` is [2][N][32] floats used in turn.
@@ -96,28 +106,87 @@ constexpr int blocks_per_sm() {
 }
 constexpr int kForwardRegs = 64, kBackwardRegs = 102;
 
-// What a row's forward and backward passes read.
-template <typename T, int VPT>
-struct Row {
-    Raw8<T> r[VPT], h[VPT], gate[VPT];
-};
+// The rows a block reads, as a ring in shared memory filled by one thread's
+// bulk copies (RING), or straight from global memory.
+constexpr int kMostStages = 4;
+constexpr int kRingHead = 128;
+enum { ERR_NORM_TIMEOUT = 5 };
 
-template <typename T, int TPR, int VPT>
-__device__ __forceinline__ void load_row(Row<T, VPT>& x, const nrn_gatednorm_t& f, int64_t row, int tid, bool vec) {
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        const int c = (tid + v * TPR) * 8, n = f.d - c;
-        x.r[v] = load8(static_cast<const T*>(f.residual) + row * f.residual_stride + (n > 0 ? c : 0), n, vec);
-        if (f.h) x.h[v] = load8(static_cast<const T*>(f.h) + row * f.h_stride + (n > 0 ? c : 0), n, vec);
-        if (f.gate) x.gate[v] = load8(static_cast<const T*>(f.gate) + row * f.gate_stride + (n > 0 ? c : 0), n, vec);
+template <typename T, int TPR, int N, bool RING>
+struct Rows {
+    const T* from[N];
+    int64_t stride[N];
+    int64_t rows, step;
+    int32_t d, stages, stage;
+    uint32_t phase;
+    bool vec;
+    uint64_t* bars;
+    unsigned char* ring;
+    int* err;
+
+    __device__ __forceinline__ void start(unsigned char* smem, int64_t row) {
+        if constexpr (RING) {
+            bars = reinterpret_cast<uint64_t*>(smem);
+            ring = smem + kRingHead;
+            stage = 0;
+            phase = 0;
+            if (threadIdx.x == 0) {
+                for (int i = 0; i < stages; ++i) tc::mbar_init(&bars[i], 1);
+                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+                for (int i = 0; i < stages; ++i) fill(row + i * step, i);
+            }
+            __syncthreads();
+        }
     }
-}
+    __device__ __forceinline__ void fill(int64_t row, int st) {
+        if (row >= rows) return;
+        const uint32_t bytes = static_cast<uint32_t>(d * sizeof(T));
+        uint32_t all = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) all += from[i] ? bytes : 0u;
+        tc::mbar_expect_tx(&bars[st], all);
+        const uint64_t once = tc::policy_evict_first();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (from[i]) tc::bulk_load(ring + (st * N + i) * static_cast<size_t>(bytes), from[i] + row * stride[i], bytes, &bars[st], once);
+    }
+    // this row is in shared memory
+    __device__ __forceinline__ void wait() {
+        if constexpr (RING) {
+            if (!tc::mbar_wait(&bars[stage], phase, nullptr) && err) atomicCAS(err, 0, ERR_NORM_TIMEOUT);
+        }
+    }
+    __device__ __forceinline__ Raw8<T> get(int i, int64_t row, int c) const {
+        if constexpr (RING) {
+            const uint4* s = reinterpret_cast<const uint4*>(ring + (stage * N + i) * (d * sizeof(T)) + (c < d ? c : 0) * sizeof(T));
+            Raw8<T> r;
+            uint4* t = reinterpret_cast<uint4*>(&r);
+#pragma unroll
+            for (int k = 0; k < static_cast<int>(sizeof(r) / 16); ++k) t[k] = c < d ? s[k] : make_uint4(0, 0, 0, 0);
+            return r;
+        } else {
+            const int n = d - c;
+            return load8(from[i] + row * stride[i] + (n > 0 ? c : 0), n, vec);
+        }
+    }
+    // every thread of the block has what it needs of this row
+    __device__ __forceinline__ void done(int64_t row) {
+        if constexpr (RING) {
+            if (threadIdx.x == 0) fill(row + stages * step, stage);
+            if (++stage == stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+    }
+};
 
 // TPR threads a row, VPT vectors of eight a thread.  Elements past the row's
 // end are loaded as 0 and stay 0: they add nothing to the sums.
-template <typename T, int TPR, int VPT>
+template <typename T, int TPR, int VPT, bool RING>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT, kForwardRegs>())
     norm_kernel(const __grid_constant__ NormArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float red[128];
     const nrn_gatednorm_t& f = a.f;
     const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
@@ -125,6 +194,11 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
     int64_t row = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= f.rows) return;
     const bool vec = a.vec != 0, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
+    Rows<T, TPR, 3, RING> in;
+    in.from[0] = static_cast<const T*>(f.residual), in.from[1] = static_cast<const T*>(f.h), in.from[2] = static_cast<const T*>(f.gate);
+    in.stride[0] = f.residual_stride, in.stride[1] = f.h_stride, in.stride[2] = f.gate_stride;
+    in.rows = f.rows, in.step = step, in.d = f.d, in.stages = a.stages, in.vec = vec, in.err = f.err;
+    in.start(smem, row);
     const float inv_d = 1.0f / static_cast<float>(f.d);
     int turn = 0;
     float aw[VPT][8], wp[VPT][8];
@@ -138,59 +212,68 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
 #pragma unroll
         for (int e = 0; e < 8; ++e) aw[v][e] *= al[e];
     }
-    Row<T, VPT> x;
-    load_row<T, TPR, VPT>(x, f, row, tid, vec);
+    const bool want_z = f.z != nullptr || a.zv != nullptr;
     for (; row < f.rows; row += step) {
         float y[VPT][8];
+        in.wait();
         if (f.h) {
+            Raw8<T> r[VPT], gate[VPT];
             float s[1] = {0.0f};
 #pragma unroll
-            for (int v = 0; v < VPT; ++v)
+            for (int v = 0; v < VPT; ++v) {
+                const int c = (tid + v * TPR) * 8;
+                const Raw8<T> h = in.get(1, row, c);
+                r[v] = in.get(0, row, c);
+                if (gated) gate[v] = in.get(2, row, c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    y[v][e] = to_f32(x.h[v].e[e]);
+                    y[v][e] = to_f32(h.e[e]);
                     s[0] = fmaf(y[v][e], y[v][e], s[0]);
                 }
+            }
             row_sum<1, TPR>(s, red, turn);
+            in.done(row);
             const float inv = rsqrtf(fmaf(s[0], inv_d, f.eps));
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    float u = y[v][e] * inv * aw[v][e];
+                    float u = inv * aw[v][e];
                     if (gated) {
-                        const float g = to_f32(x.gate[v].e[e]), sg = sigmoid(g);
+                        const float g = to_f32(gate[v].e[e]), sg = sigmoid(g);
                         u *= silu ? g * sg : sg;
                     }
-                    y[v][e] = to_f32(x.r[v].e[e]) + u;
+                    y[v][e] = fmaf(y[v][e], u, to_f32(r[v].e[e]));
                 }
+            if (f.y) {
+#pragma unroll
+                for (int v = 0; v < VPT; ++v) {
+                    const int c = (tid + v * TPR) * 8, n = f.d - c;
+                    if (n > 0) store8(static_cast<T*>(f.y) + row * f.y_stride + c, y[v], n, vec);
+                }
+            }
+            if (!want_z) continue;
         } else {
 #pragma unroll
-            for (int v = 0; v < VPT; ++v)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[v][e] = to_f32(x.r[v].e[e]);
-        }
-        if (row + step < f.rows) load_row<T, TPR, VPT>(x, f, row + step, tid, vec);
-        if (f.y) {
-#pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const int c = (tid + v * TPR) * 8, n = f.d - c;
-                if (n > 0) store8(static_cast<T*>(f.y) + row * f.y_stride + c, y[v], n, vec);
+                const Raw8<T> r = in.get(0, row, (tid + v * TPR) * 8);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[v][e] = to_f32(r.e[e]);
             }
         }
-        if (f.z == nullptr && a.zv == nullptr) continue;
         float s[1] = {0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[0] = fmaf(y[v][e], y[v][e], s[0]);
         row_sum<1, TPR>(s, red, turn);
+        if (!f.h) in.done(row);
         const float inv = rsqrtf(fmaf(s[0], inv_d, f.eps));
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = (tid + v * TPR) * 8, n = f.d - c;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[v][e] = y[v][e] * inv * wp[v][e];
+            for (int e = 0; e < 8; ++e) y[v][e] *= inv * wp[v][e];
             if (a.zv == nullptr) {
                 if (n > 0) store8(static_cast<T*>(f.z) + row * f.z_stride + c, y[v], n, vec);
                 continue;
@@ -218,9 +301,10 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
 // y is computed again from h, gate and r: reading it would cost a fifth of
 // the reads and its rounding.  Blocks take rows in turn and keep their part of
 // the two sums in registers; a second kernel adds the parts.
-template <typename T, int TPR, int VPT>
+template <typename T, int TPR, int VPT, bool RING>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT, kBackwardRegs>())
     norm_grad_kernel(const __grid_constant__ GradArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float red[128];
     const nrn_gatednorm_t& f = a.f;
     const nrn_gatednorm_grad_t& g = a.g;
@@ -244,41 +328,49 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
             s1[v][e] = s2[v][e] = 0.0f;
         }
     }
+    Rows<T, TPR, 5, RING> in;
+    in.from[0] = static_cast<const T*>(f.residual), in.from[1] = static_cast<const T*>(f.h), in.from[2] = static_cast<const T*>(f.gate);
+    in.from[3] = static_cast<const T*>(g.dy), in.from[4] = static_cast<const T*>(g.dz);
+    in.stride[0] = f.residual_stride, in.stride[1] = f.h_stride, in.stride[2] = f.gate_stride;
+    in.stride[3] = g.dy_stride, in.stride[4] = g.dz_stride;
+    in.rows = f.rows, in.step = step, in.d = f.d, in.stages = a.stages, in.vec = vec, in.err = f.err;
+    in.start(smem, slot);
     for (int64_t row = slot; row < f.rows; row += step) {
-        Row<T, VPT> x;
-        Raw8<T> ry[VPT], rz[VPT];
-        load_row<T, TPR, VPT>(x, f, row, tid, vec);
+        Raw8<T> rr[VPT], rg[VPT], ry[VPT], rz[VPT];
+        float hh[VPT][8], y[VPT][8], act[VPT][8], dact[VPT][8], inv_h = 0.0f;
+        in.wait();
+        float sh[1] = {0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int c = (tid + v * TPR) * 8, n = f.d - c;
-            if (g.dy) ry[v] = load8(static_cast<const T*>(g.dy) + row * g.dy_stride + (n > 0 ? c : 0), n, vec);
-            if (g.dz) rz[v] = load8(static_cast<const T*>(g.dz) + row * g.dz_stride + (n > 0 ? c : 0), n, vec);
-        }
-        float hh[VPT][8], y[VPT][8], act[VPT][8], dact[VPT][8], inv_h = 0.0f;
-        if (f.h) {
-            float s[1] = {0.0f};
-#pragma unroll
-            for (int v = 0; v < VPT; ++v)
+            const int c = (tid + v * TPR) * 8;
+            if (f.h) {
+                const Raw8<T> h = in.get(1, row, c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    hh[v][e] = to_f32(x.h[v].e[e]);
-                    s[0] = fmaf(hh[v][e], hh[v][e], s[0]);
+                    hh[v][e] = to_f32(h.e[e]);
+                    sh[0] = fmaf(hh[v][e], hh[v][e], sh[0]);
                 }
-            row_sum<1, TPR>(s, red, turn);
-            inv_h = rsqrtf(fmaf(s[0], inv_d, f.eps));
+            }
+            rr[v] = in.get(0, row, c);
+            if (gated) rg[v] = in.get(2, row, c);
+            if (g.dy) ry[v] = in.get(3, row, c);
+            if (g.dz) rz[v] = in.get(4, row, c);
         }
+        row_sum<1, TPR>(sh, red, turn);
+        in.done(row);
+        inv_h = rsqrtf(fmaf(sh[0], inv_d, f.eps));
         float sy[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                y[v][e] = to_f32(x.r[v].e[e]);
+                y[v][e] = to_f32(rr[v].e[e]);
                 if (f.h) {
                     hh[v][e] *= inv_h;
                     act[v][e] = 1.0f;
                     dact[v][e] = 0.0f;
                     if (gated) {
-                        const float t = to_f32(x.gate[v].e[e]), sg = sigmoid(t), ts = t * sg;
+                        const float t = to_f32(rg[v].e[e]), sg = sigmoid(t), ts = t * sg;
                         act[v][e] = silu ? ts : sg;
                         dact[v][e] = silu ? fmaf(ts, 1.0f - sg, sg) : sg * (1.0f - sg);
                     }
@@ -390,14 +482,48 @@ unsigned blocks_for(int64_t rows) {
                                                    static_cast<int64_t>(blocks_per_sm<TPR, VPT, REGS>()) * sm_count_current()));
 }
 
-template <typename T, int TPR, int VPT>
-void run_forward(const NormArgs& a, cudaStream_t s) {
-    norm_kernel<T, TPR, VPT><<<blocks_for<TPR, VPT, kForwardRegs>(a.f.rows), TPR == 32 ? 128 : TPR, 0, s>>>(a);
+// Rows that a block's share of the SM's shared memory holds; below two there is no ring.
+template <typename T, int TPR, int VPT, int REGS>
+int ring_stages(int arrays, int d, bool vec) {
+    if (TPR == 32 || !vec || d % 8 != 0) return 0;
+    const int room = (227 * 1024 / blocks_per_sm<TPR, VPT, REGS>() - 2048 - kRingHead) / (arrays * d * static_cast<int>(sizeof(T)));
+    return room < 2 ? 0 : std::min(room, kMostStages);
 }
 
 template <typename T, int TPR, int VPT>
-void run_backward(const GradArgs& a, cudaStream_t s) {
-    norm_grad_kernel<T, TPR, VPT><<<blocks_for<TPR, VPT, kBackwardRegs>(a.f.rows), TPR == 32 ? 128 : TPR, 0, s>>>(a);
+cudaError_t run_forward(NormArgs a, cudaStream_t s) {
+    constexpr int threads = TPR == 32 ? 128 : TPR;
+    const unsigned blocks = blocks_for<TPR, VPT, kForwardRegs>(a.f.rows);
+    a.stages = ring_stages<T, TPR, VPT, kForwardRegs>(3, a.f.d, a.vec != 0);
+    if constexpr (TPR > 32) {
+        if (a.stages) {
+            const int bytes = kRingHead + a.stages * 3 * a.f.d * static_cast<int>(sizeof(T));
+            const cudaError_t e = cudaFuncSetAttribute(norm_kernel<T, TPR, VPT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (e != cudaSuccess) return e;
+            norm_kernel<T, TPR, VPT, true><<<blocks, threads, bytes, s>>>(a);
+            return cudaGetLastError();
+        }
+    }
+    norm_kernel<T, TPR, VPT, false><<<blocks, threads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T, int TPR, int VPT>
+cudaError_t run_backward(GradArgs a, cudaStream_t s) {
+    constexpr int threads = TPR == 32 ? 128 : TPR;
+    const unsigned blocks = blocks_for<TPR, VPT, kBackwardRegs>(a.f.rows);
+    a.stages = ring_stages<T, TPR, VPT, kBackwardRegs>(5, a.f.d, a.vec != 0);
+    if constexpr (TPR > 32) {
+        if (a.stages) {
+            const int bytes = kRingHead + a.stages * 5 * a.f.d * static_cast<int>(sizeof(T));
+            const cudaError_t e = cudaFuncSetAttribute(norm_grad_kernel<T, TPR, VPT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (e != cudaSuccess) return e;
+            norm_grad_kernel<T, TPR, VPT, true><<<blocks, threads, bytes, s>>>(a);
+            return cudaGetLastError();
+        }
+    }
+    norm_grad_kernel<T, TPR, VPT, false><<<blocks, threads, 0, s>>>(a);
+    return cudaGetLastError();
 }
 
 // Parts of the sums over rows that the backward kernel leaves: one for each block, or warp where a warp has a row.
@@ -411,17 +537,17 @@ int grad_parts(int64_t rows, int tpr, int vpt) {
     return static_cast<int>(vpt == 1 ? blocks_for<512, 1, kBackwardRegs>(rows) : blocks_for<512, 2, kBackwardRegs>(rows));
 }
 
-#define NRN_NORM_SHAPES(T, CALL)                                \
-    do {                                                        \
-        const Shape sh = shape_of(a.f.d);                       \
-        if (sh.tpr == 32) CALL<T, 32, 1>(a, s);                 \
-        else if (sh.tpr == 64) CALL<T, 64, 1>(a, s);            \
-        else if (sh.tpr == 128) CALL<T, 128, 1>(a, s);          \
-        else if (sh.tpr == 256) CALL<T, 256, 1>(a, s);          \
-        else if (sh.tpr == 320) CALL<T, 320, 1>(a, s);          \
-        else if (sh.tpr == 1024) CALL<T, 1024, 2>(a, s);        \
-        else if (sh.vpt == 1) CALL<T, 512, 1>(a, s);            \
-        else CALL<T, 512, 2>(a, s);                             \
+#define NRN_NORM_SHAPES(T, CALL)                                               \
+    do {                                                                       \
+        const Shape sh = shape_of(a.f.d);                                      \
+        if (sh.tpr == 32) NRN_CUDA_TRY((CALL<T, 32, 1>(a, s)));                \
+        else if (sh.tpr == 64) NRN_CUDA_TRY((CALL<T, 64, 1>(a, s)));           \
+        else if (sh.tpr == 128) NRN_CUDA_TRY((CALL<T, 128, 1>(a, s)));         \
+        else if (sh.tpr == 256) NRN_CUDA_TRY((CALL<T, 256, 1>(a, s)));         \
+        else if (sh.tpr == 320) NRN_CUDA_TRY((CALL<T, 320, 1>(a, s)));         \
+        else if (sh.tpr == 1024) NRN_CUDA_TRY((CALL<T, 1024, 2>(a, s)));       \
+        else if (sh.vpt == 1) NRN_CUDA_TRY((CALL<T, 512, 1>(a, s)));           \
+        else NRN_CUDA_TRY((CALL<T, 512, 2>(a, s)));                            \
     } while (0)
 
 bool row_ok(const void* p, int64_t stride, int size) {
@@ -469,7 +595,6 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_forward(const nrn_gatednorm_t* in, nr
     if (in->dtype == NRN_BF16) NRN_NORM_SHAPES(__nv_bfloat16, run_forward);
     else if (in->dtype == NRN_FP16) NRN_NORM_SHAPES(__half, run_forward);
     else NRN_NORM_SHAPES(float, run_forward);
-    NRN_CUDA_TRY(cudaGetLastError());
     return NRN_OK;
 }
 
@@ -509,7 +634,6 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* in, c
     if (in->dtype == NRN_BF16) NRN_NORM_SHAPES(__nv_bfloat16, run_backward);
     else if (in->dtype == NRN_FP16) NRN_NORM_SHAPES(__half, run_backward);
     else NRN_NORM_SHAPES(float, run_backward);
-    NRN_CUDA_TRY(cudaGetLastError());
     if (sums) {
         norm_parts_kernel<<<dim3(static_cast<unsigned>((in->d + 31) / 32), 2), 1024, 0, s>>>(a.part, parts, in->d, in->alpha, in->w_post, g->dalpha, g->dw_post,
                                                                                           g->dw_pre);

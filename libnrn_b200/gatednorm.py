@@ -17,9 +17,10 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, Layouts, check_rows, check_vector, layout, on, ptr, require
+from ._tensors import DTYPE, Layouts, check_rows, check_vector, check_waits, error_flag, layout, on, ptr, require
 from .scaled import Scaled
 
+check = check_waits
 ACTIVATION = {"silu": 0, "sigmoid": 1}
 
 
@@ -69,7 +70,7 @@ def _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
     block, need = _layouts.get(key, residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz)
     a = N.GatedNorm.from_buffer_copy(block)
     a.residual, a.h, a.gate = residual.data_ptr(), ptr(h), ptr(gate)
-    a.alpha, a.w_post, a.w_pre = ptr(alpha), ptr(w_post), ptr(w_pre)
+    a.alpha, a.w_post, a.w_pre, a.err = ptr(alpha), ptr(w_post), ptr(w_pre), error_flag(residual.device)
     return a, need
 
 
