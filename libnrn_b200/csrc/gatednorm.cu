@@ -34,22 +34,37 @@ namespace {
 
 constexpr int kMaxD = 16384;
 
+struct RowArrays {                     // kernel arguments: read where they are used, not kept in registers
+    const void* from[5];
+    int64_t stride[5];
+    int64_t rows;
+    int32_t d, stages;
+    int32_t vec, pad;
+    int32_t* err;
+};
+
 struct NormArgs {
     nrn_gatednorm_t f;
+    RowArrays in;                      // residual, h, gate
     uint8_t* zv;
     float* zs;
     int64_t zv_stride, zs_row, zs_col;
-    int32_t vec;                       // every row starts on a 16-byte boundary
-    int32_t stages;                    // rows of the ring
 };
 
 struct GradArgs {
     nrn_gatednorm_t f;
     nrn_gatednorm_grad_t g;
+    RowArrays in;                      // residual, h, gate, dy, dz
     float* part;                       // [parts][2][d]: sums over rows
-    int32_t vec;
-    int32_t stages;
 };
+
+RowArrays row_arrays(const nrn_gatednorm_t& f, bool vec) {
+    RowArrays r{};
+    r.from[0] = f.residual, r.from[1] = f.h, r.from[2] = f.gate;
+    r.stride[0] = f.residual_stride, r.stride[1] = f.h_stride, r.stride[2] = f.gate_stride;
+    r.rows = f.rows, r.d = f.d, r.vec = vec, r.err = f.err;
+    return r;
+}
 
 __device__ __forceinline__ float sigmoid(float x) {
     float e, r;
@@ -104,7 +119,7 @@ constexpr int blocks_per_sm() {
     constexpr int regs = REGS * VPT * (TPR == 32 ? 128 : TPR);
     return 65536 / regs < 1 ? 1 : 65536 / regs;
 }
-constexpr int kForwardRegs = 64, kBackwardRegs = 102;
+constexpr int kForwardRegs = 64, kBackwardRegs = 80;
 
 // The rows a block reads, as a ring in shared memory filled by one thread's
 // bulk copies (RING), or straight from global memory.
@@ -112,17 +127,16 @@ constexpr int kMostStages = 4;
 constexpr int kRingHead = 128;
 enum { ERR_NORM_TIMEOUT = 5 };
 
-template <typename T, int TPR, int N, bool RING>
+template <typename T, int N, bool RING>
 struct Rows {
-    const T* from[N];
-    int64_t stride[N];
-    int64_t rows, step;
-    int32_t d, stages, stage;
+    const RowArrays& a;
+    int64_t step;
+    int32_t stage;
     uint32_t phase;
-    bool vec;
     uint64_t* bars;
     unsigned char* ring;
-    int* err;
+
+    __device__ __forceinline__ Rows(const RowArrays& arrays, int64_t step_) : a(arrays), step(step_) {}
 
     __device__ __forceinline__ void start(unsigned char* smem, int64_t row) {
         if constexpr (RING) {
@@ -131,49 +145,49 @@ struct Rows {
             stage = 0;
             phase = 0;
             if (threadIdx.x == 0) {
-                for (int i = 0; i < stages; ++i) tc::mbar_init(&bars[i], 1);
+                for (int i = 0; i < a.stages; ++i) tc::mbar_init(&bars[i], 1);
                 asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-                for (int i = 0; i < stages; ++i) fill(row + i * step, i);
+                for (int i = 0; i < a.stages; ++i) fill(row + i * step, i);
             }
             __syncthreads();
         }
     }
     __device__ __forceinline__ void fill(int64_t row, int st) {
-        if (row >= rows) return;
-        const uint32_t bytes = static_cast<uint32_t>(d * sizeof(T));
+        if (row >= a.rows) return;
+        const uint32_t bytes = static_cast<uint32_t>(a.d * sizeof(T));
         uint32_t all = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) all += from[i] ? bytes : 0u;
+        for (int i = 0; i < N; ++i) all += a.from[i] ? bytes : 0u;
         tc::mbar_expect_tx(&bars[st], all);
         const uint64_t once = tc::policy_evict_first();
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (from[i]) tc::bulk_load(ring + (st * N + i) * static_cast<size_t>(bytes), from[i] + row * stride[i], bytes, &bars[st], once);
+            if (a.from[i]) tc::bulk_load(ring + (st * N + i) * static_cast<size_t>(bytes), static_cast<const T*>(a.from[i]) + row * a.stride[i], bytes, &bars[st], once);
     }
     // this row is in shared memory
     __device__ __forceinline__ void wait() {
         if constexpr (RING) {
-            if (!tc::mbar_wait(&bars[stage], phase, nullptr) && err) atomicCAS(err, 0, ERR_NORM_TIMEOUT);
+            if (!tc::mbar_wait(&bars[stage], phase, nullptr) && a.err) atomicCAS(a.err, 0, ERR_NORM_TIMEOUT);
         }
     }
     __device__ __forceinline__ Raw8<T> get(int i, int64_t row, int c) const {
         if constexpr (RING) {
-            const uint4* s = reinterpret_cast<const uint4*>(ring + (stage * N + i) * (d * sizeof(T)) + (c < d ? c : 0) * sizeof(T));
+            const uint4* s = reinterpret_cast<const uint4*>(ring + (stage * N + i) * (a.d * sizeof(T)) + (c < a.d ? c : 0) * sizeof(T));
             Raw8<T> r;
             uint4* t = reinterpret_cast<uint4*>(&r);
 #pragma unroll
-            for (int k = 0; k < static_cast<int>(sizeof(r) / 16); ++k) t[k] = c < d ? s[k] : make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < static_cast<int>(sizeof(r) / 16); ++k) t[k] = c < a.d ? s[k] : make_uint4(0, 0, 0, 0);
             return r;
         } else {
-            const int n = d - c;
-            return load8(from[i] + row * stride[i] + (n > 0 ? c : 0), n, vec);
+            const int n = a.d - c;
+            return load8(static_cast<const T*>(a.from[i]) + row * a.stride[i] + (n > 0 ? c : 0), n, a.vec != 0);
         }
     }
     // every thread of the block has what it needs of this row
     __device__ __forceinline__ void done(int64_t row) {
         if constexpr (RING) {
-            if (threadIdx.x == 0) fill(row + stages * step, stage);
-            if (++stage == stages) {
+            if (threadIdx.x == 0) fill(row + a.stages * step, stage);
+            if (++stage == a.stages) {
                 stage = 0;
                 phase ^= 1u;
             }
@@ -193,11 +207,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
     const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 4 : 1);
     int64_t row = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= f.rows) return;
-    const bool vec = a.vec != 0, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
-    Rows<T, TPR, 3, RING> in;
-    in.from[0] = static_cast<const T*>(f.residual), in.from[1] = static_cast<const T*>(f.h), in.from[2] = static_cast<const T*>(f.gate);
-    in.stride[0] = f.residual_stride, in.stride[1] = f.h_stride, in.stride[2] = f.gate_stride;
-    in.rows = f.rows, in.step = step, in.d = f.d, in.stages = a.stages, in.vec = vec, in.err = f.err;
+    const bool vec = a.in.vec != 0, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
+    Rows<T, 3, RING> in(a.in, step);
     in.start(smem, row);
     const float inv_d = 1.0f / static_cast<float>(f.d);
     int turn = 0;
@@ -284,7 +295,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
 #pragma unroll
             for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));   // 16 lanes: 128 columns
             if (n <= 0) continue;
-            const float sc = block_scale(m), q = 1.0f / sc;
+            const float sc = block_scale(m), q = __frcp_rn(sc);
             if ((tid & 15) == 0) a.zs[row * a.zs_row + (c / 128) * a.zs_col] = sc;
             *reinterpret_cast<uint2*>(a.zv + row * a.zv_stride + c) =
                 make_uint2(e4m3x4(y[v][0] * q, y[v][1] * q, y[v][2] * q, y[v][3] * q),
@@ -300,7 +311,11 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
 //     s2 = sum over rows of dz yh = dw_pre
 // y is computed again from h, gate and r: reading it would cost a fifth of
 // the reads and its rounding.  Blocks take rows in turn and keep their part of
-// the two sums in registers; a second kernel adds the parts.
+// the two sums in registers; a second kernel adds the parts.  What a row
+// gives is read again from the ring by each of the four passes over it, and
+// the gate's sigmoid computed twice: kept in registers they would leave room
+// for half the threads, and spilled they cost more than the rest (d 1024:
+// 191 us with 48 bytes spilled a thread, 85 us without).
 template <typename T, int TPR, int VPT, bool RING>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT, kBackwardRegs>())
     norm_grad_kernel(const __grid_constant__ GradArgs a) {
@@ -311,74 +326,81 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
     const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
     const int slot = TPR == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 4 : 1);
-    const bool vec = a.vec != 0, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
+    const bool vec = a.in.vec != 0, block = f.h != nullptr, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
     const float inv_d = 1.0f / static_cast<float>(f.d);
     int turn = 0;
-    float s1[VPT][8], s2[VPT][8], aw[VPT][8], wp[VPT][8];
+    float s1[VPT][8], s2[VPT][8];
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s1[v][e] = s2[v][e] = 0.0f;
+    // a column's factors: in registers while there is room for them
+    constexpr bool kKeep = VPT <= 2;
+    float kaw[kKeep ? VPT : 1][8], kwp[kKeep ? VPT : 1][8];
+    auto factors = [&](int v, float* aw, float* wp) {
         const int c = (tid + v * TPR) * 8, n = f.d - c;
         float al[8];
-        load_param(f.w_post, n > 0 ? c : 0, n, aw[v]);
+        load_param(f.w_post, n > 0 ? c : 0, n, aw);
         load_param(f.alpha, n > 0 ? c : 0, n, al);
-        load_param(f.w_pre, n > 0 ? c : 0, n, wp[v]);
+        load_param(f.w_pre, n > 0 ? c : 0, n, wp);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            aw[v][e] *= al[e];
-            s1[v][e] = s2[v][e] = 0.0f;
-        }
-    }
-    Rows<T, TPR, 5, RING> in;
-    in.from[0] = static_cast<const T*>(f.residual), in.from[1] = static_cast<const T*>(f.h), in.from[2] = static_cast<const T*>(f.gate);
-    in.from[3] = static_cast<const T*>(g.dy), in.from[4] = static_cast<const T*>(g.dz);
-    in.stride[0] = f.residual_stride, in.stride[1] = f.h_stride, in.stride[2] = f.gate_stride;
-    in.stride[3] = g.dy_stride, in.stride[4] = g.dz_stride;
-    in.rows = f.rows, in.step = step, in.d = f.d, in.stages = a.stages, in.vec = vec, in.err = f.err;
+        for (int e = 0; e < 8; ++e) aw[e] *= al[e];
+    };
+    if constexpr (kKeep)
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) factors(v, kaw[v], kwp[v]);
+    Rows<T, 5, RING> in(a.in, step);
     in.start(smem, slot);
     for (int64_t row = slot; row < f.rows; row += step) {
-        Raw8<T> rr[VPT], rg[VPT], ry[VPT], rz[VPT];
-        float hh[VPT][8], y[VPT][8], act[VPT][8], dact[VPT][8], inv_h = 0.0f;
         in.wait();
-        float sh[1] = {0.0f};
+        float y[VPT][8], inv_h = 0.0f;
+        if (block) {
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const Raw8<T> h = in.get(1, row, (tid + v * TPR) * 8);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = to_f32(h.e[e]);
+                    s[0] = fmaf(x, x, s[0]);
+                }
+            }
+            row_sum<1, TPR>(s, red, turn);
+            inv_h = rsqrtf(fmaf(s[0], inv_d, f.eps));
+        }
+        float sy[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = (tid + v * TPR) * 8;
-            if (f.h) {
+            float taw[8], twp[8];
+            if constexpr (!kKeep) factors(v, taw, twp);
+            const float *aw = kKeep ? kaw[kKeep ? v : 0] : taw, *wp = kKeep ? kwp[kKeep ? v : 0] : twp;
+            const Raw8<T> r = in.get(0, row, c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[v][e] = to_f32(r.e[e]);
+            if (block) {
                 const Raw8<T> h = in.get(1, row, c);
+                if (gated) {
+                    const Raw8<T> gate = in.get(2, row, c);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float t = to_f32(gate.e[e]), sg = sigmoid(t);
+                        y[v][e] = fmaf(to_f32(h.e[e]) * inv_h * aw[e], silu ? t * sg : sg, y[v][e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[v][e] = fmaf(to_f32(h.e[e]) * inv_h, aw[e], y[v][e]);
+                }
+            }
+            if (g.dz) {
+                const Raw8<T> dz = in.get(4, row, c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    hh[v][e] = to_f32(h.e[e]);
-                    sh[0] = fmaf(hh[v][e], hh[v][e], sh[0]);
+                    sy[0] = fmaf(y[v][e], y[v][e], sy[0]);
+                    sy[1] = fmaf(to_f32(dz.e[e]) * wp[e], y[v][e], sy[1]);
                 }
             }
-            rr[v] = in.get(0, row, c);
-            if (gated) rg[v] = in.get(2, row, c);
-            if (g.dy) ry[v] = in.get(3, row, c);
-            if (g.dz) rz[v] = in.get(4, row, c);
         }
-        row_sum<1, TPR>(sh, red, turn);
-        in.done(row);
-        inv_h = rsqrtf(fmaf(sh[0], inv_d, f.eps));
-        float sy[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int v = 0; v < VPT; ++v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                y[v][e] = to_f32(rr[v].e[e]);
-                if (f.h) {
-                    hh[v][e] *= inv_h;
-                    act[v][e] = 1.0f;
-                    dact[v][e] = 0.0f;
-                    if (gated) {
-                        const float t = to_f32(rg[v].e[e]), sg = sigmoid(t), ts = t * sg;
-                        act[v][e] = silu ? ts : sg;
-                        dact[v][e] = silu ? fmaf(ts, 1.0f - sg, sg) : sg * (1.0f - sg);
-                    }
-                    y[v][e] = fmaf(hh[v][e] * aw[v][e], act[v][e], y[v][e]);
-                }
-                sy[0] = fmaf(y[v][e], y[v][e], sy[0]);
-                if (g.dz) sy[1] = fmaf(to_f32(rz[v].e[e]) * wp[v][e], y[v][e], sy[1]);
-            }
         float inv_y = 0.0f, my = 0.0f;
         if (g.dz) {
             row_sum<2, TPR>(sy, red, turn);
@@ -389,40 +411,65 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = (tid + v * TPR) * 8, n = f.d - c;
-            float d[8];
+            float taw[8], twp[8], d[8];
+            if constexpr (!kKeep) factors(v, taw, twp);
+            const float *aw = kKeep ? kaw[kKeep ? v : 0] : taw, *wp = kKeep ? kwp[kKeep ? v : 0] : twp;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                d[e] = g.dy ? to_f32(ry[v].e[e]) : 0.0f;
-                if (g.dz) {
-                    const float z = to_f32(rz[v].e[e]);
+            for (int e = 0; e < 8; ++e) d[e] = 0.0f;
+            if (g.dy) {
+                const Raw8<T> dy = in.get(3, row, c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] = to_f32(dy.e[e]);
+            }
+            if (g.dz) {
+                const Raw8<T> dz = in.get(4, row, c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float z = to_f32(dz.e[e]);
                     s2[v][e] = fmaf(z, y[v][e] * inv_y, s2[v][e]);
-                    d[e] = fmaf(inv_y, z * wp[v][e] - y[v][e] * my, d[e]);
+                    d[e] = fmaf(inv_y, z * wp[e] - y[v][e] * my, d[e]);
                 }
             }
             if (n > 0 && g.dresidual) store8(static_cast<T*>(g.dresidual) + row * g.dresidual_stride + c, d, n, vec);
-            if (f.h) {
+            if (!block) continue;
+            const Raw8<T> h = in.get(1, row, c);
+            if (gated) {
+                const Raw8<T> gate = in.get(2, row, c);
+                float dg[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    s1[v][e] = fmaf(d[e] * act[v][e], hh[v][e], s1[v][e]);
-                    const float da = d[e] * aw[v][e];
-                    dact[v][e] *= da * hh[v][e];
-                    y[v][e] = da * act[v][e];
-                    st[0] = fmaf(y[v][e], hh[v][e], st[0]);
+                    const float hh = to_f32(h.e[e]) * inv_h, t = to_f32(gate.e[e]), sg = sigmoid(t), ts = t * sg, da = d[e] * aw[e];
+                    const float act = silu ? ts : sg, dact = silu ? fmaf(ts, 1.0f - sg, sg) : sg * (1.0f - sg);
+                    s1[v][e] = fmaf(d[e] * act, hh, s1[v][e]);
+                    dg[e] = da * hh * dact;
+                    y[v][e] = da * act;
+                    st[0] = fmaf(y[v][e], hh, st[0]);
                 }
-                if (n > 0 && g.dgate && gated) store8(static_cast<T*>(g.dgate) + row * g.dgate_stride + c, dact[v], n, vec);
+                if (n > 0 && g.dgate) store8(static_cast<T*>(g.dgate) + row * g.dgate_stride + c, dg, n, vec);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float hh = to_f32(h.e[e]) * inv_h;
+                    s1[v][e] = fmaf(d[e], hh, s1[v][e]);
+                    y[v][e] = d[e] * aw[e];
+                    st[0] = fmaf(y[v][e], hh, st[0]);
+                }
             }
         }
-        if (f.h && g.dh) {
+        if (block) {
             row_sum<1, TPR>(st, red, turn);
-            const float mh = st[0] * inv_d;
+            const float mh = st[0] * inv_d * inv_h;
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 const int c = (tid + v * TPR) * 8, n = f.d - c;
+                const Raw8<T> h = in.get(1, row, c);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[v][e] = inv_h * (y[v][e] - hh[v][e] * mh);
-                if (n > 0) store8(static_cast<T*>(g.dh) + row * g.dh_stride + c, y[v], n, vec);
+                for (int e = 0; e < 8; ++e) y[v][e] = inv_h * (y[v][e] - to_f32(h.e[e]) * mh);
+                if (n > 0 && g.dh) store8(static_cast<T*>(g.dh) + row * g.dh_stride + c, y[v], n, vec);
             }
         }
+        if constexpr (RING) __syncthreads();             // the row is read: its place may be filled again
+        in.done(row);
     }
     if (a.part == nullptr) return;
     float* at = a.part + static_cast<int64_t>(slot) * 2 * f.d;
@@ -471,7 +518,7 @@ Shape shape_of(int d) {
     if (vecs <= 320) return {320, 1};
     if (vecs <= 512) return {512, 1};
     if (vecs <= 1024) return {512, 2};
-    return {1024, 2};
+    return {512, 4};
 }
 
 // Blocks that take the rows in turn: as many as are on the GPU at once.
@@ -494,10 +541,10 @@ template <typename T, int TPR, int VPT>
 cudaError_t run_forward(NormArgs a, cudaStream_t s) {
     constexpr int threads = TPR == 32 ? 128 : TPR;
     const unsigned blocks = blocks_for<TPR, VPT, kForwardRegs>(a.f.rows);
-    a.stages = ring_stages<T, TPR, VPT, kForwardRegs>(3, a.f.d, a.vec != 0);
+    a.in.stages = ring_stages<T, TPR, VPT, kForwardRegs>(3, a.f.d, a.in.vec != 0);
     if constexpr (TPR > 32) {
-        if (a.stages) {
-            const int bytes = kRingHead + a.stages * 3 * a.f.d * static_cast<int>(sizeof(T));
+        if (a.in.stages) {
+            const int bytes = kRingHead + a.in.stages * 3 * a.f.d * static_cast<int>(sizeof(T));
             const cudaError_t e = cudaFuncSetAttribute(norm_kernel<T, TPR, VPT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
             if (e != cudaSuccess) return e;
             norm_kernel<T, TPR, VPT, true><<<blocks, threads, bytes, s>>>(a);
@@ -512,10 +559,10 @@ template <typename T, int TPR, int VPT>
 cudaError_t run_backward(GradArgs a, cudaStream_t s) {
     constexpr int threads = TPR == 32 ? 128 : TPR;
     const unsigned blocks = blocks_for<TPR, VPT, kBackwardRegs>(a.f.rows);
-    a.stages = ring_stages<T, TPR, VPT, kBackwardRegs>(5, a.f.d, a.vec != 0);
+    a.in.stages = ring_stages<T, TPR, VPT, kBackwardRegs>(5, a.f.d, a.in.vec != 0);
     if constexpr (TPR > 32) {
-        if (a.stages) {
-            const int bytes = kRingHead + a.stages * 5 * a.f.d * static_cast<int>(sizeof(T));
+        if (a.in.stages) {
+            const int bytes = kRingHead + a.in.stages * 5 * a.f.d * static_cast<int>(sizeof(T));
             const cudaError_t e = cudaFuncSetAttribute(norm_grad_kernel<T, TPR, VPT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
             if (e != cudaSuccess) return e;
             norm_grad_kernel<T, TPR, VPT, true><<<blocks, threads, bytes, s>>>(a);
@@ -533,8 +580,8 @@ int grad_parts(int64_t rows, int tpr, int vpt) {
     if (tpr == 128) return static_cast<int>(blocks_for<128, 1, kBackwardRegs>(rows));
     if (tpr == 256) return static_cast<int>(blocks_for<256, 1, kBackwardRegs>(rows));
     if (tpr == 320) return static_cast<int>(blocks_for<320, 1, kBackwardRegs>(rows));
-    if (tpr == 1024) return static_cast<int>(blocks_for<1024, 2, kBackwardRegs>(rows));
-    return static_cast<int>(vpt == 1 ? blocks_for<512, 1, kBackwardRegs>(rows) : blocks_for<512, 2, kBackwardRegs>(rows));
+    if (vpt == 1) return static_cast<int>(blocks_for<512, 1, kBackwardRegs>(rows));
+    return static_cast<int>(vpt == 2 ? blocks_for<512, 2, kBackwardRegs>(rows) : blocks_for<512, 4, kBackwardRegs>(rows));
 }
 
 #define NRN_NORM_SHAPES(T, CALL)                                               \
@@ -545,9 +592,9 @@ int grad_parts(int64_t rows, int tpr, int vpt) {
         else if (sh.tpr == 128) NRN_CUDA_TRY((CALL<T, 128, 1>(a, s)));         \
         else if (sh.tpr == 256) NRN_CUDA_TRY((CALL<T, 256, 1>(a, s)));         \
         else if (sh.tpr == 320) NRN_CUDA_TRY((CALL<T, 320, 1>(a, s)));         \
-        else if (sh.tpr == 1024) NRN_CUDA_TRY((CALL<T, 1024, 2>(a, s)));       \
         else if (sh.vpt == 1) NRN_CUDA_TRY((CALL<T, 512, 1>(a, s)));           \
-        else NRN_CUDA_TRY((CALL<T, 512, 2>(a, s)));                            \
+        else if (sh.vpt == 2) NRN_CUDA_TRY((CALL<T, 512, 2>(a, s)));           \
+        else NRN_CUDA_TRY((CALL<T, 512, 4>(a, s)));                            \
     } while (0)
 
 bool row_ok(const void* p, int64_t stride, int size) {
@@ -589,8 +636,8 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_forward(const nrn_gatednorm_t* in, nr
         a.zs_row = q->scale_stride[0], a.zs_col = q->scale_stride[1];
     }
     if (in->rows == 0 || (!in->y && !in->z && !a.zv)) return NRN_OK;
-    a.vec = row_ok(in->residual, in->residual_stride, size) && row_ok(in->h, in->h_stride, size) &&
-            row_ok(in->gate, in->gate_stride, size) && row_ok(in->y, in->y_stride, size) && row_ok(in->z, in->z_stride, size);
+    a.in = row_arrays(*in, row_ok(in->residual, in->residual_stride, size) && row_ok(in->h, in->h_stride, size) &&
+                               row_ok(in->gate, in->gate_stride, size) && row_ok(in->y, in->y_stride, size) && row_ok(in->z, in->z_stride, size));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (in->dtype == NRN_BF16) NRN_NORM_SHAPES(__nv_bfloat16, run_forward);
     else if (in->dtype == NRN_FP16) NRN_NORM_SHAPES(__half, run_forward);
@@ -628,9 +675,11 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* in, c
         NRN_CHECK_ARG(g->workspace && g->workspace_bytes >= static_cast<int64_t>(parts) * 2 * in->d * 4, who + ": workspace too small");
         a.part = static_cast<float*>(g->workspace);
     }
-    a.vec = row_ok(in->residual, in->residual_stride, size) && row_ok(in->h, in->h_stride, size) &&
-            row_ok(in->gate, in->gate_stride, size) && row_ok(g->dy, g->dy_stride, size) && row_ok(g->dz, g->dz_stride, size) &&
-            row_ok(g->dresidual, g->dresidual_stride, size) && row_ok(g->dh, g->dh_stride, size) && row_ok(g->dgate, g->dgate_stride, size);
+    a.in = row_arrays(*in, row_ok(in->residual, in->residual_stride, size) && row_ok(in->h, in->h_stride, size) &&
+                               row_ok(in->gate, in->gate_stride, size) && row_ok(g->dy, g->dy_stride, size) && row_ok(g->dz, g->dz_stride, size) &&
+                               row_ok(g->dresidual, g->dresidual_stride, size) && row_ok(g->dh, g->dh_stride, size) && row_ok(g->dgate, g->dgate_stride, size));
+    a.in.from[3] = g->dy, a.in.from[4] = g->dz;
+    a.in.stride[3] = g->dy_stride, a.in.stride[4] = g->dz_stride;
     if (in->dtype == NRN_BF16) NRN_NORM_SHAPES(__nv_bfloat16, run_backward);
     else if (in->dtype == NRN_FP16) NRN_NORM_SHAPES(__half, run_backward);
     else NRN_NORM_SHAPES(float, run_backward);

@@ -50,16 +50,29 @@ __device__ __forceinline__ Raw8<T> load8(const T* p, int n, bool vec) {
     return r;
 }
 
+// Two results as one word (16-bit types), the first in the low half.
+__device__ __forceinline__ uint32_t pack2_f32(__nv_bfloat16, float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2_f32(__half, float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* x, int n, bool vec) {
     if (vec && n >= 8) {
-        Raw8<T> r;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.e[i] = from_f32<T>(x[i]);
-        const uint4* s = reinterpret_cast<const uint4*>(&r);
         uint4* d = reinterpret_cast<uint4*>(p);
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = s[i];
+        if constexpr (sizeof(T) == 2) {
+            const T k{};
+            d[0] = make_uint4(pack2_f32(k, x[0], x[1]), pack2_f32(k, x[2], x[3]), pack2_f32(k, x[4], x[5]), pack2_f32(k, x[6], x[7]));
+        } else {
+            d[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+            d[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
