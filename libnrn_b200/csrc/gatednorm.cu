@@ -116,7 +116,7 @@ __device__ __forceinline__ void load_param(const float* p, int c, int n, float* 
 // Blocks of one SM that the kernels' registers leave room for.
 template <int TPR, int VPT, int REGS>
 constexpr int blocks_per_sm() {
-    constexpr int regs = REGS * VPT * (TPR == 32 ? 128 : TPR);
+    constexpr int regs = (VPT == 1 ? REGS : 64 * VPT) * (TPR == 32 ? 128 : TPR);
     return 65536 / regs < 1 ? 1 : 65536 / regs;
 }
 constexpr int kForwardRegs = 64, kBackwardRegs = 80;
@@ -509,14 +509,14 @@ __global__ void __launch_bounds__(1024) norm_parts_kernel(const float* part, int
 struct Shape {
     int tpr, vpt;
 };
-Shape shape_of(int d) {
+Shape shape_of(int d, bool backward) {
     const int vecs = (d + 7) / 8;
     if (vecs <= 32) return {32, 1};
     if (vecs <= 64) return {64, 1};
-    if (vecs <= 128) return {128, 1};
-    if (vecs <= 256) return {256, 1};
-    if (vecs <= 320) return {320, 1};
-    if (vecs <= 512) return {512, 1};
+    if (vecs <= 128) return backward ? Shape{128, 1} : Shape{64, 2};
+    if (vecs <= 256) return backward ? Shape{256, 1} : Shape{128, 2};
+    if (vecs <= 320) return backward ? Shape{320, 1} : Shape{160, 2};
+    if (vecs <= 512) return {256, 2};
     if (vecs <= 1024) return {512, 2};
     return {512, 4};
 }
@@ -574,28 +574,43 @@ cudaError_t run_backward(GradArgs a, cudaStream_t s) {
 }
 
 // Parts of the sums over rows that the backward kernel leaves: one for each block, or warp where a warp has a row.
-int grad_parts(int64_t rows, int tpr, int vpt) {
-    if (tpr == 32) return 4 * static_cast<int>(blocks_for<32, 1, kBackwardRegs>(rows));
-    if (tpr == 64) return static_cast<int>(blocks_for<64, 1, kBackwardRegs>(rows));
-    if (tpr == 128) return static_cast<int>(blocks_for<128, 1, kBackwardRegs>(rows));
-    if (tpr == 256) return static_cast<int>(blocks_for<256, 1, kBackwardRegs>(rows));
-    if (tpr == 320) return static_cast<int>(blocks_for<320, 1, kBackwardRegs>(rows));
-    if (vpt == 1) return static_cast<int>(blocks_for<512, 1, kBackwardRegs>(rows));
-    return static_cast<int>(vpt == 2 ? blocks_for<512, 2, kBackwardRegs>(rows) : blocks_for<512, 4, kBackwardRegs>(rows));
+int grad_parts(int64_t rows, int d) {
+    const Shape sh = shape_of(d, true);
+    switch (sh.tpr) {
+        case 32: return 4 * static_cast<int>(blocks_for<32, 1, kBackwardRegs>(rows));
+        case 64: return static_cast<int>(blocks_for<64, 1, kBackwardRegs>(rows));
+        case 128: return static_cast<int>(blocks_for<128, 1, kBackwardRegs>(rows));
+        case 256: return static_cast<int>(sh.vpt == 1 ? blocks_for<256, 1, kBackwardRegs>(rows) : blocks_for<256, 2, kBackwardRegs>(rows));
+        case 320: return static_cast<int>(blocks_for<320, 1, kBackwardRegs>(rows));
+        default: return static_cast<int>(sh.vpt == 2 ? blocks_for<512, 2, kBackwardRegs>(rows) : blocks_for<512, 4, kBackwardRegs>(rows));
+    }
 }
 
-#define NRN_NORM_SHAPES(T, CALL)                                               \
-    do {                                                                       \
-        const Shape sh = shape_of(a.f.d);                                      \
-        if (sh.tpr == 32) NRN_CUDA_TRY((CALL<T, 32, 1>(a, s)));                \
-        else if (sh.tpr == 64) NRN_CUDA_TRY((CALL<T, 64, 1>(a, s)));           \
-        else if (sh.tpr == 128) NRN_CUDA_TRY((CALL<T, 128, 1>(a, s)));         \
-        else if (sh.tpr == 256) NRN_CUDA_TRY((CALL<T, 256, 1>(a, s)));         \
-        else if (sh.tpr == 320) NRN_CUDA_TRY((CALL<T, 320, 1>(a, s)));         \
-        else if (sh.vpt == 1) NRN_CUDA_TRY((CALL<T, 512, 1>(a, s)));           \
-        else if (sh.vpt == 2) NRN_CUDA_TRY((CALL<T, 512, 2>(a, s)));           \
-        else NRN_CUDA_TRY((CALL<T, 512, 4>(a, s)));                            \
-    } while (0)
+template <typename T>
+cudaError_t forward_any(const NormArgs& a, cudaStream_t s) {
+    const Shape sh = shape_of(a.f.d, false);
+    switch (sh.tpr) {
+        case 32: return run_forward<T, 32, 1>(a, s);
+        case 64: return sh.vpt == 1 ? run_forward<T, 64, 1>(a, s) : run_forward<T, 64, 2>(a, s);
+        case 128: return run_forward<T, 128, 2>(a, s);
+        case 160: return run_forward<T, 160, 2>(a, s);
+        case 256: return run_forward<T, 256, 2>(a, s);
+        default: return sh.vpt == 2 ? run_forward<T, 512, 2>(a, s) : run_forward<T, 512, 4>(a, s);
+    }
+}
+
+template <typename T>
+cudaError_t backward_any(const GradArgs& a, cudaStream_t s) {
+    const Shape sh = shape_of(a.f.d, true);
+    switch (sh.tpr) {
+        case 32: return run_backward<T, 32, 1>(a, s);
+        case 64: return run_backward<T, 64, 1>(a, s);
+        case 128: return run_backward<T, 128, 1>(a, s);
+        case 256: return sh.vpt == 1 ? run_backward<T, 256, 1>(a, s) : run_backward<T, 256, 2>(a, s);
+        case 320: return run_backward<T, 320, 1>(a, s);
+        default: return sh.vpt == 2 ? run_backward<T, 512, 2>(a, s) : run_backward<T, 512, 4>(a, s);
+    }
+}
 
 bool row_ok(const void* p, int64_t stride, int size) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0);
@@ -639,17 +654,16 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_forward(const nrn_gatednorm_t* in, nr
     a.in = row_arrays(*in, row_ok(in->residual, in->residual_stride, size) && row_ok(in->h, in->h_stride, size) &&
                                row_ok(in->gate, in->gate_stride, size) && row_ok(in->y, in->y_stride, size) && row_ok(in->z, in->z_stride, size));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (in->dtype == NRN_BF16) NRN_NORM_SHAPES(__nv_bfloat16, run_forward);
-    else if (in->dtype == NRN_FP16) NRN_NORM_SHAPES(__half, run_forward);
-    else NRN_NORM_SHAPES(float, run_forward);
+    if (in->dtype == NRN_BF16) NRN_CUDA_TRY(forward_any<__nv_bfloat16>(a, s));
+    else if (in->dtype == NRN_FP16) NRN_CUDA_TRY(forward_any<__half>(a, s));
+    else NRN_CUDA_TRY(forward_any<float>(a, s));
     return NRN_OK;
 }
 
 extern "C" nrn_status_t nrn_cuda_gatednorm_workspace(const nrn_gatednorm_t* a, int64_t* bytes) {
     NRN_CHECK_ARG(a && bytes, "nrn_cuda_gatednorm_workspace: null argument");
     NRN_CHECK_ARG(a->rows >= 0 && a->d >= 1 && a->d <= kMaxD, "nrn_cuda_gatednorm_workspace: sizes out of range");
-    const Shape sh = shape_of(a->d);
-    *bytes = static_cast<int64_t>(grad_parts(a->rows, sh.tpr, sh.vpt)) * 2 * a->d * 4;
+    *bytes = static_cast<int64_t>(grad_parts(a->rows, a->d)) * 2 * a->d * 4;
     return NRN_OK;
 }
 
@@ -669,8 +683,7 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* in, c
     a.f = *in;
     a.g = *g;
     const int size = in->dtype == NRN_FP32 ? 4 : 2;
-    const Shape sh = shape_of(in->d);
-    const int parts = grad_parts(in->rows, sh.tpr, sh.vpt);
+    const int parts = grad_parts(in->rows, in->d);
     if (sums) {
         NRN_CHECK_ARG(g->workspace && g->workspace_bytes >= static_cast<int64_t>(parts) * 2 * in->d * 4, who + ": workspace too small");
         a.part = static_cast<float*>(g->workspace);
@@ -680,9 +693,9 @@ extern "C" nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* in, c
                                row_ok(g->dresidual, g->dresidual_stride, size) && row_ok(g->dh, g->dh_stride, size) && row_ok(g->dgate, g->dgate_stride, size));
     a.in.from[3] = g->dy, a.in.from[4] = g->dz;
     a.in.stride[3] = g->dy_stride, a.in.stride[4] = g->dz_stride;
-    if (in->dtype == NRN_BF16) NRN_NORM_SHAPES(__nv_bfloat16, run_backward);
-    else if (in->dtype == NRN_FP16) NRN_NORM_SHAPES(__half, run_backward);
-    else NRN_NORM_SHAPES(float, run_backward);
+    if (in->dtype == NRN_BF16) NRN_CUDA_TRY(backward_any<__nv_bfloat16>(a, s));
+    else if (in->dtype == NRN_FP16) NRN_CUDA_TRY(backward_any<__half>(a, s));
+    else NRN_CUDA_TRY(backward_any<float>(a, s));
     if (sums) {
         norm_parts_kernel<<<dim3(static_cast<unsigned>((in->d + 31) / 32), 2), 1024, 0, s>>>(a.part, parts, in->d, in->alpha, in->w_post, g->dalpha, g->dw_post,
                                                                                           g->dw_pre);
