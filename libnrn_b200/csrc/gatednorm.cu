@@ -73,15 +73,15 @@ __device__ __forceinline__ float sigmoid(float x) {
     return r;
 }
 
-// N sums over the threads of a row; every thread gets them.  Rows of one
-// warp need no barrier; else `red` is [2][N][32] floats used in turn.
-template <int N, int TPR>
+// N sums over the threads of a row; every thread gets them.  A row of one
+// warp needs no barrier; else `red` is [2][N][32] floats used in turn.
+template <int N, bool WARP>
 __device__ __forceinline__ void row_sum(float (&x)[N], float* red, int& turn) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
-    if constexpr (TPR > 32) {
+    if constexpr (!WARP) {
         float* at = red + (turn & 1) * 64;
         ++turn;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -91,10 +91,10 @@ __device__ __forceinline__ void row_sum(float (&x)[N], float* red, int& turn) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            float s = lane < TPR / 32 ? at[i * 32 + lane] : 0.0f;
+            float s = lane < static_cast<int>(blockDim.x >> 5) ? at[i * 32 + lane] : 0.0f;
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            x[i] = s;
+            for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);   // at most 16 warps
+            x[i] = __shfl_sync(0xffffffffu, s, 0);
         }
     }
 }
@@ -113,13 +113,12 @@ __device__ __forceinline__ void load_param(const float* p, int c, int n, float* 
     }
 }
 
-// Blocks of one SM that the kernels' registers leave room for.
-template <int TPR, int VPT, int REGS>
-constexpr int blocks_per_sm() {
-    constexpr int regs = (VPT == 1 ? REGS : 64 * VPT) * (TPR == 32 ? 128 : TPR);
-    return 65536 / regs < 1 ? 1 : 65536 / regs;
+// Threads of a block, at most: 128 with a row for each warp, else 512 (128
+// registers a thread; 64 where it has eight elements).
+template <bool WARP>
+constexpr int most_threads() {
+    return WARP ? 128 : 512;
 }
-constexpr int kForwardRegs = 64, kBackwardRegs = 80;
 
 // The rows a block reads, as a ring in shared memory filled by one thread's
 // bulk copies (RING), or straight from global memory.
@@ -195,17 +194,17 @@ struct Rows {
     }
 };
 
-// TPR threads a row, VPT vectors of eight a thread.  Elements past the row's
+// A warp or a block a row, VPT vectors of eight a thread.  Elements past the row's
 // end are loaded as 0 and stay 0: they add nothing to the sums.
-template <typename T, int TPR, int VPT, bool RING>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT, kForwardRegs>())
+template <typename T, bool WARP, int VPT, bool RING>
+__global__ void __launch_bounds__(most_threads<WARP>(), WARP ? 8 / VPT : 1)
     norm_kernel(const __grid_constant__ NormArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float red[128];
     const nrn_gatednorm_t& f = a.f;
-    const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 4 : 1);
-    int64_t row = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    const int tpr = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? 4 : 1);
+    int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= f.rows) return;
     const bool vec = a.in.vec != 0, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
     Rows<T, 3, RING> in(a.in, step);
@@ -215,7 +214,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
     float aw[VPT][8], wp[VPT][8];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-        const int c = (tid + v * TPR) * 8, n = f.d - c;
+        const int c = (tid + v * tpr) * 8, n = f.d - c;
         float al[8];
         load_param(f.w_post, n > 0 ? c : 0, n, aw[v]);
         load_param(f.alpha, n > 0 ? c : 0, n, al);
@@ -232,7 +231,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
             float s[1] = {0.0f};
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const int c = (tid + v * TPR) * 8;
+                const int c = (tid + v * tpr) * 8;
                 const Raw8<T> h = in.get(1, row, c);
                 r[v] = in.get(0, row, c);
                 if (gated) gate[v] = in.get(2, row, c);
@@ -242,7 +241,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
                     s[0] = fmaf(y[v][e], y[v][e], s[0]);
                 }
             }
-            row_sum<1, TPR>(s, red, turn);
+            row_sum<1, WARP>(s, red, turn);
             in.done(row);
             const float inv = rsqrtf(fmaf(s[0], inv_d, f.eps));
 #pragma unroll
@@ -259,7 +258,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
             if (f.y) {
 #pragma unroll
                 for (int v = 0; v < VPT; ++v) {
-                    const int c = (tid + v * TPR) * 8, n = f.d - c;
+                    const int c = (tid + v * tpr) * 8, n = f.d - c;
                     if (n > 0) store8(static_cast<T*>(f.y) + row * f.y_stride + c, y[v], n, vec);
                 }
             }
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
         } else {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const Raw8<T> r = in.get(0, row, (tid + v * TPR) * 8);
+                const Raw8<T> r = in.get(0, row, (tid + v * tpr) * 8);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[v][e] = to_f32(r.e[e]);
             }
@@ -277,25 +276,26 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[0] = fmaf(y[v][e], y[v][e], s[0]);
-        row_sum<1, TPR>(s, red, turn);
+        row_sum<1, WARP>(s, red, turn);
         if (!f.h) in.done(row);
         const float inv = rsqrtf(fmaf(s[0], inv_d, f.eps));
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int c = (tid + v * TPR) * 8, n = f.d - c;
+            const int c = (tid + v * tpr) * 8, n = f.d - c;
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[v][e] *= inv * wp[v][e];
             if (a.zv == nullptr) {
                 if (n > 0) store8(static_cast<T*>(f.z) + row * f.z_stride + c, y[v], n, vec);
                 continue;
             }
-            uint32_t m = 0;
+            // a value that is no number makes its whole row so: fmaxf need not find it
+            float m = fabsf(y[v][0]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = max(m, abs_bits(y[v][e]));
+            for (int e = 1; e < 8; ++e) m = fmaxf(m, fabsf(y[v][e]));
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));   // 16 lanes: 128 columns
+            for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));   // 16 lanes: 128 columns
             if (n <= 0) continue;
-            const float sc = block_scale(m), q = __frcp_rn(sc);
+            const float sc = block_scale(__float_as_uint(m)), q = __frcp_rn(sc);
             if ((tid & 15) == 0) a.zs[row * a.zs_row + (c / 128) * a.zs_col] = sc;
             *reinterpret_cast<uint2*>(a.zv + row * a.zv_stride + c) =
                 make_uint2(e4m3x4(y[v][0] * q, y[v][1] * q, y[v][2] * q, y[v][3] * q),
@@ -316,16 +316,16 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
 // the gate's sigmoid computed twice: kept in registers they would leave room
 // for half the threads, and spilled they cost more than the rest (d 1024:
 // 191 us with 48 bytes spilled a thread, 85 us without).
-template <typename T, int TPR, int VPT, bool RING>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT, kBackwardRegs>())
+template <typename T, bool WARP, int VPT, bool RING>
+__global__ void __launch_bounds__(most_threads<WARP>(), WARP ? 8 / VPT : 1)
     norm_grad_kernel(const __grid_constant__ GradArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float red[128];
     const nrn_gatednorm_t& f = a.f;
     const nrn_gatednorm_grad_t& g = a.g;
-    const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int slot = TPR == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 4 : 1);
+    const int tpr = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
+    const int slot = WARP ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? 4 : 1);
     const bool vec = a.in.vec != 0, block = f.h != nullptr, gated = f.gate != nullptr, silu = f.act == NRN_ACT_SILU;
     const float inv_d = 1.0f / static_cast<float>(f.d);
     int turn = 0;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
     constexpr bool kKeep = VPT <= 2;
     float kaw[kKeep ? VPT : 1][8], kwp[kKeep ? VPT : 1][8];
     auto factors = [&](int v, float* aw, float* wp) {
-        const int c = (tid + v * TPR) * 8, n = f.d - c;
+        const int c = (tid + v * tpr) * 8, n = f.d - c;
         float al[8];
         load_param(f.w_post, n > 0 ? c : 0, n, aw);
         load_param(f.alpha, n > 0 ? c : 0, n, al);
@@ -358,20 +358,20 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
             float s[1] = {0.0f};
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const Raw8<T> h = in.get(1, row, (tid + v * TPR) * 8);
+                const Raw8<T> h = in.get(1, row, (tid + v * tpr) * 8);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float x = to_f32(h.e[e]);
                     s[0] = fmaf(x, x, s[0]);
                 }
             }
-            row_sum<1, TPR>(s, red, turn);
+            row_sum<1, WARP>(s, red, turn);
             inv_h = rsqrtf(fmaf(s[0], inv_d, f.eps));
         }
         float sy[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int c = (tid + v * TPR) * 8;
+            const int c = (tid + v * tpr) * 8;
             float taw[8], twp[8];
             if constexpr (!kKeep) factors(v, taw, twp);
             const float *aw = kKeep ? kaw[kKeep ? v : 0] : taw, *wp = kKeep ? kwp[kKeep ? v : 0] : twp;
@@ -403,14 +403,14 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
         }
         float inv_y = 0.0f, my = 0.0f;
         if (g.dz) {
-            row_sum<2, TPR>(sy, red, turn);
+            row_sum<2, WARP>(sy, red, turn);
             inv_y = rsqrtf(fmaf(sy[0], inv_d, f.eps));
             my = inv_y * inv_y * sy[1] * inv_d;      // mean(dz w_pre yh) inv_y
         }
         float st[1] = {0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int c = (tid + v * TPR) * 8, n = f.d - c;
+            const int c = (tid + v * tpr) * 8, n = f.d - c;
             float taw[8], twp[8], d[8];
             if constexpr (!kKeep) factors(v, taw, twp);
             const float *aw = kKeep ? kaw[kKeep ? v : 0] : taw, *wp = kKeep ? kwp[kKeep ? v : 0] : twp;
@@ -457,11 +457,11 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
             }
         }
         if (block) {
-            row_sum<1, TPR>(st, red, turn);
+            row_sum<1, WARP>(st, red, turn);
             const float mh = st[0] * inv_d * inv_h;
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const int c = (tid + v * TPR) * 8, n = f.d - c;
+                const int c = (tid + v * tpr) * 8, n = f.d - c;
                 const Raw8<T> h = in.get(1, row, c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[v][e] = inv_h * (y[v][e] - to_f32(h.e[e]) * mh);
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, blocks_per_sm<TPR, VPT,
     float* at = a.part + static_cast<int64_t>(slot) * 2 * f.d;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-        const int c = (tid + v * TPR) * 8, n = f.d - c;
+        const int c = (tid + v * tpr) * 8, n = f.d - c;
         if (n <= 0) continue;
         store8(at + c, s1[v], n, f.d % 4 == 0);
         store8(at + f.d + c, s2[v], n, f.d % 4 == 0);
@@ -505,111 +505,68 @@ __global__ void __launch_bounds__(1024) norm_parts_kernel(const float* part, int
     }
 }
 
-// Threads of a row and vectors of a thread.
+// A row of up to 512 elements has a warp, a longer one a block whose threads
+// have 16 elements each (measured at d 4096: 8 elements a thread 131 us, 16
+// 111 us: the reductions cost each thread the same), past 8,192 elements 32.
 struct Shape {
-    int tpr, vpt;
+    bool warp;
+    int vpt, threads;
 };
-Shape shape_of(int d, bool backward) {
+Shape shape_of(int d) {
     const int vecs = (d + 7) / 8;
-    if (vecs <= 32) return {32, 1};
-    if (vecs <= 64) return {64, 1};
-    if (vecs <= 128) return backward ? Shape{128, 1} : Shape{64, 2};
-    if (vecs <= 256) return backward ? Shape{256, 1} : Shape{128, 2};
-    if (vecs <= 320) return backward ? Shape{320, 1} : Shape{160, 2};
-    if (vecs <= 512) return {256, 2};
-    if (vecs <= 1024) return {512, 2};
-    return {512, 4};
+    if (vecs <= 64) return {true, vecs <= 32 ? 1 : 2, 128};
+    const int vpt = vecs <= 1024 ? 2 : 4;
+    return {false, vpt, ((vecs + vpt - 1) / vpt + 31) / 32 * 32};
 }
 
 // Blocks that take the rows in turn: as many as are on the GPU at once.
-template <int TPR, int VPT, int REGS>
-unsigned blocks_for(int64_t rows) {
-    constexpr int rows_per = TPR == 32 ? 4 : 1;
-    return static_cast<unsigned>(std::min<int64_t>((rows + rows_per - 1) / rows_per,
-                                                   static_cast<int64_t>(blocks_per_sm<TPR, VPT, REGS>()) * sm_count_current()));
+int blocks_per_sm(const Shape& sh) { return (sh.vpt == 1 ? 1024 : 512) / sh.threads; }
+unsigned blocks_for(const Shape& sh, int64_t rows) {
+    const int rows_per = sh.warp ? 4 : 1;
+    return static_cast<unsigned>(std::min<int64_t>((rows + rows_per - 1) / rows_per, static_cast<int64_t>(blocks_per_sm(sh)) * sm_count_current()));
+}
+// Parts of the sums over rows that the backward kernel leaves: one for each block, or warp where a warp has a row.
+int grad_parts(int64_t rows, int d) {
+    const Shape sh = shape_of(d);
+    return static_cast<int>(blocks_for(sh, rows)) * (sh.warp ? 4 : 1);
 }
 
 // Rows that a block's share of the SM's shared memory holds; below two there is no ring.
-template <typename T, int TPR, int VPT, int REGS>
-int ring_stages(int arrays, int d, bool vec) {
-    if (TPR == 32 || !vec || d % 8 != 0) return 0;
-    const int room = (227 * 1024 / blocks_per_sm<TPR, VPT, REGS>() - 2048 - kRingHead) / (arrays * d * static_cast<int>(sizeof(T)));
+int ring_stages(const Shape& sh, int arrays, int d, int size, bool vec) {
+    if (sh.warp || !vec || d % 8 != 0) return 0;
+    const int room = (227 * 1024 / blocks_per_sm(sh) - 2048 - kRingHead) / (arrays * d * size);
     return room < 2 ? 0 : std::min(room, kMostStages);
 }
 
-template <typename T, int TPR, int VPT>
-cudaError_t run_forward(NormArgs a, cudaStream_t s) {
-    constexpr int threads = TPR == 32 ? 128 : TPR;
-    const unsigned blocks = blocks_for<TPR, VPT, kForwardRegs>(a.f.rows);
-    a.in.stages = ring_stages<T, TPR, VPT, kForwardRegs>(3, a.f.d, a.in.vec != 0);
-    if constexpr (TPR > 32) {
-        if (a.in.stages) {
-            const int bytes = kRingHead + a.in.stages * 3 * a.f.d * static_cast<int>(sizeof(T));
-            const cudaError_t e = cudaFuncSetAttribute(norm_kernel<T, TPR, VPT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-            if (e != cudaSuccess) return e;
-            norm_kernel<T, TPR, VPT, true><<<blocks, threads, bytes, s>>>(a);
-            return cudaGetLastError();
-        }
-    }
-    norm_kernel<T, TPR, VPT, false><<<blocks, threads, 0, s>>>(a);
+template <typename K, typename A>
+cudaError_t launch(K kernel, const Shape& sh, const A& a, int bytes, cudaStream_t s) {
+    const cudaError_t e = bytes ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
+    if (e != cudaSuccess) return e;
+    kernel<<<blocks_for(sh, a.f.rows), sh.threads, bytes, s>>>(a);
     return cudaGetLastError();
 }
 
-template <typename T, int TPR, int VPT>
-cudaError_t run_backward(GradArgs a, cudaStream_t s) {
-    constexpr int threads = TPR == 32 ? 128 : TPR;
-    const unsigned blocks = blocks_for<TPR, VPT, kBackwardRegs>(a.f.rows);
-    a.in.stages = ring_stages<T, TPR, VPT, kBackwardRegs>(5, a.f.d, a.in.vec != 0);
-    if constexpr (TPR > 32) {
-        if (a.in.stages) {
-            const int bytes = kRingHead + a.in.stages * 5 * a.f.d * static_cast<int>(sizeof(T));
-            const cudaError_t e = cudaFuncSetAttribute(norm_grad_kernel<T, TPR, VPT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-            if (e != cudaSuccess) return e;
-            norm_grad_kernel<T, TPR, VPT, true><<<blocks, threads, bytes, s>>>(a);
-            return cudaGetLastError();
-        }
-    }
-    norm_grad_kernel<T, TPR, VPT, false><<<blocks, threads, 0, s>>>(a);
-    return cudaGetLastError();
-}
-
-// Parts of the sums over rows that the backward kernel leaves: one for each block, or warp where a warp has a row.
-int grad_parts(int64_t rows, int d) {
-    const Shape sh = shape_of(d, true);
-    switch (sh.tpr) {
-        case 32: return 4 * static_cast<int>(blocks_for<32, 1, kBackwardRegs>(rows));
-        case 64: return static_cast<int>(blocks_for<64, 1, kBackwardRegs>(rows));
-        case 128: return static_cast<int>(blocks_for<128, 1, kBackwardRegs>(rows));
-        case 256: return static_cast<int>(sh.vpt == 1 ? blocks_for<256, 1, kBackwardRegs>(rows) : blocks_for<256, 2, kBackwardRegs>(rows));
-        case 320: return static_cast<int>(blocks_for<320, 1, kBackwardRegs>(rows));
-        default: return static_cast<int>(sh.vpt == 2 ? blocks_for<512, 2, kBackwardRegs>(rows) : blocks_for<512, 4, kBackwardRegs>(rows));
-    }
+template <typename T>
+cudaError_t forward_any(NormArgs a, cudaStream_t s) {
+    const Shape sh = shape_of(a.f.d);
+    const int size = static_cast<int>(sizeof(T));
+    a.in.stages = ring_stages(sh, 3, a.f.d, size, a.in.vec != 0);
+    const int bytes = a.in.stages ? kRingHead + a.in.stages * 3 * a.f.d * size : 0;
+    if (sh.warp) return sh.vpt == 1 ? launch(norm_kernel<T, true, 1, false>, sh, a, 0, s) : launch(norm_kernel<T, true, 2, false>, sh, a, 0, s);
+    if (sh.vpt == 2) return bytes ? launch(norm_kernel<T, false, 2, true>, sh, a, bytes, s) : launch(norm_kernel<T, false, 2, false>, sh, a, 0, s);
+    return bytes ? launch(norm_kernel<T, false, 4, true>, sh, a, bytes, s) : launch(norm_kernel<T, false, 4, false>, sh, a, 0, s);
 }
 
 template <typename T>
-cudaError_t forward_any(const NormArgs& a, cudaStream_t s) {
-    const Shape sh = shape_of(a.f.d, false);
-    switch (sh.tpr) {
-        case 32: return run_forward<T, 32, 1>(a, s);
-        case 64: return sh.vpt == 1 ? run_forward<T, 64, 1>(a, s) : run_forward<T, 64, 2>(a, s);
-        case 128: return run_forward<T, 128, 2>(a, s);
-        case 160: return run_forward<T, 160, 2>(a, s);
-        case 256: return run_forward<T, 256, 2>(a, s);
-        default: return sh.vpt == 2 ? run_forward<T, 512, 2>(a, s) : run_forward<T, 512, 4>(a, s);
-    }
-}
-
-template <typename T>
-cudaError_t backward_any(const GradArgs& a, cudaStream_t s) {
-    const Shape sh = shape_of(a.f.d, true);
-    switch (sh.tpr) {
-        case 32: return run_backward<T, 32, 1>(a, s);
-        case 64: return run_backward<T, 64, 1>(a, s);
-        case 128: return run_backward<T, 128, 1>(a, s);
-        case 256: return sh.vpt == 1 ? run_backward<T, 256, 1>(a, s) : run_backward<T, 256, 2>(a, s);
-        case 320: return run_backward<T, 320, 1>(a, s);
-        default: return sh.vpt == 2 ? run_backward<T, 512, 2>(a, s) : run_backward<T, 512, 4>(a, s);
-    }
+cudaError_t backward_any(GradArgs a, cudaStream_t s) {
+    const Shape sh = shape_of(a.f.d);
+    const int size = static_cast<int>(sizeof(T));
+    a.in.stages = ring_stages(sh, 5, a.f.d, size, a.in.vec != 0);
+    const int bytes = a.in.stages ? kRingHead + a.in.stages * 5 * a.f.d * size : 0;
+    if (sh.warp) return sh.vpt == 1 ? launch(norm_grad_kernel<T, true, 1, false>, sh, a, 0, s) : launch(norm_grad_kernel<T, true, 2, false>, sh, a, 0, s);
+    if (sh.vpt == 2)
+        return bytes ? launch(norm_grad_kernel<T, false, 2, true>, sh, a, bytes, s) : launch(norm_grad_kernel<T, false, 2, false>, sh, a, 0, s);
+    return bytes ? launch(norm_grad_kernel<T, false, 4, true>, sh, a, bytes, s) : launch(norm_grad_kernel<T, false, 4, false>, sh, a, 0, s);
 }
 
 bool row_ok(const void* p, int64_t stride, int size) {
