@@ -8,15 +8,17 @@
 // TMEM); because the scales change with every block, each block's sums leave
 // TMEM and are scaled and added in fp32 registers.
 //
-// Kernel (persistent, one CTA per SM, 10 warps), for a tile of 128 rows of
+// Kernel (persistent, one CTA per SM, 12 warps), for a tile of 128 rows of
 // one operand ("rows", the MMA's M) by NT rows of the other ("cols", its N):
 //   warp 0    producer: per block one TMA box of each operand (128-byte
 //             swizzle, zeros outside the matrix) into a ring of stages;
 //   warp 1    issuer (one thread): per block four tcgen05.mma (K = 32) into
 //             one of the TMEM accumulators; the commit frees the stage and
 //             hands the accumulator on;
-//   warps 2-9 two warpgroups, each half of the columns: tcgen05.ld, scale,
-//             add, and at the end write the tile.
+//   warps 4-11 two warpgroups, each half of the columns: tcgen05.ld, scale,
+//             add, and at the end write the tile.  With NT = 256 a thread
+//             holds 128 sums: the first warpgroup gives its registers up
+//             (12 x 168 at launch: 4 x 56 + 8 x 224).
 // With NT = 256 an accumulator is 128 x 256: per block 512 cycles of MMA at
 // the dense e4m3 rate against 256 cycles of TMEM reads and 256 (128 as
 // packed pairs) of FMA issue, so the promotion hides behind the MMA of the
@@ -48,7 +50,7 @@ using namespace tc;
 constexpr int kBlock = 128;            // columns (and weight rows) of a scale block
 constexpr int kRowTile = 128;
 constexpr int kEpiThreads = 256;
-constexpr int kThreads = 64 + kEpiThreads;
+constexpr int kThreads = 128 + kEpiThreads;
 constexpr int kMaxStages = 8;
 enum { ERR_SCALED_TIMEOUT = 5 };
 
@@ -77,7 +79,7 @@ struct Smem {
     int abort;
     int last;
     int stop;
-    float cscale[2][256];
+    alignas(16) float cscale[2][256];
 };
 constexpr int kSmemHead = 4096;        // Smem, padded so that the tiles start 1 KB aligned
 static_assert(sizeof(Smem) <= kSmemHead, "barrier block too large");
@@ -196,8 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         k1 = static_cast<int>(static_cast<int64_t>(a.blocks) * (sp + 1) / a.splits);
     };
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < 4) {
+        if constexpr (NT == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0 && lane == 0) {
             long long it = 0;
             int stage = 0;
             uint32_t phase = 0;
@@ -224,9 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the copies still in flight land before the CTA exits
             for (long long q = it - 1; q >= 0 && q >= it - stages; --q)
                 mbar_wait(&M.full[q % stages], static_cast<uint32_t>((q / stages) & 1), nullptr);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
+        } else if (warp == 1 && lane == 0) {
             int stage = 0, buf = 0;
             uint32_t phase = 0, bphase = 0;
             bool ok = true;
@@ -262,7 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_wait(&M.drain, 0, nullptr);
         }
     } else {
-        const int et = threadIdx.x - 64;             // 0 .. 255
+        if constexpr (NT == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int et = threadIdx.x - 128;            // 0 .. 255
         const int half = et >> 7;                    // this warpgroup's half of the columns
         const int sub = warp & 3;                    // TMEM lanes 32 sub ..
         const int row_l = sub * 32 + lane;
@@ -306,10 +308,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float* sc = &M.cscale[kb & 1][half * S::kCols];
                     auto add = [&](const uint32_t* v, int c0) {
 #pragma unroll
-                        for (int j = 0; j < S::kChunk; j += 2) {
-                            uint64_t f = uu;
-                            if (!CBLOCK) f = mul2(uu, *reinterpret_cast<const uint64_t*>(sc + c0 + j));
+                        for (int j = 0; j < S::kChunk; j += 4) {
+                            uint64_t f = uu, h = uu;
+                            if (!CBLOCK) {
+                                const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(sc + c0 + j);
+                                f = mul2(uu, s4.x);
+                                h = mul2(uu, s4.y);
+                            }
                             acc[(c0 + j) / 2] = fma2(pack2(v[j], v[j + 1]), f, acc[(c0 + j) / 2]);
+                            acc[(c0 + j) / 2 + 1] = fma2(pack2(v[j + 2], v[j + 3]), h, acc[(c0 + j) / 2 + 1]);
                         }
                     };
                     if constexpr (S::kCols == 8) {

@@ -41,6 +41,7 @@ def _describe(values, scales, row_block):
 
 
 _matrices = Layouts(_describe)
+_fresh: dict = {}        # descriptions of the matrices that Scaled.empty makes, by (rows, cols, row_block)
 
 
 class Scaled:
@@ -69,11 +70,25 @@ class Scaled:
 
     @classmethod
     def empty(cls, rows: int, cols: int, device, row_block: int = 1) -> "Scaled":
-        pitch = -(-cols // 16) * 16
+        pitch, kind = -(-cols // 16) * 16, (rows, cols, row_block)
         values = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=device)
+        if pitch != cols:
+            values = values[:, :cols]
         # scales of neighbouring rows next to each other: as the product's threads read them
-        scales = torch.empty((-(-cols // BLOCK), -(-rows // row_block)), dtype=torch.float32, device=device).t()
-        return cls(values[:, :cols] if pitch != cols else values, scales, row_block)
+        shape = (-(-rows // row_block), -(-cols // BLOCK))
+        scales = torch.empty_strided(shape, (1, shape[0]), dtype=torch.float32, device=device)
+        block = _fresh.get(kind)
+        if block is None:
+            if len(_fresh) > 4096:
+                _fresh.clear()
+            new = cls(values, scales, row_block)
+            _fresh[kind] = bytes(new.desc)
+            return new
+        new = object.__new__(cls)
+        new.values, new.scales, new.row_block = values, scales, row_block
+        d = new.desc = N.Scaled.from_buffer_copy(block)
+        d.values, d.scales = values.data_ptr(), scales.data_ptr()
+        return new
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """What the matrix stands for, by torch operations (for checks and export)."""
