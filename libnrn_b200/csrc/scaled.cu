@@ -588,10 +588,13 @@ struct Plan {
     int64_t row_tiles, col_tiles, blocks;
 };
 
-// The tile width and the split of k: the fewest cycles by a simple model --
-// whole rounds of tiles over the SMs, per block of 128 columns the slower of
-// MMA (2 NT cycles) and shared memory (128 + NT), per tile a fixed cost and,
-// where k is split, the parts' way through L2.
+// The tile width and the split of k: the fewest cycles by a model of what
+// bounds the kernel.  Rounds of tiles over the SMs; per block of 128 columns
+// both operands' way from L2, which all SMs together get at about 36 bytes a
+// cycle each and one alone at 64 (measured: 128 x 256 tiles 1,300 cycles a
+// block on a full GPU, 128 x 128 tiles 1,000, against 512 and 256 of MMA); per
+// tile a fixed cost and the result's way out; where k is split, the parts' way
+// out and, in the last block of a tile, all parts' way back.
 Plan plan_of(int64_t m, int64_t n, int64_t k) {
     Plan best{};
     best.swap = m <= 128;
@@ -607,9 +610,10 @@ Plan plan_of(int64_t m, int64_t n, int64_t k) {
             if (splits > 1 && (best.blocks / splits < 2 || best.row_tiles * ct > kMaxSplitTiles)) break;
             const int64_t items = best.row_tiles * ct * splits;
             const double rounds = static_cast<double>((items + sms - 1) / sms);
-            const double per = std::max<double>(2 * nt, 128 + nt);
-            const double c = rounds * (static_cast<double>((best.blocks + splits - 1) / splits) * per + 1000 + 4 * nt +
-                                       (splits > 1 ? 1500 + 2.0 * nt * splits : 0.0));
+            const double busy = static_cast<double>(std::min(items, sms)) / static_cast<double>(sms);
+            const double per = static_cast<double>(kRowTile + nt) * std::max(2.0, 3.6 * busy);
+            const double c = rounds * (static_cast<double>((best.blocks + splits - 1) / splits) * per + 1000 + 7.0 * nt +
+                                       (splits > 1 ? 1500 + 14.0 * nt * (1 + splits) : 0.0));
             if (c < cost) {
                 cost = c;
                 best.nt = nt;
