@@ -25,6 +25,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "launch.h"
 #include "scaled.cuh"
 #include "tc.cuh"
 #include "vecio.cuh"
@@ -523,7 +524,7 @@ Shape shape_of(int d) {
 int blocks_per_sm(const Shape& sh) { return (sh.vpt == 1 ? 1024 : 512) / sh.threads; }
 unsigned blocks_for(const Shape& sh, int64_t rows) {
     const int rows_per = sh.warp ? 4 : 1;
-    return static_cast<unsigned>(std::min<int64_t>((rows + rows_per - 1) / rows_per, static_cast<int64_t>(blocks_per_sm(sh)) * sm_count_current()));
+    return static_cast<unsigned>(std::min<int64_t>((rows + rows_per - 1) / rows_per, static_cast<int64_t>(blocks_per_sm(sh)) * sm_count()));
 }
 // Parts of the sums over rows that the backward kernel leaves: one for each block, or warp where a warp has a row.
 int grad_parts(int64_t rows, int d) {
@@ -538,11 +539,11 @@ int ring_stages(const Shape& sh, int arrays, int d, int size, bool vec) {
     return room < 2 ? 0 : std::min(room, kMostStages);
 }
 
-template <typename K, typename A>
-cudaError_t launch(K kernel, const Shape& sh, const A& a, int bytes, cudaStream_t s) {
-    const cudaError_t e = bytes ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
+template <auto Kernel, typename A>
+cudaError_t launch(const Shape& sh, const A& a, int bytes, cudaStream_t s) {
+    const cudaError_t e = bytes ? allow_shared<Kernel>(bytes) : cudaSuccess;
     if (e != cudaSuccess) return e;
-    kernel<<<blocks_for(sh, a.f.rows), sh.threads, bytes, s>>>(a);
+    Kernel<<<blocks_for(sh, a.f.rows), sh.threads, bytes, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -552,9 +553,9 @@ cudaError_t forward_any(NormArgs a, cudaStream_t s) {
     const int size = static_cast<int>(sizeof(T));
     a.in.stages = ring_stages(sh, 3, a.f.d, size, a.in.vec != 0);
     const int bytes = a.in.stages ? kRingHead + a.in.stages * 3 * a.f.d * size : 0;
-    if (sh.warp) return sh.vpt == 1 ? launch(norm_kernel<T, true, 1, false>, sh, a, 0, s) : launch(norm_kernel<T, true, 2, false>, sh, a, 0, s);
-    if (sh.vpt == 2) return bytes ? launch(norm_kernel<T, false, 2, true>, sh, a, bytes, s) : launch(norm_kernel<T, false, 2, false>, sh, a, 0, s);
-    return bytes ? launch(norm_kernel<T, false, 4, true>, sh, a, bytes, s) : launch(norm_kernel<T, false, 4, false>, sh, a, 0, s);
+    if (sh.warp) return sh.vpt == 1 ? launch<norm_kernel<T, true, 1, false>>(sh, a, 0, s) : launch<norm_kernel<T, true, 2, false>>(sh, a, 0, s);
+    if (sh.vpt == 2) return bytes ? launch<norm_kernel<T, false, 2, true>>(sh, a, bytes, s) : launch<norm_kernel<T, false, 2, false>>(sh, a, 0, s);
+    return bytes ? launch<norm_kernel<T, false, 4, true>>(sh, a, bytes, s) : launch<norm_kernel<T, false, 4, false>>(sh, a, 0, s);
 }
 
 template <typename T>
@@ -563,10 +564,10 @@ cudaError_t backward_any(GradArgs a, cudaStream_t s) {
     const int size = static_cast<int>(sizeof(T));
     a.in.stages = ring_stages(sh, 5, a.f.d, size, a.in.vec != 0);
     const int bytes = a.in.stages ? kRingHead + a.in.stages * 5 * a.f.d * size : 0;
-    if (sh.warp) return sh.vpt == 1 ? launch(norm_grad_kernel<T, true, 1, false>, sh, a, 0, s) : launch(norm_grad_kernel<T, true, 2, false>, sh, a, 0, s);
+    if (sh.warp) return sh.vpt == 1 ? launch<norm_grad_kernel<T, true, 1, false>>(sh, a, 0, s) : launch<norm_grad_kernel<T, true, 2, false>>(sh, a, 0, s);
     if (sh.vpt == 2)
-        return bytes ? launch(norm_grad_kernel<T, false, 2, true>, sh, a, bytes, s) : launch(norm_grad_kernel<T, false, 2, false>, sh, a, 0, s);
-    return bytes ? launch(norm_grad_kernel<T, false, 4, true>, sh, a, bytes, s) : launch(norm_grad_kernel<T, false, 4, false>, sh, a, 0, s);
+        return bytes ? launch<norm_grad_kernel<T, false, 2, true>>(sh, a, bytes, s) : launch<norm_grad_kernel<T, false, 2, false>>(sh, a, 0, s);
+    return bytes ? launch<norm_grad_kernel<T, false, 4, true>>(sh, a, bytes, s) : launch<norm_grad_kernel<T, false, 4, false>>(sh, a, 0, s);
 }
 
 bool row_ok(const void* p, int64_t stride, int size) {

@@ -26,6 +26,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "launch.h"
 #include "tc.cuh"
 #include "tensor_map.h"
 #include "vecio.cuh"
@@ -1253,7 +1254,7 @@ template <int DK, int CH, int TERMS, bool STATE_ONLY>
 cudaError_t launch_mma(const ScanArgs& p, cudaStream_t s) {
     const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kMmaCols - 1) / kMmaCols);
     constexpr int bytes = sizeof(MmaSmem<DK, CH>);
-    const cudaError_t e = cudaFuncSetAttribute(scan_mma_kernel<DK, CH, TERMS, STATE_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = allow_shared<scan_mma_kernel<DK, CH, TERMS, STATE_ONLY>>(bytes);
     if (e != cudaSuccess) return e;
     scan_mma_kernel<DK, CH, TERMS, STATE_ONLY><<<static_cast<unsigned>(blocks), kMmaThreads, bytes, s>>>(p);
     return cudaGetLastError();
@@ -1284,7 +1285,7 @@ template <int DK, int TERMS, bool STATE_ONLY>
 cudaError_t launch_tc(const ScanArgs& p, const CUtensorMap* maps, cudaStream_t s) {
     const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kTcCols - 1) / kTcCols);
     constexpr int bytes = TcSmem<DK, TERMS, STATE_ONLY>::kBytes;
-    const cudaError_t e = cudaFuncSetAttribute(scan_tc_kernel<DK, TERMS, STATE_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = allow_shared<scan_tc_kernel<DK, TERMS, STATE_ONLY>>(bytes);
     if (e != cudaSuccess) return e;
     scan_tc_kernel<DK, TERMS, STATE_ONLY><<<static_cast<unsigned>(blocks), kTcThreads, bytes, s>>>(maps[0], maps[1], maps[2], p);
     return cudaGetLastError();
@@ -1316,7 +1317,7 @@ int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
 // sequences are split.
 int64_t segment_length(const nrn_linattn_t* a, int dc) {
     const int64_t tiles = (dc + kTcCols - 1) / kTcCols;
-    const int64_t want = sm_count_current();                          // blocks that fill the GPU
+    const int64_t want = sm_count();                          // blocks that fill the GPU
     const int64_t rows = static_cast<int64_t>(a->heads) * tiles;
     const int64_t all = a->cu_seqlens ? a->tokens : a->tokens * a->seqs;
     if (all == 0) return kChunk;
@@ -1512,7 +1513,7 @@ extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const 
         const int64_t n = all_tokens(a);
         if (share == 1 || n == 0) continue;
         const int64_t total = n * a->kv_heads * dd, per = a->cu_seqlens ? n : a->tokens;
-        const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 16LL * sm_count_current()));
+        const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 16LL * sm_count()));
         if (a->dtype == NRN_BF16)
             sum_heads_kernel<<<blocks, 256, 0, s>>>(part, n, a->kv_heads, share, dd, static_cast<__nv_bfloat16*>(out), st[0], st[1], st[2], per);
         else if (a->dtype == NRN_FP16)

@@ -37,6 +37,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "launch.h"
 #include "scaled.cuh"
 #include "tc.cuh"
 #include "tensor_map.h"
@@ -601,7 +602,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k) {
     const int64_t rows = best.swap ? n : m, cols = best.swap ? m : n;
     best.row_tiles = (rows + kRowTile - 1) / kRowTile;
     best.blocks = (k + kBlock - 1) / kBlock;
-    const int64_t sms = std::max(1, sm_count_current());
+    const int64_t sms = std::max(1, sm_count());
     double cost = 1e300;
     for (int nt : {256, 128, 64, 32, 16}) {
         if (nt > 16 && nt / 2 >= cols) continue;                 // a narrower tile holds them all
@@ -647,8 +648,8 @@ nrn_status_t launch_product(const CUtensorMap& rm, const CUtensorMap& cm, Produc
     constexpr int stage = Shape<NT>::kStageBytes;
     a.stages = std::min(kMaxStages, (227 * 1024 - kSmemHead) / stage);
     const int bytes = kSmemHead + a.stages * stage;
-    NRN_CUDA_TRY(cudaFuncSetAttribute(product_kernel<NT, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    const int grid = std::min(a.row_tiles * a.col_tiles * a.splits, sm_count_current());
+    NRN_CUDA_TRY((allow_shared<product_kernel<NT, CB>>(bytes)));
+    const int grid = std::min(a.row_tiles * a.col_tiles * a.splits, sm_count());
     product_kernel<NT, CB><<<grid, kThreads, bytes, s>>>(rm, cm, a);
     NRN_CUDA_TRY(cudaGetLastError());
     return NRN_OK;
@@ -673,7 +674,7 @@ nrn_status_t quantize(const void* x, int64_t rows, int64_t cols, int64_t stride,
     const int64_t rb = (rows + kBlock - 1) / kBlock;
     if (!transpose && o->row_block == 1) {
         const int64_t work = rows * ((cols + kBlock - 1) / kBlock);
-        const int64_t blocks = std::min<int64_t>((work + kQuantThreads / 16 - 1) / (kQuantThreads / 16), 32LL * sm_count_current());
+        const int64_t blocks = std::min<int64_t>((work + kQuantThreads / 16 - 1) / (kQuantThreads / 16), 32LL * sm_count());
         quant_rows_kernel<T><<<static_cast<unsigned>(blocks), kQuantThreads, 0, s>>>(
             p, rows, cols, stride, vec, o->values, o->value_stride, o->scales, o->scale_stride[0], o->scale_stride[1]);
     } else {

@@ -84,13 +84,13 @@ def forward(residual, h=None, gate=None, *, alpha=None, w_post=None, w_pre=None,
     y, z = residual, None
     with on(dev, stream) as st:
         if h is not None:
-            y = torch.empty((rows, d), dtype=residual.dtype, device=dev)
+            y = torch.empty_strided((rows, d), (d, 1), dtype=residual.dtype, device=dev)
             a.y, a.y_stride = y.data_ptr(), d
         if want_z and scaled:
             z = Scaled.empty(rows, d, dev)
             a.z_scaled = C.pointer(z.desc)
         elif want_z:
-            z = torch.empty((rows, d), dtype=residual.dtype, device=dev)
+            z = torch.empty_strided((rows, d), (d, 1), dtype=residual.dtype, device=dev)
             a.z, a.z_stride = z.data_ptr(), d
         N.check(N.lib().nrn_cuda_gatednorm_forward(C.byref(a), st), "nrn_cuda_gatednorm_forward")
     return y, z
@@ -106,7 +106,7 @@ def backward(dy, dz, residual, h=None, gate=None, *, alpha=None, w_post=None, w_
     with on(dev, stream) as st:
         g = N.GatedNormGrad()
         g.dy, g.dz, g.dy_stride, g.dz_stride = ptr(dy), ptr(dz), _stride(dy), _stride(dz)
-        like = [torch.empty((rows, d), dtype=dt, device=dev) if want else None for want in (True, h is not None, gate is not None)]
+        like = [torch.empty_strided((rows, d), (d, 1), dtype=dt, device=dev) if want else None for want in (True, h is not None, gate is not None)]
         sums = [torch.empty(d, dtype=torch.float32, device=dev) if t is not None else None for t in (alpha, w_post, w_pre)]
         g.dresidual, g.dh, g.dgate = (ptr(t) for t in like)
         g.dresidual_stride = g.dh_stride = g.dgate_stride = d

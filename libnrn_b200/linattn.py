@@ -157,7 +157,7 @@ def _describe_step(q, k, v, log_decay, state, scale, slots, out):
     for f, x in ((a.q_stride, q), (a.k_stride, k), (a.v_stride, v)):
         f[0], f[2] = x.stride(0), x.stride(1)
     a.o_stride[0], a.o_stride[2] = (out.stride(0), out.stride(1)) if out is not None else (h * dv, dv)
-    return bytes(a), (b, h, dv), state.stride(0), state.shape[0]
+    return bytes(a), (b, h, dv), (h * dv, dv, 1), state.stride(0), state.shape[0]
 
 
 _steps = Layouts(_describe_step)
@@ -169,10 +169,10 @@ def step(q, k, v, log_decay, state, *, scale=None, slots=None, out=None, stream=
     output is 0, and one past the states gives NaN."""
     _check_q(q)
     key = (layout(q), layout(k), layout(v), layout(log_decay), layout(state), scale, layout(slots), layout(out))
-    block, shape, stride, count = _steps.get(key, q, k, v, log_decay, state, scale, slots, out)
+    block, shape, strides, stride, count = _steps.get(key, q, k, v, log_decay, state, scale, slots, out)
     with on(q.device, stream) as st:
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_strided(shape, strides, dtype=q.dtype, device=q.device)
         a = N.LinAttn.from_buffer_copy(block)
         a.q, a.k, a.v, a.o, a.log_decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr()
         N.check(N.lib().nrn_cuda_linattn_step(C.byref(a), state.data_ptr(), stride, count, ptr(slots), st), "nrn_cuda_linattn_step")

@@ -41,7 +41,20 @@ def _describe(values, scales, row_block):
 
 
 _matrices = Layouts(_describe)
-_fresh: dict = {}        # descriptions of the matrices that Scaled.empty makes, by (rows, cols, row_block)
+
+
+def _describe_empty(rows, cols, row_block):
+    """(bytes, where the scales start, row pitch, shape of the scales, description) of a matrix of Scaled.empty."""
+    require(row_block in (1, BLOCK), f"row_block: must be 1 or {BLOCK}, is {row_block}")
+    pitch, shape = -(-max(cols, 1) // 16) * 16, (-(-rows // row_block), -(-cols // BLOCK))
+    at = -(-rows * pitch // 16) * 16
+    d = N.Scaled()
+    d.rows, d.cols, d.value_stride, d.row_block = rows, cols, pitch, row_block
+    d.scale_stride[0], d.scale_stride[1] = 1, max(shape[0], 1)
+    return max(at + 4 * shape[0] * shape[1], 16), at, pitch, shape, bytes(d)
+
+
+_empties = Layouts(_describe_empty)
 
 
 class Scaled:
@@ -49,46 +62,46 @@ class Scaled:
     [ceil(rows / row_block), ceil(cols / 128)], any strides).  ``quantize`` makes one; values and scales of a checkpoint
     can be given as they are."""
 
-    __slots__ = ("values", "scales", "row_block", "desc")
+    __slots__ = ("_values", "_scales", "_base", "_at", "_pitch", "_scale_shape", "row_block", "desc", "shape", "device")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, row_block: int = 1):
         require(isinstance(values, torch.Tensor) and values.is_cuda, "values: a CUDA matrix is needed")
         block = _matrices.get((layout(values), layout(scales), row_block), values, scales, row_block)
-        self.values, self.scales, self.row_block = values, scales, row_block
+        self._values, self._scales, self.row_block = values, scales, row_block
+        self.shape, self.device = values.shape, values.device
+        at = values.data_ptr()
+        require(at % 16 == 0, "values: rows must start on 16-byte boundaries (Scaled.empty allocates them so)")
         self.desc = N.Scaled.from_buffer_copy(block)
-        self.desc.values, self.desc.scales = values.data_ptr(), scales.data_ptr()
-        require(self.desc.values is None or self.desc.values % 16 == 0,
-                "values: rows must start on 16-byte boundaries (Scaled.empty allocates them so)")
-
-    @property
-    def shape(self):
-        return self.values.shape
-
-    @property
-    def device(self):
-        return self.values.device
+        self.desc.values, self.desc.scales = at, scales.data_ptr()
 
     @classmethod
     def empty(cls, rows: int, cols: int, device, row_block: int = 1) -> "Scaled":
-        pitch, kind = -(-cols // 16) * 16, (rows, cols, row_block)
-        values = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=device)
-        if pitch != cols:
-            values = values[:, :cols]
-        # scales of neighbouring rows next to each other: as the product's threads read them
-        shape = (-(-rows // row_block), -(-cols // BLOCK))
-        scales = torch.empty_strided(shape, (1, shape[0]), dtype=torch.float32, device=device)
-        block = _fresh.get(kind)
-        if block is None:
-            if len(_fresh) > 4096:
-                _fresh.clear()
-            new = cls(values, scales, row_block)
-            _fresh[kind] = bytes(new.desc)
-            return new
+        """A matrix to be filled: one allocation, of which ``values`` and ``scales`` are views."""
+        n, at, pitch, scale_shape, block = _empties.get((rows, cols, row_block), rows, cols, row_block)
         new = object.__new__(cls)
-        new.values, new.scales, new.row_block = values, scales, row_block
+        new._base = base = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device)
+        new._values = new._scales = None
+        new._at, new._pitch, new._scale_shape = at, pitch, scale_shape
+        new.row_block, new.shape, new.device = row_block, torch.Size((rows, cols)), base.device
         d = new.desc = N.Scaled.from_buffer_copy(block)
-        d.values, d.scales = values.data_ptr(), scales.data_ptr()
+        p = base.data_ptr()
+        d.values, d.scales = p, p + at
         return new
+
+    @property
+    def values(self) -> torch.Tensor:
+        if self._values is None:
+            rows, cols = self.shape
+            self._values = self._base[:rows * self._pitch].view(torch.float8_e4m3fn).view(rows, self._pitch)[:, :cols]
+        return self._values
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            # scales of neighbouring rows next to each other: as the product's threads read them
+            rows, cols = self._scale_shape
+            self._scales = self._base[self._at:self._at + 4 * rows * cols].view(torch.float32).view(cols, rows).t()
+        return self._scales
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """What the matrix stands for, by torch operations (for checks and export)."""
@@ -181,7 +194,8 @@ def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None
     kind, stride, need = _products.get(key, a, b, dtype, out)
     with on(dev, stream) as st:
         if out is None:
-            out = torch.empty((a.shape[0], b.shape[0]), dtype=dtype, device=dev)
+            n = b.shape[0]
+            out = torch.empty_strided((a.shape[0], n), (n, 1), dtype=dtype, device=dev)
         w = _workspace(need, dev, st).data_ptr() if need else None
         N.check(N.lib().nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), kind, stride, w, need, error_flag(dev), st),
                 "nrn_cuda_scaled_product")
