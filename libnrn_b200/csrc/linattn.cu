@@ -609,19 +609,26 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
 //     inter [128 x 64]  = X16^T a^T             X16: the entering state in bf16
 //     U     [128 x b.d] = sum over terms of (w c)^T b
 //     intra [128 x 64]  = c^T P^T
-// 18 warps, one block an SM:
-//   warp 0    copies: a, b and c of a chunk by TMA into one of two stages;
-//   warp 1    issues the MMAs (one thread);
-//   warps 2-  everything else, in the order that keeps the tensor cores busy
-//             behind them: (1) c^T, its decayed terms and b^T through
-//             ldmatrix/stmatrix into K-major tiles, while P and inter run;
-//             (2) P out of TMEM, decay and mask, bf16, while U runs; (3) the
-//             fp32 state, kept in registers (32 a thread): lam^n X + U, and
-//             its bf16 copy, while intra runs; (4) the results.
-// About 70 warp instructions a token and head against 270 with mma.sync
+// 20 warps, one block an SM:
+//   warp 0      copies: a, b and c of a chunk by TMA into one of two stages;
+//   warp 1      issues the MMAs (one thread); warps 2 and 3 only give up
+//               their registers;
+//   warps 4-11  (1) c^T, its decayed terms and b^T through ldmatrix/stmatrix
+//               into K-major tiles, while P and inter run; (2) P out of TMEM,
+//               decay and mask, bf16, while U runs;
+//   warps 12-19 (3) the fp32 state, kept in registers (64 a thread):
+//               lam^n X + U, and its bf16 copy; (4) the results.
+// The two groups work on neighbouring chunks at once: all sixteen warps on one
+// phase after the other took 6,600 cycles a chunk (of which 2,700 issue slots),
+// most of it latency and waits for the MMAs of the same chunk.
+// About 170 warp instructions a token and head against 270 with mma.sync
 // (whose operands pass through registers in every warp).
-constexpr int kTcWarps = 16;            // that are not copying or issuing
-constexpr int kTcThreads = 64 + 32 * kTcWarps;
+//
+// A value of c that is no number must not reach earlier tokens of its chunk
+// through the zeros of P (0 * inf): it goes into the tiles as 0, and from its
+// token on the column's results are NaN.
+constexpr int kTcThreads = 640;
+constexpr int kTcGroup = 8;             // warps of each of the two groups
 constexpr int kTcCols = 128;
 enum { ERR_LINATTN_TIMEOUT = 5 };
 
@@ -638,17 +645,20 @@ struct TcSmem {
     static constexpr int kBt = kWt + TERMS * 128 * 128;               // b^T [DK][64]
     static constexpr int kX16 = kBt + DK * 128;                       // [128][DK]
     static constexpr int kProb = kX16 + (STATE_ONLY ? 0 : 128 * DK * 2);   // [64][64]
-    static constexpr int kBytes = kProb + (STATE_ONLY ? 0 : kTile);
+    static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 1 KB for each warp of results
+    static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 1024);
 };
 static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
 
 struct TcHead {
-    uint64_t full[2], empty[2], pready, psm, x16, vk, uready, oready, drain;
+    uint64_t full[2], empty[2], oready[2], pready, psm, x16, vk, uready, drain;
     uint32_t tmem;
     int abort;
-    float lag[128];                // factor of P at token i - token j, from -63 on
-    float w[kChunk];               // decay of each token to the chunk's end
-    float out[kChunk];             // and of the entering state to each token, times out_mul
+    alignas(16) float lag[128];    // factor of P at token i - token j, from -63 on
+    alignas(16) float w[kChunk];   // decay of each token to the chunk's end
+    alignas(16) float out[kChunk]; // and of the entering state to each token, times out_mul
+    uint8_t bad[2][kTcGroup];      // 16 columns of c hold a value that is no number, and each column's first, in scan order
+    uint8_t first_bad[2][kTcCols];
 };
 static_assert(sizeof(TcHead) <= 2048, "barriers and factors");
 
@@ -688,22 +698,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
         : "memory");
 }
-// 16 lanes x 16 columns as the fragments of two 16x8 accumulators.
+// 16 lanes x 32 columns as the fragments of four 16x8 accumulators.
 __device__ __forceinline__ void tc_ld_frag(uint32_t taddr, uint32_t* v) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void tc_ld1(uint32_t taddr, uint32_t& v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v)::"memory");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_ld32(uint32_t* v) {
-    tc_wait_ld16(v);
-    tc_wait_ld16(v + 16);
-}
-
 template <int DK, int TERMS, bool STATE_ONLY>
 __global__ void __launch_bounds__(kTcThreads, 1)
     scan_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
@@ -722,20 +725,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const Unit u = unit_of(p, unit);
     if (!u.any) return;
     const int chunks = static_cast<int>((u.end - u.begin + kChunk - 1) / kChunk);
-    constexpr uint32_t kP = 0, kU = 64, kIntra = 192, kInter = 256;      // TMEM columns
+    constexpr uint32_t kP = 0, kU = 64, kIntra = 192, kInter = 320;      // TMEM columns; the last two in turn
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&M.full[i], 1);
             mbar_init(&M.empty[i], 1);
+            mbar_init(&M.oready[i], 1);   // two: the next chunk's may come before this one's is looked at
         }
         mbar_init(&M.pready, 1);
         mbar_init(&M.uready, 1);
-        mbar_init(&M.oready, 1);
         mbar_init(&M.drain, 1);
-        mbar_init(&M.psm, kTcWarps);
-        mbar_init(&M.x16, kTcWarps);
-        mbar_init(&M.vk, kTcWarps);
+        mbar_init(&M.psm, kTcGroup);
+        mbar_init(&M.x16, kTcGroup);
+        mbar_init(&M.vk, kTcGroup);
         M.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -758,8 +761,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return p.reverse ? u.len - t - tokens(c) : t;
     };
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0 && lane == 0) {
             int c = 0;
             for (; c < chunks; ++c) {
                 const int st = c & 1;
@@ -779,9 +783,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             // the copies still in flight land before the block ends
             for (int q = c - 1; q >= 0 && q >= c - 2; --q) mbar_wait(&M.full[q & 1], (q >> 1) & 1, nullptr);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
+        } else if (warp == 1 && lane == 0) {
             bool ok = true;
             for (int c = 0; c < chunks && ok; ++c) {
                 const int st = c & 1;
@@ -797,9 +799,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         mma_bf16<64, 64>(tmem + kP, desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32),
                                          desc_swizzled(sb + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
                     tc_commit(&M.pready);
-                    ok = mbar_wait(&M.x16, ph, abort);
-                    if (!ok) break;
-                    tc_fence_after();
+                }
+                ok = mbar_wait(&M.x16, ph, abort);       // X16 is there, and U of the last chunk read
+                if (!ok) break;
+                tc_fence_after();
+                if constexpr (!STATE_ONLY) {
 #pragma unroll
                     for (int kk = 0; kk < DK / 16; ++kk)
                         mma_bf16<128, 64>(tmem + kInter + 64 * st, desc_plain(base + L::kX16 + kk * 256, DK * 16),
@@ -821,9 +825,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        mma_bf16<128, 64>(tmem + kIntra, desc_plain(base + L::kCt + kk * 256, 1024),
+                        mma_bf16<128, 64>(tmem + kIntra + 64 * st, desc_plain(base + L::kCt + kk * 256, 1024),
                                           desc_plain(base + L::kProb + kk * 256, 1024), kk > 0);
-                    tc_commit(&M.oready);
+                    tc_commit(&M.oready[st]);
                 }
                 tc_commit(&M.empty[st]);
             }
@@ -832,92 +836,58 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_commit(&M.drain);
             mbar_wait(&M.drain, 0, nullptr);
         }
-    } else {
-        const int ew = warp - 2, sub = warp & 3, part = ew >> 2;      // TMEM lanes 32 sub ..; this warp's fourth of the columns
-        const int et = threadIdx.x - 64;
+    } else if (warp < 4 + kTcGroup) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const int ew = warp - 4, sub = warp & 3, half = ew >> 2;      // rows 16 sub and columns 32 half of P; 16 columns of c and b
+        const int et = threadIdx.x - 128;
         const int l7 = lane & 7, l8 = (lane >> 3) & 1, l16 = lane >> 4, q = lane & 3, g8 = lane >> 2;
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * sub) << 16);
         const float g = p.log_decay[head];
-        const int row = tile * kTcCols + 32 * sub + lane;             // column of c
-        const int64_t sh = (static_cast<int64_t>(u.seq) * p.heads + head) * db * dc;
-        const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
-        constexpr int kX = DK / 4;
-        const int x0 = part * kX;                                     // first row of b's dimension of this thread
-        float x[kX];
-        const bool given = !STATE_ONLY && (p.seg != nullptr || p.s_in != nullptr) && row < dc;
-#pragma unroll
-        for (int i = 0; i < kX; ++i) {
-            x[i] = 0.0f;
-            if (given && x0 + i < db)
-                x[i] = p.seg ? p.seg[gh + static_cast<int64_t>(x0 + i) * dc + row] : p.s_in[sh + (x0 + i) * p.s_i + row * p.s_j] * p.in_mul;
-        }
-        // the bf16 copy of this thread's part of the state: 16-byte rows of core matrices
-        auto copy_state = [&]() {
-            const uint32_t at = base + L::kX16 + ((32 * sub + lane) >> 3) * (DK * 16) + (lane & 7) * 16 + (x0 / 8) * 128;
-#pragma unroll
-            for (int i = 0; i < kX; i += 8)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 16), "r"(bf16x2(x[i], x[i + 1])),
-                             "r"(bf16x2(x[i + 2], x[i + 3])), "r"(bf16x2(x[i + 4], x[i + 5])), "r"(bf16x2(x[i + 6], x[i + 7]))
-                             : "memory");
-            proxy_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&M.x16);
-        };
-        if (!STATE_ONLY && chunks > 0) copy_state();
-        if (et < 127) M.lag[et] = p.out_mul * ((p.reverse ? et <= 63 : et >= 63) ? decay_power(g, p.reverse ? 63 - et : et - 63) : 0.0f);
-        float whole = 0.0f;
+        if (!STATE_ONLY && et < 127)
+            M.lag[et] = p.out_mul * ((p.reverse ? et <= 63 : et >= 63) ? decay_power(g, p.reverse ? 63 - et : et - 63) : 0.0f);
         bool ok = true;
         for (int c = 0; c < chunks; ++c) {
             const int st = c & 1, n = tokens(c);
             const uint32_t ph = c & 1;
             const uint32_t sb = base + L::kHead + st * L::kStage + L::kTilesA * L::kTile, sc = sb + L::kTilesB * L::kTile;
-            // everybody is done with the last chunk's tiles and factors
-            asm volatile("bar.sync 1, 512;" ::: "memory");
+            if (c > 0) {                 // the last chunk's tiles have been read
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph ^ 1u, abort));
+                if (!STATE_ONLY) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.oready[st ^ 1], ((c - 1) >> 1) & 1, abort));
+            }
             if (c == 0 || n < kChunk) {
-                if (et < kChunk) {
-                    const int pos = p.reverse ? n - 1 - et : et;
-                    M.w[et] = et < n ? decay_power(g, n - p.off - pos) : 0.0f;
-                    M.out[et] = et < n ? p.out_mul * decay_power(g, pos + p.off) : 0.0f;
-                }
-                whole = decay_power(g, n);
-                asm volatile("bar.sync 1, 512;" ::: "memory");
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (et < kChunk) M.w[et] = et < n ? decay_power(g, n - p.off - (p.reverse ? n - 1 - et : et)) : 0.0f;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
             }
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
             if (ok) {
-                // (1) c^T, its terms and b^T, in blocks of 16 columns by 16 tokens: two of c and two (DK = 64: one) of b a warp
-                constexpr int kCb = 2, kBb = DK / 64;
-                const int ccol = ew & 7, ckk = kCb * (ew >> 3), bcol = DK == 128 ? ew & 7 : ew & 3, bkk = DK == 128 ? 2 * (ew >> 3) : ew >> 2;
-                const uint32_t lrow = (l7 + 8 * l16) * 128, trow = l8 * 1024 + l16 * 128 + l7 * 16;
-                const uint32_t cfrom = sc + (ccol >> 2) * L::kTile + lrow + (((2 * (ccol & 3) + l8) ^ l7) << 4) + ckk * 2048;
-                const uint32_t bfrom = sb + (bcol >> 2) * L::kTile + lrow + (((2 * (bcol & 3) + l8) ^ l7) << 4) + bkk * 2048;
-                const uint32_t cto = 2 * ccol * 1024 + trow + ckk * 256, bto = 2 * bcol * 1024 + trow + bkk * 256;
-                uint32_t fc[kCb][4], fb[kBb][4];
+                // (1) 16 columns, 16 tokens at a time
+                const uint32_t to = (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
+                const uint32_t from = (ew >> 2) * L::kTile + (l7 + 8 * l16) * 128 + (((2 * (ew & 3) + l8) ^ l7) << 4);
+                uint32_t f[4][4];
 #pragma unroll
-                for (int i = 0; i < kCb; ++i) ldsm4t_at(fc[i], cfrom + i * 2048);
-#pragma unroll
-                for (int i = 0; i < kBb; ++i) ldsm4t_at(fb[i], bfrom + i * 2048);
+                for (int kk = 0; kk < 4; ++kk) ldsm4t_at(f[kk], sc + from + kk * 2048);
                 if (n < kChunk) {
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        auto keep = [&](int kk) {
+                    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
                             const int j = kk * 16 + (h >> 1) * 8 + 2 * q;
-                            return j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
-                        };
-#pragma unroll
-                        for (int i = 0; i < kCb; ++i) fc[i][h] &= keep(ckk + i);
-#pragma unroll
-                        for (int i = 0; i < kBb; ++i) fb[i][h] &= keep(bkk + i);
-                    }
+                            f[kk][h] &= j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
+                        }
                 }
+                float finite = 0.0f;                     // stays 0 while all values are numbers
 #pragma unroll
-                for (int i = 0; i < kCb; ++i) {
+                for (int kk = 0; kk < 4; ++kk) {
                     uint32_t term[TERMS][4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float2 w = *reinterpret_cast<const float2*>(&M.w[(ckk + i) * 16 + 8 * h + 2 * q]);
+                        const float2 w = *reinterpret_cast<const float2*>(&M.w[kk * 16 + 8 * h + 2 * q]);
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            float y = low_f32(fc[i][2 * h + r]) * w.x, z = high_f32(fc[i][2 * h + r]) * w.y;
+                            float y = low_f32(f[kk][2 * h + r]), z = high_f32(f[kk][2 * h + r]);
+                            finite = fmaf(y, 0.0f, fmaf(z, 0.0f, finite));
+                            y *= w.x;
+                            z *= w.y;
 #pragma unroll
                             for (int k = 0; k < TERMS; ++k) {
                                 const uint32_t b2 = bf16x2(y, z);
@@ -929,141 +899,218 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             }
                         }
                     }
-                    if (!STATE_ONLY) stsm4(base + L::kCt + cto + i * 256, fc[i][0], fc[i][1], fc[i][2], fc[i][3]);
 #pragma unroll
                     for (int k = 0; k < TERMS; ++k)
-                        stsm4(base + L::kWt + k * 128 * 128 + cto + i * 256, term[k][0], term[k][1], term[k][2], term[k][3]);
+                        stsm4(base + L::kWt + k * 128 * 128 + to + kk * 256, term[k][0], term[k][1], term[k][2], term[k][3]);
                 }
+                if constexpr (!STATE_ONLY) {
+                    const bool bad = __any_sync(0xffffffffu, finite != 0.0f);
+                    if (bad) {
+                        int first[2] = {255, 255};
 #pragma unroll
-                for (int i = 0; i < kBb; ++i) stsm4(base + L::kBt + bto + i * 256, fb[i][0], fb[i][1], fb[i][2], fb[i][3]);
+                        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const uint32_t part = e ? f[kk][h] >> 16 : f[kk][h] & 0xffffu;
+                                    if ((part & 0x7f80u) != 0x7f80u) continue;
+                                    f[kk][h] &= e ? 0xffffu : 0xffff0000u;
+                                    const int j = kk * 16 + (h >> 1) * 8 + 2 * q + e;
+                                    first[h & 1] = min(first[h & 1], p.reverse ? n - 1 - j : j);
+                                }
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 1));
+                            first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 2));
+                            if (q == 0) M.first_bad[st][16 * ew + 8 * r + g8] = static_cast<uint8_t>(first[r]);
+                        }
+                    }
+                    if (lane == 0) M.bad[st][ew] = bad;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) stsm4(base + L::kCt + to + kk * 256, f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
+                }
+                if (ew < DK / 16) {
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) ldsm4t_at(f[kk], sb + from + kk * 2048);
+                    if (n < kChunk) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                const int j = kk * 16 + (h >> 1) * 8 + 2 * q;
+                                f[kk][h] &= j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
+                            }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) stsm4(base + L::kBt + to + kk * 256, f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
+                }
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&M.vk);
             }
             if constexpr (!STATE_ONLY) {
-                // (2) P
+                // (2) rows i = 16 sub + g and + 8, columns j = 32 half + 8 nt + 2 q and + 1: v[4 nt ..]
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.pready, ph, abort));
                 if (ok) {
                     tc_fence_after();
-                    // rows i = 16 sub + g and + 8, columns j = 16 part + 8 nt + 2 q and + 1: v[4 nt ..]
-                    uint32_t v[8];
-                    tc_ld_frag(lanes + kP + 16 * part, v);
-                    tc_wait_ld8(v);
-                    const int i = 16 * sub + g8, j0 = 16 * part + 2 * q, jn = n - j0;
+                    uint32_t v[16];
+                    tc_ld_frag(tmem + (static_cast<uint32_t>(32 * sub) << 16) + kP + 32 * half, v);
+                    tc_wait_ld16(v);
+                    const int i = 16 * sub + g8, j0 = 32 * half + 2 * q;
                     const float* lag = &M.lag[63 + i - j0];
-                    const int d = i - j0;
-                    uint32_t r[4];
+                    // token j of column e from here counts for token i if before < e <= upto
+                    const int d = i - j0, before = p.reverse ? d - 1 : -1000, upto = p.reverse ? n - 1 - j0 : d;
+                    uint32_t r[8];
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
+                    for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const int e = 8 * nt - 8 * h;                // token j - token i is e - d
-                            // in reverse the tokens past the sequence's end come before: they are masked here
-                            const bool s0 = p.reverse ? d <= e && 8 * nt < jn : d >= e, s1 = p.reverse ? d <= e + 1 && 8 * nt + 1 < jn : d >= e + 1;
+                            const int e = 8 * nt - 8 * h;                // against row i + 8 h
+                            // in reverse the tokens past the sequence's end come before: they are masked by upto
+                            const bool s0 = e > before && (p.reverse ? 8 * nt : e) <= upto;
+                            const bool s1 = e + 1 > before && (p.reverse ? 8 * nt + 1 : e + 1) <= upto;
                             r[2 * nt + h] = bf16x2(s0 ? __uint_as_float(v[4 * nt + 2 * h]) * lag[-e] : 0.0f,
                                                    s1 ? __uint_as_float(v[4 * nt + 2 * h + 1]) * lag[-e - 1] : 0.0f);
                         }
-                    // matrices (rows 0-7, 8-15) x (columns 0-7, 8-15)
-                    stsm4(base + L::kProb + (2 * sub + l8) * 1024 + (2 * part + l16) * 128 + l7 * 16, r[0], r[1], r[2], r[3]);
+                    // matrices (rows 0-7, 8-15) x (columns 8 nt, 8 nt + 8)
+                    const uint32_t at = base + L::kProb + (2 * sub + l8) * 1024 + (4 * half + l16) * 128 + l7 * 16;
+                    stsm4(at, r[0], r[1], r[2], r[3]);
+                    stsm4(at + 256, r[4], r[5], r[6], r[7]);
                     tc_fence_before();
                     proxy_fence();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&M.psm);
                 }
             }
+        }
+        if (!ok && lane == 0) fail();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        const int ew = warp - 4 - kTcGroup, sub = warp & 3, half = ew >> 2;   // TMEM lanes 32 sub ..; half of their columns
+        const int et = threadIdx.x - 128 - 32 * kTcGroup;
+        const int q = lane & 3;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * sub) << 16);
+        const float g = p.log_decay[head];
+        const int row = tile * kTcCols + 32 * sub + lane;             // column of c
+        const int64_t sh = (static_cast<int64_t>(u.seq) * p.heads + head) * db * dc;
+        const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
+        constexpr int kX = DK / 2;
+        const int x0 = half * kX;                                     // first row of b's dimension of this thread
+        float x[kX];
+        const bool given = !STATE_ONLY && (p.seg != nullptr || p.s_in != nullptr) && row < dc;
+#pragma unroll
+        for (int i = 0; i < kX; ++i) {
+            x[i] = 0.0f;
+            if (given && x0 + i < db)
+                x[i] = p.seg ? p.seg[gh + static_cast<int64_t>(x0 + i) * dc + row] : p.s_in[sh + (x0 + i) * p.s_i + row * p.s_j] * p.in_mul;
+        }
+        // the bf16 copy of this thread's part of the state, in 16-byte rows of core matrices; U has been read
+        auto copy_state = [&]() {
+            if constexpr (!STATE_ONLY) {
+                const uint32_t at = base + L::kX16 + ((32 * sub + lane) >> 3) * (DK * 16) + (lane & 7) * 16 + (x0 / 8) * 128;
+#pragma unroll
+                for (int i = 0; i < kX; i += 8)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 16), "r"(bf16x2(x[i], x[i + 1])),
+                                 "r"(bf16x2(x[i + 2], x[i + 3])), "r"(bf16x2(x[i + 4], x[i + 5])), "r"(bf16x2(x[i + 6], x[i + 7]))
+                                 : "memory");
+                proxy_fence();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&M.x16);
+        };
+        if (chunks > 0) copy_state();
+        float whole = 0.0f;
+        bool ok = true;
+        for (int c = 0; c < chunks; ++c) {
+            const int st = c & 1, n = tokens(c);
+            const uint32_t ph = c & 1;
+            if (c == 0 || n < kChunk) {
+                asm volatile("bar.sync 2, 256;" ::: "memory");
+                if (et < kChunk) M.out[et] = et < n ? p.out_mul * decay_power(g, (p.reverse ? n - 1 - et : et) + p.off) : 0.0f;
+                whole = decay_power(g, n);
+                asm volatile("bar.sync 2, 256;" ::: "memory");
+            }
             // (3) the state
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph, abort));
-            bool bad = false;
             if (ok) {
                 tc_fence_after();
-                uint32_t v[kX];
-                tc_ld16(lanes + kU + x0, v);
-                if constexpr (kX == 32) {
-                    tc_ld16(lanes + kU + x0 + 16, v + 16);
-                    tc_wait_ld16(v + 16);
-                }
-                tc_wait_ld16(v);
-                // a column of c with a value that is no number shows in every element of its row of U
-                bad = !(fabsf(__uint_as_float(v[0])) <= 3.4028234e38f);
 #pragma unroll
-                for (int i = 0; i < kX; ++i) x[i] = fmaf(whole, x[i], __uint_as_float(v[i]));
+                for (int i0 = 0; i0 < kX; i0 += 16) {
+                    uint32_t v[16];
+                    tc_ld16(lanes + kU + x0 + i0, v);
+                    tc_wait_ld16(v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i0 + i] = fmaf(whole, x[i0 + i], __uint_as_float(v[i]));
+                }
                 tc_fence_before();
-                if (!STATE_ONLY && c + 1 < chunks) copy_state();
+                if (c + 1 < chunks) copy_state();
             }
             if constexpr (!STATE_ONLY) {
-                // (4) the results: 16 tokens of this lane's column
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.oready, ph, abort));
+                // (4) the results: 32 tokens of this lane's column
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.oready[st], (c >> 1) & 1, abort));
                 if (ok) {
                     tc_fence_after();
-                    const int m = n - 16 * part;         // tokens of this part
-                    uint32_t a[16], b[16];
-                    tc_ld16(lanes + kIntra + 16 * part, a);
-                    tc_ld16(lanes + kInter + 64 * st + 16 * part, b);
-                    tc_wait_ld16(a);
-                    tc_wait_ld16(b);
+                    const bool bad = (M.bad[st][2 * sub] | M.bad[st][2 * sub + 1]) != 0;
+                    unsigned char* own = smem + L::kOut + ew * 1024;
+                    const int64_t at = (u.row0 + first(c) + 32 * half) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head;
+                    // this lane's place when results leave eight tokens at a time
+                    const int t8 = lane >> 2, j8 = tile * kTcCols + 32 * sub + 8 * q;
+                    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + at + t8 * p.o_tok + j8;
 #pragma unroll
-                    for (int t = 0; t < 16; t += 4) {
-                        const float4 w = *reinterpret_cast<const float4*>(&M.out[16 * part + t]);
-                        a[t] = __float_as_uint(fmaf(w.x, __uint_as_float(b[t]), __uint_as_float(a[t])));
-                        a[t + 1] = __float_as_uint(fmaf(w.y, __uint_as_float(b[t + 1]), __uint_as_float(a[t + 1])));
-                        a[t + 2] = __float_as_uint(fmaf(w.z, __uint_as_float(b[t + 2]), __uint_as_float(a[t + 2])));
-                        a[t + 3] = __float_as_uint(fmaf(w.w, __uint_as_float(b[t + 3]), __uint_as_float(a[t + 3])));
-                    }
-                    const int64_t at = (u.row0 + first(c) + 16 * part) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head;
-                    // bf16 results pass through 1 KB of this warp's own (the terms were read when U was done)
-                    unsigned char* own = smem + L::kWt + ew * 1024;
-                    if (p.o_f32) {
-                        float* to = static_cast<float*>(p.o) + at + row;
+                    for (int t0 = 0; t0 < 32; t0 += 16) {
+                        const int m = n - 32 * half - t0;    // tokens left
+                        uint32_t a[16], b[16];
+                        tc_ld16(lanes + kIntra + 64 * st + 32 * half + t0, a);
+                        tc_ld16(lanes + kInter + 64 * st + 32 * half + t0, b);
+                        tc_wait_ld16(a);
+                        tc_wait_ld16(b);
 #pragma unroll
-                        for (int t = 0; t < 16; ++t, to += p.o_tok)
-                            if (t < m && row < dc) *to = __uint_as_float(a[t]);
-                    } else {
-#pragma unroll
-                        for (int t = 0; t < 16; t += 2) {
-                            const uint32_t two = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
-                            *reinterpret_cast<uint16_t*>(own + t * 64 + lane * 2) = static_cast<uint16_t>(two);
-                            *reinterpret_cast<uint16_t*>(own + (t + 1) * 64 + lane * 2) = static_cast<uint16_t>(two >> 16);
+                        for (int t = 0; t < 16; t += 4) {
+                            const float4 w = *reinterpret_cast<const float4*>(&M.out[32 * half + t0 + t]);
+                            a[t] = __float_as_uint(fmaf(w.x, __uint_as_float(b[t]), __uint_as_float(a[t])));
+                            a[t + 1] = __float_as_uint(fmaf(w.y, __uint_as_float(b[t + 1]), __uint_as_float(a[t + 1])));
+                            a[t + 2] = __float_as_uint(fmaf(w.z, __uint_as_float(b[t + 2]), __uint_as_float(a[t + 2])));
+                            a[t + 3] = __float_as_uint(fmaf(w.w, __uint_as_float(b[t + 3]), __uint_as_float(a[t + 3])));
                         }
-                    }
-                    if (__any_sync(0xffffffffu, bad)) {
-                        // sum again over the tokens that count alone
-#pragma unroll 1
-                        for (int t = 0; t < 16; ++t) {
-                            const int i = 16 * part + t;
-                            const unsigned char* pp = smem + L::kProb + (i >> 3) * 1024 + (i & 7) * 16;
-                            const unsigned char* cc = smem + L::kCt + (4 * sub + (lane >> 3)) * 1024 + l7 * 16;
-                            uint32_t entering;
-                            tc_ld1(lanes + kInter + 64 * st + i, entering);
-                            float y = 0.0f;
-#pragma unroll 1
-                            for (int j = p.reverse ? i : 0; j < (p.reverse ? n : i + 1); ++j)
-                                y = fmaf(to_f32(*reinterpret_cast<const __nv_bfloat16*>(pp + (j >> 3) * 128 + (j & 7) * 2)),
-                                         to_f32(*reinterpret_cast<const __nv_bfloat16*>(cc + (j >> 3) * 128 + (j & 7) * 2)), y);
-                            y = fmaf(M.out[i], __uint_as_float(entering), y);
-                            if (!p.o_f32) *reinterpret_cast<__nv_bfloat16*>(own + t * 64 + lane * 2) = __float2bfloat16_rn(y);
-                            else if (t < m && row < dc) static_cast<float*>(p.o)[at + t * p.o_tok + row] = y;
+                        if (bad && M.bad[st][2 * sub + (lane >> 4)]) {
+                            const int from = M.first_bad[st][32 * sub + lane];
+#pragma unroll
+                            for (int t = 0; t < 16; ++t) {
+                                const int i = 32 * half + t0 + t;
+                                if ((p.reverse ? n - 1 - i : i) >= from) a[t] = 0x7fffffffu;
+                            }
                         }
-                    }
-                    tc_fence_before();
-                    if (!p.o_f32) {
-                        __syncwarp();
-                        // 64 bytes a token, eight tokens at a time
-                        const int t = lane >> 2, j = tile * kTcCols + 32 * sub + 8 * q;
-                        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + at + t * p.o_tok + j;
+                        if (p.o_f32) {
+                            float* f = static_cast<float*>(p.o) + at + t0 * p.o_tok + row;
 #pragma unroll
-                        for (int k = 0; k < 2; ++k, to += 8 * p.o_tok) {
-                            const uint4 r = *reinterpret_cast<const uint4*>(own + (8 * k + t) * 64 + q * 16);
-                            if (8 * k + t >= m || j >= dc) continue;
-                            if (p.o_vec) {
-                                *reinterpret_cast<uint4*>(to) = r;
-                            } else {
-                                const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&r);
+                            for (int t = 0; t < 16; ++t, f += p.o_tok)
+                                if (t < m && row < dc) *f = __uint_as_float(a[t]);
+                        } else {
+                            __syncwarp();
 #pragma unroll
-                                for (int x8 = 0; x8 < 8; ++x8)
-                                    if (j + x8 < dc) to[x8] = e[x8];
+                            for (int t = 0; t < 16; t += 2) {
+                                const uint32_t two = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
+                                *reinterpret_cast<uint16_t*>(own + t * 64 + lane * 2) = static_cast<uint16_t>(two);
+                                *reinterpret_cast<uint16_t*>(own + (t + 1) * 64 + lane * 2) = static_cast<uint16_t>(two >> 16);
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (int k = 0; k < 2; ++k, to += 8 * p.o_tok) {
+                                const uint4 r = *reinterpret_cast<const uint4*>(own + (8 * k + t8) * 64 + q * 16);
+                                if (8 * k + t8 >= m || j8 >= dc) continue;
+                                if (p.o_vec) {
+                                    *reinterpret_cast<uint4*>(to) = r;
+                                } else {
+                                    const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&r);
+#pragma unroll
+                                    for (int x8 = 0; x8 < 8; ++x8)
+                                        if (j8 + x8 < dc) to[x8] = e[x8];
+                                }
                             }
                         }
                     }
+                    tc_fence_before();
                 }
             }
         }
