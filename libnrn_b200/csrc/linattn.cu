@@ -640,18 +640,15 @@ struct TcSmem {
     static constexpr int kTilesA = STATE_ONLY ? 0 : DK / 64, kTilesB = DK / 64, kTilesC = 2;
     static constexpr int kStage = (kTilesA + kTilesB + kTilesC) * kTile;
     static constexpr int kHead = 2048;
-    static constexpr int kCt = kHead + 2 * kStage;                    // c^T [128][64]
-    static constexpr int kWt = kCt + (STATE_ONLY ? 0 : 128 * 128);    // its terms
-    static constexpr int kBt = kWt + TERMS * 128 * 128;               // b^T [DK][64]
-    static constexpr int kX16 = kBt + DK * 128;                       // [128][DK]
-    static constexpr int kProb = kX16 + (STATE_ONLY ? 0 : 128 * DK * 2);   // [64][64]
+    static constexpr int kBt = kHead + 2 * kStage;                    // b^T [DK][64]
+    static constexpr int kProb = kBt + DK * 128;                      // [64][64]
     static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 1 KB for each warp of results
     static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 1024);
 };
 static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
 
 struct TcHead {
-    uint64_t full[2], empty[2], oready[2], pready, psm, x16, vk, uready, drain;
+    uint64_t full[2], empty[2], oready[2], pready, psm, x16, vk, uready, odone, drain;
     uint32_t tmem;
     int abort;
     alignas(16) float lag[128];    // factor of P at token i - token j, from -63 on
@@ -673,6 +670,40 @@ __device__ __forceinline__ uint64_t desc_swizzled(uint32_t addr) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
 }
+// The same with A in TMEM: lane = row, two elements of K a column.
+template <int NN>
+__device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint64_t b, bool accumulate) {
+    constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NN >> 3) << 17) | (128u >> 4 << 24);
+    const uint32_t zero = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(zero)
+        : "memory");
+}
+// One thread of a converged warp, chosen so that the compiler keeps what the warp computed alike in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+// 16 lanes by 32 columns from eight pairs of fragment registers (row g and g + 8 of four columns each).
+__device__ __forceinline__ void tc_st_frag(uint32_t taddr, const uint32_t (&v)[4][4]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(v[0][0]), "r"(v[0][1]), "r"(v[0][2]), "r"(v[0][3]), "r"(v[1][0]), "r"(v[1][1]), "r"(v[1][2]), "r"(v[1][3]), "r"(v[2][0]),
+        "r"(v[2][1]), "r"(v[2][2]), "r"(v[2][3]), "r"(v[3][0]), "r"(v[3][1]), "r"(v[3][2]), "r"(v[3][3])
+        : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int MM, int NN>
 __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, bool accumulate) {
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NN >> 3) << 17) | (static_cast<uint32_t>(MM >> 4) << 24);
@@ -716,7 +747,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     TcHead& M = *reinterpret_cast<TcHead*>(smem);
     const uint32_t base = smem_u32(smem);
     volatile int* abort = &M.abort;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int db = p.b.d, dc = p.c.d;
     const int tiles = (dc + kTcCols - 1) / kTcCols;
     const int tile = blockIdx.x % tiles;
@@ -725,7 +756,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const Unit u = unit_of(p, unit);
     if (!u.any) return;
     const int chunks = static_cast<int>((u.end - u.begin + kChunk - 1) / kChunk);
-    constexpr uint32_t kP = 0, kU = 64, kIntra = 192, kInter = 320;      // TMEM columns; the last two in turn
+    // TMEM columns: accumulators, then the left operands X16, c^T's terms and c^T
+    constexpr uint32_t kP = 0, kU = 64, kIntra = 192, kInter = 256, kX16 = 320, kWt = 384, kCt = 480;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -739,6 +771,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_init(&M.psm, kTcGroup);
         mbar_init(&M.x16, kTcGroup);
         mbar_init(&M.vk, kTcGroup);
+        mbar_init(&M.odone, kTcGroup);
         M.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -762,7 +795,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0 && lane == 0) {
             int c = 0;
             for (; c < chunks; ++c) {
@@ -783,62 +816,78 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             // the copies still in flight land before the block ends
             for (int q = c - 1; q >= 0 && q >= c - 2; --q) mbar_wait(&M.full[q & 1], (q >> 1) & 1, nullptr);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
+            // the whole warp walks the chunks, one thread issues
+            const bool leader = elect_one();
             bool ok = true;
-            for (int c = 0; c < chunks && ok; ++c) {
+            for (int c = 0; c < chunks; ++c) {
                 const int st = c & 1;
                 const uint32_t ph = c & 1;
                 const uint32_t sa = base + L::kHead + st * L::kStage, sb = sa + L::kTilesA * L::kTile;
-                ok = mbar_wait(&M.full[st], (c >> 1) & 1, abort);
+                ok = __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
                 if (!ok) break;
                 tc_fence_after();
                 if constexpr (!STATE_ONLY) {
                     // P: the last chunk's was read before psm of that chunk, on which intra waited
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < DK / 16; ++kk)
-                        mma_bf16<64, 64>(tmem + kP, desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32),
-                                         desc_swizzled(sb + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
-                    tc_commit(&M.pready);
+                        for (int kk = 0; kk < DK / 16; ++kk)
+                            mma_bf16<64, 64>(tmem + kP, desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32),
+                                             desc_swizzled(sb + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
+                        tc_commit(&M.pready);
+                    }
+                    __syncwarp();
                 }
-                ok = mbar_wait(&M.x16, ph, abort);       // X16 is there, and U of the last chunk read
+                ok = __all_sync(0xffffffffu, mbar_wait(&M.x16, ph, abort));       // X16 is there, and U of the last chunk read
+                if (!STATE_ONLY && c > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.odone, ph ^ 1u, abort));   // and its results
                 if (!ok) break;
                 tc_fence_after();
                 if constexpr (!STATE_ONLY) {
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < DK / 16; ++kk)
-                        mma_bf16<128, 64>(tmem + kInter + 64 * st, desc_plain(base + L::kX16 + kk * 256, DK * 16),
-                                          desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
+                        for (int kk = 0; kk < DK / 16; ++kk)
+                            mma_bf16_ta<64>(tmem + kInter, tmem + kX16 + kk * 8, desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
+                    }
+                    __syncwarp();
                 }
-                ok = mbar_wait(&M.vk, ph, abort);
+                ok = __all_sync(0xffffffffu, mbar_wait(&M.vk, ph, abort));
                 if (!ok) break;
                 tc_fence_after();
+                if (leader) {
 #pragma unroll
-                for (int t = 0; t < TERMS; ++t)
+                    for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_bf16<128, DK>(tmem + kU, desc_plain(base + L::kWt + t * 128 * 128 + kk * 256, 1024),
-                                          desc_plain(base + L::kBt + kk * 256, 1024), t + kk > 0);
-                tc_commit(&M.uready);
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_bf16_ta<DK>(tmem + kU, tmem + kWt + t * 32 + kk * 8, desc_plain(base + L::kBt + kk * 256, 1024), t + kk > 0);
+                    tc_commit(&M.uready);
+                }
+                __syncwarp();
                 if constexpr (!STATE_ONLY) {
-                    ok = mbar_wait(&M.psm, ph, abort);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&M.psm, ph, abort));
                     if (!ok) break;
                     tc_fence_after();
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_bf16<128, 64>(tmem + kIntra + 64 * st, desc_plain(base + L::kCt + kk * 256, 1024),
-                                          desc_plain(base + L::kProb + kk * 256, 1024), kk > 0);
-                    tc_commit(&M.oready[st]);
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_bf16_ta<64>(tmem + kIntra, tmem + kCt + kk * 8, desc_plain(base + L::kProb + kk * 256, 1024), kk > 0);
+                        tc_commit(&M.oready[st]);
+                    }
+                    __syncwarp();
                 }
-                tc_commit(&M.empty[st]);
+                if (leader) tc_commit(&M.empty[st]);
+                __syncwarp();
             }
-            if (!ok) fail();
+            if (!ok && leader) fail();
             // every MMA issued has completed before the accumulators are freed
-            tc_commit(&M.drain);
-            mbar_wait(&M.drain, 0, nullptr);
+            if (leader) {
+                tc_commit(&M.drain);
+                mbar_wait(&M.drain, 0, nullptr);
+            }
         }
     } else if (warp < 4 + kTcGroup) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int ew = warp - 4, sub = warp & 3, half = ew >> 2;      // rows 16 sub and columns 32 half of P; 16 columns of c and b
+        const int ccol = 2 * sub + half;                              // these 16 of c: this warp's lanes of TMEM
         const int et = threadIdx.x - 128;
         const int l7 = lane & 7, l8 = (lane >> 3) & 1, l16 = lane >> 4, q = lane & 3, g8 = lane >> 2;
         const float g = p.log_decay[head];
@@ -860,12 +909,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
             if (ok) {
-                // (1) 16 columns, 16 tokens at a time
-                const uint32_t to = (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
-                const uint32_t from = (ew >> 2) * L::kTile + (l7 + 8 * l16) * 128 + (((2 * (ew & 3) + l8) ^ l7) << 4);
+                // (1) 16 columns of c
+                const uint32_t lrow = (l7 + 8 * l16) * 128;
+                const uint32_t cfrom = sc + (ccol >> 2) * L::kTile + lrow + (((2 * (ccol & 3) + l8) ^ l7) << 4);
+                const uint32_t lanes = tmem + (static_cast<uint32_t>(16 * ccol) << 16);
                 uint32_t f[4][4];
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) ldsm4t_at(f[kk], sc + from + kk * 2048);
+                for (int kk = 0; kk < 4; ++kk) ldsm4t_at(f[kk], cfrom + kk * 2048);
                 if (n < kChunk) {
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
@@ -875,61 +925,63 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             f[kk][h] &= j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
                         }
                 }
-                float finite = 0.0f;                     // stays 0 while all values are numbers
+                {
+                    float y[4][4], z[4][4], finite = 0.0f;       // stays 0 while all values are numbers
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    uint32_t term[TERMS][4];
+                    for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float2 w = *reinterpret_cast<const float2*>(&M.w[kk * 16 + 8 * h + 2 * q]);
+                        for (int h = 0; h < 4; ++h) {
+                            const float2 w = *reinterpret_cast<const float2*>(&M.w[kk * 16 + 8 * (h >> 1) + 2 * q]);
+                            y[kk][h] = low_f32(f[kk][h]);
+                            z[kk][h] = high_f32(f[kk][h]);
+                            if (!STATE_ONLY) finite = fmaf(y[kk][h], 0.0f, fmaf(z[kk][h], 0.0f, finite));
+                            y[kk][h] *= w.x;
+                            z[kk][h] *= w.y;
+                        }
+                    if constexpr (!STATE_ONLY) {
+                        const bool bad = __any_sync(0xffffffffu, finite != 0.0f);
+                        if (bad) {
+                            int first[2] = {255, 255};
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float y = low_f32(f[kk][2 * h + r]), z = high_f32(f[kk][2 * h + r]);
-                            finite = fmaf(y, 0.0f, fmaf(z, 0.0f, finite));
-                            y *= w.x;
-                            z *= w.y;
+                            for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-                            for (int k = 0; k < TERMS; ++k) {
-                                const uint32_t b2 = bf16x2(y, z);
-                                term[k][2 * h + r] = b2;
-                                if (k + 1 < TERMS) {
-                                    y -= low_f32(b2);
-                                    z -= high_f32(b2);
-                                }
+                                for (int h = 0; h < 4; ++h)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        const uint32_t part = e ? f[kk][h] >> 16 : f[kk][h] & 0xffffu;
+                                        if ((part & 0x7f80u) != 0x7f80u) continue;
+                                        f[kk][h] &= e ? 0xffffu : 0xffff0000u;
+                                        const int j = kk * 16 + (h >> 1) * 8 + 2 * q + e;
+                                        first[h & 1] = min(first[h & 1], p.reverse ? n - 1 - j : j);
+                                    }
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 1));
+                                first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 2));
+                                if (q == 0) M.first_bad[st][16 * ccol + 8 * r + g8] = static_cast<uint8_t>(first[r]);
                             }
                         }
+                        if (lane == 0) M.bad[st][ccol] = bad;
+                        tc_st_frag(lanes + kCt, f);
                     }
 #pragma unroll
-                    for (int k = 0; k < TERMS; ++k)
-                        stsm4(base + L::kWt + k * 128 * 128 + to + kk * 256, term[k][0], term[k][1], term[k][2], term[k][3]);
-                }
-                if constexpr (!STATE_ONLY) {
-                    const bool bad = __any_sync(0xffffffffu, finite != 0.0f);
-                    if (bad) {
-                        int first[2] = {255, 255};
+                    for (int k = 0; k < TERMS; ++k) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-                            for (int h = 0; h < 4; ++h)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const uint32_t part = e ? f[kk][h] >> 16 : f[kk][h] & 0xffffu;
-                                    if ((part & 0x7f80u) != 0x7f80u) continue;
-                                    f[kk][h] &= e ? 0xffffu : 0xffff0000u;
-                                    const int j = kk * 16 + (h >> 1) * 8 + 2 * q + e;
-                                    first[h & 1] = min(first[h & 1], p.reverse ? n - 1 - j : j);
+                            for (int h = 0; h < 4; ++h) {
+                                f[kk][h] = bf16x2(y[kk][h], z[kk][h]);
+                                if (k + 1 < TERMS) {
+                                    y[kk][h] -= low_f32(f[kk][h]);
+                                    z[kk][h] -= high_f32(f[kk][h]);
                                 }
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 1));
-                            first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 2));
-                            if (q == 0) M.first_bad[st][16 * ew + 8 * r + g8] = static_cast<uint8_t>(first[r]);
-                        }
+                            }
+                        tc_st_frag(lanes + kWt + 32 * k, f);
                     }
-                    if (lane == 0) M.bad[st][ew] = bad;
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) stsm4(base + L::kCt + to + kk * 256, f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
                 }
+                // and 16 of b
+                const uint32_t to = (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
+                const uint32_t from = (ew >> 2) * L::kTile + lrow + (((2 * (ew & 3) + l8) ^ l7) << 4);
                 if (ew < DK / 16) {
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) ldsm4t_at(f[kk], sb + from + kk * 2048);
@@ -945,6 +997,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) stsm4(base + L::kBt + to + kk * 256, f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
                 }
+                tc_wait_st();
+                tc_fence_before();
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&M.vk);
@@ -986,7 +1040,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (!ok && lane == 0) fail();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         const int ew = warp - 4 - kTcGroup, sub = warp & 3, half = ew >> 2;   // TMEM lanes 32 sub ..; half of their columns
         const int et = threadIdx.x - 128 - 32 * kTcGroup;
         const int q = lane & 3;
@@ -1005,16 +1059,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (given && x0 + i < db)
                 x[i] = p.seg ? p.seg[gh + static_cast<int64_t>(x0 + i) * dc + row] : p.s_in[sh + (x0 + i) * p.s_i + row * p.s_j] * p.in_mul;
         }
-        // the bf16 copy of this thread's part of the state, in 16-byte rows of core matrices; U has been read
+        // the bf16 copy of this thread's part of the state; U has been read
         auto copy_state = [&]() {
             if constexpr (!STATE_ONLY) {
-                const uint32_t at = base + L::kX16 + ((32 * sub + lane) >> 3) * (DK * 16) + (lane & 7) * 16 + (x0 / 8) * 128;
 #pragma unroll
-                for (int i = 0; i < kX; i += 8)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 16), "r"(bf16x2(x[i], x[i + 1])),
-                                 "r"(bf16x2(x[i + 2], x[i + 3])), "r"(bf16x2(x[i + 4], x[i + 5])), "r"(bf16x2(x[i + 6], x[i + 7]))
-                                 : "memory");
-                proxy_fence();
+                for (int i = 0; i < kX; i += 32) {
+                    uint32_t v[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] = bf16x2(x[i + 2 * k], x[i + 2 * k + 1]);
+                    tc_st16(lanes + kX16 + (x0 + i) / 2, v);
+                }
+                tc_wait_st();
+                tc_fence_before();
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&M.x16);
@@ -1061,10 +1117,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int t0 = 0; t0 < 32; t0 += 16) {
                         const int m = n - 32 * half - t0;    // tokens left
                         uint32_t a[16], b[16];
-                        tc_ld16(lanes + kIntra + 64 * st + 32 * half + t0, a);
-                        tc_ld16(lanes + kInter + 64 * st + 32 * half + t0, b);
+                        tc_ld16(lanes + kIntra + 32 * half + t0, a);
+                        tc_ld16(lanes + kInter + 32 * half + t0, b);
                         tc_wait_ld16(a);
                         tc_wait_ld16(b);
+                        if (t0 == 16) {                      // read: the next chunk's may come
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&M.odone);
+                        }
 #pragma unroll
                         for (int t = 0; t < 16; t += 4) {
                             const float4 w = *reinterpret_cast<const float4*>(&M.out[32 * half + t0 + t]);
@@ -1110,7 +1171,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             }
                         }
                     }
-                    tc_fence_before();
                 }
             }
         }
