@@ -642,8 +642,8 @@ struct TcSmem {
     static constexpr int kHead = 2048;
     static constexpr int kBt = kHead + 2 * kStage;                    // b^T [DK][64]
     static constexpr int kProb = kBt + DK * 128;                      // [64][64]
-    static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 1 KB for each warp of results
-    static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 1024);
+    static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 2 KB for each warp of results
+    static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 2048);
 };
 static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
 
@@ -737,6 +737,7 @@ __device__ __forceinline__ void tc_ld_frag(uint32_t taddr, uint32_t* v) {
           "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr));
 }
+constexpr uint64_t kMinusOnes = 0xbf800000bf800000ull;
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <int DK, int TERMS, bool STATE_ONLY>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -885,7 +886,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
     } else if (warp < 4 + kTcGroup) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         const int ew = warp - 4, sub = warp & 3, half = ew >> 2;      // rows 16 sub and columns 32 half of P; 16 columns of c and b
         const int ccol = 2 * sub + half;                              // these 16 of c: this warp's lanes of TMEM
         const int et = threadIdx.x - 128;
@@ -926,20 +927,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                 }
                 {
-                    float y[4][4], z[4][4], finite = 0.0f;       // stays 0 while all values are numbers
+                    uint64_t y[4][4], numbers = 0;       // two tokens' values; `numbers` stays 0 while all values are
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
-                            const float2 w = *reinterpret_cast<const float2*>(&M.w[kk * 16 + 8 * (h >> 1) + 2 * q]);
-                            y[kk][h] = low_f32(f[kk][h]);
-                            z[kk][h] = high_f32(f[kk][h]);
-                            if (!STATE_ONLY) finite = fmaf(y[kk][h], 0.0f, fmaf(z[kk][h], 0.0f, finite));
-                            y[kk][h] *= w.x;
-                            z[kk][h] *= w.y;
+                            const uint64_t w = *reinterpret_cast<const uint64_t*>(&M.w[kk * 16 + 8 * (h >> 1) + 2 * q]);
+                            y[kk][h] = pack2(f[kk][h] << 16, f[kk][h] & 0xffff0000u);
+                            if (!STATE_ONLY) numbers = fma2(y[kk][h], 0ull, numbers);
+                            y[kk][h] = mul2(y[kk][h], w);
                         }
                     if constexpr (!STATE_ONLY) {
-                        const bool bad = __any_sync(0xffffffffu, finite != 0.0f);
+                        const float2 finite = unpack2(numbers);
+                        const bool bad = __any_sync(0xffffffffu, finite.x != 0.0f || finite.y != 0.0f);
                         if (bad) {
                             int first[2] = {255, 255};
 #pragma unroll
@@ -970,11 +970,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                             for (int h = 0; h < 4; ++h) {
-                                f[kk][h] = bf16x2(y[kk][h], z[kk][h]);
-                                if (k + 1 < TERMS) {
-                                    y[kk][h] -= low_f32(f[kk][h]);
-                                    z[kk][h] -= high_f32(f[kk][h]);
-                                }
+                                const float2 v = unpack2(y[kk][h]);
+                                f[kk][h] = bf16x2(v.x, v.y);
+                                if (k + 1 < TERMS)       // what the term leaves
+                                    y[kk][h] = fma2(pack2(f[kk][h] << 16, f[kk][h] & 0xffff0000u), kMinusOnes, y[kk][h]);
                             }
                         tc_st_frag(lanes + kWt + 32 * k, f);
                     }
@@ -1040,7 +1039,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (!ok && lane == 0) fail();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
         const int ew = warp - 4 - kTcGroup, sub = warp & 3, half = ew >> 2;   // TMEM lanes 32 sub ..; half of their columns
         const int et = threadIdx.x - 128 - 32 * kTcGroup;
         const int q = lane & 3;
@@ -1051,13 +1050,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
         constexpr int kX = DK / 2;
         const int x0 = half * kX;                                     // first row of b's dimension of this thread
-        float x[kX];
+        uint64_t x[kX / 2];                                           // pairs
         const bool given = !STATE_ONLY && (p.seg != nullptr || p.s_in != nullptr) && row < dc;
 #pragma unroll
-        for (int i = 0; i < kX; ++i) {
-            x[i] = 0.0f;
-            if (given && x0 + i < db)
-                x[i] = p.seg ? p.seg[gh + static_cast<int64_t>(x0 + i) * dc + row] : p.s_in[sh + (x0 + i) * p.s_i + row * p.s_j] * p.in_mul;
+        for (int i = 0; i < kX; i += 2) {
+            float v[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (given && x0 + i + e < db)
+                    v[e] = p.seg ? p.seg[gh + static_cast<int64_t>(x0 + i + e) * dc + row] : p.s_in[sh + (x0 + i + e) * p.s_i + row * p.s_j] * p.in_mul;
+            x[i / 2] = pack2(__float_as_uint(v[0]), __float_as_uint(v[1]));
         }
         // the bf16 copy of this thread's part of the state; U has been read
         auto copy_state = [&]() {
@@ -1066,7 +1068,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int i = 0; i < kX; i += 32) {
                     uint32_t v[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) v[k] = bf16x2(x[i + 2 * k], x[i + 2 * k + 1]);
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 y = unpack2(x[i / 2 + k]);
+                        v[k] = bf16x2(y.x, y.y);
+                    }
                     tc_st16(lanes + kX16 + (x0 + i) / 2, v);
                 }
                 tc_wait_st();
@@ -1076,7 +1081,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 0) mbar_arrive(&M.x16);
         };
         if (chunks > 0) copy_state();
-        float whole = 0.0f;
+        uint64_t whole2 = 0;
         bool ok = true;
         for (int c = 0; c < chunks; ++c) {
             const int st = c & 1, n = tokens(c);
@@ -1084,7 +1089,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (c == 0 || n < kChunk) {
                 asm volatile("bar.sync 2, 256;" ::: "memory");
                 if (et < kChunk) M.out[et] = et < n ? p.out_mul * decay_power(g, (p.reverse ? n - 1 - et : et) + p.off) : 0.0f;
-                whole = decay_power(g, n);
+                const uint32_t whole = __float_as_uint(decay_power(g, n));
+                whole2 = pack2(whole, whole);
                 asm volatile("bar.sync 2, 256;" ::: "memory");
             }
             // (3) the state
@@ -1097,7 +1103,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tc_ld16(lanes + kU + x0 + i0, v);
                     tc_wait_ld16(v);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i0 + i] = fmaf(whole, x[i0 + i], __uint_as_float(v[i]));
+                    for (int i = 0; i < 16; i += 2) x[(i0 + i) / 2] = fma2(whole2, x[(i0 + i) / 2], pack2(v[i], v[i + 1]));
                 }
                 tc_fence_before();
                 if (c + 1 < chunks) copy_state();
@@ -1108,31 +1114,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (ok) {
                     tc_fence_after();
                     const bool bad = (M.bad[st][2 * sub] | M.bad[st][2 * sub + 1]) != 0;
-                    unsigned char* own = smem + L::kOut + ew * 1024;
                     const int64_t at = (u.row0 + first(c) + 32 * half) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head;
-                    // this lane's place when results leave eight tokens at a time
-                    const int t8 = lane >> 2, j8 = tile * kTcCols + 32 * sub + 8 * q;
-                    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + at + t8 * p.o_tok + j8;
+                    const int m = n - 32 * half;             // tokens of this half
+                    // bf16 results pass through 2 KB of this warp's own, two tokens a word
+                    unsigned char* own = smem + L::kOut + ew * 2048;
 #pragma unroll
                     for (int t0 = 0; t0 < 32; t0 += 16) {
-                        const int m = n - 32 * half - t0;    // tokens left
                         uint32_t a[16], b[16];
                         tc_ld16(lanes + kIntra + 32 * half + t0, a);
                         tc_ld16(lanes + kInter + 32 * half + t0, b);
                         tc_wait_ld16(a);
                         tc_wait_ld16(b);
-                        if (t0 == 16) {                      // read: the next chunk's may come
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&M.odone);
-                        }
 #pragma unroll
                         for (int t = 0; t < 16; t += 4) {
-                            const float4 w = *reinterpret_cast<const float4*>(&M.out[32 * half + t0 + t]);
-                            a[t] = __float_as_uint(fmaf(w.x, __uint_as_float(b[t]), __uint_as_float(a[t])));
-                            a[t + 1] = __float_as_uint(fmaf(w.y, __uint_as_float(b[t + 1]), __uint_as_float(a[t + 1])));
-                            a[t + 2] = __float_as_uint(fmaf(w.z, __uint_as_float(b[t + 2]), __uint_as_float(a[t + 2])));
-                            a[t + 3] = __float_as_uint(fmaf(w.w, __uint_as_float(b[t + 3]), __uint_as_float(a[t + 3])));
+                            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&M.out[32 * half + t0 + t]);
+                            const float2 lo = unpack2(fma2(w.x, pack2(b[t], b[t + 1]), pack2(a[t], a[t + 1])));
+                            const float2 hi = unpack2(fma2(w.y, pack2(b[t + 2], b[t + 3]), pack2(a[t + 2], a[t + 3])));
+                            a[t] = __float_as_uint(lo.x), a[t + 1] = __float_as_uint(lo.y);
+                            a[t + 2] = __float_as_uint(hi.x), a[t + 3] = __float_as_uint(hi.y);
                         }
                         if (bad && M.bad[st][2 * sub + (lane >> 4)]) {
                             const int from = M.first_bad[st][32 * sub + lane];
@@ -1146,30 +1145,40 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             float* f = static_cast<float*>(p.o) + at + t0 * p.o_tok + row;
 #pragma unroll
                             for (int t = 0; t < 16; ++t, f += p.o_tok)
-                                if (t < m && row < dc) *f = __uint_as_float(a[t]);
-                        } else {
-                            __syncwarp();
+                                if (t0 + t < m && row < dc) *f = __uint_as_float(a[t]);
+                        }
 #pragma unroll
-                            for (int t = 0; t < 16; t += 2) {
-                                const uint32_t two = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
-                                *reinterpret_cast<uint16_t*>(own + t * 64 + lane * 2) = static_cast<uint16_t>(two);
-                                *reinterpret_cast<uint16_t*>(own + (t + 1) * 64 + lane * 2) = static_cast<uint16_t>(two >> 16);
-                            }
-                            __syncwarp();
+                        for (int t = 0; t < 16; t += 2)
+                            *reinterpret_cast<uint32_t*>(own + (t0 + t) * 64 + lane * 4) = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&M.odone);    // read: the next chunk's may come
+                    if (!p.o_f32) {
+                        // out of there as four columns of two tokens a lane: 64 bytes a token
+                        const int t8 = 2 * (lane >> 3), j4 = tile * kTcCols + 32 * sub + 4 * (lane & 7);
+                        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + at + t8 * p.o_tok + j4;
 #pragma unroll
-                            for (int k = 0; k < 2; ++k, to += 8 * p.o_tok) {
-                                const uint4 r = *reinterpret_cast<const uint4*>(own + (8 * k + t8) * 64 + q * 16);
-                                if (8 * k + t8 >= m || j8 >= dc) continue;
-                                if (p.o_vec) {
-                                    *reinterpret_cast<uint4*>(to) = r;
-                                } else {
-                                    const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&r);
+                        for (int k = 0; k < 4; ++k, to += 8 * p.o_tok) {
+                            const uint4 r = *reinterpret_cast<const uint4*>(own + (4 * k + (lane >> 3)) * 128 + (lane & 7) * 16);
+                            const uint2 even = make_uint2(__byte_perm(r.x, r.y, 0x5410), __byte_perm(r.z, r.w, 0x5410));
+                            const uint2 odd = make_uint2(__byte_perm(r.x, r.y, 0x7632), __byte_perm(r.z, r.w, 0x7632));
+                            const int left = m - 8 * k - t8;
+                            if (j4 >= dc) continue;
+                            if (p.o_vec) {
+                                if (left > 0) *reinterpret_cast<uint2*>(to) = even;
+                                if (left > 1) *reinterpret_cast<uint2*>(to + p.o_tok) = odd;
+                            } else {
+                                const __nv_bfloat16 *e0 = reinterpret_cast<const __nv_bfloat16*>(&even), *e1 = reinterpret_cast<const __nv_bfloat16*>(&odd);
 #pragma unroll
-                                    for (int x8 = 0; x8 < 8; ++x8)
-                                        if (j8 + x8 < dc) to[x8] = e[x8];
+                                for (int e = 0; e < 4; ++e) {
+                                    if (j4 + e >= dc) continue;
+                                    if (left > 0) to[e] = e0[e];
+                                    if (left > 1) to[p.o_tok + e] = e1[e];
                                 }
                             }
                         }
+                        __syncwarp();
                     }
                 }
             }
@@ -1179,8 +1188,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int i = 0; i < kX; ++i) {
                 if (x0 + i >= db) continue;
-                if (STATE_ONLY) to[gh + static_cast<int64_t>(x0 + i) * dc + row] = x[i];
-                else to[sh + (x0 + i) * p.s_i + row * p.s_j] = x[i] * p.end_mul;
+                const float2 y = unpack2(x[i / 2]);
+                const float v = i & 1 ? y.y : y.x;
+                if (STATE_ONLY) to[gh + static_cast<int64_t>(x0 + i) * dc + row] = v;
+                else to[sh + (x0 + i) * p.s_i + row * p.s_j] = v * p.end_mul;
             }
         }
         if (!ok && lane == 0) fail();
