@@ -1206,8 +1206,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 //
 // The segments' own end states (from zero) become the states that enter
 // them: X_{g+1} = lam^len(g) X_g + E_g with X_0 the given state; the state
-// after the last segment is the final one.  One thread an element.
-__global__ void scan_join_kernel(const __grid_constant__ ScanArgs p) {
+// after the last segment is the final one.  One thread an element (two at
+// once where they lie in pairs), the loads of four segments in flight; a
+// segment's state is read and written once.
+template <int V>
+__global__ void __launch_bounds__(128) scan_join_kernel(const __grid_constant__ ScanArgs p) {
+    __shared__ float power[2];
     const int64_t n = static_cast<int64_t>(p.b.d) * p.c.d;
     const int head = blockIdx.y % p.heads, seq = blockIdx.y / p.heads;
     int64_t len = p.tokens, first;
@@ -1218,22 +1222,49 @@ __global__ void scan_join_kernel(const __grid_constant__ ScanArgs p) {
         len = b > a ? b - a : 0;
         first = a / p.seg_len + seq;
     }
-    const float whole = decay_power(p.log_decay[head], p.seg_len);
     const int64_t segs = (len + p.seg_len - 1) / p.seg_len;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n;
-         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t i = e / p.c.d, j = e - i * p.c.d;
-        const int64_t sh = (static_cast<int64_t>(seq) * p.heads + head) * n;
-        float x = p.s_in ? p.s_in[sh + i * p.s_i + j * p.s_j] * p.in_mul : 0.0f;
-        for (int64_t g = 0; g < segs; ++g) {
-            float* at = p.seg + ((first + g) * p.heads + head) * n + e;
-            const float own = *at;
-            *at = x;
-            const int64_t m = len - g * p.seg_len;
-            x = fmaf(m < p.seg_len ? decay_power(p.log_decay[head], m) : whole, x, own);
-        }
-        if (p.s_out) p.s_out[sh + i * p.s_i + j * p.s_j] = x * p.end_mul;
+    if (threadIdx.x == 0) power[0] = decay_power(p.log_decay[head], p.seg_len);
+    if (threadIdx.x == 32) power[1] = decay_power(p.log_decay[head], len - (segs - 1) * p.seg_len);
+    __syncthreads();
+    const int64_t e = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * V;
+    if (e >= n) return;
+    const int64_t sh = (static_cast<int64_t>(seq) * p.heads + head) * n;
+    float x[V];
+    int64_t at_state[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int64_t i = (e + v) / p.c.d, j = e + v - i * p.c.d;
+        at_state[v] = sh + i * p.s_i + j * p.s_j;
+        x[v] = p.s_in ? p.s_in[at_state[v]] * p.in_mul : 0.0f;
     }
+    const int64_t step = static_cast<int64_t>(p.heads) * n;
+    float* at = p.seg + (first * p.heads + head) * n + e;
+    for (int64_t g = 0; g < segs; g += 4) {
+        float own[4][V];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) own[k][v] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (g + k >= segs) break;
+            if constexpr (V == 2) *reinterpret_cast<float2*>(own[k]) = *reinterpret_cast<const float2*>(at + k * step);
+            else own[k][0] = at[k * step];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (g + k >= segs) break;
+            if constexpr (V == 2) *reinterpret_cast<float2*>(at + k * step) = make_float2(x[0], x[1]);
+            else at[k * step] = x[0];
+            const float w = power[g + k == segs - 1];
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = fmaf(w, x[v], own[k][v]);
+        }
+        at += 4 * step;
+    }
+    if (p.s_out)
+#pragma unroll
+        for (int v = 0; v < V; ++v) p.s_out[at_state[v]] = x[v] * p.end_mul;
 }
 
 // Sums the partial gradients of `share` heads that read one key or value
@@ -1488,8 +1519,10 @@ nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, cudaStream_t s) {
         p.seg = static_cast<float*>(a->workspace);
         NRN_CUDA_TRY(launch_scan(p, a->dtype, true, s));
         const int64_t n = static_cast<int64_t>(p.b.d) * p.c.d;
-        const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 64)), static_cast<unsigned>(p.seqs * p.heads));
-        scan_join_kernel<<<grid, 256, 0, s>>>(p);
+        const int v = n % 2 == 0 ? 2 : 1;      // every state starts on an even element then
+        const dim3 grid(static_cast<unsigned>((n / v + 127) / 128), static_cast<unsigned>(p.seqs * p.heads));
+        if (v == 2) scan_join_kernel<2><<<grid, 128, 0, s>>>(p);
+        else scan_join_kernel<1><<<grid, 128, 0, s>>>(p);
         NRN_CUDA_TRY(cudaGetLastError());
     }
     NRN_CUDA_TRY(launch_scan(p, a->dtype, false, s));
