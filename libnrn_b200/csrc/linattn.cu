@@ -1461,20 +1461,42 @@ cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, cudaStrea
 
 int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
 
-// Tokens of a segment.  A scan is serial in time, so its parallelism is
-// sequences x heads x 64-column tiles; where that leaves most SMs idle the
-// sequences are split.
+// Tokens of a segment.  A scan is serial in time and one block holds an SM, so
+// its parallelism is sequences x heads x 128-column tiles; where that leaves
+// SMs idle, or a last round of blocks nearly empty, the sequences are split.
+// Splitting costs a pass over b and c for the segments' states and the join,
+// so the least time is looked for, by a model of microseconds measured on
+// d 128: 2.0 a chunk and 8 a block, 1.2 and 6 for the states, 4 for the join
+// and its bytes.  Packed sequences' lengths are not known here: their segments
+// are counted as if half of them were cut short.
 int64_t segment_length(const nrn_linattn_t* a, int dc) {
-    const int64_t tiles = (dc + kTcCols - 1) / kTcCols;
-    const int64_t want = sm_count();                          // blocks that fill the GPU
-    const int64_t rows = static_cast<int64_t>(a->heads) * tiles;
-    const int64_t all = a->cu_seqlens ? a->tokens : a->tokens * a->seqs;
-    if (all == 0) return kChunk;
-    const int64_t units = std::max<int64_t>(1, want / rows);          // segments of all sequences together
-    const bool whole = a->cu_seqlens == nullptr && a->seqs * 2 >= units;
-    if (whole) return std::max<int64_t>(kChunk, (a->tokens + kChunk - 1) / kChunk * kChunk);
-    const int64_t len = std::max<int64_t>(8 * kChunk, ((all + units - 1) / units + kChunk - 1) / kChunk * kChunk);
-    return len;
+    const int64_t rows = static_cast<int64_t>(a->heads) * ((dc + kTcCols - 1) / kTcCols), sms = sm_count();
+    const bool packed = a->cu_seqlens != nullptr;
+    const int64_t chunks = (a->tokens + kChunk - 1) / kChunk;              // of each sequence, or of all packed ones
+    if (chunks <= 1) return kChunk;
+    const auto rounds = [&](double blocks) {
+        const double r = blocks / static_cast<double>(sms);
+        return packed ? std::max(1.0, r + 0.5) : std::ceil(r);
+    };
+    int64_t best = 0;
+    double cost = 1e300;
+    for (int64_t k = 1; k <= std::min<int64_t>(chunks, 4 * sms); ++k) {     // segments of a sequence, or of all
+        const int64_t s = (chunks + k - 1) / k;
+        const double units = packed ? static_cast<double>(chunks) / s + 0.5 * a->seqs
+                                    : static_cast<double>(a->seqs) * ((chunks + s - 1) / s);
+        const double r = rounds(units * rows);
+        double t = r * (2.0 * s + 8.0);
+        // packed sequences that are whole: the longest is about twice the mean
+        if (packed && k == 1) t = std::max(rounds(static_cast<double>(a->seqs) * rows) * (2.0 * chunks / std::max(1, a->seqs) + 8.0),
+                                           2.0 * std::min<double>(chunks, 2.0 * chunks / std::max(1, a->seqs)) + 8.0);
+        else if (k > 1) t += r * (1.2 * s + 6.0) + 4.0 + units * rows * a->dk * static_cast<double>(std::min(dc, kTcCols)) * 8.0 / 3e6;
+        if (t < cost) {
+            cost = t;
+            best = s;
+        }
+        if (units * rows > 4.0 * sms) break;
+    }
+    return best * kChunk;
 }
 
 int64_t unit_count(const nrn_linattn_t* a, int64_t seg_len) {
