@@ -1269,20 +1269,52 @@ __global__ void __launch_bounds__(128) scan_join_kernel(const __grid_constant__ 
 
 // Sums the partial gradients of `share` heads that read one key or value
 // head, in the heads' order: out[token][kv][d] = sum_h part[token][kv*share + h][d].
-template <typename T>
-__global__ void sum_heads_kernel(const float* part, int64_t tokens, int kv, int share, int d, T* out, int64_t o_seq,
-                                 int64_t o_tok, int64_t o_head, int64_t per_seq) {
-    const int64_t total = tokens * kv * d;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < total;
-         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t t = e / (static_cast<int64_t>(kv) * d);
-        const int rem = static_cast<int>(e - t * kv * d), h = rem / d, i = rem - h * d;
-        const float* at = part + (t * kv + h) * share * d + i;
-        float x = 0.0f;
-        for (int g = 0; g < share; ++g) x += at[static_cast<int64_t>(g) * d];
-        const int64_t s = t / per_seq;
-        out[s * o_seq + (t - s * per_seq) * o_tok + h * o_head + i] = from_f32<T>(x);
+// V elements a thread, bound by HBM: 4 share bytes in and one result out an
+// element.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) sum_heads_kernel(const float* part, uint32_t tokens, uint32_t kv, uint32_t share, uint32_t d, T* out,
+                                                        int64_t o_seq, int64_t o_tok, int64_t o_head, uint32_t per_seq) {
+    const uint32_t vecs = d / V, row = kv * vecs;
+    const uint32_t t = blockIdx.x * blockDim.y + threadIdx.y;
+    if (t >= tokens) return;
+    const float* from = part + static_cast<int64_t>(t) * kv * share * d;
+    const uint32_t s = t / per_seq;
+    T* to = out + s * o_seq + (t - s * per_seq) * o_tok;
+    for (uint32_t e = threadIdx.x; e < row; e += blockDim.x) {
+        const uint32_t h = e / vecs, i = (e - h * vecs) * V;
+        const float* at = from + static_cast<int64_t>(h) * share * d + i;
+        float x[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] = 0.0f;
+        for (uint32_t g = 0; g < share; ++g, at += d) {
+            if constexpr (V == 8) {
+                const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4);
+                x[0] += a.x, x[1] += a.y, x[2] += a.z, x[3] += a.w;
+                x[4] += b.x, x[5] += b.y, x[6] += b.z, x[7] += b.w;
+            } else {
+                x[0] += at[0];
+            }
+        }
+        if constexpr (V == 8) store8(to + h * o_head + i, x, 8, true);
+        else to[h * o_head + i] = from_f32<T>(x[0]);
     }
+}
+
+template <typename T>
+cudaError_t sum_heads(const float* part, int64_t tokens, int kv, int share, int d, void* out, const int64_t* st, int64_t per_seq, cudaStream_t s) {
+    const int64_t n = 16 / static_cast<int64_t>(sizeof(T));
+    const bool vec = d % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 && st[0] % n == 0 && st[1] % n == 0 && st[2] % n == 0;
+    const unsigned row = static_cast<unsigned>(kv * d / (vec ? 8 : 1));
+    const dim3 block(row >= 256 ? 256 : (row > 128 ? 256 : (row > 64 ? 128 : (row > 32 ? 64 : 32))), 1);
+    const dim3 threads(block.x, 256 / block.x);
+    const unsigned blocks = static_cast<unsigned>((tokens + threads.y - 1) / threads.y);
+    if (vec)
+        sum_heads_kernel<T, 8><<<blocks, threads, 0, s>>>(part, static_cast<uint32_t>(tokens), kv, share, d, static_cast<T*>(out), st[0], st[1], st[2],
+                                                          static_cast<uint32_t>(per_seq));
+    else
+        sum_heads_kernel<T, 1><<<blocks, threads, 0, s>>>(part, static_cast<uint32_t>(tokens), kv, share, d, static_cast<T*>(out), st[0], st[1], st[2],
+                                                          static_cast<uint32_t>(per_seq));
+    return cudaGetLastError();
 }
 
 // -------------------------------------------------------------- one token
@@ -1570,6 +1602,7 @@ nrn_status_t check_common(const nrn_linattn_t* a, const char* who) {
     NRN_CHECK_ARG(a != nullptr, w + ": null arguments");
     NRN_CHECK_ARG(a->dtype == NRN_BF16 || a->dtype == NRN_FP16 || a->dtype == NRN_FP32, w + ": unknown type");
     NRN_CHECK_ARG(a->seqs >= 0 && a->tokens >= 0, w + ": negative sizes");
+    NRN_CHECK_ARG(a->tokens < (int64_t(1) << 31) && (a->cu_seqlens || a->tokens * a->seqs < (int64_t(1) << 31)), w + ": at most 2^31 - 1 tokens");
     NRN_CHECK_ARG(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0,
                   w + ": heads must be a multiple of kv_heads");
     NRN_CHECK_ARG(a->dk >= 1 && a->dk <= kMaxDim && a->dv >= 1 && a->dv <= kMaxDim, w + ": key and value dimensions are 1 to 256");
@@ -1685,15 +1718,10 @@ extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const 
         NRN_TRY(run_scan(p, a, s));
         const int64_t n = all_tokens(a);
         if (share == 1 || n == 0) continue;
-        const int64_t total = n * a->kv_heads * dd, per = a->cu_seqlens ? n : a->tokens;
-        const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 16LL * sm_count()));
-        if (a->dtype == NRN_BF16)
-            sum_heads_kernel<<<blocks, 256, 0, s>>>(part, n, a->kv_heads, share, dd, static_cast<__nv_bfloat16*>(out), st[0], st[1], st[2], per);
-        else if (a->dtype == NRN_FP16)
-            sum_heads_kernel<<<blocks, 256, 0, s>>>(part, n, a->kv_heads, share, dd, static_cast<__half*>(out), st[0], st[1], st[2], per);
-        else
-            sum_heads_kernel<<<blocks, 256, 0, s>>>(part, n, a->kv_heads, share, dd, static_cast<float*>(out), st[0], st[1], st[2], per);
-        NRN_CUDA_TRY(cudaGetLastError());
+        const int64_t per = a->cu_seqlens ? n : a->tokens;
+        if (a->dtype == NRN_BF16) NRN_CUDA_TRY(sum_heads<__nv_bfloat16>(part, n, a->kv_heads, share, dd, out, st, per, s));
+        else if (a->dtype == NRN_FP16) NRN_CUDA_TRY(sum_heads<__half>(part, n, a->kv_heads, share, dd, out, st, per, s));
+        else NRN_CUDA_TRY(sum_heads<float>(part, n, a->kv_heads, share, dd, out, st, per, s));
     }
     return NRN_OK;
 }
