@@ -61,7 +61,9 @@ struct ScanArgs {
     const float* s_in;             // [seqs][heads] states, element (i of b, j of c) at i*s_i + j*s_j; or null
     float* s_out;                  // the same layout, or null
     int64_t s_i, s_j;
-    float* seg;                    // [units][heads][b.d][c.d]: states of segments, or null
+    float* seg;                    // [units][heads]: states of segments, element (i of b, j of c) at i*g_i + j*g_j; or null
+    int64_t g_i, g_j;
+    int32_t seg_made;              // the states that enter the segments are there already
     int64_t seg_len;               // tokens of a segment (a multiple of the chunk)
     int32_t units;
     int32_t* err;                  // set when a device-side wait gives up, or null
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
         for (int g = 0; g < 4 * G; ++g) {
             const int i = ((g >> 2) * 8 + part) * 4 + (g & 3);
             if (i < db)
-                s[g] = p.seg ? p.seg[gh + static_cast<int64_t>(i) * dc + col] : p.s_in[sh + i * p.s_i + col * p.s_j] * p.in_mul;
+                s[g] = p.seg ? p.seg[gh + i * p.g_i + col * p.g_j] : p.s_in[sh + i * p.s_i + col * p.s_j] * p.in_mul;
         }
     }
     for (int64_t t0 = u.begin; t0 < u.end; t0 += kSerialTokens) {
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
 #pragma unroll
         for (int g = 0; g < 4 * G; ++g) {
             const int i = ((g >> 2) * 8 + part) * 4 + (g & 3);
-            if (i < db) p.seg[gh + static_cast<int64_t>(i) * dc + col] = s[g];
+            if (i < db) p.seg[gh + i * p.g_i + col * p.g_j] = s[g];
         }
     } else if (u.last && p.s_out != nullptr && p.seg == nullptr) {
 #pragma unroll
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
             const int i = nt * 8 + 2 * q + (e & 1), j = wcol + g + 8 * (e >> 1);
             s[nt][e] = 0.0f;
             if (given && i < db && j < dc)
-                s[nt][e] = p.seg ? p.seg[gh + static_cast<int64_t>(i) * dc + j] : p.s_in[sh + i * p.s_i + j * p.s_j] * p.in_mul;
+                s[nt][e] = p.seg ? p.seg[gh + i * p.g_i + j * p.g_j] : p.s_in[sh + i * p.s_i + j * p.s_j] * p.in_mul;
         }
 
     RowLoader<CH, DK> la(p.a, p, u, head, 0), lb(p.b, p, u, head, 0);
@@ -595,7 +597,7 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
         for (int e = 0; e < 4; ++e) {
             const int i = nt * 8 + 2 * q + (e & 1), j = wcol + g + 8 * (e >> 1);
             if (i >= db || j >= dc) continue;
-            if (STATE_ONLY) to[gh + static_cast<int64_t>(i) * dc + j] = s[nt][e];
+            if (STATE_ONLY) to[gh + i * p.g_i + j * p.g_j] = s[nt][e];
             else to[sh + i * p.s_i + j * p.s_j] = s[nt][e] * p.end_mul;
         }
 }
@@ -1058,7 +1060,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 if (given && x0 + i + e < db)
-                    v[e] = p.seg ? p.seg[gh + static_cast<int64_t>(x0 + i + e) * dc + row] : p.s_in[sh + (x0 + i + e) * p.s_i + row * p.s_j] * p.in_mul;
+                    v[e] = p.seg ? p.seg[gh + (x0 + i + e) * p.g_i + row * p.g_j] : p.s_in[sh + (x0 + i + e) * p.s_i + row * p.s_j] * p.in_mul;
             x[i / 2] = pack2(__float_as_uint(v[0]), __float_as_uint(v[1]));
         }
         // the bf16 copy of this thread's part of the state; U has been read
@@ -1190,7 +1192,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (x0 + i >= db) continue;
                 const float2 y = unpack2(x[i / 2]);
                 const float v = i & 1 ? y.y : y.x;
-                if (STATE_ONLY) to[gh + static_cast<int64_t>(x0 + i) * dc + row] = v;
+                if (STATE_ONLY) to[gh + (x0 + i) * p.g_i + row * p.g_j] = v;
                 else to[sh + (x0 + i) * p.s_i + row * p.s_j] = v * p.end_mul;
             }
         }
@@ -1569,8 +1571,9 @@ nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, cudaStream_t s) {
     NRN_CHECK_ARG(static_cast<int64_t>(p.seqs) * p.heads < 65536 || !is_split(a, p.seg_len),
                   "nrn_cuda_linattn: at most 65,535 sequences times heads when sequences are split");
     p.units = static_cast<int32_t>(units);
-    if (is_split(a, p.seg_len)) {
-        p.seg = static_cast<float*>(a->workspace);
+    p.seg = is_split(a, p.seg_len) ? static_cast<float*>(a->workspace) : nullptr;
+    if (!p.seg_made) p.g_i = p.c.d, p.g_j = 1;
+    if (p.seg != nullptr && !p.seg_made) {
         NRN_CUDA_TRY(launch_scan(p, a->dtype, true, s));
         const int64_t n = static_cast<int64_t>(p.b.d) * p.c.d;
         const int v = n % 2 == 0 ? 2 : 1;      // every state starts on an even element then
@@ -1698,8 +1701,13 @@ extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const 
     p.end_mul = a->scale;
     p.s_in = g->dstate_out;
     float* part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + seg_bytes(a));
-    for (int which = 0; which < 2; ++which) {
+    // both carry the state of q and do, one transposed: where their segments
+    // are alike, the values' scan leaves the keys' its entering states
+    const bool alike = segment_length(a, a->dv) == segment_length(a, a->dk);
+    for (int which : {1, 0}) {
         p.a = which ? k : v, p.b = which ? q : d, p.c = which ? d : q;
+        p.seg_made = !which && alike;
+        p.g_i = 1, p.g_j = a->dv;
         const int dd = which ? a->dv : a->dk;
         const int64_t* st = which ? g->dv_stride : g->dk_stride;
         void* out = which ? g->dv : g->dk;
