@@ -476,12 +476,24 @@ NRN_API nrn_status_t nrn_cuda_scaled_transpose(const nrn_scaled_t* in, const nrn
 /* out [a.rows][b.rows] = a b^T: products of 8-bit values summed in fp32 over
  * each block of 128 columns, times both scales, summed in fp32.  Work split
  * over the columns leaves partial sums in the workspace
- * (nrn_cuda_scaled_workspace bytes, zeroed once before its first use and
- * left zeroed where it has to be; not shared by calls that run at once). */
+ * (nrn_cuda_scaled_workspace bytes; the first 4,096 zero before its first
+ * use and left so; not shared by calls that run at once). */
 NRN_API nrn_status_t nrn_cuda_scaled_workspace(const nrn_scaled_t* a, const nrn_scaled_t* b, int64_t* bytes);
 NRN_API nrn_status_t nrn_cuda_scaled_product(const nrn_scaled_t* a, const nrn_scaled_t* b, void* out, int32_t dtype,
                                              int64_t out_stride, void* workspace, int64_t workspace_bytes,
                                              int32_t* err, nrn_stream_t stream);
+/* Gradients of y = x w^T (x [rows][w.cols], y [rows][w.rows], w with a
+ * row_block of 128): dx = dy w and dw = dy^T x, contiguous, with dy and x
+ * quantised along the axis that each of the two sums over.  Workspace:
+ * `bytes`, 256-byte aligned, the first `zeroed` (4,096) of them zero before
+ * its first use and left so, as a product's: one workspace serves both.  Not
+ * shared by calls that run at once. */
+NRN_API nrn_status_t nrn_cuda_scaled_backward_workspace(int64_t rows, const nrn_scaled_t* w, int64_t* bytes,
+                                                        int64_t* zeroed);
+NRN_API nrn_status_t nrn_cuda_scaled_backward(const void* dy, const void* x, int32_t dtype, int64_t rows,
+                                              int64_t dy_stride, int64_t x_stride, const nrn_scaled_t* w, void* dx,
+                                              int32_t dx_dtype, void* dw, int32_t dw_dtype, void* workspace,
+                                              int64_t workspace_bytes, int32_t* err, nrn_stream_t stream);
 
 /* The norms before and after a block with its gate and residual scale, for
  * rows of d elements, norm(x) = x / sqrt(mean(x^2) + eps):

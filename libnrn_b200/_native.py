@@ -43,6 +43,7 @@ EXPORTS = [
     "nrn_engine_set_deterministic", "nrn_engine_add_probe", "nrn_engine_clear_probes",
     "nrn_cuda_linattn_workspace", "nrn_cuda_linattn_forward", "nrn_cuda_linattn_backward", "nrn_cuda_linattn_step",
     "nrn_cuda_scaled_quantize", "nrn_cuda_scaled_transpose", "nrn_cuda_scaled_workspace", "nrn_cuda_scaled_product",
+    "nrn_cuda_scaled_backward", "nrn_cuda_scaled_backward_workspace",
     "nrn_cuda_gatednorm_forward", "nrn_cuda_gatednorm_workspace", "nrn_cuda_gatednorm_backward",
 ]
 
@@ -263,6 +264,8 @@ def lib() -> C.CDLL:
             "nrn_cuda_scaled_transpose": [C.POINTER(Scaled), C.POINTER(Scaled), vp],
             "nrn_cuda_scaled_workspace": [C.POINTER(Scaled), C.POINTER(Scaled), C.POINTER(i64)],
             "nrn_cuda_scaled_product": [C.POINTER(Scaled), C.POINTER(Scaled), vp, i32, i64, vp, i64, vp, vp],
+            "nrn_cuda_scaled_backward_workspace": [i64, C.POINTER(Scaled), C.POINTER(i64), C.POINTER(i64)],
+            "nrn_cuda_scaled_backward": [vp, vp, i32, i64, i64, i64, C.POINTER(Scaled), vp, i32, vp, i32, vp, i64, vp, vp],
             "nrn_cuda_gatednorm_forward": [C.POINTER(GatedNorm), vp],
             "nrn_cuda_gatednorm_workspace": [C.POINTER(GatedNorm), C.POINTER(i64)],
             "nrn_cuda_gatednorm_backward": [C.POINTER(GatedNorm), C.POINTER(GatedNormGrad), vp],

@@ -404,80 +404,135 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 constexpr int kQuantThreads = 256;
 
-// A scale for each row and 128 columns: 16 lanes of eight elements a block.
+// A scale for each row and 128 columns: 16 lanes of eight elements a block,
+// two blocks of the result at a time so that enough loads are in flight.
+// Bound by HBM: one read and a write of half or a quarter of it.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
-    quant_rows_kernel(const T* x, int64_t rows, int64_t cols, int64_t x_stride, int vec, uint8_t* values, int64_t v_stride,
-                      float* scales, int64_t s_row, int64_t s_col) {
-    const int64_t blocks = (cols + kBlock - 1) / kBlock, total = rows * blocks;
-    const int part = threadIdx.x & 15;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kQuantThreads / 16);
+    quant_rows_kernel(const T* x, uint32_t rows, uint32_t cols, int64_t x_stride, int vec, uint8_t* values, int64_t v_stride,
+                      float* scales, int64_t s_row, int64_t s_col, uint32_t blocks) {
+    const uint32_t total = rows * blocks, part = threadIdx.x & 15;
+    const uint32_t step = gridDim.x * (kQuantThreads / 16);
+    constexpr int kAtOnce = 2;
     // every lane of a warp takes part in the shuffles: the loop is uniform
-    for (int64_t w0 = static_cast<int64_t>(blockIdx.x) * (kQuantThreads / 16) + (threadIdx.x >> 5) * 2; w0 < total; w0 += step) {
-        const int64_t w = w0 + ((threadIdx.x >> 4) & 1);
-        const int64_t r = w / blocks, b = w - r * blocks, c = b * kBlock + part * 8;
-        const int n = w < total ? static_cast<int>(cols - c < 8 ? (cols - c < 0 ? 0 : cols - c) : 8) : 0;
-        float f[8];
-        uint32_t m = 0;
-        const Raw8<T> raw = load8(x + (n > 0 ? r * x_stride + c : 0), n, vec != 0);
+    for (uint32_t w0 = blockIdx.x * (kQuantThreads / 16) + (threadIdx.x >> 5) * 2; w0 < total; w0 += kAtOnce * step) {
+        Raw8<T> raw[kAtOnce];
+        uint32_t r[kAtOnce], b[kAtOnce];
+        int n[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            f[e] = to_f32(raw.e[e]);
-            m = max(m, abs_bits(f[e]));
+        for (int k = 0; k < kAtOnce; ++k) {
+            const uint32_t w = w0 + k * step + ((threadIdx.x >> 4) & 1);
+            r[k] = w / blocks;
+            b[k] = w - r[k] * blocks;
+            const int left = static_cast<int>(cols - b[k] * kBlock) - static_cast<int>(part) * 8;
+            n[k] = w < total && left > 0 ? min(left, 8) : (w < total ? 0 : -1);
+            raw[k] = load8(x + (n[k] > 0 ? r[k] * x_stride + b[k] * kBlock + part * 8 : 0), n[k], vec != 0);
         }
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const float s = block_scale(m), inv = 1.0f / s;
-        if (w < total && part == 0) scales[r * s_row + b * s_col] = s;
-        if (n > 0) {
-            const uint2 q = make_uint2(e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                                       e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-            uint8_t* d = values + r * v_stride + c;   // rows are padded to 16 bytes: a whole store fits
-            *reinterpret_cast<uint2*>(d) = q;
+        for (int k = 0; k < kAtOnce; ++k) {
+            float f[8];
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[e] = to_f32(raw[k].e[e]);
+                m = max(m, abs_bits(f[e]));
+            }
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const float s = block_scale(m), inv = __frcp_rn(s);
+            if (n[k] >= 0 && part == 0) scales[r[k] * s_row + b[k] * s_col] = s;
+            if (n[k] > 0)          // rows are padded to 16 bytes: a whole store fits
+                *reinterpret_cast<uint2*>(values + r[k] * v_stride + b[k] * kBlock + part * 8) =
+                    make_uint2(e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
         }
     }
 }
 
-// x^T with a scale for each of its rows (columns of x) and 128 rows of x: a
-// tile of 128 rows by 64 columns passes through shared memory.
-constexpr int kTransCols = 64;
-template <typename T>
+struct QuantOut {
+    uint8_t* values;
+    int64_t v_stride;
+    float* scales;
+    int64_t s_row, s_col;
+};
+
+// x^T with a scale for each of its rows (columns of x) and 128 rows of x, and
+// with ROWS also x itself with a scale for each row and 128 columns, from one
+// read: a gradient is wanted both ways.  A block has a 128 x 128 tile, a
+// thread eight rows by eight columns of it in registers; the transposed bytes
+// pass through shared memory, eight at a time, their places exclusive-ored
+// with the column's so that neither way has bank conflicts.
+template <typename T, bool ROWS>
 __global__ void __launch_bounds__(kQuantThreads)
-    quant_cols_kernel(const T* x, int64_t rows, int64_t cols, int64_t x_stride, int vec, uint8_t* values, int64_t v_stride,
-                      float* scales, int64_t s_row, int64_t s_col) {
-    __shared__ float tile[kBlock][kTransCols + 1];
-    __shared__ float inv_s[kTransCols];
-    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kBlock, c0 = static_cast<int64_t>(blockIdx.x) * kTransCols;
-    for (int e = threadIdx.x; e < kBlock * kTransCols / 8; e += kQuantThreads) {
-        const int r = e / (kTransCols / 8), c = (e % (kTransCols / 8)) * 8;
-        const int64_t left = cols - c0 - c;
-        const int n = r0 + r < rows ? static_cast<int>(left < 0 ? 0 : (left < 8 ? left : 8)) : 0;
-        const Raw8<T> raw = load8(x + (n > 0 ? (r0 + r) * x_stride + c0 + c : 0), n, vec != 0);
+    quant_cols_kernel(const T* x, int64_t rows, int64_t cols, int64_t x_stride, int vec, const QuantOut by_cols, const QuantOut by_rows) {
+    __shared__ alignas(16) uint8_t bytes[kBlock][kBlock];
+    __shared__ uint32_t amax[kQuantThreads / 16][kBlock];
+    __shared__ float inv_s[kBlock];
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kBlock, c0 = static_cast<int64_t>(blockIdx.x) * kBlock;
+    const int part = threadIdx.x & 15, rg = threadIdx.x >> 4;        // columns 8 part ..; rows 8 rg ..
+    const int64_t left = cols - c0 - part * 8;
+    const int n = static_cast<int>(left < 0 ? 0 : (left < 8 ? left : 8));
+    Raw8<T> raw[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) tile[r][c + i] = to_f32(raw.e[i]);
+    for (int i = 0; i < 8; ++i) {
+        const int64_t r = r0 + rg * 8 + i;
+        raw[i] = load8(x + (r < rows && n > 0 ? r * x_stride + c0 + part * 8 : 0), r < rows ? n : 0, vec != 0);
     }
-    __syncthreads();
-    {
-        const int c = threadIdx.x >> 2, q = threadIdx.x & 3;     // four lanes a column
-        uint32_t m = 0;
-        for (int r = q; r < kBlock; r += 4) m = max(m, abs_bits(tile[r][c]));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float s = block_scale(m);
-        if (q == 0) {
-            inv_s[c] = 1.0f / s;
-            if (c0 + c < cols) scales[(c0 + c) * s_row + blockIdx.y * s_col] = s;
+    uint32_t m[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[e] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint32_t mr = 0;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            f[e] = to_f32(raw[i].e[e]);
+            const uint32_t a = abs_bits(f[e]);
+            m[e] = max(m[e], a);
+            if (ROWS) mr = max(mr, a);
+        }
+        if constexpr (ROWS) {
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) mr = max(mr, __shfl_xor_sync(0xffffffffu, mr, d));
+            const float s = block_scale(mr), inv = __frcp_rn(s);
+            const int64_t r = r0 + rg * 8 + i;
+            if (r < rows) {
+                if (part == 0) by_rows.scales[r * by_rows.s_row + blockIdx.x * by_rows.s_col] = s;
+                if (n > 0)
+                    *reinterpret_cast<uint2*>(by_rows.values + r * by_rows.v_stride + c0 + part * 8) =
+                        make_uint2(e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+            }
         }
     }
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) *reinterpret_cast<uint4*>(&amax[rg][part * 8 + e]) = make_uint4(m[e], m[e + 1], m[e + 2], m[e + 3]);
     __syncthreads();
-    // a warp writes the 128 bytes of one column, four a lane
-    for (int c = threadIdx.x >> 5; c < kTransCols; c += kQuantThreads / 32) {
-        if (c0 + c >= cols) continue;
-        const int r = (threadIdx.x & 31) * 4;
+    if (threadIdx.x < kBlock) {
+        uint32_t a = 0;
+#pragma unroll
+        for (int g = 0; g < kQuantThreads / 16; ++g) a = max(a, amax[g][threadIdx.x]);
+        const float s = block_scale(a);
+        inv_s[threadIdx.x] = __frcp_rn(s);
+        if (c0 + threadIdx.x < cols) by_cols.scales[(c0 + threadIdx.x) * by_cols.s_row + blockIdx.y * by_cols.s_col] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = part * 8 + e;
         const float inv = inv_s[c];
-        if (r0 + r < rows)        // rows of the result are padded to 16 bytes
-            *reinterpret_cast<uint32_t*>(values + (c0 + c) * v_stride + r0 + r) =
-                e4m3x4(tile[r][c] * inv, tile[r + 1][c] * inv, tile[r + 2][c] * inv, tile[r + 3][c] * inv);
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(raw[i].e[e]) * inv;
+        *reinterpret_cast<uint2*>(&bytes[c][(rg ^ part) * 8]) = make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int c = k * 32 + (threadIdx.x >> 3), q = threadIdx.x & 7, pc = c >> 3;      // rows 16 q .. of column c
+        if (c0 + c >= cols || r0 + q * 16 >= rows) continue;
+        uint4 v = *reinterpret_cast<const uint4*>(&bytes[c][(q ^ (pc >> 1)) * 16]);
+        if (pc & 1) v = make_uint4(v.z, v.w, v.x, v.y);
+        *reinterpret_cast<uint4*>(by_cols.values + (c0 + c) * by_cols.v_stride + r0 + q * 16) = v;   // rows are padded to 16 bytes
     }
 }
 
@@ -520,24 +575,41 @@ __global__ void __launch_bounds__(kQuantThreads)
     }
 }
 
-// Values of a matrix transposed, 128 x 128 bytes at a time.
+// Values of a matrix transposed, 128 x 128 bytes at a time: four rows by
+// four columns a step, through shared memory on both sides.
 __global__ void __launch_bounds__(kQuantThreads)
     transpose_kernel(const uint8_t* in, int64_t rows, int64_t cols, int64_t in_stride, uint8_t* out, int64_t out_stride) {
-    __shared__ uint32_t tile[kBlock][33];
+    __shared__ alignas(8) uint32_t from[kBlock][34], to[kBlock][34];   // 34: four rows on are 8 banks on
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kBlock, c0 = static_cast<int64_t>(blockIdx.x) * kBlock;
-    for (int e = threadIdx.x; e < kBlock * 32; e += kQuantThreads) {
-        const int r = e >> 5, c = (e & 31) * 4;
-        // rows are padded to 16 bytes: a word that starts inside a row ends inside its storage
-        tile[r][e & 31] = r0 + r < rows && c0 + c < cols ? *reinterpret_cast<const uint32_t*>(in + (r0 + r) * in_stride + c0 + c) : 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int r = k * 32 + (threadIdx.x >> 3), q = threadIdx.x & 7;
+        // rows are padded to 16 bytes: 16 that start inside a row end inside its storage
+        const uint4 v = r0 + r < rows && c0 + q * 16 < cols ? *reinterpret_cast<const uint4*>(in + (r0 + r) * in_stride + c0 + q * 16) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint2*>(&from[r][q * 4]) = make_uint2(v.x, v.y);
+        *reinterpret_cast<uint2*>(&from[r][q * 4 + 2]) = make_uint2(v.z, v.w);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < kBlock * 32; e += kQuantThreads) {
-        const int c = e >> 5, r = (e & 31) * 4;      // column c of the input, four of its rows
-        if (c0 + c >= cols || r0 + r >= rows) continue;
-        uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= ((tile[r + i][c >> 2] >> (8 * (c & 3))) & 0xffu) << (8 * i);
-        *reinterpret_cast<uint32_t*>(out + (c0 + c) * out_stride + r0 + r) = w;
+    for (int k = 0; k < 4; ++k) {
+        // columns 4 cw .., rows 4 rw ..: a warp has eight by four of them
+        const int e = k * (kQuantThreads / 32) + (threadIdx.x >> 5), cw = (e & 3) * 8 + (threadIdx.x & 7), rw = (e >> 2) * 4 + ((threadIdx.x >> 3) & 3);
+        const uint32_t a = from[4 * rw][cw], b = from[4 * rw + 1][cw], c = from[4 * rw + 2][cw], d = from[4 * rw + 3][cw];
+        const uint32_t ab = __byte_perm(a, b, 0x5140), cd = __byte_perm(c, d, 0x5140), ab2 = __byte_perm(a, b, 0x7362), cd2 = __byte_perm(c, d, 0x7362);
+        to[4 * cw][rw] = __byte_perm(ab, cd, 0x5410);
+        to[4 * cw + 1][rw] = __byte_perm(ab, cd, 0x7632);
+        to[4 * cw + 2][rw] = __byte_perm(ab2, cd2, 0x5410);
+        to[4 * cw + 3][rw] = __byte_perm(ab2, cd2, 0x7632);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int c = k * 32 + (threadIdx.x >> 3), q = threadIdx.x & 7;
+        if (c0 + c < cols && r0 + q * 16 < rows)
+{
+            const uint2 lo = *reinterpret_cast<const uint2*>(&to[c][q * 4]), hi = *reinterpret_cast<const uint2*>(&to[c][q * 4 + 2]);
+            *reinterpret_cast<uint4*>(out + (c0 + c) * out_stride + r0 + q * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
     }
 }
 
@@ -644,6 +716,21 @@ nrn_status_t launch_nt(int nt, const CUtensorMap& rm, const CUtensorMap& cm, con
     }
 }
 
+QuantOut quant_out(const nrn_scaled_t* o) {
+    return QuantOut{o->values, o->value_stride, o->scales, o->scale_stride[0], o->scale_stride[1]};
+}
+
+// x both ways, for a gradient.
+template <typename T>
+nrn_status_t quantize_both(const void* x, int64_t rows, int64_t cols, int64_t stride, const nrn_scaled_t* by_cols, const nrn_scaled_t* by_rows,
+                           cudaStream_t s) {
+    const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * sizeof(T) % 16 == 0;
+    const dim3 grid(static_cast<unsigned>((cols + kBlock - 1) / kBlock), static_cast<unsigned>((rows + kBlock - 1) / kBlock));
+    quant_cols_kernel<T, true><<<grid, kQuantThreads, 0, s>>>(static_cast<const T*>(x), rows, cols, stride, vec, quant_out(by_cols), quant_out(by_rows));
+    NRN_CUDA_TRY(cudaGetLastError());
+    return NRN_OK;
+}
+
 template <typename T>
 nrn_status_t quantize(const void* x, int64_t rows, int64_t cols, int64_t stride, bool transpose, const nrn_scaled_t* o,
                       cudaStream_t s) {
@@ -651,17 +738,19 @@ nrn_status_t quantize(const void* x, int64_t rows, int64_t cols, int64_t stride,
     const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * sizeof(T) % 16 == 0;
     const int64_t rb = (rows + kBlock - 1) / kBlock;
     if (!transpose && o->row_block == 1) {
-        const int64_t work = rows * ((cols + kBlock - 1) / kBlock);
-        const int64_t blocks = std::min<int64_t>((work + kQuantThreads / 16 - 1) / (kQuantThreads / 16), 32LL * sm_count());
+        const int64_t per_row = (cols + kBlock - 1) / kBlock, work = rows * per_row;
+        NRN_CHECK_ARG(work < (int64_t(1) << 30), "nrn_cuda_scaled_quantize: too many blocks for one launch");
+        const int64_t blocks = std::min<int64_t>((work + kQuantThreads / 16 - 1) / (kQuantThreads / 16), 16LL * sm_count());
         quant_rows_kernel<T><<<static_cast<unsigned>(blocks), kQuantThreads, 0, s>>>(
-            p, rows, cols, stride, vec, o->values, o->value_stride, o->scales, o->scale_stride[0], o->scale_stride[1]);
+            p, static_cast<uint32_t>(rows), static_cast<uint32_t>(cols), stride, vec, o->values, o->value_stride, o->scales, o->scale_stride[0],
+            o->scale_stride[1], static_cast<uint32_t>(per_row));
     } else {
         NRN_CHECK_ARG(rb < 65536, "nrn_cuda_scaled_quantize: at most 8,388,480 rows");
+        const dim3 grid(static_cast<unsigned>((cols + kBlock - 1) / kBlock), static_cast<unsigned>(rb));
         if (transpose)
-            quant_cols_kernel<T><<<dim3(static_cast<unsigned>((cols + kTransCols - 1) / kTransCols), static_cast<unsigned>(rb)), kQuantThreads, 0, s>>>(
-                p, rows, cols, stride, vec, o->values, o->value_stride, o->scales, o->scale_stride[0], o->scale_stride[1]);
+            quant_cols_kernel<T, false><<<grid, kQuantThreads, 0, s>>>(p, rows, cols, stride, vec, quant_out(o), QuantOut{});
         else
-            quant_blocks_kernel<T><<<dim3(static_cast<unsigned>((cols + kBlock - 1) / kBlock), static_cast<unsigned>(rb)), kQuantThreads, 0, s>>>(
+            quant_blocks_kernel<T><<<grid, kQuantThreads, 0, s>>>(
                 p, rows, cols, stride, vec, o->values, o->value_stride, o->scales, o->scale_stride[0], o->scale_stride[1]);
     }
     NRN_CUDA_TRY(cudaGetLastError());
@@ -770,4 +859,93 @@ extern "C" nrn_status_t nrn_cuda_scaled_product(const nrn_scaled_t* a, const nrn
     g.part = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes) : nullptr;
     g.err = err;
     return c->row_block == 1 ? launch_nt<false>(p.nt, rm, cm, g, s) : launch_nt<true>(p.nt, rm, cm, g, s);
+}
+
+namespace nrn {
+namespace {
+
+// The 8-bit operands of a backward pass, one after the other in the workspace.
+struct BackwardPlan {
+    nrn_scaled_t dy, dyt, xt, wt;
+    int64_t product_bytes, bytes;
+};
+
+BackwardPlan backward_plan(int64_t rows, const nrn_scaled_t* w, uint8_t* base) {
+    BackwardPlan p{};
+    // the products' own workspace first, its counters at least: they stay zero from call to call
+    const auto need = [](int64_t m, int64_t n, int64_t k) { return m == 0 || n == 0 || k == 0 ? 0 : plan_workspace(plan_of(m, n, k)); };
+    p.product_bytes = std::max({kCountBytes, need(rows, w->cols, w->rows), need(w->rows, w->cols, rows)});
+    int64_t at = (p.product_bytes + 255) / 256 * 256;
+    const auto make = [&](int64_t r, int64_t c, bool scales) {
+        nrn_scaled_t m{};
+        m.rows = r, m.cols = c, m.row_block = 1;
+        m.value_stride = (std::max<int64_t>(c, 1) + 15) / 16 * 16;
+        m.values = base + at;
+        at += (r * m.value_stride + 255) / 256 * 256;
+        if (scales) {
+            const int64_t kb = (c + kBlock - 1) / kBlock;
+            m.scales = reinterpret_cast<float*>(base + at);
+            m.scale_stride[0] = 1, m.scale_stride[1] = std::max<int64_t>(r, 1);
+            at += (r * kb * 4 + 255) / 256 * 256;
+        }
+        return m;
+    };
+    p.dy = make(rows, w->rows, true);
+    p.dyt = make(w->rows, rows, true);
+    p.xt = make(w->cols, rows, true);
+    p.wt = make(w->cols, w->rows, false);
+    p.wt.row_block = kBlock;
+    p.wt.scales = w->scales;
+    p.wt.scale_stride[0] = w->scale_stride[1], p.wt.scale_stride[1] = w->scale_stride[0];
+    p.bytes = at;
+    return p;
+}
+
+}  // namespace
+}  // namespace nrn
+
+extern "C" nrn_status_t nrn_cuda_scaled_backward_workspace(int64_t rows, const nrn_scaled_t* w, int64_t* bytes, int64_t* zeroed) {
+    const std::string who = "nrn_cuda_scaled_backward_workspace";
+    NRN_CHECK_ARG(w && bytes && zeroed, who + ": null argument");
+    NRN_CHECK_ARG(rows >= 0 && w->rows >= 0 && w->cols >= 0, who + ": negative sizes");
+    const BackwardPlan p = backward_plan(rows, w, nullptr);
+    *bytes = p.bytes;
+    *zeroed = kCountBytes;
+    return NRN_OK;
+}
+
+extern "C" nrn_status_t nrn_cuda_scaled_backward(const void* dy, const void* x, int32_t dtype, int64_t rows, int64_t dy_stride, int64_t x_stride,
+                                                 const nrn_scaled_t* w, void* dx, int32_t dx_dtype, void* dw, int32_t dw_dtype, void* workspace,
+                                                 int64_t workspace_bytes, int32_t* err, nrn_stream_t stream) {
+    const std::string who = "nrn_cuda_scaled_backward";
+    NRN_TRY(check_scaled(w, who));
+    NRN_CHECK_ARG(w->row_block == kBlock, who + ": weights have a row_block of 128");
+    NRN_CHECK_ARG(dtype == NRN_BF16 || dtype == NRN_FP16 || dtype == NRN_FP32, who + ": unknown type");
+    NRN_CHECK_ARG(rows >= 0 && rows < (int64_t(1) << 23) - 128 && w->rows < (int64_t(1) << 23) - 128, who + ": at most 8,388,480 rows");
+    NRN_CHECK_ARG(dy_stride >= 0 && x_stride >= 0, who + ": negative strides");
+    if (w->rows == 0 || w->cols == 0) return NRN_OK;
+    NRN_CHECK_ARG((rows == 0 || (dy && x && dx)) && dw, who + ": null array");
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        NRN_CUDA_TRY(cudaMemsetAsync(dw, 0, static_cast<size_t>(w->rows) * w->cols * (dw_dtype == NRN_FP32 ? 4 : 2), s));
+        return NRN_OK;
+    }
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    const BackwardPlan p = backward_plan(rows, w, base);
+    NRN_CHECK_ARG(workspace && workspace_bytes >= p.bytes, who + ": workspace too small");
+    NRN_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, who + ": the workspace must be 256-byte aligned");
+    const int64_t n = w->rows, k = w->cols;
+    if (dtype == NRN_BF16) {
+        NRN_TRY(quantize_both<__nv_bfloat16>(dy, rows, n, dy_stride, &p.dyt, &p.dy, s));
+        NRN_TRY(quantize<__nv_bfloat16>(x, rows, k, x_stride, true, &p.xt, s));
+    } else if (dtype == NRN_FP16) {
+        NRN_TRY(quantize_both<__half>(dy, rows, n, dy_stride, &p.dyt, &p.dy, s));
+        NRN_TRY(quantize<__half>(x, rows, k, x_stride, true, &p.xt, s));
+    } else {
+        NRN_TRY(quantize_both<float>(dy, rows, n, dy_stride, &p.dyt, &p.dy, s));
+        NRN_TRY(quantize<float>(x, rows, k, x_stride, true, &p.xt, s));
+    }
+    NRN_TRY(nrn_cuda_scaled_transpose(w, &p.wt, stream));
+    NRN_TRY(nrn_cuda_scaled_product(&p.dy, &p.wt, dx, dx_dtype, k, workspace, p.product_bytes, err, stream));
+    return nrn_cuda_scaled_product(&p.dyt, &p.xt, dw, dw_dtype, k, workspace, p.product_bytes, err, stream);
 }

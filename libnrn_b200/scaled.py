@@ -153,13 +153,18 @@ def transpose(w: Scaled, *, stream=None) -> Scaled:
 _workspaces: dict = {}
 
 
+_COUNTERS = 4096        # bytes at a workspace's start that are zero between calls
+
+
 def _workspace(n: int, device, stream: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.uint8, device=device)      # belongs to the graph, zeroed by it
+    capturing = torch.cuda.is_current_stream_capturing()     # then it belongs to the graph
     key = (device.index, stream)
-    w = _workspaces.get(key)
+    w = None if capturing else _workspaces.get(key)
     if w is None or w.numel() < n:
-        w = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=device)
+        w = torch.empty(max(n, _COUNTERS), dtype=torch.uint8, device=device)
+        w[:_COUNTERS].zero_()
+        if not capturing:
+            _workspaces[key] = w
     return w
 
 
@@ -202,14 +207,42 @@ def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None
     return out
 
 
+def _describe_backward(dy, x, w, dx_dtype, dw_dtype):
+    """(row strides of dy and x, their type, types of the results, bytes of workspace)."""
+    require(w.row_block == BLOCK, "w: must be Scaled with a row_block of 128")
+    for name, t, cols in (("dy", dy, w.shape[0]), ("x", x, w.shape[1])):
+        require(isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[1] == cols, f"{name}: must be [rows, {cols}]")
+        check_tensor(t, name, dy.dtype, w.device)
+        require(cols <= 1 or t.stride(1) == 1, f"{name}: the last dimension must have stride 1")
+        require(t.shape[0] <= 1 or t.stride(0) >= cols, f"{name}: rows overlap")
+    rows = dy.shape[0]
+    require(rows == x.shape[0], f"dy: has {rows} rows, x has {x.shape[0]}")
+    for name, t in (("dy", dy.dtype), ("dx_dtype", dx_dtype), ("dw_dtype", dw_dtype)):
+        require(t in DTYPE, f"{name}: must be bfloat16, float16 or float32, is {t}")
+    need, zeroed = C.c_int64(), C.c_int64()
+    N.check(N.lib().nrn_cuda_scaled_backward_workspace(rows, C.byref(w.desc), C.byref(need), C.byref(zeroed)),
+            "nrn_cuda_scaled_backward_workspace")
+    return (rows, *(t.stride(0) if rows > 1 else max(t.shape[1], 1) for t in (dy, x)), DTYPE[dy.dtype], DTYPE[dx_dtype], DTYPE[dw_dtype],
+            need.value)
+
+
+_backwards = Layouts(_describe_backward)
+
+
 def product_backward(dy: torch.Tensor, x: torch.Tensor, w: Scaled, *, dx_dtype=None, dw_dtype=torch.float32, stream=None):
     """(dx, dw) of y = x @ w^T: dx = dy @ w and dw = dy^T @ x, with dy and x quantised along the axis that each of the two
     sums over (dy's rows for dx; the columns of dy and x for dw)."""
-    require(isinstance(w, Scaled) and w.row_block == BLOCK, "w: must be Scaled with a row_block of 128")
-    for name, t, cols in (("dy", dy, w.shape[0]), ("x", x, w.shape[1])):
-        require(isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[1] == cols, f"{name}: must be [rows, {cols}]")
-    require(dy.shape[0] == x.shape[0], f"dy: has {dy.shape[0]} rows, x has {x.shape[0]}")
-    dx = product(quantize(dy, stream=stream), transpose(w, stream=stream), dtype=dx_dtype or dy.dtype, stream=stream)
-    dw = product(quantize(dy, transpose=True, stream=stream), quantize(x, transpose=True, stream=stream), dtype=dw_dtype,
-                 stream=stream)
+    require(isinstance(w, Scaled), "w: must be Scaled with a row_block of 128")
+    require(isinstance(dy, torch.Tensor) and dy.is_cuda, "dy: a CUDA tensor is needed")
+    dx_dtype = dx_dtype or dy.dtype
+    key = (layout(dy), layout(x), w.shape, w.row_block, w.device, dx_dtype, dw_dtype)
+    rows, dy_stride, x_stride, kind, dx_kind, dw_kind, need = _backwards.get(key, dy, x, w, dx_dtype, dw_dtype)
+    dev, (n, k) = w.device, w.shape
+    with on(dev, stream) as st:
+        dx = torch.empty_strided((rows, k), (k, 1), dtype=dx_dtype, device=dev)
+        dw = torch.empty_strided((n, k), (k, 1), dtype=dw_dtype, device=dev)
+        work = _workspace(need, dev, st) if need else None
+        N.check(N.lib().nrn_cuda_scaled_backward(dy.data_ptr(), x.data_ptr(), kind, rows, dy_stride, x_stride, C.byref(w.desc), dx.data_ptr(),
+                                                 dx_kind, dw.data_ptr(), dw_kind, None if work is None else work.data_ptr(), need,
+                                                 error_flag(dev), st), "nrn_cuda_scaled_backward")
     return dx, dw
