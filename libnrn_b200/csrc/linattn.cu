@@ -655,7 +655,8 @@ struct TcHead {
     int abort;
     alignas(16) float lag[128];    // factor of P at token i - token j, from -63 on
     alignas(16) float w[kChunk];   // decay of each token to the chunk's end
-    alignas(16) float out[kChunk]; // and of the entering state to each token, times out_mul
+    alignas(16) float out[2][kChunk];   // and of the entering state to each token, times out_mul; [1]: of a shorter last chunk
+    float whole[2];                // lam^(tokens of the chunk), likewise
     uint8_t bad[2][kTcGroup];      // 16 columns of c hold a value that is no number, and each column's first, in scan order
     uint8_t first_bad[2][kTcCols];
 };
@@ -894,8 +895,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int et = threadIdx.x - 128;
         const int l7 = lane & 7, l8 = (lane >> 3) & 1, l16 = lane >> 4, q = lane & 3, g8 = lane >> 2;
         const float g = p.log_decay[head];
-        if (!STATE_ONLY && et < 127)
-            M.lag[et] = p.out_mul * ((p.reverse ? et <= 63 : et >= 63) ? decay_power(g, p.reverse ? 63 - et : et - 63) : 0.0f);
+        // the factors of a chunk of n tokens, one thread each; the results' group reads its own after the MMAs that follow these
+        auto factors = [&](int n, int last) {
+            int64_t power = -1;
+            if (et < 127) power = last ? -1 : (p.reverse ? 63 - et : et - 63);
+            else if (et == 127) power = n;
+            else if (et < 192) power = et - 128 < n ? n - p.off - (p.reverse ? n - 1 - (et - 128) : et - 128) : -1;
+            else power = et - 192 < n ? (p.reverse ? n - 1 - (et - 192) : et - 192) + p.off : -1;
+            const float f = power < 0 ? 0.0f : decay_power(g, power);
+            if (et < 127 && !last) M.lag[et] = p.out_mul * f;
+            if (et == 127) M.whole[last] = f;
+            if (et >= 128 && et < 192) M.w[et - 128] = f;
+            if (et >= 192) M.out[last][et - 192] = p.out_mul * f;
+        };
         bool ok = true;
         for (int c = 0; c < chunks; ++c) {
             const int st = c & 1, n = tokens(c);
@@ -907,7 +919,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (c == 0 || n < kChunk) {
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (et < kChunk) M.w[et] = et < n ? decay_power(g, n - p.off - (p.reverse ? n - 1 - et : et)) : 0.0f;
+                factors(n, c > 0);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
@@ -1043,9 +1055,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
         const int ew = warp - 4 - kTcGroup, sub = warp & 3, half = ew >> 2;   // TMEM lanes 32 sub ..; half of their columns
-        const int et = threadIdx.x - 128 - 32 * kTcGroup;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * sub) << 16);
-        const float g = p.log_decay[head];
         const int row = tile * kTcCols + 32 * sub + lane;             // column of c
         const int64_t sh = (static_cast<int64_t>(u.seq) * p.heads + head) * db * dc;
         const int64_t gh = (static_cast<int64_t>(unit) * p.heads + head) * db * dc;
@@ -1095,22 +1105,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 0) mbar_arrive(&M.x16);
         };
         if (chunks > 0) copy_state();
-        uint64_t whole2 = 0;
         bool ok = true;
         for (int c = 0; c < chunks; ++c) {
             const int st = c & 1, n = tokens(c);
             const uint32_t ph = c & 1;
-            if (c == 0 || n < kChunk) {
-                asm volatile("bar.sync 2, 256;" ::: "memory");
-                if (et < kChunk) M.out[et] = et < n ? p.out_mul * decay_power(g, (p.reverse ? n - 1 - et : et) + p.off) : 0.0f;
-                const uint32_t whole = __float_as_uint(decay_power(g, n));
-                whole2 = pack2(whole, whole);
-                asm volatile("bar.sync 2, 256;" ::: "memory");
-            }
             // (3) the state
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph, abort));
+            const int last = c > 0 && n < kChunk;
             if (ok) {
                 tc_fence_after();
+                const uint32_t whole = __float_as_uint(M.whole[last]);
+                const uint64_t whole2 = pack2(whole, whole);
 #pragma unroll
                 for (int i0 = 0; i0 < kX; i0 += 16) {
                     uint32_t v[16];
@@ -1141,7 +1146,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tc_wait_ld16(b);
 #pragma unroll
                         for (int t = 0; t < 16; t += 4) {
-                            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&M.out[32 * half + t0 + t]);
+                            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&M.out[last][32 * half + t0 + t]);
                             const float2 lo = unpack2(fma2(w.x, pack2(b[t], b[t + 1]), pack2(a[t], a[t + 1])));
                             const float2 hi = unpack2(fma2(w.y, pack2(b[t + 2], b[t + 3]), pack2(a[t + 2], a[t + 3])));
                             a[t] = __float_as_uint(lo.x), a[t + 1] = __float_as_uint(lo.y);
@@ -1513,7 +1518,7 @@ int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
 // SMs idle, or a last round of blocks nearly empty, the sequences are split.
 // Splitting costs a pass over b and c for the segments' states and the join,
 // so the least time is looked for, by a model of microseconds measured on
-// d 128: 2.0 a chunk and 8 a block, 1.2 and 6 for the states, 4 for the join
+// d 128: 2.0 a chunk and 5 a block, 1.2 and 4 for the states, 4 for the join
 // and its bytes.  Packed sequences' lengths are not known here: their segments
 // are counted as if half of them were cut short.
 int64_t segment_length(const nrn_linattn_t* a, int dc) {
@@ -1532,11 +1537,11 @@ int64_t segment_length(const nrn_linattn_t* a, int dc) {
         const double units = packed ? static_cast<double>(chunks) / s + 0.5 * a->seqs
                                     : static_cast<double>(a->seqs) * ((chunks + s - 1) / s);
         const double r = rounds(units * rows);
-        double t = r * (2.0 * s + 8.0);
+        double t = r * (2.0 * s + 5.0);
         // packed sequences that are whole: the longest is about twice the mean
-        if (packed && k == 1) t = std::max(rounds(static_cast<double>(a->seqs) * rows) * (2.0 * chunks / std::max(1, a->seqs) + 8.0),
-                                           2.0 * std::min<double>(chunks, 2.0 * chunks / std::max(1, a->seqs)) + 8.0);
-        else if (k > 1) t += r * (1.2 * s + 6.0) + 4.0 + units * rows * a->dk * static_cast<double>(std::min(dc, kTcCols)) * 8.0 / 3e6;
+        if (packed && k == 1) t = std::max(rounds(static_cast<double>(a->seqs) * rows) * (2.0 * chunks / std::max(1, a->seqs) + 5.0),
+                                           2.0 * std::min<double>(chunks, 2.0 * chunks / std::max(1, a->seqs)) + 5.0);
+        else if (k > 1) t += r * (1.2 * s + 4.0) + 4.0 + units * rows * a->dk * static_cast<double>(std::min(dc, kTcCols)) * 8.0 / 3e6;
         if (t < cost) {
             cost = t;
             best = s;
