@@ -650,7 +650,7 @@ struct TcSmem {
 static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
 
 struct TcHead {
-    uint64_t full[2], empty[2], oready[2], pready, psm, x16, vk, uready, odone, drain;
+    uint64_t full[2], empty[2], oready[2], pready, psm, x16, vk, uready, iready, odone, drain;
     uint32_t tmem;
     int abort;
     alignas(16) float lag[128];    // factor of P at token i - token j, from -63 on
@@ -771,6 +771,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         mbar_init(&M.pready, 1);
         mbar_init(&M.uready, 1);
+        mbar_init(&M.iready, 1);
         mbar_init(&M.drain, 1);
         mbar_init(&M.psm, kTcGroup);
         mbar_init(&M.x16, kTcGroup);
@@ -842,19 +843,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     __syncwarp();
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&M.x16, ph, abort));       // X16 is there, and U of the last chunk read
-                if (!STATE_ONLY && c > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.odone, ph ^ 1u, abort));   // and its results
-                if (!ok) break;
-                tc_fence_after();
-                if constexpr (!STATE_ONLY) {
-                    if (leader) {
-#pragma unroll
-                        for (int kk = 0; kk < DK / 16; ++kk)
-                            mma_bf16_ta<64>(tmem + kInter, tmem + kX16 + kk * 8, desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
-                    }
-                    __syncwarp();
-                }
-                ok = __all_sync(0xffffffffu, mbar_wait(&M.vk, ph, abort));
+                // X16 is there, U of the last chunk read, and c's terms are there: U first, the state waits for it
+                ok = __all_sync(0xffffffffu, mbar_wait(&M.x16, ph, abort) && mbar_wait(&M.vk, ph, abort));
                 if (!ok) break;
                 tc_fence_after();
                 if (leader) {
@@ -866,6 +856,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tc_commit(&M.uready);
                 }
                 __syncwarp();
+                if constexpr (!STATE_ONLY) {
+                    // the last chunk's results have been read
+                    if (c > 0) ok = __all_sync(0xffffffffu, mbar_wait(&M.odone, ph ^ 1u, abort));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
+#pragma unroll
+                        for (int kk = 0; kk < DK / 16; ++kk)
+                            mma_bf16_ta<64>(tmem + kInter, tmem + kX16 + kk * 8, desc_swizzled(sa + (kk >> 2) * L::kTile + (kk & 3) * 32), kk > 0);
+                        tc_commit(&M.iready);
+                    }
+                    __syncwarp();
+                }
                 if constexpr (!STATE_ONLY) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&M.psm, ph, abort));
                     if (!ok) break;
@@ -913,22 +916,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int st = c & 1, n = tokens(c);
             const uint32_t ph = c & 1;
             const uint32_t sb = base + L::kHead + st * L::kStage + L::kTilesA * L::kTile, sc = sb + L::kTilesB * L::kTile;
-            if (c > 0) {                 // the last chunk's tiles have been read
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph ^ 1u, abort));
-                if (!STATE_ONLY) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.oready[st ^ 1], ((c - 1) >> 1) & 1, abort));
-            }
+            if (c > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph ^ 1u, abort));   // U has read the last chunk's terms
             if (c == 0 || n < kChunk) {
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 factors(n, c > 0);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
+            uint32_t f[4][4];                            // two tokens of two columns each
+            uint64_t numbers = 0;                        // stays 0 while all values are
             if (ok) {
+                tc_fence_after();
                 // (1) 16 columns of c
                 const uint32_t lrow = (l7 + 8 * l16) * 128;
                 const uint32_t cfrom = sc + (ccol >> 2) * L::kTile + lrow + (((2 * (ccol & 3) + l8) ^ l7) << 4);
                 const uint32_t lanes = tmem + (static_cast<uint32_t>(16 * ccol) << 16);
-                uint32_t f[4][4];
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) ldsm4t_at(f[kk], cfrom + kk * 2048);
                 if (n < kChunk) {
@@ -941,7 +943,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                 }
                 {
-                    uint64_t y[4][4], numbers = 0;       // two tokens' values; `numbers` stays 0 while all values are
+                    uint64_t y[4][4];                    // two tokens' values
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
@@ -951,33 +953,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             if (!STATE_ONLY) numbers = fma2(y[kk][h], 0ull, numbers);
                             y[kk][h] = mul2(y[kk][h], w);
                         }
-                    if constexpr (!STATE_ONLY) {
-                        const float2 finite = unpack2(numbers);
-                        const bool bad = __any_sync(0xffffffffu, finite.x != 0.0f || finite.y != 0.0f);
-                        if (bad) {
-                            int first[2] = {255, 255};
-#pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-                                for (int h = 0; h < 4; ++h)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        const uint32_t part = e ? f[kk][h] >> 16 : f[kk][h] & 0xffffu;
-                                        if ((part & 0x7f80u) != 0x7f80u) continue;
-                                        f[kk][h] &= e ? 0xffffu : 0xffff0000u;
-                                        const int j = kk * 16 + (h >> 1) * 8 + 2 * q + e;
-                                        first[h & 1] = min(first[h & 1], p.reverse ? n - 1 - j : j);
-                                    }
-#pragma unroll
-                            for (int r = 0; r < 2; ++r) {
-                                first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 1));
-                                first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 2));
-                                if (q == 0) M.first_bad[st][16 * ccol + 8 * r + g8] = static_cast<uint8_t>(first[r]);
-                            }
-                        }
-                        if (lane == 0) M.bad[st][ccol] = bad;
-                        tc_st_frag(lanes + kCt, f);
-                    }
+                    uint32_t term[4][4];
 #pragma unroll
                     for (int k = 0; k < TERMS; ++k) {
 #pragma unroll
@@ -985,30 +961,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                             for (int h = 0; h < 4; ++h) {
                                 const float2 v = unpack2(y[kk][h]);
-                                f[kk][h] = bf16x2(v.x, v.y);
+                                term[kk][h] = bf16x2(v.x, v.y);
                                 if (k + 1 < TERMS)       // what the term leaves
-                                    y[kk][h] = fma2(pack2(f[kk][h] << 16, f[kk][h] & 0xffff0000u), kMinusOnes, y[kk][h]);
+                                    y[kk][h] = fma2(pack2(term[kk][h] << 16, term[kk][h] & 0xffff0000u), kMinusOnes, y[kk][h]);
                             }
-                        tc_st_frag(lanes + kWt + 32 * k, f);
+                        tc_st_frag(lanes + kWt + 32 * k, term);
                     }
                 }
                 // and 16 of b
                 const uint32_t to = (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
                 const uint32_t from = (ew >> 2) * L::kTile + lrow + (((2 * (ew & 3) + l8) ^ l7) << 4);
                 if (ew < DK / 16) {
+                    uint32_t t[4][4];
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) ldsm4t_at(f[kk], sb + from + kk * 2048);
+                    for (int kk = 0; kk < 4; ++kk) ldsm4t_at(t[kk], sb + from + kk * 2048);
                     if (n < kChunk) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                             for (int h = 0; h < 4; ++h) {
                                 const int j = kk * 16 + (h >> 1) * 8 + 2 * q;
-                                f[kk][h] &= j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
+                                t[kk][h] &= j + 1 < n ? 0xffffffffu : (j < n ? 0xffffu : 0u);
                             }
                     }
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) stsm4(base + L::kBt + to + kk * 256, f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
+                    for (int kk = 0; kk < 4; ++kk) stsm4(base + L::kBt + to + kk * 256, t[kk][0], t[kk][1], t[kk][2], t[kk][3]);
                 }
                 tc_wait_st();
                 tc_fence_before();
@@ -1017,6 +994,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (lane == 0) mbar_arrive(&M.vk);
             }
             if constexpr (!STATE_ONLY) {
+                // c^T itself goes out with P: intra of the last chunk has read its own, and the results' group what is said of it
+                if (c > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.oready[st ^ 1], ((c - 1) >> 1) & 1, abort));
+                if (ok) {
+                    tc_fence_after();
+                    const float2 finite = unpack2(numbers);
+                    const bool bad = __any_sync(0xffffffffu, finite.x != 0.0f || finite.y != 0.0f);
+                    if (bad) {
+                        int first[2] = {255, 255};
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const uint32_t part = e ? f[kk][h] >> 16 : f[kk][h] & 0xffffu;
+                                    if ((part & 0x7f80u) != 0x7f80u) continue;
+                                    f[kk][h] &= e ? 0xffffu : 0xffff0000u;
+                                    const int j = kk * 16 + (h >> 1) * 8 + 2 * q + e;
+                                    first[h & 1] = min(first[h & 1], p.reverse ? n - 1 - j : j);
+                                }
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 1));
+                            first[r] = min(first[r], __shfl_xor_sync(0xffffffffu, first[r], 2));
+                            if (q == 0) M.first_bad[st][16 * ccol + 8 * r + g8] = static_cast<uint8_t>(first[r]);
+                        }
+                    }
+                    if (lane == 0) M.bad[st][ccol] = bad;
+                    tc_st_frag(tmem + (static_cast<uint32_t>(16 * ccol) << 16) + kCt, f);
+                }
                 // (2) rows i = 16 sub + g and + 8, columns j = 32 half + 8 nt + 2 q and + 1: v[4 nt ..]
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.pready, ph, abort));
                 if (ok) {
@@ -1044,6 +1051,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const uint32_t at = base + L::kProb + (2 * sub + l8) * 1024 + (4 * half + l16) * 128 + l7 * 16;
                     stsm4(at, r[0], r[1], r[2], r[3]);
                     stsm4(at + 256, r[4], r[5], r[6], r[7]);
+                    tc_wait_st();
                     tc_fence_before();
                     proxy_fence();
                     __syncwarp();
@@ -1125,7 +1133,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int i = 0; i < 16; i += 2) x[(i0 + i) / 2] = fma2(whole2, x[(i0 + i) / 2], pack2(v[i], v[i + 1]));
                 }
                 tc_fence_before();
-                if (c + 1 < chunks) copy_state();
+                if (c + 1 < chunks) {
+                    if (!STATE_ONLY) ok = __all_sync(0xffffffffu, mbar_wait(&M.iready, ph, abort));   // inter has read the last copy
+                    tc_fence_after();
+                    if (ok) copy_state();
+                }
             }
             if constexpr (!STATE_ONLY) {
                 // (4) the results: 32 tokens of this lane's column
