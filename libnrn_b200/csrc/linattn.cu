@@ -632,6 +632,7 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
 constexpr int kTcThreads = 640;
 constexpr int kTcGroup = 8;             // warps of each of the two groups
 constexpr int kTcCols = 128;
+constexpr int kTcStages = 3;             // chunks of a, b and c in shared memory: with two, the copies' latency showed
 enum { ERR_LINATTN_TIMEOUT = 5 };
 
 using namespace tc;
@@ -641,8 +642,8 @@ struct TcSmem {
     static constexpr int kTile = kChunk * 128;                        // 64 rows of 64 bf16: 8 KB
     static constexpr int kTilesA = STATE_ONLY ? 0 : DK / 64, kTilesB = DK / 64, kTilesC = 2;
     static constexpr int kStage = (kTilesA + kTilesB + kTilesC) * kTile;
-    static constexpr int kHead = 2048;
-    static constexpr int kBt = kHead + 2 * kStage;                    // b^T [DK][64]
+    static constexpr int kHead = 3072;
+    static constexpr int kBt = kHead + kTcStages * kStage;                    // b^T [DK][64]
     static constexpr int kProb = kBt + DK * 128;                      // [64][64]
     static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 2 KB for each warp of results
     static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 2048);
@@ -650,7 +651,7 @@ struct TcSmem {
 static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
 
 struct TcHead {
-    uint64_t full[2], empty[2], oready[2], pready, psm, x16, vk, uready, iready, odone, drain;
+    uint64_t full[kTcStages], empty[kTcStages], oready[2], pready, psm, x16, vk, uready, iready, odone, drain;
     uint32_t tmem;
     int abort;
     alignas(16) float lag[128];    // factor of P at token i - token j, from -63 on
@@ -660,7 +661,7 @@ struct TcHead {
     uint8_t bad[2][kTcGroup];      // 16 columns of c hold a value that is no number, and each column's first, in scan order
     uint8_t first_bad[2][kTcCols];
 };
-static_assert(sizeof(TcHead) <= 2048, "barriers and factors");
+static_assert(sizeof(TcHead) <= 3072, "barriers and factors");
 
 // No swizzle: rows of 16 bytes, eight rows to a core matrix, core matrices of
 // one row group 128 bytes apart, row groups `group` bytes apart.
@@ -764,9 +765,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr uint32_t kP = 0, kU = 64, kIntra = 192, kInter = 256, kX16 = 320, kWt = 384, kCt = 480;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kTcStages; ++i) {
             mbar_init(&M.full[i], 1);
             mbar_init(&M.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&M.oready[i], 1);   // two: the next chunk's may come before this one's is looked at
         }
         mbar_init(&M.pready, 1);
@@ -802,10 +805,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0 && lane == 0) {
-            int c = 0;
+            int c = 0, st = 0;
+            uint32_t phase = 0;
             for (; c < chunks; ++c) {
-                const int st = c & 1;
-                if (!mbar_wait(&M.empty[st], ((c >> 1) & 1) ^ 1u, abort)) {
+                if (!mbar_wait(&M.empty[st], phase ^ 1u, abort)) {
                     fail();
                     break;
                 }
@@ -818,18 +821,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tma_load_4d(dst + (L::kTilesA + i) * L::kTile, &bmap, 64 * i, head / p.b.share, tok, seq, &M.full[st]);
                 for (int i = 0; i < L::kTilesC; ++i)
                     tma_load_4d(dst + (L::kTilesA + L::kTilesB + i) * L::kTile, &cmap, tile * kTcCols + 64 * i, head / p.c.share, tok, seq, &M.full[st]);
+                if (++st == kTcStages) {
+                    st = 0;
+                    phase ^= 1u;
+                }
             }
             // the copies still in flight land before the block ends
-            for (int q = c - 1; q >= 0 && q >= c - 2; --q) mbar_wait(&M.full[q & 1], (q >> 1) & 1, nullptr);
+            for (int q = c - 1; q >= 0 && q >= c - kTcStages; --q) mbar_wait(&M.full[q % kTcStages], (q / kTcStages) & 1, nullptr);
         } else if (warp == 1) {
             // the whole warp walks the chunks, one thread issues
             const bool leader = elect_one();
             bool ok = true;
+            int stage = 0;
+            uint32_t phase = 0;
             for (int c = 0; c < chunks; ++c) {
-                const int st = c & 1;
                 const uint32_t ph = c & 1;
-                const uint32_t sa = base + L::kHead + st * L::kStage, sb = sa + L::kTilesA * L::kTile;
-                ok = __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
+                const uint32_t sa = base + L::kHead + stage * L::kStage, sb = sa + L::kTilesA * L::kTile;
+                ok = __all_sync(0xffffffffu, mbar_wait(&M.full[stage], phase, abort));
                 if (!ok) break;
                 tc_fence_after();
                 if constexpr (!STATE_ONLY) {
@@ -877,12 +885,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
                             mma_bf16_ta<64>(tmem + kIntra, tmem + kCt + kk * 8, desc_plain(base + L::kProb + kk * 256, 1024), kk > 0);
-                        tc_commit(&M.oready[st]);
+                        tc_commit(&M.oready[ph]);
                     }
                     __syncwarp();
                 }
-                if (leader) tc_commit(&M.empty[st]);
+                if (leader) tc_commit(&M.empty[stage]);
                 __syncwarp();
+                if (++stage == kTcStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
             if (!ok && leader) fail();
             // every MMA issued has completed before the accumulators are freed
@@ -912,17 +924,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (et >= 192) M.out[last][et - 192] = p.out_mul * f;
         };
         bool ok = true;
+        int stage = kTcStages - 1;
+        uint32_t phase = 1;
         for (int c = 0; c < chunks; ++c) {
+            if (++stage == kTcStages) {
+                stage = 0;
+                phase ^= 1u;
+            }
             const int st = c & 1, n = tokens(c);
             const uint32_t ph = c & 1;
-            const uint32_t sb = base + L::kHead + st * L::kStage + L::kTilesA * L::kTile, sc = sb + L::kTilesB * L::kTile;
+            const uint32_t sb = base + L::kHead + stage * L::kStage + L::kTilesA * L::kTile, sc = sb + L::kTilesB * L::kTile;
             if (c > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph ^ 1u, abort));   // U has read the last chunk's terms
             if (c == 0 || n < kChunk) {
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 factors(n, c > 0);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[st], (c >> 1) & 1, abort));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.full[stage], phase, abort));
             uint32_t f[4][4];                            // two tokens of two columns each
             uint64_t numbers = 0;                        // stays 0 while all values are
             if (ok) {
