@@ -38,4 +38,23 @@ cudaError_t allow_shared(int bytes) {
     return e;
 }
 
+// Kernels that follow one another in one call: with `after`, the blocks of
+// this one take their places as those of the one before leave, and wait
+// (previous_done) before they touch what it wrote, or write what it reads.
+// Each kernel of such a chain lets the next one in (let_next) and waits on
+// every path, so that the end of one is the end of all before it; a kernel that
+// does neither may stand in the chain, launched as usual.
+template <typename... P, typename... A>
+cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, int shared, cudaStream_t s, bool after, const A&... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid, c.blockDim = block, c.dynamicSmemBytes = static_cast<size_t>(shared), c.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at, c.numAttrs = after ? 1 : 0;
+    return cudaLaunchKernelEx(&c, kernel, args...);
+}
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 }  // namespace nrn

@@ -767,7 +767,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int head = (blockIdx.x / tiles) % p.heads;
     const int unit = blockIdx.x / tiles / p.heads;
     const Unit u = unit_of(p, unit);
-    if (!u.any) return;
+    let_next();
+    if (!u.any) {
+        previous_done();
+        return;
+    }
     const int chunks = static_cast<int>((u.end - u.begin + kChunk - 1) / kChunk);
     // TMEM columns: accumulators, then the left operands X16, c^T's terms and c^T
     constexpr uint32_t kP = 0, kU = 64, kIntra = kU + DK, kInter = kIntra + 64, kX16 = kInter + 64, kCt = kX16 + DK / 2,
@@ -802,6 +806,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = M.tmem;
+    previous_done();
     auto fail = [&]() {
         *abort = 1;
         if (p.err) atomicCAS(p.err, 0, ERR_LINATTN_TIMEOUT);
@@ -1289,6 +1294,8 @@ __global__ void __launch_bounds__(128) scan_join_kernel(const __grid_constant__ 
     if (threadIdx.x == 0) power[0] = decay_power(p.log_decay[head], p.seg_len);
     if (threadIdx.x == 32) power[1] = decay_power(p.log_decay[head], len - (segs - 1) * p.seg_len);
     __syncthreads();
+    let_next();
+    previous_done();
     const int64_t e = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * V;
     if (e >= n) return;
     const int64_t sh = (static_cast<int64_t>(seq) * p.heads + head) * n;
@@ -1339,6 +1346,8 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* part, uint3
                                                         int64_t o_seq, int64_t o_tok, int64_t o_head, uint32_t per_seq) {
     const uint32_t vecs = d / V, row = kv * vecs;
     const uint32_t t = blockIdx.x * blockDim.y + threadIdx.y;
+    let_next();
+    previous_done();
     if (t >= tokens) return;
     const float* from = part + static_cast<int64_t>(t) * kv * share * d;
     const uint32_t s = t / per_seq;
@@ -1363,6 +1372,7 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* part, uint3
     }
 }
 
+// Always after the scan that made the parts.
 template <typename T>
 cudaError_t sum_heads(const float* part, int64_t tokens, int kv, int share, int d, void* out, const int64_t* st, int64_t per_seq, cudaStream_t s) {
     const int64_t n = 16 / static_cast<int64_t>(sizeof(T));
@@ -1372,12 +1382,10 @@ cudaError_t sum_heads(const float* part, int64_t tokens, int kv, int share, int 
     const dim3 threads(block.x, 256 / block.x);
     const unsigned blocks = static_cast<unsigned>((tokens + threads.y - 1) / threads.y);
     if (vec)
-        sum_heads_kernel<T, 8><<<blocks, threads, 0, s>>>(part, static_cast<uint32_t>(tokens), kv, share, d, static_cast<T*>(out), st[0], st[1], st[2],
-                                                          static_cast<uint32_t>(per_seq));
-    else
-        sum_heads_kernel<T, 1><<<blocks, threads, 0, s>>>(part, static_cast<uint32_t>(tokens), kv, share, d, static_cast<T*>(out), st[0], st[1], st[2],
-                                                          static_cast<uint32_t>(per_seq));
-    return cudaGetLastError();
+        return launch_chained(sum_heads_kernel<T, 8>, blocks, threads, 0, s, true, part, static_cast<uint32_t>(tokens), kv, share, d, static_cast<T*>(out),
+                              st[0], st[1], st[2], static_cast<uint32_t>(per_seq));
+    return launch_chained(sum_heads_kernel<T, 1>, blocks, threads, 0, s, true, part, static_cast<uint32_t>(tokens), kv, share, d, static_cast<T*>(out), st[0],
+                          st[1], st[2], static_cast<uint32_t>(per_seq));
 }
 
 // -------------------------------------------------------------- one token
@@ -1529,26 +1537,27 @@ bool make_scan_map(const Strided& m, const ScanArgs& p, CUtensorMap* map) {
 }
 
 template <int DK, int TERMS, bool STATE_ONLY>
-cudaError_t launch_tc(const ScanArgs& p, const CUtensorMap* maps, cudaStream_t s) {
+cudaError_t launch_tc(const ScanArgs& p, const CUtensorMap* maps, bool after, cudaStream_t s) {
     const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kTcCols - 1) / kTcCols);
     constexpr int bytes = TcSmem<DK, TERMS, STATE_ONLY>::kBytes;
     const cudaError_t e = allow_shared<scan_tc_kernel<DK, TERMS, STATE_ONLY>>(bytes);
     if (e != cudaSuccess) return e;
-    scan_tc_kernel<DK, TERMS, STATE_ONLY><<<static_cast<unsigned>(blocks), kTcThreads, bytes, s>>>(maps[0], maps[1], maps[2], p);
-    return cudaGetLastError();
+    return launch_chained(scan_tc_kernel<DK, TERMS, STATE_ONLY>, dim3(static_cast<unsigned>(blocks)), dim3(kTcThreads), bytes, s, after, maps[0], maps[1],
+                          maps[2], p);
 }
 
 template <int DK>
-cudaError_t launch_tc_any(const ScanArgs& p, const CUtensorMap* maps, bool state_only, cudaStream_t s) {
-    if (state_only) return launch_tc<DK, 3, true>(p, maps, s);
-    return p.seg == nullptr && p.s_out != nullptr ? launch_tc<DK, 3, false>(p, maps, s) : launch_tc<DK, 2, false>(p, maps, s);
+cudaError_t launch_tc_any(const ScanArgs& p, const CUtensorMap* maps, bool state_only, bool after, cudaStream_t s) {
+    if (state_only) return launch_tc<DK, 3, true>(p, maps, after, s);
+    return p.seg == nullptr && p.s_out != nullptr ? launch_tc<DK, 3, false>(p, maps, after, s) : launch_tc<DK, 2, false>(p, maps, after, s);
 }
 
-cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, cudaStream_t s) {
+// after: a kernel of the same call comes before it
+cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, bool after, cudaStream_t s) {
     if (dtype == NRN_BF16 && p.b.d <= 128 && p.vec && p.tokens > 0 && p.tokens < (int64_t(1) << 31) - kChunk) {
         CUtensorMap maps[3];
         if (make_scan_map(p.a, p, &maps[0]) && make_scan_map(p.b, p, &maps[1]) && make_scan_map(p.c, p, &maps[2]))
-            return p.b.d <= 64 ? launch_tc_any<64>(p, maps, state_only, s) : launch_tc_any<128>(p, maps, state_only, s);
+            return p.b.d <= 64 ? launch_tc_any<64>(p, maps, state_only, after, s) : launch_tc_any<128>(p, maps, state_only, after, s);
     }
     if (dtype == NRN_BF16 && p.b.d <= 64) return launch_mma_any<64>(p, state_only, s);
     if (dtype == NRN_BF16 && p.b.d <= 128) return launch_mma_any<128>(p, state_only, s);
@@ -1625,7 +1634,7 @@ int64_t workspace_need(const nrn_linattn_t* a, bool backward) {
     return n;
 }
 
-nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, cudaStream_t s) {
+nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, bool after, cudaStream_t s) {
     const int per16 = 16 / elem_size(a->dtype);
     p.o_vec = reinterpret_cast<uintptr_t>(p.o) % 16 == 0 && p.o_seq % per16 == 0 && p.o_tok % per16 == 0 && p.o_head % per16 == 0 && p.c.d % per16 == 0;
     if (p.cu) p.a.seq = p.b.seq = p.c.seq = p.o_seq = 0;      // packed: a token's row counts from the arrays' start
@@ -1638,15 +1647,14 @@ nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, cudaStream_t s) {
     p.seg = is_split(a, p.seg_len) ? static_cast<float*>(a->workspace) : nullptr;
     if (!p.seg_made) p.g_i = p.c.d, p.g_j = 1;
     if (p.seg != nullptr && !p.seg_made) {
-        NRN_CUDA_TRY(launch_scan(p, a->dtype, true, s));
+        NRN_CUDA_TRY(launch_scan(p, a->dtype, true, after, s));
         const int64_t n = static_cast<int64_t>(p.b.d) * p.c.d;
         const int v = n % 2 == 0 ? 2 : 1;      // every state starts on an even element then
         const dim3 grid(static_cast<unsigned>((n / v + 127) / 128), static_cast<unsigned>(p.seqs * p.heads));
-        if (v == 2) scan_join_kernel<2><<<grid, 128, 0, s>>>(p);
-        else scan_join_kernel<1><<<grid, 128, 0, s>>>(p);
-        NRN_CUDA_TRY(cudaGetLastError());
+        NRN_CUDA_TRY(launch_chained(v == 2 ? scan_join_kernel<2> : scan_join_kernel<1>, grid, dim3(128), 0, s, true, p));
+        after = true;
     }
-    NRN_CUDA_TRY(launch_scan(p, a->dtype, false, s));
+    NRN_CUDA_TRY(launch_scan(p, a->dtype, false, after, s));
     return NRN_OK;
 }
 
@@ -1731,7 +1739,7 @@ extern "C" nrn_status_t nrn_cuda_linattn_forward(const nrn_linattn_t* a, nrn_str
     p.o_seq = a->o_stride[0], p.o_tok = a->o_stride[1], p.o_head = a->o_stride[2];
     p.s_in = a->state_in, p.s_out = a->state_out;
     p.s_i = a->dv, p.s_j = 1;
-    return run_scan(p, a, reinterpret_cast<cudaStream_t>(stream));
+    return run_scan(p, a, false, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const nrn_linattn_grad_t* g, nrn_stream_t stream) {
@@ -1755,7 +1763,7 @@ extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const 
     p.o_seq = g->dq_stride[0], p.o_tok = g->dq_stride[1], p.o_head = g->dq_stride[2];
     p.s_in = a->state_in;
     p.s_i = 1, p.s_j = a->dv;
-    NRN_TRY(run_scan(p, a, s));
+    NRN_TRY(run_scan(p, a, false, s));
 
     // the gradients of keys and values run backwards in time; heads that
     // share one key or value head leave fp32 parts, summed in a fixed order
@@ -1787,7 +1795,7 @@ extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const 
             p.o_tok = static_cast<int64_t>(a->heads) * dd;
             p.o_seq = a->cu_seqlens ? 0 : p.o_tok * a->tokens;
         }
-        NRN_TRY(run_scan(p, a, s));
+        NRN_TRY(run_scan(p, a, true, s));
         const int64_t n = all_tokens(a);
         if (share == 1 || n == 0) continue;
         const int64_t per = a->cu_seqlens ? n : a->tokens;
