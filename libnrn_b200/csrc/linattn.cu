@@ -653,8 +653,8 @@ struct TcSmem {
     static constexpr int kBt = kHead + kTcStages * kStage;                    // b^T [DK][64]
     static constexpr int kBuffers = STATE_ONLY ? 2 : 1;   // of the left operand's terms and b^T: the state's pass has room
     static constexpr int kProb = kBt + kBuffers * DK * 128;           // [64][64]
-    static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 2 KB for each warp of results
-    static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 2048);
+    static constexpr int kOut = kProb + (STATE_ONLY ? 0 : kTile);          // 4 KB for each warp of results
+    static constexpr int kBytes = kOut + (STATE_ONLY ? 0 : kTcGroup * 4096);
 };
 static_assert(TcSmem<128, 3, false>::kBytes <= 227 * 1024, "shared memory of one block");
 
@@ -751,7 +751,8 @@ __device__ __forceinline__ void tc_ld_frag(uint32_t taddr, uint32_t* v) {
 }
 constexpr uint64_t kMinusOnes = 0xbf800000bf800000ull;
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-template <int DK, int TERMS, bool STATE_ONLY>
+// F32: the results are fp32 parts (shared heads); both kinds in one kernel cost it registers (4%)
+template <int DK, int TERMS, bool STATE_ONLY, bool F32>
 __global__ void __launch_bounds__(kTcThreads, 1)
     scan_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                    const __grid_constant__ CUtensorMap cmap, const __grid_constant__ ScanArgs p) {
@@ -1183,8 +1184,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const bool bad = (M.bad[st][2 * sub] | M.bad[st][2 * sub + 1]) != 0;
                     const int64_t at = (u.row0 + first(c) + 32 * half) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head;
                     const int m = n - 32 * half;             // tokens of this half
-                    // bf16 results pass through 2 KB of this warp's own, two tokens a word
-                    unsigned char* own = smem + L::kOut + ew * 2048;
+                    // results pass through shared memory of this warp's own, bf16 ones two tokens a word
+                    unsigned char* own = smem + L::kOut + ew * 4096;
 #pragma unroll
                     for (int t0 = 0; t0 < 32; t0 += 16) {
                         uint32_t a[16], b[16];
@@ -1208,22 +1209,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 if ((p.reverse ? n - 1 - i : i) >= from) a[t] = 0x7fffffffu;
                             }
                         }
-                        if (p.o_f32) {
-                            float* f = static_cast<float*>(p.o) + at + t0 * p.o_tok + row;
+                        if constexpr (F32) {
 #pragma unroll
-                            for (int t = 0; t < 16; ++t, f += p.o_tok)
-                                if (t0 + t < m && row < dc) *f = __uint_as_float(a[t]);
+                            for (int t = 0; t < 16; ++t) *reinterpret_cast<uint32_t*>(own + (t0 + t) * 128 + lane * 4) = a[t];
+                        } else {
+#pragma unroll
+                            for (int t = 0; t < 16; t += 2)
+                                *reinterpret_cast<uint32_t*>(own + (t0 + t) * 64 + lane * 4) = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
                         }
-#pragma unroll
-                        for (int t = 0; t < 16; t += 2)
-                            *reinterpret_cast<uint32_t*>(own + (t0 + t) * 64 + lane * 4) = bf16x2(__uint_as_float(a[t]), __uint_as_float(a[t + 1]));
                     }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&M.odone);    // read: the next chunk's may come
-                    if (!p.o_f32) {
+                    const int j4 = tile * kTcCols + 32 * sub + 4 * (lane & 7);
+                    if constexpr (F32) {
+                        // four tokens at a time, 128 bytes each (a store a token straight from the registers: a scan of 106 us takes 78 so)
+                        float* to = static_cast<float*>(p.o) + at + (lane >> 3) * p.o_tok + j4;
+#pragma unroll
+                        for (int t = lane >> 3; t < 32; t += 4, to += 4 * p.o_tok) {
+                            const float4 r = *reinterpret_cast<const float4*>(own + t * 128 + (lane & 7) * 16);
+                            if (t >= m || j4 >= dc) continue;
+                            if (p.o_vec) {
+                                *reinterpret_cast<float4*>(to) = r;
+                            } else {
+                                to[0] = r.x;
+                                if (j4 + 1 < dc) to[1] = r.y;
+                                if (j4 + 2 < dc) to[2] = r.z;
+                                if (j4 + 3 < dc) to[3] = r.w;
+                            }
+                        }
+                        __syncwarp();
+                    } else {
                         // out of there as four columns of two tokens a lane: 64 bytes a token
-                        const int t8 = 2 * (lane >> 3), j4 = tile * kTcCols + 32 * sub + 4 * (lane & 7);
+                        const int t8 = 2 * (lane >> 3);
                         __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + at + t8 * p.o_tok + j4;
 #pragma unroll
                         for (int k = 0; k < 4; ++k, to += 8 * p.o_tok) {
@@ -1536,20 +1554,22 @@ bool make_scan_map(const Strided& m, const ScanArgs& p, CUtensorMap* map) {
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DK, int TERMS, bool STATE_ONLY>
+template <int DK, int TERMS, bool STATE_ONLY, bool F32>
 cudaError_t launch_tc(const ScanArgs& p, const CUtensorMap* maps, bool after, cudaStream_t s) {
     const int64_t blocks = static_cast<int64_t>(p.units) * p.heads * ((p.c.d + kTcCols - 1) / kTcCols);
     constexpr int bytes = TcSmem<DK, TERMS, STATE_ONLY>::kBytes;
-    const cudaError_t e = allow_shared<scan_tc_kernel<DK, TERMS, STATE_ONLY>>(bytes);
+    const cudaError_t e = allow_shared<scan_tc_kernel<DK, TERMS, STATE_ONLY, F32>>(bytes);
     if (e != cudaSuccess) return e;
-    return launch_chained(scan_tc_kernel<DK, TERMS, STATE_ONLY>, dim3(static_cast<unsigned>(blocks)), dim3(kTcThreads), bytes, s, after, maps[0], maps[1],
+    return launch_chained(scan_tc_kernel<DK, TERMS, STATE_ONLY, F32>, dim3(static_cast<unsigned>(blocks)), dim3(kTcThreads), bytes, s, after, maps[0], maps[1],
                           maps[2], p);
 }
 
 template <int DK>
 cudaError_t launch_tc_any(const ScanArgs& p, const CUtensorMap* maps, bool state_only, bool after, cudaStream_t s) {
-    if (state_only) return launch_tc<DK, 3, true>(p, maps, after, s);
-    return p.seg == nullptr && p.s_out != nullptr ? launch_tc<DK, 3, false>(p, maps, after, s) : launch_tc<DK, 2, false>(p, maps, after, s);
+    if (state_only) return launch_tc<DK, 3, true, false>(p, maps, after, s);
+    const bool whole = p.seg == nullptr && p.s_out != nullptr;
+    if (p.o_f32) return whole ? launch_tc<DK, 3, false, true>(p, maps, after, s) : launch_tc<DK, 2, false, true>(p, maps, after, s);
+    return whole ? launch_tc<DK, 3, false, false>(p, maps, after, s) : launch_tc<DK, 2, false, false>(p, maps, after, s);
 }
 
 // after: a kernel of the same call comes before it
