@@ -40,6 +40,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -120,6 +121,13 @@ struct Shape {
     static constexpr uint32_t kTmem = NT * kBufs < 32 ? 32 : NT * kBufs;
     static constexpr int kStageBytes = (kRowTile + NT) * kBlock;
 };
+// Results whose rows do not start on 16 bytes, or that end inside a tile, pass
+// through 32 x 16 floats of a warp's own, so that a store covers two rows: one
+// element of 32 rows a store made 6992 x 4411 results (213 columns) 336 us
+// that take 53.  A kernel of its own (ODD): in one with the rest the backward
+// pass took 175 us where it takes 166.
+constexpr int kOutPitch = 17;          // floats: no bank conflicts either way
+constexpr int kOutBytes = kEpiThreads / 32 * 32 * kOutPitch * 4;
 
 template <typename T>
 __device__ __forceinline__ void put(void* out, int64_t at, float x) {
@@ -133,7 +141,7 @@ __device__ __forceinline__ void put_any(void* out, int dtype, int64_t at, float 
 
 // CBLOCK: the cols operand has one scale for 128 rows (uniform over a
 // warpgroup's columns); otherwise one for each, staged in shared memory.
-template <int NT, bool CBLOCK>
+template <int NT, bool CBLOCK, bool ODD>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap rmap, const __grid_constant__ CUtensorMap cmap,
                    const __grid_constant__ ProductArgs a) {
@@ -374,8 +382,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (et == 0) a.count[tile] = 0;
             }
-            if (row < a.n_rows) {
-                if (a.vec && col0 + S::kCols <= a.n_cols && S::kCols >= 8) {
+            const bool whole = a.vec && col0 + S::kCols <= a.n_cols;      // this warpgroup's columns
+            if (ODD && !whole) {
+                float* st = reinterpret_cast<float*>(tiles + stages * S::kStageBytes) + (et >> 5) * 32 * kOutPitch;
+                const int e = lane % S::kChunk, first = rt * kRowTile + sub * 32;
+#pragma unroll
+                for (int j = 0; j < S::kCols; j += S::kChunk) {
+                    if (col0 + j >= a.n_cols) continue;
+#pragma unroll
+                    for (int c = 0; c < S::kChunk; c += 2) {
+                        const float2 y = unpack2(acc[(j + c) / 2]);
+                        st[lane * kOutPitch + c] = y.x, st[lane * kOutPitch + c + 1] = y.y;
+                    }
+                    __syncwarp();
+                    if (col0 + j + e < a.n_cols) {
+                        const int64_t at = first * a.out_row + col0 + j + e;
+                        const int rows = min(a.n_rows - first, 32);
+                        if (a.dtype == NRN_FP32) {
+                            for (int r = lane / S::kChunk; r < rows; r += 32 / S::kChunk) static_cast<float*>(a.out)[at + r * a.out_row] = st[r * kOutPitch + e];
+                        } else if (a.dtype == NRN_BF16) {
+                            for (int r = lane / S::kChunk; r < rows; r += 32 / S::kChunk) put<__nv_bfloat16>(a.out, at + r * a.out_row, st[r * kOutPitch + e]);
+                        } else {
+                            for (int r = lane / S::kChunk; r < rows; r += 32 / S::kChunk) put<__half>(a.out, at + r * a.out_row, st[r * kOutPitch + e]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            } else if (row < a.n_rows) {
+                if (whole) {
                     // 8 columns at a time: 16 bytes (32 in fp32)
 #pragma unroll
                     for (int j = 0; j < S::kCols; j += 8) {
@@ -390,7 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         else if (a.dtype == NRN_FP16) store8(static_cast<__half*>(a.out) + at, x, 8, true);
                         else store8(static_cast<float*>(a.out) + at, x, 8, true);
                     }
-                } else {
+                } else if constexpr (!ODD) {
+                    // swapped: neighbouring lanes' rows are neighbours in the result
 #pragma unroll
                     for (int j = 0; j < S::kCols; ++j) {
                         const float2 y = unpack2(acc[j / 2]);
@@ -712,25 +747,30 @@ nrn_status_t check_scaled(const nrn_scaled_t* m, const std::string& who) {
     return NRN_OK;
 }
 
-template <int NT, bool CB>
+template <int NT, bool CB, bool ODD>
 nrn_status_t launch_product(const CUtensorMap& rm, const CUtensorMap& cm, ProductArgs a, bool after, cudaStream_t s) {
     constexpr int stage = Shape<NT>::kStageBytes;
-    a.stages = std::min(kMaxStages, (227 * 1024 - kSmemHead) / stage);
-    const int bytes = kSmemHead + a.stages * stage;
-    NRN_CUDA_TRY((allow_shared<product_kernel<NT, CB>>(bytes)));
+    a.stages = std::min(kMaxStages, (227 * 1024 - kSmemHead - (ODD ? kOutBytes : 0)) / stage);
+    const int bytes = kSmemHead + a.stages * stage + (ODD ? kOutBytes : 0);
+    NRN_CUDA_TRY((allow_shared<product_kernel<NT, CB, ODD>>(bytes)));
     const int grid = std::min(a.row_tiles * a.col_tiles * a.splits, sm_count());
-    NRN_CUDA_TRY(launch_chained(product_kernel<NT, CB>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), bytes, s, after, rm, cm, a));
+    NRN_CUDA_TRY(launch_chained(product_kernel<NT, CB, ODD>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), bytes, s, after, rm, cm, a));
     return NRN_OK;
 }
 
 template <bool CB>
 nrn_status_t launch_nt(int nt, const CUtensorMap& rm, const CUtensorMap& cm, const ProductArgs& a, bool after, cudaStream_t s) {
+    // rows of results that end inside a warpgroup's columns, or start anywhere
+    const bool odd = a.out_col == 1 && !(a.vec && a.n_cols % (nt / 2) == 0);
+    const auto run = [&](auto width) {
+        return odd ? launch_product<width(), CB, true>(rm, cm, a, after, s) : launch_product<width(), CB, false>(rm, cm, a, after, s);
+    };
     switch (nt) {
-        case 256: return launch_product<256, CB>(rm, cm, a, after, s);
-        case 128: return launch_product<128, CB>(rm, cm, a, after, s);
-        case 64: return launch_product<64, CB>(rm, cm, a, after, s);
-        case 32: return launch_product<32, CB>(rm, cm, a, after, s);
-        default: return launch_product<16, CB>(rm, cm, a, after, s);
+        case 256: return run(std::integral_constant<int, 256>());
+        case 128: return run(std::integral_constant<int, 128>());
+        case 64: return run(std::integral_constant<int, 64>());
+        case 32: return run(std::integral_constant<int, 32>());
+        default: return run(std::integral_constant<int, 16>());
     }
 }
 
