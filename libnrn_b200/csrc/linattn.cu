@@ -137,9 +137,11 @@ __device__ __forceinline__ const T* row_ptr(const Strided& m, const Unit& u, int
 // columns (c) of one state: 8 lanes share a column, each with every eighth
 // group of four rows in registers, so a token costs each thread
 // 3 * b.d / 8 operations and three shuffles; 16 tokens at a time are staged
-// in shared memory as fp32.  Bound by the fp32 pipe: 3 b.d c.d operations a
-// token and head.  It serves fp16, fp32 and b.d > 128; bf16 with b.d <= 128
-// has the kernels below.
+// in shared memory as fp32.  It does 3 b.d c.d operations a token and head on
+// the fp32 pipe, at about a sixth of the pipe's rate (256 x 64 fp32 tokens of
+// 16 heads of 128 x 128: 2.1 ms): every token is a chain of shared-memory
+// loads, products and shuffles that the next one waits for.  It serves fp16,
+// fp32 and b.d > 128; bf16 with b.d <= 128 has the kernels below.
 //
 // lam in fp32 is off by up to 3e-8, which over a memory of thousands of
 // tokens would show; the error of its powers is taken out of the state after
