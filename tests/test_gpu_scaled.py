@@ -188,3 +188,21 @@ def test_refusals():
                  lambda: scaled.Scaled(q.values[:, 1:129], q.scales[:, :1])):
         with pytest.raises(N.NrnError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=str)
+@pytest.mark.parametrize("shape", [(700, 1001, 130), (2100, 1344, 100), (2051, 2176, 300), (700, 129, 256), (1500, 264, 64)], ids=str)
+def test_product_ragged_edges(shape, dtype):
+    """Results that end inside a tile or inside one half of it, rows on 16 bytes and off: nothing beside them is written."""
+    from libnrn_b200 import scaled
+    m, n, k = shape
+    a, b = scaled.quantize(randn(m, k, seed=3)), scaled.quantize(randn(n, k, seed=4), row_block=128)
+    want = a.dequantize(torch.float64) @ b.dequantize(torch.float64).t()
+    for first, pitch in ((0, n + 24 - n % 8), (5, n + 11)):
+        out = torch.full((m + 2, pitch), 7.0, device="cuda", dtype=dtype)
+        y = out[1:m + 1, first:first + n]
+        scaled.product(a, b, out=y)
+        scaled.check()
+        assert R.rel(y, want) <= tol(dtype, k)
+        y.fill_(7.0)
+        assert bool((out == 7.0).all())
