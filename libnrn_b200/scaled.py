@@ -13,6 +13,7 @@ products summed in fp32 within a block, scaled, and summed in fp32.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -149,23 +150,37 @@ def transpose(w: Scaled, *, stream=None) -> Scaled:
     return out
 
 
-# Split products' workspaces, one for each stream (calls on one stream follow one another).
-_workspaces: dict = {}
-
-
 _COUNTERS = 4096        # bytes at a workspace's start that are zero between calls
 
 
-def _workspace(n: int, device, stream: int) -> torch.Tensor:
-    capturing = torch.cuda.is_current_stream_capturing()     # then it belongs to the graph
+class _Stream:
+    """What calls on one stream share: their workspace (they follow one another there), and whose turn it is to enqueue.  The
+    library lets other threads run while it launches: without turns another thread's kernels could come between those of
+    one call and overwrite what they hand on, or free the workspace before they are in the stream."""
+
+    __slots__ = ("turn", "work")
+
+    def __init__(self):
+        self.turn, self.work = threading.Lock(), None
+
+    def workspace(self, n: int, device) -> torch.Tensor:
+        """n bytes; for the thread whose turn it is, which keeps hold of them until its launches are made."""
+        capturing = torch.cuda.is_current_stream_capturing()     # then it belongs to the graph
+        w = None if capturing else self.work
+        if w is None or w.numel() < n:
+            w = torch.empty(max(n, _COUNTERS), dtype=torch.uint8, device=device)
+            w[:_COUNTERS].zero_()
+            if not capturing:
+                self.work = w
+        return w
+
+
+_streams: dict = {}
+
+
+def _on_stream(device, stream: int) -> _Stream:
     key = (device.index, stream)
-    w = None if capturing else _workspaces.get(key)
-    if w is None or w.numel() < n:
-        w = torch.empty(max(n, _COUNTERS), dtype=torch.uint8, device=device)
-        w[:_COUNTERS].zero_()
-        if not capturing:
-            _workspaces[key] = w
-    return w
+    return _streams.get(key) or _streams.setdefault(key, _Stream())
 
 
 check = check_waits
@@ -201,9 +216,14 @@ def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None
         if out is None:
             n = b.shape[0]
             out = torch.empty_strided((a.shape[0], n), (n, 1), dtype=dtype, device=dev)
-        w = _workspace(need, dev, st).data_ptr() if need else None
-        N.check(N.lib().nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), kind, stride, w, need, error_flag(dev), st),
-                "nrn_cuda_scaled_product")
+        if need:
+            shared = _on_stream(dev, st)
+            with shared.turn:
+                w = shared.workspace(need, dev)
+                s = N.lib().nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), kind, stride, w.data_ptr(), need, error_flag(dev), st)
+        else:
+            s = N.lib().nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), kind, stride, None, 0, error_flag(dev), st)
+        N.check(s, "nrn_cuda_scaled_product")
     return out
 
 
@@ -241,8 +261,10 @@ def product_backward(dy: torch.Tensor, x: torch.Tensor, w: Scaled, *, dx_dtype=N
     with on(dev, stream) as st:
         dx = torch.empty_strided((rows, k), (k, 1), dtype=dx_dtype, device=dev)
         dw = torch.empty_strided((n, k), (k, 1), dtype=dw_dtype, device=dev)
-        work = _workspace(need, dev, st) if need else None
-        N.check(N.lib().nrn_cuda_scaled_backward(dy.data_ptr(), x.data_ptr(), kind, rows, dy_stride, x_stride, C.byref(w.desc), dx.data_ptr(),
-                                                 dx_kind, dw.data_ptr(), dw_kind, None if work is None else work.data_ptr(), need,
-                                                 error_flag(dev), st), "nrn_cuda_scaled_backward")
+        shared = _on_stream(dev, st)
+        with shared.turn:
+            work = shared.workspace(need, dev)
+            s = N.lib().nrn_cuda_scaled_backward(dy.data_ptr(), x.data_ptr(), kind, rows, dy_stride, x_stride, C.byref(w.desc), dx.data_ptr(),
+                                                 dx_kind, dw.data_ptr(), dw_kind, work.data_ptr(), need, error_flag(dev), st)
+        N.check(s, "nrn_cuda_scaled_backward")
     return dx, dw

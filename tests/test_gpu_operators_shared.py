@@ -1,0 +1,78 @@
+"""What the tensor operators (linattn, scaled, gatednorm) share."""
+import threading
+import time
+
+import pytest
+import torch
+
+from libnrn_b200 import _native as N
+
+pytestmark = pytest.mark.gpu
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def randn(*s, seed=0, dtype=FP32):
+    return torch.randn(*s, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+
+
+def together(*calls):
+    """Runs the calls in a thread each; the first error is raised here."""
+    errors, start = [], threading.Barrier(len(calls))
+
+    def run(f):
+        try:
+            start.wait()
+            f()
+        except BaseException as e:      # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(f,)) for f in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if errors:
+        raise errors[0]
+
+
+# ------------------------------------------------------------------- threads
+
+def test_threads_on_one_stream_take_turns(monkeypatch):
+    """Two calls that use one workspace are never in the library at once, whatever their threads: between the launches of
+    one, another's would overwrite its operands.  (Nothing is launched here.)"""
+    from libnrn_b200 import scaled
+    x, dy = randn(8, 4096, dtype=BF16), randn(8, 2048, seed=1, dtype=BF16)
+    a, w = scaled.quantize(x), scaled.quantize(randn(2048, 4096, seed=2), row_block=128)
+    guard, inside, most = threading.Lock(), [0], [0]
+
+    def slowly(*_):
+        with guard:
+            inside[0] += 1
+            most[0] = max(most[0], inside[0])
+        time.sleep(0.02)
+        with guard:
+            inside[0] -= 1
+        return 0
+    for name in ("nrn_cuda_scaled_product", "nrn_cuda_scaled_backward"):
+        monkeypatch.setattr(N.lib(), name, slowly)
+    together(*[lambda: [scaled.product_backward(dy, x, w) for _ in range(4)]] * 2, lambda: [scaled.product(a, w) for _ in range(4)])
+    assert most[0] == 1
+    # on streams of their own they need not wait
+    side = [torch.cuda.Stream() for _ in range(2)]
+    together(*[lambda s=s: [scaled.product(a, w, stream=s) for _ in range(8)] for s in side])
+    assert most[0] == 2
+
+
+def test_threads_on_one_stream_are_right():
+    from libnrn_b200 import scaled
+    cases = []
+    for i, (m, n, k) in enumerate([(200, 512, 1024), (300, 256, 640), (8, 2048, 4096), (16, 4096, 4096)]):
+        x, dy = randn(m, k, seed=10 + i, dtype=BF16), randn(m, n, seed=20 + i, dtype=BF16)
+        w = scaled.quantize(randn(n, k, seed=30 + i), row_block=128)
+        cases.append((x, dy, w, scaled.product(scaled.quantize(x), w), scaled.product_backward(dy, x, w)))
+
+    def work(x, dy, w, y, grads):
+        for _ in range(40):
+            assert torch.equal(scaled.product(scaled.quantize(x), w), y)
+            assert all(torch.equal(a, b) for a, b in zip(scaled.product_backward(dy, x, w), grads))
+    together(*[lambda c=c: work(*c) for c in cases])
+    scaled.check()
