@@ -66,13 +66,15 @@ class Readout:
         for i in range(blocks):
             self.weights |= {"in.%d" % i: w(sum(self.parts), width), "out.%d" % i: w(width, heads * dv), "alpha.%d" % i: ones(0.5),
                              "w_pre.%d" % i: ones(), "w_post.%d" % i: ones()}
-        self._small = {}
 
     def small(self, name: str) -> scaled.Scaled:
-        """A projection's weights in 8 bits, made once until they change."""
-        if name not in self._small:
-            self._small[name] = scaled.quantize(self.weights[name], row_block=128)
-        return self._small[name]
+        """A projection's weights in 8 bits, as they are now."""
+        return scaled.quantize(self.weights[name], row_block=128)
+
+    def quantized(self) -> dict:
+        """All projections' weights in 8 bits by name: made once by a caller who reads or steps many times with weights that
+        stay, and given to those calls as ``small``.  They do not follow ``weights``."""
+        return {n: self.small(n) for n in self.weights if n.split(".")[0] in ("embed", "in", "out", "head")}
 
     def new_states(self, sessions: int) -> list:
         """Zero states, one tensor [sessions, heads, dk, dv] for each block."""
@@ -89,19 +91,21 @@ class Readout:
         w = self.weights
         return {"alpha": w["alpha.%d" % i], "w_post": w["w_post.%d" % i], "w_pre": w["w_pre.%d" % (i + 1)], "eps": self.eps}
 
-    def _through(self, counts, attend):
-        x = scaled.product(scaled.quantize(counts), self.small("embed"))
+    def _through(self, counts, attend, small):
+        w = self.small if small is None else small.__getitem__
+        x = scaled.product(scaled.quantize(counts), w("embed"))
         _, z = gatednorm.forward(x, w_pre=self.weights["w_pre.0"], eps=self.eps, scaled=True)
         for i in range(self.blocks):
-            q, k, v, gate = self._split(scaled.product(z, self.small("in.%d" % i)))
+            q, k, v, gate = self._split(scaled.product(z, w("in.%d" % i)))
             o = attend(i, q, k, v)
-            h = scaled.product(scaled.quantize(o), self.small("out.%d" % i))
+            h = scaled.product(scaled.quantize(o), w("out.%d" % i))
             x, z = gatednorm.forward(x, h, gate, scaled=True, **self._norms(i))
-        return scaled.product(z, self.small("head"))
+        return scaled.product(z, w("head"))
 
-    def read(self, counts, states=None, cu_seqlens=None):
+    def read(self, counts, states=None, cu_seqlens=None, small=None):
         """(answers [batch, bins, outputs], states) of whole recordings [batch, bins, features] (bf16), or of packed ones
-        [1, bins, features] with ``cu_seqlens``, that go on from ``states`` (default: nothing remembered)."""
+        [1, bins, features] with ``cu_seqlens``, that go on from ``states`` (default: nothing remembered).  ``small``:
+        weights in 8 bits that the caller keeps (``quantized``; default: made from ``weights`` in the call)."""
         check_rows(counts, "counts", torch.bfloat16, self.device, (*counts.shape[:2], self.features))
         b, t = counts.shape[:2]
         after = []
@@ -111,48 +115,49 @@ class Readout:
                                      state=None if states is None else states[i], cu_seqlens=cu_seqlens)
             after.append(end)
             return o.reshape(b * t, -1)
-        return self._through(counts.reshape(b * t, -1), attend).view(b, t, -1), after
+        return self._through(counts.reshape(b * t, -1), attend, small).view(b, t, -1), after
 
-    def step(self, counts, states, slots=None):
+    def step(self, counts, states, slots=None, small=None):
         """Answers [batch, outputs] for one bin [batch, features] of each session; ``states`` are updated in place
-        (session i in ``slots[i]``, default i)."""
+        (session i in ``slots[i]``, default i).  ``small`` as in ``read``."""
         check_rows(counts, "counts", torch.bfloat16, self.device, (counts.shape[0], self.features))
-        return self._through(counts, lambda i, q, k, v: linattn.step(q, k, v, self.log_decay, states[i], slots=slots).flatten(1))
+        return self._through(counts, lambda i, q, k, v: linattn.step(q, k, v, self.log_decay, states[i], slots=slots).flatten(1), small)
 
     def gradients(self, counts, targets, cu_seqlens=None):
         """(loss, gradients by the weights' names) of the mean squared error of ``read``'s answers."""
         check_rows(counts, "counts", torch.bfloat16, self.device, (*counts.shape[:2], self.features))
         b, t = counts.shape[:2]
         c = counts.reshape(b * t, -1)
-        x = scaled.product(scaled.quantize(c), self.small("embed"))
+        w = self.quantized().__getitem__
+        x = scaled.product(scaled.quantize(c), w("embed"))
         _, z = gatednorm.forward(x, w_pre=self.weights["w_pre.0"], eps=self.eps)
         kept = []
         for i in range(self.blocks):
-            p = scaled.product(scaled.quantize(z), self.small("in.%d" % i))
+            p = scaled.product(scaled.quantize(z), w("in.%d" % i))
             q, k, v, gate = self._split(p)
             qkv = tuple(y.unflatten(0, (b, t)) for y in (q, k, v))
             o, _ = linattn.forward(*qkv, self.log_decay, cu_seqlens=cu_seqlens)
             o = o.reshape(b * t, -1)
-            h = scaled.product(scaled.quantize(o), self.small("out.%d" % i))
+            h = scaled.product(scaled.quantize(o), w("out.%d" % i))
             kept.append((x, z, qkv, gate, o, h))
             x, z = gatednorm.forward(x, h, gate, **self._norms(i))
-        answers = scaled.product(scaled.quantize(z), self.small("head"), dtype=torch.float32)
+        answers = scaled.product(scaled.quantize(z), w("head"), dtype=torch.float32)
         off = answers - targets.reshape(b * t, -1).float()
         grads = {}
-        dz, grads["head"] = scaled.product_backward((off * (2.0 / off.numel())).to(torch.bfloat16), z, self.small("head"))
+        dz, grads["head"] = scaled.product_backward((off * (2.0 / off.numel())).to(torch.bfloat16), z, w("head"))
         dx = None
         for i in range(self.blocks - 1, -1, -1):
             x, z, qkv, gate, o, h = kept[i]
             g = gatednorm.backward(dx, dz, x, h, gate, **self._norms(i))
             grads["alpha.%d" % i], grads["w_post.%d" % i], grads["w_pre.%d" % (i + 1)] = g.alpha, g.w_post, g.w_pre
-            do, grads["out.%d" % i] = scaled.product_backward(g.h, o, self.small("out.%d" % i))
+            do, grads["out.%d" % i] = scaled.product_backward(g.h, o, w("out.%d" % i))
             dqkv = linattn.backward(do.view(b, t, self.heads, self.dv), *qkv, self.log_decay, cu_seqlens=cu_seqlens)[:3]
             dp = torch.cat([y.reshape(b * t, -1) for y in dqkv] + [g.gate], dim=1)
-            dz, grads["in.%d" % i] = scaled.product_backward(dp, z, self.small("in.%d" % i))
+            dz, grads["in.%d" % i] = scaled.product_backward(dp, z, w("in.%d" % i))
             dx = g.residual
         g = gatednorm.backward(dx, dz, kept[0][0], w_pre=self.weights["w_pre.0"], eps=self.eps)
         grads["w_pre.0"] = g.w_pre
-        grads["embed"] = scaled.product_backward(g.residual, c, self.small("embed"))[1]
+        grads["embed"] = scaled.product_backward(g.residual, c, w("embed"))[1]
         return off.square().mean(), grads
 
     def learn(self, grads, rate: float) -> None:
@@ -160,7 +165,6 @@ class Readout:
         for name, g in grads.items():
             w = self.weights[name]
             w -= rate * w.square().mean().sqrt() * g / g.square().mean().sqrt().clamp_min(1e-30)
-        self._small.clear()
 
 
 def main() -> None:
@@ -183,9 +187,9 @@ def main() -> None:
         r.learn(grads, 0.02)
     # one bin at a time gives what the whole recording gives
     whole, _ = r.read(past)
-    states = r.new_states(1)
+    states, small = r.new_states(1), r.quantized()
     for t in range(past.shape[1]):
-        last = r.step(past[:, t], states)
+        last = r.step(past[:, t], states, small=small)
     scaled.check()
     d = float((last - whole[:, -1]).float().norm() / whole[:, -1].float().norm())
     print(f"last bin read step by step differs by {d:.1e} from the whole recording's")

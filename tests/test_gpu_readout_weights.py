@@ -1,0 +1,60 @@
+"""A readout answers by the weights that it has at the call, and its ends."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def make(seed=0, **kw):
+    from libnrn_b200 import readout
+    return readout.Readout(24, 16, width=64, heads=2, dk=32, dv=32, blocks=1, seed=seed, **kw)
+
+
+def counts(*s):
+    return torch.poisson(torch.full(s, 0.7, device="cuda"), generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("how", ["assign", "in place", "data", "update", "all"])
+def test_answers_follow_the_weights(how):
+    a, b, x = make(0), make(1), counts(2, 30, 24)
+    before = a.read(x)[0]
+    assert not torch.equal(before, b.read(x)[0])
+    for n, w in b.weights.items():
+        if how == "assign":
+            a.weights[n] = w
+        elif how == "in place":
+            a.weights[n].copy_(w)
+        elif how == "data":
+            a.weights[n].data.copy_(w)
+    if how == "update":
+        a.weights.update(b.weights)
+    elif how == "all":
+        a.weights = dict(b.weights)
+    assert torch.equal(a.read(x)[0], b.read(x)[0])
+    sa, sb = a.new_states(2), b.new_states(2)
+    assert torch.equal(a.step(x[:, 0], sa), b.step(x[:, 0], sb)) and torch.equal(sa[0], sb[0])
+    la, ga = a.gradients(x[:1, :-1], x[:1, 1:, :16])
+    lb, gb = b.gradients(x[:1, :-1], x[:1, 1:, :16])
+    assert torch.equal(la, lb) and all(torch.equal(ga[n], gb[n]) for n in gb)
+
+
+def test_a_captured_step_follows_the_weights():
+    r, x = make(), counts(2, 24)
+    states, mine = r.new_states(2), r.new_states(2)
+    r.step(x, r.new_states(2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = r.step(x, states)
+    r.weights["head"].mul_(-2.0)
+    graph.replay()
+    assert torch.equal(got, r.step(x, mine))
+
+
+def test_weights_that_the_caller_keeps():
+    """8-bit weights made once are the caller's, and stay as they were."""
+    r, x = make(), counts(2, 30, 24)
+    kept, before = r.quantized(), r.read(x)[0]
+    assert torch.equal(r.read(x, small=kept)[0], before)
+    assert torch.equal(r.step(x[:, 0], r.new_states(2), small=kept), r.step(x[:, 0], r.new_states(2)))
+    r.weights["head"].zero_()
+    assert torch.equal(r.read(x, small=kept)[0], before) and not r.read(x)[0].any()
