@@ -50,6 +50,11 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def number(x):
+    """x as a Python number, read at every call: a tensor would stand in a key for what it held at its first use."""
+    return x if x is None or type(x) is float else float(x)
+
+
 def layout(t):
     """All of a tensor argument that its checks look at (None and anything else stand for themselves)."""
     return (t.shape, t.stride(), t.dtype, t.device) if isinstance(t, torch.Tensor) else (t if t is None else type(t))

@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, Layouts, check_rows, check_vector, check_waits, error_flag, layout, on, ptr, require
+from ._tensors import DTYPE, Layouts, check_rows, check_vector, check_waits, error_flag, layout, number, on, ptr, require
 from .scaled import Scaled
 
 check = check_waits
@@ -54,7 +54,7 @@ def _describe(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
         if t is not None:
             check_vector(t, name, d, dev)
     a = N.GatedNorm()
-    a.dtype, a.act, a.rows, a.d, a.eps = DTYPE[dt], ACTIVATION[activation], rows, d, float(eps)
+    a.dtype, a.act, a.rows, a.d, a.eps = DTYPE[dt], ACTIVATION[activation], rows, d, eps
     a.residual_stride, a.h_stride, a.gate_stride = residual.stride(0), _stride(h), _stride(gate)
     n = C.c_int64()
     N.check(N.lib().nrn_cuda_gatednorm_workspace(C.byref(a), C.byref(n)), "nrn_cuda_gatednorm_workspace")
@@ -66,6 +66,7 @@ _layouts = Layouts(_describe)
 
 def _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
     require(isinstance(residual, torch.Tensor) and residual.is_cuda, "residual: a CUDA tensor is needed")
+    eps = number(eps)
     key = (layout(residual), layout(h), layout(gate), layout(alpha), layout(w_post), layout(w_pre), eps, activation, layout(dy), layout(dz))
     block, need = _layouts.get(key, residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz)
     a = N.GatedNorm.from_buffer_copy(block)

@@ -21,8 +21,8 @@ import ctypes as C
 import torch
 
 from . import _native as N
-from ._tensors import (DTYPE, Layouts, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, layout, on,
-                       ptr, require)
+from ._tensors import (DTYPE, Layouts, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, layout, number,
+                       on, ptr, require)
 
 check = check_waits
 
@@ -67,7 +67,7 @@ def _describe(q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out):
         if x is not None:
             check_rows(x, name, dt, dev, (b, t, h, dv))
     a.log_decay = log_decay.data_ptr()
-    a.scale = dk ** -0.5 if scale is None else float(scale)
+    a.scale = dk ** -0.5 if scale is None else scale
     a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
     if out is not None:
         a.o_stride[:] = _strides(out)
@@ -83,6 +83,7 @@ _sequences = Layouts(_describe)
 
 def _call(q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out):
     """(argument block with the inputs' pointers, workspace bytes, shape of the states)."""
+    scale = number(scale)
     key = (layout(q), layout(k), layout(v), layout(log_decay), scale, layout(cu_seqlens), layout(state), layout(dstate), layout(do),
            layout(out))
     block, need, shape = _sequences.get(key, q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out)
@@ -153,7 +154,7 @@ def _describe_step(q, k, v, log_decay, state, scale, slots, out):
         check_rows(out, "out", q.dtype, dev, (b, h, dv))
     a = N.LinAttn()
     a.dtype, a.seqs, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[q.dtype], b, h, hk, dk, dv, 1
-    a.scale = dk ** -0.5 if scale is None else float(scale)
+    a.scale = dk ** -0.5 if scale is None else scale
     for f, x in ((a.q_stride, q), (a.k_stride, k), (a.v_stride, v)):
         f[0], f[2] = x.stride(0), x.stride(1)
     a.o_stride[0], a.o_stride[2] = (out.stride(0), out.stride(1)) if out is not None else (h * dv, dv)
@@ -168,6 +169,7 @@ def step(q, k, v, log_decay, state, *, scale=None, slots=None, out=None, stream=
     ``state[slots[i]]`` (int32, default: state[i]); a slot appears at most once in a call, a negative one is padding whose
     output is 0, and one past the states gives NaN."""
     _check_q(q)
+    scale = number(scale)
     key = (layout(q), layout(k), layout(v), layout(log_decay), layout(state), scale, layout(slots), layout(out))
     block, shape, strides, stride, count = _steps.get(key, q, k, v, log_decay, state, scale, slots, out)
     with on(q.device, stream) as st:

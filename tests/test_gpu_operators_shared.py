@@ -76,3 +76,23 @@ def test_threads_on_one_stream_are_right():
             assert all(torch.equal(a, b) for a, b in zip(scaled.product_backward(dy, x, w), grads))
     together(*[lambda c=c: work(*c) for c in cases])
     scaled.check()
+
+
+# -------------------------------------------------------- numbers as tensors
+
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_a_number_in_a_tensor_is_read_at_every_call(device):
+    from libnrn_b200 import gatednorm, linattn
+    q, k, v = (randn(1, 20, 2, 32, seed=i) for i in range(3))
+    g = torch.full((2,), -0.1, device="cuda")
+    scale, eps = torch.tensor(0.5, device=device), torch.tensor(1e-6, device=device)
+    r, state = randn(4, 64), torch.zeros(1, 2, 32, 32, device="cuda")
+    for s, e in ((0.5, 1e-6), (0.25, 0.5)):
+        scale.fill_(s)
+        eps.fill_(e)
+        assert torch.equal(linattn.forward(q, k, v, g, scale=scale)[0], linattn.forward(q, k, v, g, scale=s)[0])
+        assert all(torch.equal(a, b) for a, b in zip(linattn.backward(q, q, k, v, g, scale=scale), linattn.backward(q, q, k, v, g, scale=s)))
+        one = [linattn.step(q[:, 0], k[:, 0], v[:, 0], g, state.clone(), scale=f) for f in (scale, s)]
+        assert torch.equal(*one)
+        assert torch.equal(gatednorm.forward(r, eps=eps)[1], gatednorm.forward(r, eps=float(eps))[1])
+        assert torch.equal(gatednorm.backward(None, r, r, eps=eps).residual, gatednorm.backward(None, r, r, eps=float(eps)).residual)
