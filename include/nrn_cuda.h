@@ -543,6 +543,11 @@ NRN_API nrn_status_t nrn_cuda_gatednorm_workspace(const nrn_gatednorm_t* a, int6
 NRN_API nrn_status_t nrn_cuda_gatednorm_backward(const nrn_gatednorm_t* a, const nrn_gatednorm_grad_t* g,
                                                  nrn_stream_t stream);
 
+/* A device word for these calls' `err`, one for each device: zero when it is
+ * made, at the first call, which may come while a stream is being captured.
+ * It belongs to the library. */
+NRN_API nrn_status_t nrn_cuda_wait_flag(int32_t device, int32_t** flag);
+
 /* ------------------------------------------------------------------------ */
 /* Engine: a network resident on one GPU                                   */
 /* ------------------------------------------------------------------------ */

@@ -44,7 +44,7 @@ EXPORTS = [
     "nrn_cuda_linattn_workspace", "nrn_cuda_linattn_forward", "nrn_cuda_linattn_backward", "nrn_cuda_linattn_step",
     "nrn_cuda_scaled_quantize", "nrn_cuda_scaled_transpose", "nrn_cuda_scaled_workspace", "nrn_cuda_scaled_product",
     "nrn_cuda_scaled_backward", "nrn_cuda_scaled_backward_workspace",
-    "nrn_cuda_gatednorm_forward", "nrn_cuda_gatednorm_workspace", "nrn_cuda_gatednorm_backward",
+    "nrn_cuda_gatednorm_forward", "nrn_cuda_gatednorm_workspace", "nrn_cuda_gatednorm_backward", "nrn_cuda_wait_flag",
 ]
 
 
@@ -269,6 +269,7 @@ def lib() -> C.CDLL:
             "nrn_cuda_gatednorm_forward": [C.POINTER(GatedNorm), vp],
             "nrn_cuda_gatednorm_workspace": [C.POINTER(GatedNorm), C.POINTER(i64)],
             "nrn_cuda_gatednorm_backward": [C.POINTER(GatedNorm), C.POINTER(GatedNormGrad), vp],
+            "nrn_cuda_wait_flag": [i32, C.POINTER(vp)],
         }
         for name, args in sig.items():
             f = getattr(L, name)

@@ -8,6 +8,7 @@ pointers (``Layouts``)."""
 from __future__ import annotations
 
 import contextlib
+import ctypes as C
 
 import torch
 
@@ -115,21 +116,42 @@ def on(device, stream=None):
     return _switched(device, stream)
 
 
-# A flag on each device that kernels set when one of their bounded waits gives up.
-_errors: dict = {}
+class _Flag:
+    """A device's word that kernels set when one of their bounded waits gives up, and the same as a tensor.  The library
+    makes it: made here by the first call it could become part of a graph that is being captured, whose replays would clear
+    it."""
+
+    def __init__(self, index: int):
+        p = C.c_void_p()
+        N.check(N.lib().nrn_cuda_wait_flag(index, C.byref(p)), "nrn_cuda_wait_flag")
+        self.index, self.address = index, p.value
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (p.value, False), "version": 2}
+
+    def tensor(self) -> torch.Tensor:
+        return torch.as_tensor(self, device=torch.device("cuda", self.index))
+
+
+_flags: dict = {}
+
+
+def flag(index: int) -> _Flag:
+    f = _flags.get(index)
+    if f is None:
+        f = _flags[index] = _Flag(index)
+    return f
 
 
 def error_flag(device) -> int:
     """Address of the device's flag."""
-    t = _errors.get(device.index)
-    if t is None:
-        t = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-    return t.data_ptr()
+    return flag(device.index).address
 
 
 def check_waits(device=None) -> None:
     """Raises if a device-side wait of an earlier call on `device` (default: the current one) gave up.  Waits for the GPU."""
     i = torch.cuda.current_device() if device is None else torch.device(device).index
-    t = _errors.get(i)
-    if t is not None and int(t.item()) != 0:
-        raise N.NrnError(7, f"a device-side wait timed out (code {int(t.item())})")
+    f = _flags.get(i)
+    if f is None:
+        return
+    code = int(f.tensor().item())
+    if code != 0:
+        raise N.NrnError(7, f"a device-side wait timed out (code {code})")

@@ -26,7 +26,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-fmad=false", "-cudart=shared", "-Xcompiler", "-fPIC", "-Xcompiler",
          "-fvisibility=hidden", f"-I{os.path.join(ROOT, 'include')}", f"-I{CSRC}"]
 SOURCES = ["neuron.cu", "deliver.cu", "connect.cu", "engine.cu", "comm.cu", "blockdense.cu", "raster_noalloc.cu", "plastic.cu",
-           "exchange.cu", "bsr.cu", "linattn.cu", "scaled.cu", "gatednorm.cu"]
+           "exchange.cu", "bsr.cu", "linattn.cu", "scaled.cu", "gatednorm.cu", "waits.cu"]
 
 
 def _nccl_dir():

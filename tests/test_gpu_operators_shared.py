@@ -1,4 +1,7 @@
 """What the tensor operators (linattn, scaled, gatednorm) share."""
+import os
+import subprocess
+import sys
 import threading
 import time
 
@@ -9,6 +12,7 @@ from libnrn_b200 import _native as N
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def randn(*s, seed=0, dtype=FP32):
@@ -96,3 +100,35 @@ def test_a_number_in_a_tensor_is_read_at_every_call(device):
         assert torch.equal(*one)
         assert torch.equal(gatednorm.forward(r, eps=eps)[1], gatednorm.forward(r, eps=float(eps))[1])
         assert torch.equal(gatednorm.backward(None, r, r, eps=eps).residual, gatednorm.backward(None, r, r, eps=float(eps)).residual)
+
+
+# -------------------------------------------------- waits that gave up, graphs
+
+FIRST = """
+import torch
+from libnrn_b200 import _native as N, _tensors, {module}
+x = torch.randn(8, 4096, device="cuda"); big = torch.full((1 << 20,), 7, dtype=torch.int32, device="cuda"); del big
+torch.cuda.synchronize()
+q = torch.randn(1, 70, 2, 64, device="cuda").bfloat16(); ld = torch.full((2,), -0.1, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    {call}
+{module}.check()                                   # nothing ran yet: nothing gave up
+graph.replay()
+{module}.check()
+_tensors.flag(0).tensor().fill_(5)
+graph.replay()                                     # a replay takes no flag down
+try:
+    {module}.check()
+    raise SystemExit("the flag was lost")
+except N.NrnError:
+    pass
+print("told")
+"""
+
+
+@pytest.mark.parametrize("module,call", [("linattn", "linattn.forward(q, q, q, ld)"), ("gatednorm", "gatednorm.forward(x, x)"),
+                                         ("scaled", "scaled.product(scaled.quantize(x), scaled.quantize(x, row_block=128))")], ids=["linattn", "gatednorm", "scaled"])
+def test_the_first_call_of_a_process_may_be_captured(module, call):
+    r = subprocess.run([sys.executable, "-c", FIRST.format(module=module, call=call)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "told" in r.stdout, r.stdout + r.stderr
