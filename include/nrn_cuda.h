@@ -477,7 +477,8 @@ NRN_API nrn_status_t nrn_cuda_scaled_transpose(const nrn_scaled_t* in, const nrn
  * each block of 128 columns, times both scales, summed in fp32.  Work split
  * over the columns leaves partial sums in the workspace
  * (nrn_cuda_scaled_workspace bytes; the first 4,096 zero before its first
- * use and left so; not shared by calls that run at once). */
+ * use and left so, but after a wait that gave up, when they must be zeroed
+ * again; not shared by calls that run at once). */
 NRN_API nrn_status_t nrn_cuda_scaled_workspace(const nrn_scaled_t* a, const nrn_scaled_t* b, int64_t* bytes);
 NRN_API nrn_status_t nrn_cuda_scaled_product(const nrn_scaled_t* a, const nrn_scaled_t* b, void* out, int32_t dtype,
                                              int64_t out_stride, void* workspace, int64_t workspace_bytes,

@@ -146,12 +146,23 @@ def error_flag(device) -> int:
     return flag(device.index).address
 
 
+# Called with a device's index when a wait there gave up: what later calls would take over from the unfinished ones.
+after_timeout: list = []
+
+
 def check_waits(device=None) -> None:
-    """Raises if a device-side wait of an earlier call on `device` (default: the current one) gave up.  Waits for the GPU."""
+    """Raises if a device-side wait of an earlier call on `device` (default: the current one) gave up.  Waits for the GPU.
+    What gave up is told once: the flag is down afterwards and later calls start afresh.  Results of the calls before, and
+    graphs that were captured, are the caller's to make again."""
     i = torch.cuda.current_device() if device is None else torch.device(device).index
     f = _flags.get(i)
     if f is None:
         return
     code = int(f.tensor().item())
     if code != 0:
+        torch.cuda.synchronize(i)
+        for drop in after_timeout:
+            drop(i)
+        f.tensor().zero_()
+        torch.cuda.synchronize(i)
         raise N.NrnError(7, f"a device-side wait timed out (code {code})")

@@ -18,7 +18,7 @@ import threading
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, Layouts, check_tensor, check_waits, error_flag, layout, on, require
+from ._tensors import DTYPE, Layouts, after_timeout, check_tensor, check_waits, error_flag, layout, on, require
 
 BLOCK = 128
 
@@ -181,6 +181,17 @@ _streams: dict = {}
 def _on_stream(device, stream: int) -> _Stream:
     key = (device.index, stream)
     return _streams.get(key) or _streams.setdefault(key, _Stream())
+
+
+def _drop_workspaces(index: int) -> None:
+    """A product that gave up leaves counters above zero: the next one on its stream gets a new workspace."""
+    for (i, _), shared in list(_streams.items()):
+        if i == index:
+            with shared.turn:
+                shared.work = None
+
+
+after_timeout.append(_drop_workspaces)
 
 
 check = check_waits

@@ -132,3 +132,19 @@ print("told")
 def test_the_first_call_of_a_process_may_be_captured(module, call):
     r = subprocess.run([sys.executable, "-c", FIRST.format(module=module, call=call)], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "told" in r.stdout, r.stdout + r.stderr
+
+
+def test_a_wait_that_gave_up_is_told_once_and_leaves_nothing():
+    """After the flag is told it is down again, and products whose counters were left above zero are right."""
+    from libnrn_b200 import _tensors, linattn, scaled
+    a, w = scaled.quantize(randn(8, 4096)), scaled.quantize(randn(2048, 4096, seed=1), row_block=128)
+    want = scaled.product(a, w)
+    linattn.check()
+    for shared in scaled._streams.values():
+        if shared.work is not None:
+            shared.work[:4096].view(torch.int32).fill_(1)
+    _tensors.flag(torch.cuda.current_device()).tensor().fill_(5)
+    with pytest.raises(N.NrnError, match="timed out"):
+        scaled.check()
+    scaled.check()
+    assert torch.equal(scaled.product(a, w), want) and torch.equal(scaled.product(a, w), want)
