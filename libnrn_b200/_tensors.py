@@ -154,13 +154,14 @@ def check_waits(device=None) -> None:
     """Raises if a device-side wait of an earlier call on `device` (default: the current one) gave up.  Waits for the GPU.
     What gave up is told once: the flag is down afterwards and later calls start afresh.  Results of the calls before, and
     graphs that were captured, are the caller's to make again."""
-    i = torch.cuda.current_device() if device is None else torch.device(device).index
+    i = None if device is None else torch.device(device).index
+    i = torch.cuda.current_device() if i is None else i
     f = _flags.get(i)
     if f is None:
         return
+    torch.cuda.synchronize(i)            # a call on any stream
     code = int(f.tensor().item())
     if code != 0:
-        torch.cuda.synchronize(i)
         for drop in after_timeout:
             drop(i)
         f.tensor().zero_()

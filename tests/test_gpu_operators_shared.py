@@ -148,3 +148,26 @@ def test_a_wait_that_gave_up_is_told_once_and_leaves_nothing():
         scaled.check()
     scaled.check()
     assert torch.equal(scaled.product(a, w), want) and torch.equal(scaled.product(a, w), want)
+
+
+def test_check_names_a_device_as_torch_does():
+    from libnrn_b200 import _tensors, scaled
+    scaled.product(scaled.quantize(randn(8, 256)), scaled.quantize(randn(20, 256), row_block=128))
+    i = torch.cuda.current_device()
+    for name in (None, "cuda", torch.device("cuda"), f"cuda:{i}", torch.device("cuda", i), i):
+        scaled.check(name)
+        _tensors.flag(i).tensor().fill_(5)
+        with pytest.raises(N.NrnError):
+            scaled.check(name)
+
+
+def test_check_waits_for_every_stream():
+    from libnrn_b200 import _tensors, scaled
+    flag, side = _tensors.flag(torch.cuda.current_device()).tensor(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        flag.fill_(5)
+    with pytest.raises(N.NrnError):
+        scaled.check()
+    scaled.check()
