@@ -10,8 +10,7 @@
 //
 // Bound by HBM: three rows in, two out (five and three backward), if the
 // operations an element stay near 30: the sigmoid is two special-function
-// operations (its error, about 2^-22 where the gate is not small, is below
-// every output's rounding), alpha and w_post are one factor, and a block keeps
+// operations for 16-bit types, alpha and w_post are one factor, and a block keeps
 // its columns' factors in registers over all the rows it takes in turn.  A row
 // is held in registers, eight elements a thread and vector (16 bytes of bf16):
 // 32 threads a row where the row is short, else a block a row.  The reductions
@@ -19,7 +18,7 @@
 // their way meanwhile: rows on 16-byte boundaries come by bulk copies into a
 // ring of two to four in shared memory.  Measured, bf16 rows of 4096: forward
 // with z as e4m3 606 MB in 129 us (71% of the measured copy); backward, rows
-// of 2560, 336 MB in 98 us (52%): there the operations an element, about 60,
+// of 2560, 336 MB in 99 us (52%): there the operations an element, about 60,
 // and two reductions a row count as much as the bytes.
 #include <cuda_runtime.h>
 
@@ -70,11 +69,30 @@ RowArrays row_arrays(const nrn_gatednorm_t& f, bool vec) {
     return r;
 }
 
-__device__ __forceinline__ float sigmoid(float x) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+// The sigmoid's error, relative: for 16-bit types ex2.approx (2^-22), its
+// argument's rounding (|x| 2^-23: 2^-18 at 30) and rcp.approx (2^-23), far
+// below the results' 2^-9 and 2^-12; fp32 takes expf (2^-22 in all).  Below
+// -87 a 16-bit type's is 0.
+template <typename T>
+__device__ __forceinline__ float exp_of(float x) {
+    if constexpr (sizeof(T) == 4) return expf(x);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 1.4426950408889634f));
+    return e;
+}
+__device__ __forceinline__ float inverse(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float x) { return inverse(1.0f + exp_of<T>(-x)); }
+// sigmoid(x) and its derivative sigmoid(x) sigmoid(-x).  1 - sigmoid(x) in
+// place of sigmoid(-x) would have none of its bits left at 17.
+template <typename T>
+__device__ __forceinline__ float2 sigmoid_grad(float x) {
+    const float t = exp_of<T>(-fabsf(x)), r = inverse(1.0f + t), u = t * r;
+    return make_float2(x < 0.0f ? u : r, u * r);
 }
 
 // N sums over the threads of a row; every thread gets them.  A row of one
@@ -254,7 +272,7 @@ __global__ void __launch_bounds__(most_threads<WARP>(), WARP ? 8 / VPT : 1)
                 for (int e = 0; e < 8; ++e) {
                     float u = inv * aw[v][e];
                     if (gated) {
-                        const float g = to_f32(gate[v].e[e]), sg = sigmoid(g);
+                        const float g = to_f32(gate[v].e[e]), sg = sigmoid<T>(g);
                         u *= silu ? g * sg : sg;
                     }
                     y[v][e] = fmaf(y[v][e], u, to_f32(r[v].e[e]));
@@ -388,7 +406,7 @@ __global__ void __launch_bounds__(most_threads<WARP>(), WARP ? 8 / VPT : 1)
                     const Raw8<T> gate = in.get(2, row, c);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float t = to_f32(gate.e[e]), sg = sigmoid(t);
+                        const float t = to_f32(gate.e[e]), sg = sigmoid<T>(t);
                         y[v][e] = fmaf(to_f32(h.e[e]) * inv_h * aw[e], silu ? t * sg : sg, y[v][e]);
                     }
                 } else {
@@ -442,8 +460,9 @@ __global__ void __launch_bounds__(most_threads<WARP>(), WARP ? 8 / VPT : 1)
                 float dg[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float hh = to_f32(h.e[e]) * inv_h, t = to_f32(gate.e[e]), sg = sigmoid(t), ts = t * sg, da = d[e] * aw[e];
-                    const float act = silu ? ts : sg, dact = silu ? fmaf(ts, 1.0f - sg, sg) : sg * (1.0f - sg);
+                    const float hh = to_f32(h.e[e]) * inv_h, t = to_f32(gate.e[e]), da = d[e] * aw[e];
+                    const float2 sg = sigmoid_grad<T>(t);
+                    const float act = silu ? t * sg.x : sg.x, dact = silu ? fmaf(t, sg.y, sg.x) : sg.y;
                     s1[v][e] = fmaf(d[e] * act, hh, s1[v][e]);
                     dg[e] = da * hh * dact;
                     y[v][e] = da * act;
