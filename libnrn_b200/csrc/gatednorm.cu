@@ -95,6 +95,12 @@ __device__ __forceinline__ float2 sigmoid_grad(float x) {
     return make_float2(x < 0.0f ? u : r, u * r);
 }
 
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // N sums over the threads of a row; every thread gets them.  A row of one
 // warp needs no barrier; else `red` is [2][N][32] floats used in turn.
 template <int N, bool WARP>
@@ -310,12 +316,12 @@ __global__ void __launch_bounds__(most_threads<WARP>(), WARP ? 8 / VPT : 1)
                 if (n > 0) store8(static_cast<T*>(f.z) + row * f.z_stride + c, y[v], n, vec);
                 continue;
             }
-            // a value that is no number makes its whole row so: fmaxf need not find it
+            // an infinity in y gives a NaN among zeros, which has to win
             float m = fabsf(y[v][0]);
 #pragma unroll
-            for (int e = 1; e < 8; ++e) m = fmaxf(m, fabsf(y[v][e]));
+            for (int e = 1; e < 8; ++e) m = max_or_nan(m, fabsf(y[v][e]));
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));   // 16 lanes: 128 columns
+            for (int d = 1; d < 16; d <<= 1) m = max_or_nan(m, __shfl_xor_sync(0xffffffffu, m, d));   // 16 lanes: 128 columns
             if (n <= 0) continue;
             const float sc = block_scale(__float_as_uint(m)), q = __frcp_rn(sc);
             if ((tid & 15) == 0) a.zs[row * a.zs_row + (c / 128) * a.zs_col] = sc;

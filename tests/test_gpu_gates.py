@@ -1,4 +1,5 @@
-"""The norms' gates where they saturate, element by element.
+"""The norms' gates where they saturate, element by element, and rows with
+an infinity as 8 bits.
 
 Tolerances, relative and for each element.  fp32: the row's norm (a sum of 64
 squares and a reciprocal root, 2^-21), the exponential (2 ulp) and its
@@ -43,3 +44,17 @@ def test_saturated_gates(dtype, act, d):
     assert off(y, hh * (x * sg if act == "silu" else sg)) <= TOL[dtype]
     ref = dy.double() * hh * (sg * (1.0 + x * other) if act == "silu" else sg * other)
     assert off(g.gate, ref) <= TOL[dtype], off(g.gate, ref)
+
+
+@pytest.mark.parametrize("shape", [(5, 256), (4, 1000), (3, 4096)], ids=str)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_an_infinity_as_8_bits(bad, shape):
+    """z's block that holds no number is NaN throughout, as the quantiser makes it; the row's other blocks are what z is."""
+    from libnrn_b200 import gatednorm, scaled
+    x = torch.randn(*shape, device="cuda")
+    x[1, 140] = bad
+    _, z = gatednorm.forward(x, scaled=True)
+    _, plain = gatednorm.forward(x)
+    want = scaled.quantize(plain)
+    assert torch.equal(z.dequantize().isnan(), want.dequantize().isnan())
+    assert bool(z.dequantize()[1, 128:256].isnan().all()) and torch.equal(z.scales.isnan(), want.scales.isnan())
