@@ -989,9 +989,16 @@ extern "C" nrn_status_t nrn_cuda_scaled_backward(const void* dy, const void* x, 
     NRN_CHECK_ARG(dtype == NRN_BF16 || dtype == NRN_FP16 || dtype == NRN_FP32, who + ": unknown type");
     NRN_CHECK_ARG(rows >= 0 && rows < (int64_t(1) << 23) - 128 && w->rows < (int64_t(1) << 23) - 128, who + ": at most 8,388,480 rows");
     NRN_CHECK_ARG(dy_stride >= 0 && x_stride >= 0, who + ": negative strides");
-    if (w->rows == 0 || w->cols == 0) return NRN_OK;
-    NRN_CHECK_ARG((rows == 0 || (dy && x && dx)) && dw, who + ": null array");
+    NRN_CHECK_ARG(dx_dtype == NRN_BF16 || dx_dtype == NRN_FP16 || dx_dtype == NRN_FP32, who + ": unknown type of dx");
+    NRN_CHECK_ARG(dw_dtype == NRN_BF16 || dw_dtype == NRN_FP16 || dw_dtype == NRN_FP32, who + ": unknown type of dw");
+    if (w->cols == 0) return NRN_OK;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (w->rows == 0) {
+        NRN_CHECK_ARG(rows == 0 || dx, who + ": null array");
+        if (rows) NRN_CUDA_TRY(cudaMemsetAsync(dx, 0, static_cast<size_t>(rows) * w->cols * (dx_dtype == NRN_FP32 ? 4 : 2), s));
+        return NRN_OK;
+    }
+    NRN_CHECK_ARG((rows == 0 || (dy && x && dx)) && dw, who + ": null array");
     if (rows == 0) {
         NRN_CUDA_TRY(cudaMemsetAsync(dw, 0, static_cast<size_t>(w->rows) * w->cols * (dw_dtype == NRN_FP32 ? 4 : 2), s));
         return NRN_OK;
