@@ -248,7 +248,10 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
         }
         if (n == kSerialTokens) {
 #pragma unroll
-            for (int g = 0; g < 4 * G; ++g) s[g] = fmaf(s[g], mend, s[g]);
+            for (int g = 0; g < 4 * G; ++g) {
+                const float x = fmaf(s[g], mend, s[g]);
+                s[g] = x == x ? x : s[g];            // an infinity times the error would leave no number
+            }
         }
     }
     if (col >= dc) return;

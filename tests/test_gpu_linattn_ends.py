@@ -1,0 +1,30 @@
+"""Linear attention at its ends.  Tolerances as in test_gpu_linattn.py."""
+import pytest
+import torch
+
+import operator_refs as R
+from test_gpu_linattn import STATE_TOL, TOL, close, decays, make
+
+pytestmark = pytest.mark.gpu
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("t", [1, 16, 40, 150])
+@pytest.mark.parametrize("kind", ["bf16", "bf16 off 16 bytes", "fp16", "fp32"])
+def test_an_infinite_state_stays_infinite(kind, t):
+    from libnrn_b200 import linattn
+    dtype = {"fp16": FP16, "fp32": FP32}.get(kind, BF16)
+    q, k, v, s0, _, _ = make(1, t, 3, 3, 64, 64, dtype)
+    if kind == "bf16 off 16 bytes":
+        q, k, v = (torch.cat([x[..., :1], x], -1)[..., 1:] for x in (q, k, v))
+    q[q == 0] = 1
+    s0[0, :, 5, 7] = float("inf")
+    g = torch.tensor([0.0, -0.01, -0.5], device="cuda")      # the first decay has no error to take out
+    o, end = linattn.forward(q, k, v, g, state=s0)
+    ro, rend = R.linattn(q, k, v, g, 0.125, s0)
+    assert bool(ro[..., 7].isinf().all())
+    assert torch.equal(o[..., 7].double(), ro[..., 7]) and torch.equal(end[..., 5, 7].double(), rend[..., 5, 7])
+    rest = [i for i in range(64) if i != 7]
+    close(o[..., rest], ro[..., rest], TOL[dtype])
+    end[..., 5, 7] = rend[..., 5, 7] = 0
+    close(end, rend, STATE_TOL)
