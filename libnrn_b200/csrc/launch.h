@@ -43,7 +43,9 @@ cudaError_t allow_shared(int bytes) {
 // (previous_done) before they touch what it wrote, or write what it reads.
 // Each kernel of such a chain lets the next one in (let_next) and waits on
 // every path, so that the end of one is the end of all before it; a kernel that
-// does neither may stand in the chain, launched as usual.
+// does neither may stand in the chain, launched as usual.  A kernel that
+// allocates TMEM does so before it lets the next one in: the allocation waits
+// for as long as another block of its SM holds the columns.
 template <typename... P, typename... A>
 cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, int shared, cudaStream_t s, bool after, const A&... args) {
     cudaLaunchConfig_t c{};

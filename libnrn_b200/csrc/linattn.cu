@@ -773,8 +773,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int head = (blockIdx.x / tiles) % p.heads;
     const int unit = blockIdx.x / tiles / p.heads;
     const Unit u = unit_of(p, unit);
-    let_next();
     if (!u.any) {
+        let_next();
         previous_done();
         return;
     }
@@ -812,6 +812,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = M.tmem;
+    let_next();              // not before this block has its TMEM: a block of the next kernel could take it and wait for this one
     previous_done();
     auto fail = [&]() {
         *abort = 1;
