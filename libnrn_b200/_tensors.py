@@ -23,8 +23,18 @@ def require(cond: bool, msg: str) -> None:
         raise N.NrnError(1, msg)
 
 
+_recorded = torch.is_grad_enabled
+
+
+def check_gradient(t, name: str) -> None:
+    """The operators' results have no graph: a gradient would be lost without a word."""
+    require(not (t.requires_grad and _recorded()), f"{name}: requires a gradient, which this call does not record: call it under torch.no_grad() and use the "
+                                   "operator's backward")
+
+
 def check_tensor(t, name: str, dtype, device, shape=None) -> None:
     require(isinstance(t, torch.Tensor), f"{name}: a tensor is needed")
+    check_gradient(t, name)
     require(t.is_cuda and t.device == device, f"{name}: must be on {device}, is on {t.device}")
     require(t.dtype == dtype, f"{name}: must be {dtype}, is {t.dtype}")
     if shape is not None:
@@ -58,7 +68,9 @@ def number(x):
 
 def layout(t):
     """All of a tensor argument that its checks look at (None and anything else stand for themselves)."""
-    return (t.shape, t.stride(), t.dtype, t.device) if isinstance(t, torch.Tensor) else (t if t is None else type(t))
+    if t is None:
+        return None
+    return (t.shape, t.stride(), t.dtype, t.device, t.requires_grad and _recorded()) if isinstance(t, torch.Tensor) else type(t)
 
 
 class Layouts:

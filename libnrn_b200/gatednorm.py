@@ -7,7 +7,8 @@ norm(x) = x / sqrt(mean(x^2) + eps):
 
 h is the block's output; without it y is the residual and only z is computed.
 gate (like h), alpha, w_post and w_pre (fp32 [d]) may be None: 1.  All sums
-and z's input are fp32; y and z are rounded once.
+and z's input are fp32; y and z are rounded once.  Results have no autograd
+graph: tensors that require gradients are refused where these are recorded.
 """
 from __future__ import annotations
 

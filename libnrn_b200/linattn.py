@@ -12,7 +12,8 @@ sequences, [sequences + 1], on the device, from 0 to the number of tokens) the
 batch dimension is 1 and states have one entry for each sequence.  dk and dv
 are at most 256; ``log_decay`` (fp32 [heads]) is at most 0, -inf forgets
 everything at each token.  The decays are time constants, not learned: they
-have no gradient.
+have no gradient.  Results have no autograd graph: tensors that require
+gradients are refused where these are recorded, and ``backward`` gives them.
 """
 from __future__ import annotations
 

@@ -9,6 +9,9 @@ products summed in fp32 within a block, scaled, and summed in fp32.
     w = scaled.quantize(weights, row_block=128)          # once
     y = scaled.product(scaled.quantize(x), w)            # x @ weights^T, bf16
     dx, dw = scaled.product_backward(dy, x, w)
+
+Results have no autograd graph: tensors that require gradients are refused
+where these are recorded.
 """
 from __future__ import annotations
 
@@ -18,7 +21,7 @@ import threading
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, Layouts, after_timeout, check_tensor, check_waits, error_flag, layout, on, require
+from ._tensors import DTYPE, Layouts, after_timeout, check_gradient, check_tensor, check_waits, error_flag, layout, on, require
 
 BLOCK = 128
 
@@ -113,6 +116,7 @@ class Scaled:
 
 def _describe_quantize(x, row_block, transpose):
     require(x.dim() == 2, "x: must be a matrix")
+    check_gradient(x, "x")
     require(x.dtype in DTYPE, f"x: must be bfloat16, float16 or float32, is {x.dtype}")
     require(row_block in (1, BLOCK), f"row_block: must be 1 or {BLOCK}, is {row_block}")
     rows, cols = x.shape

@@ -171,3 +171,29 @@ def test_check_waits_for_every_stream():
     with pytest.raises(N.NrnError):
         scaled.check()
     scaled.check()
+
+
+# ------------------------------------------------------------------ gradients
+
+def test_tensors_that_want_gradients_are_refused():
+    """Results have no graph: a call that would lose a gradient without a word is refused where gradients are recorded."""
+    from libnrn_b200 import gatednorm, linattn, scaled
+    q, k, v = (randn(1, 20, 2, 32, seed=i) for i in range(3))
+    g, r, p = torch.full((2,), -0.1, device="cuda"), randn(4, 64), torch.ones(64, device="cuda")
+    state = torch.zeros(1, 2, 32, 32, device="cuda")
+    w = scaled.quantize(randn(16, 64), row_block=128)
+    calls = [lambda q=q, k=k, v=v, state=state: linattn.forward(q, k, v, g, state=state),
+             lambda q=q, k=k, v=v: linattn.backward(q, q, k, v, g),
+             lambda q=q, k=k, v=v, state=state: linattn.step(q[:, 0], k[:, 0], v[:, 0], g, state),
+             lambda r=r: scaled.quantize(r), lambda r=r: scaled.product_backward(r[:, :16].contiguous(), r, w),
+             lambda r=r, p=p: gatednorm.forward(r, r, w_post=p), lambda r=r: gatednorm.backward(r, None, r)]
+    for call in calls:
+        call()
+        for name in call.__code__.co_varnames[:call.__code__.co_argcount]:
+            wants = {"q": q, "k": k, "v": v, "state": state, "r": r, "p": p}[name].clone().requires_grad_(True)
+            with pytest.raises(N.NrnError, match="gradient"):
+                call(**{name: wants})
+            with torch.no_grad():
+                call(**{name: wants})
+            with pytest.raises(N.NrnError, match="gradient"):      # what was allowed there is not remembered here
+                call(**{name: wants})
