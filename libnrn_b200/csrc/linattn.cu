@@ -1837,6 +1837,7 @@ extern "C" nrn_status_t nrn_cuda_linattn_step(const nrn_linattn_t* a, float* sta
     NRN_TRY(check_common(a, "nrn_cuda_linattn_step"));
     NRN_CHECK_ARG(a->tokens == 1 && a->cu_seqlens == nullptr, "nrn_cuda_linattn_step: one token for each sequence");
     NRN_CHECK_ARG(n_slots >= 0 && (slots || n_slots >= a->seqs), "nrn_cuda_linattn_step: fewer states than sequences");
+    NRN_CHECK_ARG(n_slots <= 1 || slot_stride >= static_cast<int64_t>(a->heads) * a->dk * a->dv, "nrn_cuda_linattn_step: states lie on one another");
     if (a->seqs == 0) return NRN_OK;
     NRN_CHECK_ARG(a->q && a->k && a->v && a->o && state, "nrn_cuda_linattn_step: null array");
     NRN_CHECK_ARG(static_cast<int64_t>(a->seqs) * a->heads * ((a->dv + 7) / 8) < (int64_t(1) << 31),

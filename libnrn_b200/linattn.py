@@ -146,6 +146,7 @@ def _describe_step(q, k, v, log_decay, state, scale, slots, out):
     require(isinstance(state, torch.Tensor) and state.dim() == 4, "state: must be [states, heads, dk, dv]")
     check_tensor(state, "state", torch.float32, dev, (state.shape[0], h, dk, dv))
     require(state.shape[0] == 0 or state[0].is_contiguous(), "state: each state must be contiguous")
+    require(state.shape[0] <= 1 or state.stride(0) >= h * dk * dv, "state: states lie on one another")
     if slots is not None:
         check_tensor(slots, "slots", torch.int32, dev, (b,))
         require(slots.is_contiguous(), "slots: must be contiguous")

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import operator_refs as R
+from libnrn_b200 import _native as N
 from test_gpu_linattn import STATE_TOL, TOL, close, decays, make
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +29,19 @@ def test_an_infinite_state_stays_infinite(kind, t):
     close(o[..., rest], ro[..., rest], TOL[dtype])
     end[..., 5, 7] = rend[..., 5, 7] = 0
     close(end, rend, STATE_TOL)
+
+
+def test_states_on_one_another_are_refused(monkeypatch):
+    """Sequences that would update one state, or states that overlap.  (Nothing is launched here.)"""
+    from libnrn_b200 import linattn
+    monkeypatch.setattr(N.lib(), "nrn_cuda_linattn_step", lambda *a: 0)
+    q, k, v, _, _, _ = make(3, 1, 2, 2, 32, 32, BF16)
+    q, k, v, g = q[:, 0], k[:, 0], v[:, 0], decays(2)
+    one = torch.zeros(1, 2, 32, 32, device="cuda")
+    linattn.step(q[:1], k[:1], v[:1], g, one)
+    linattn.step(q[:1], k[:1], v[:1], g, one.expand(1, 2, 32, 32))
+    for state in (one.expand(3, 2, 32, 32), torch.zeros(4 * 2048, device="cuda").as_strided((3, 2, 32, 32), (1024, 1024, 32, 1))):
+        with pytest.raises(N.NrnError, match="state"):
+            linattn.step(q, k, v, g, state)
+        with pytest.raises(N.NrnError, match="state"):
+            linattn.step(q[:1], k[:1], v[:1], g, state, slots=torch.zeros(1, dtype=torch.int32, device="cuda"))

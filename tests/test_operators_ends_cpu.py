@@ -18,3 +18,11 @@ def test_gradients_of_an_unknown_type():
         assert backward(9, 0, w) == 1 and b"dx" in N.lib().nrn_last_error()
         assert backward(0, -1, w) == 1 and b"dw" in N.lib().nrn_last_error()
     assert backward(0, 0, weights(rows=0)) == 0 and backward(0, 0, weights(cols=0)) == 0
+
+
+def test_steps_of_states_that_overlap():
+    a = N.LinAttn()
+    a.dtype, a.seqs, a.heads, a.kv_heads, a.dk, a.dv, a.tokens, a.scale, a.log_decay = 0, 0, 4, 2, 8, 16, 1, 1.0, 256
+    step = lambda stride, n: N.lib().nrn_cuda_linattn_step(C.byref(a), 256, stride, n, None, None)      # noqa: E731
+    assert step(0, 2) == 1 and step(511, 2) == 1 and b"one another" in N.lib().nrn_last_error()
+    assert step(512, 2) == 0 and step(0, 1) == 0
