@@ -47,6 +47,15 @@ def check_rows(t, name: str, dtype, device, shape) -> None:
     require(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the last dimension must have stride 1, has {t.stride(-1)}")
 
 
+def check_result(t, name: str, dtype, device, shape) -> None:
+    """Rows that are written: no two elements at one place (each dimension steps over what lies inside it)."""
+    check_rows(t, name, dtype, device, shape)
+    inside = 1
+    for stride, n in sorted((t.stride(i), n) for i, n in enumerate(t.shape) if n > 1):
+        require(stride >= inside, f"{name}: elements lie on one another")
+        inside += (n - 1) * stride
+
+
 def check_vector(t, name: str, n: int, device) -> None:
     check_tensor(t, name, torch.float32, device, (n,))
     require(t.is_contiguous(), f"{name}: must be contiguous")

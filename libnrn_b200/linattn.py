@@ -5,8 +5,9 @@ time (``step``).  For each sequence and head, with lam = exp(log_decay[head]):
     S_t = lam S_{t-1} + k_t v_t^T          o_t = scale * S_t^T q_t
 
 Tokens are [batch, tokens, heads, d] tensors with any strides but the last,
-which is 1; bf16, fp16 or fp32.  k and v may have fewer heads (a divisor of
-q's), each read by as many heads of q.  States are fp32
+which is 1; bf16, fp16 or fp32.  A result given as ``out`` lies on none of the
+inputs, and its elements not on one another.  k and v may have fewer heads (a
+divisor of q's), each read by as many heads of q.  States are fp32
 [batch, heads, dk, dv].  With ``cu_seqlens`` (int32 starts of packed
 sequences, [sequences + 1], on the device, from 0 to the number of tokens) the
 batch dimension is 1 and states have one entry for each sequence.  dk and dv
@@ -22,7 +23,7 @@ import ctypes as C
 import torch
 
 from . import _native as N
-from ._tensors import (DTYPE, Layouts, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, layout, number,
+from ._tensors import (DTYPE, Layouts, check_result, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, layout, number,
                        on, ptr, require)
 
 check = check_waits
@@ -64,9 +65,10 @@ def _describe(q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out):
     for name, x in (("state", state), ("dstate", dstate)):
         if x is not None:
             check_state(x, name, dev, shape)
-    for name, x in (("do", do), ("out", out)):
-        if x is not None:
-            check_rows(x, name, dt, dev, (b, t, h, dv))
+    if do is not None:
+        check_rows(do, "do", dt, dev, (b, t, h, dv))
+    if out is not None:
+        check_result(out, "out", dt, dev, (b, t, h, dv))
     a.log_decay = log_decay.data_ptr()
     a.scale = dk ** -0.5 if scale is None else scale
     a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
@@ -153,7 +155,7 @@ def _describe_step(q, k, v, log_decay, state, scale, slots, out):
     else:
         require(state.shape[0] >= b, f"state: {state.shape[0]} states for {b} sequences")
     if out is not None:
-        check_rows(out, "out", q.dtype, dev, (b, h, dv))
+        check_result(out, "out", q.dtype, dev, (b, h, dv))
     a = N.LinAttn()
     a.dtype, a.seqs, a.heads, a.kv_heads, a.dk, a.dv, a.tokens = DTYPE[q.dtype], b, h, hk, dk, dv, 1
     a.scale = dk ** -0.5 if scale is None else scale

@@ -45,3 +45,24 @@ def test_states_on_one_another_are_refused(monkeypatch):
             linattn.step(q, k, v, g, state)
         with pytest.raises(N.NrnError, match="state"):
             linattn.step(q[:1], k[:1], v[:1], g, state, slots=torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+def test_results_on_one_another_are_refused(monkeypatch):
+    """An `out` whose tokens share memory.  (Nothing is launched here.)"""
+    from libnrn_b200 import linattn
+    for name in ("nrn_cuda_linattn_step", "nrn_cuda_linattn_forward"):
+        monkeypatch.setattr(N.lib(), name, lambda *a: 0)
+    q, k, v, s0, _, _ = make(2, 10, 2, 2, 32, 32, BF16)
+    g = decays(2)
+    for out in (torch.empty(2, 1, 2, 32, device="cuda", dtype=BF16).expand(2, 10, 2, 32), torch.empty(1, 10, 2, 32, device="cuda", dtype=BF16).expand(2, 10, 2, 32),
+                torch.empty(2, 10, 1, 32, device="cuda", dtype=BF16).expand(2, 10, 2, 32),
+                torch.empty(4000, device="cuda", dtype=BF16).as_strided((2, 10, 2, 32), (640, 32, 32, 1))):
+        with pytest.raises(N.NrnError, match="out"):
+            linattn.forward(q, k, v, g, out=out)
+    for out in (torch.empty(1, 2, 32, device="cuda", dtype=BF16).expand(2, 2, 32), torch.empty(2, 1, 32, device="cuda", dtype=BF16).expand(2, 2, 32)):
+        with pytest.raises(N.NrnError, match="out"):
+            linattn.step(q[:, 0], k[:, 0], v[:, 0], g, s0, out=out)
+    # heads outside tokens, parts of something wider
+    linattn.forward(q, k, v, g, out=torch.empty(2, 2, 10, 32, device="cuda", dtype=BF16).transpose(1, 2))
+    linattn.forward(q, k, v, g, out=torch.empty(2, 10, 2, 96, device="cuda", dtype=BF16)[..., 32:64])
+    linattn.forward(q, k, v, g, out=torch.empty(10, 2, 2, 32, device="cuda", dtype=BF16).transpose(0, 1))
