@@ -65,8 +65,11 @@ def _describe(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
 _layouts = Layouts(_describe)
 
 
-def _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
+def _check_residual(residual):
     require(isinstance(residual, torch.Tensor) and residual.is_cuda, "residual: a CUDA tensor is needed")
+
+
+def _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz):
     eps = number(eps)
     key = (layout(residual), layout(h), layout(gate), layout(alpha), layout(w_post), layout(w_pre), eps, activation, layout(dy), layout(dz))
     block, need = _layouts.get(key, residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz)
@@ -80,11 +83,12 @@ def forward(residual, h=None, gate=None, *, alpha=None, w_post=None, w_pre=None,
             scaled=False, want_z=True, stream=None):
     """(y, z) of [rows, d] tensors (bf16, fp16 or fp32; last stride 1).  z is None without ``want_z``, and a ``Scaled``
     matrix with ``scaled``: the next block's 8-bit input.  Without h, y is ``residual`` itself."""
-    a, _ = _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, None, None)
-    rows, d = residual.shape
+    _check_residual(residual)
     dev = residual.device
     y, z = residual, None
     with on(dev, stream) as st:
+        a, _ = _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, None, None)
+        rows, d = residual.shape
         if h is not None:
             y = torch.empty_strided((rows, d), (d, 1), dtype=residual.dtype, device=dev)
             a.y, a.y_stride = y.data_ptr(), d
@@ -102,10 +106,11 @@ def backward(dy, dz, residual, h=None, gate=None, *, alpha=None, w_post=None, w_
              stream=None) -> Gradients:
     """Gradients of a ``forward`` call with these arguments, given those of y and z (None: zero).  Those of alpha, w_post
     and w_pre are fp32 sums over the rows, added in a fixed order."""
-    a, need = _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz)
-    rows, d = residual.shape
+    _check_residual(residual)
     dev, dt = residual.device, residual.dtype
     with on(dev, stream) as st:
+        a, need = _call(residual, h, gate, alpha, w_post, w_pre, eps, activation, dy, dz)
+        rows, d = residual.shape
         g = N.GatedNormGrad()
         g.dy, g.dz, g.dy_stride, g.dz_stride = ptr(dy), ptr(dz), _stride(dy), _stride(dz)
         like = [torch.empty_strided((rows, d), (d, 1), dtype=dt, device=dev) if want else None for want in (True, h is not None, gate is not None)]

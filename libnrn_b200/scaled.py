@@ -226,8 +226,8 @@ def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None
     require(isinstance(a, Scaled) and isinstance(b, Scaled), "a, b: must be Scaled (scaled.quantize)")
     dev = a.device
     key = (a.shape, b.shape, dev, b.device, dtype, layout(out))
-    kind, stride, need = _products.get(key, a, b, dtype, out)
     with on(dev, stream) as st:
+        kind, stride, need = _products.get(key, a, b, dtype, out)
         if out is None:
             n = b.shape[0]
             out = torch.empty_strided((a.shape[0], n), (n, 1), dtype=dtype, device=dev)
@@ -271,9 +271,9 @@ def product_backward(dy: torch.Tensor, x: torch.Tensor, w: Scaled, *, dx_dtype=N
     require(isinstance(dy, torch.Tensor) and dy.is_cuda, "dy: a CUDA tensor is needed")
     dx_dtype = dx_dtype or dy.dtype
     key = (layout(dy), layout(x), w.shape, w.row_block, w.device, dx_dtype, dw_dtype)
-    rows, dy_stride, x_stride, kind, dx_kind, dw_kind, need = _backwards.get(key, dy, x, w, dx_dtype, dw_dtype)
     dev, (n, k) = w.device, w.shape
     with on(dev, stream) as st:
+        rows, dy_stride, x_stride, kind, dx_kind, dw_kind, need = _backwards.get(key, dy, x, w, dx_dtype, dw_dtype)
         dx = torch.empty_strided((rows, k), (k, 1), dtype=dx_dtype, device=dev)
         dw = torch.empty_strided((n, k), (k, 1), dtype=dw_dtype, device=dev)
         shared = _on_stream(dev, st)

@@ -1,4 +1,5 @@
 """What the tensor operators (linattn, scaled, gatednorm) share."""
+import contextlib
 import os
 import subprocess
 import sys
@@ -197,3 +198,42 @@ def test_tensors_that_want_gradients_are_refused():
                 call(**{name: wants})
             with pytest.raises(N.NrnError, match="gradient"):      # what was allowed there is not remembered here
                 call(**{name: wants})
+
+
+# -------------------------------------------------------------------- devices
+
+def test_sizes_are_asked_for_on_the_tensors_device(monkeypatch):
+    """The workspaces' sizes depend on the device: they are asked for after the switch to it."""
+    from libnrn_b200 import gatednorm, scaled
+    switched = [0]
+
+    def watched(real):
+        @contextlib.contextmanager
+        def on(*a):
+            with real(*a) as s:
+                switched[0] += 1
+                try:
+                    yield s
+                finally:
+                    switched[0] -= 1
+        return on
+    asked = []
+
+    def sizes(name):
+        real = getattr(N.lib(), name)
+
+        def call(*a):
+            asked.append((name, switched[0]))
+            return real(*a)
+        return call
+    for m in (scaled, gatednorm):
+        monkeypatch.setattr(m, "on", watched(m.on))
+    names = ["nrn_cuda_scaled_workspace", "nrn_cuda_scaled_backward_workspace", "nrn_cuda_gatednorm_workspace"]
+    for n in names:
+        monkeypatch.setattr(N.lib(), n, sizes(n))
+    x = randn(37, 1111, dtype=BF16)                 # layouts that no other test has
+    w = scaled.quantize(randn(53, 1111), row_block=128)
+    scaled.product(scaled.quantize(x), w)
+    scaled.product_backward(randn(37, 53, dtype=BF16), x, w)
+    gatednorm.forward(x)
+    assert sorted(n for n, _ in asked) == sorted(names) and all(s == 1 for _, s in asked), asked
