@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "internal.h"
 
@@ -27,14 +28,20 @@ inline int sm_count() {
     return n;
 }
 
-// Lets a kernel use `bytes` of dynamic shared memory.
+// Lets a kernel use `bytes` of dynamic shared memory.  The limit is only ever
+// raised, and one thread at a time sets it: another thread's launch may need
+// the larger one.
 template <auto Kernel>
 cudaError_t allow_shared(int bytes) {
     static std::atomic<int> most[kMaxDevices];
+    static std::mutex turn;
     const int d = device_index();
-    if (d >= 0 && d < kMaxDevices && most[d].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+    if (d < 0 || d >= kMaxDevices) return cudaErrorInvalidDevice;
+    if (most[d].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+    std::lock_guard<std::mutex> lock(turn);
+    if (most[d].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && d >= 0 && d < kMaxDevices) most[d].store(bytes, std::memory_order_relaxed);
+    if (e == cudaSuccess) most[d].store(bytes, std::memory_order_release);
     return e;
 }
 
