@@ -27,16 +27,17 @@ from ._tensors import check_rows, require
 
 
 def bin_spikes(step: np.ndarray, gid: np.ndarray, n: int, bin_steps: int, bins: int, *, first: int = 0, group: int = 1,
-               start: int = 0, device="cuda") -> torch.Tensor:
-    """Spike counts [bins, ceil(n / group)] (bf16) of neurons first .. first + n - 1 of a raster (``Network.raster``),
-    ``group`` neighbours together, in ``bins`` bins of ``bin_steps`` steps from step ``start`` on."""
+               start: int = 0, device="cuda", dtype=torch.bfloat16) -> torch.Tensor:
+    """Spike counts [bins, ceil(n / group)] of neurons first .. first + n - 1 of a raster (``Network.raster``), ``group``
+    neighbours together, in ``bins`` bins of ``bin_steps`` steps from step ``start`` on.  bf16, which a ``Readout`` takes,
+    holds counts to 256 and rounds larger ones to eight bits; another ``dtype`` for more."""
     width = -(-n // group)
     s = torch.from_numpy(np.ascontiguousarray(step)).to(device).long()
     g = torch.from_numpy(np.ascontiguousarray(gid)).to(device).long() - first
     b = (s - start) // bin_steps
     keep = (g >= 0) & (g < n) & (s >= start) & (b < bins)
     at = b[keep] * width + g[keep] // group
-    return torch.bincount(at, minlength=bins * width).view(bins, width).to(torch.bfloat16)
+    return torch.bincount(at, minlength=bins * width).view(bins, width).to(dtype)
 
 
 class Readout:

@@ -1,4 +1,5 @@
 """A readout answers by the weights that it has at the call, and its ends."""
+import numpy as np
 import pytest
 import torch
 
@@ -58,3 +59,13 @@ def test_weights_that_the_caller_keeps():
     assert torch.equal(r.step(x[:, 0], r.new_states(2), small=kept), r.step(x[:, 0], r.new_states(2)))
     r.weights["head"].zero_()
     assert torch.equal(r.read(x, small=kept)[0], before) and not r.read(x)[0].any()
+
+
+def test_counts_past_256():
+    """bf16 has eight bits: larger counts are exact in the type that is asked for."""
+    from libnrn_b200 import readout
+    step, gid = np.repeat([3, 11], [257, 1001]), np.zeros(1258, np.int64)
+    exact = readout.bin_spikes(step, gid, 4, 10, 2, group=4, dtype=torch.float32)
+    assert exact.dtype == torch.float32 and exact.tolist() == [[257.0], [1001.0]]
+    assert torch.equal(readout.bin_spikes(step, gid, 4, 10, 2, group=4), exact.to(torch.bfloat16))
+    assert "256" in readout.bin_spikes.__doc__
