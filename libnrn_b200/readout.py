@@ -53,7 +53,9 @@ class Readout:
         self.features, self.outputs, self.width, self.eps = features, outputs, width, eps
         self.heads, self.kv_heads, self.dk, self.dv, self.blocks = heads, kv_heads, dk, dv, blocks
         self.parts = (heads * dk, kv_heads * dk, kv_heads * dv, width)          # q, k, v, gate
-        self.device = torch.device(device, torch.cuda.current_device()) if device == "cuda" else torch.device(device)
+        self.device = torch.device(device)
+        if self.device.index is None:
+            self.device = torch.device(self.device.type, torch.cuda.current_device())
         memory = torch.logspace(math.log10(tau[0]), math.log10(tau[1]), heads, dtype=torch.float64)
         self.log_decay = (-bin_s / memory).float().to(self.device)
         gen = torch.Generator(device=self.device).manual_seed(seed)

@@ -69,3 +69,10 @@ def test_counts_past_256():
     assert exact.dtype == torch.float32 and exact.tolist() == [[257.0], [1001.0]]
     assert torch.equal(readout.bin_spikes(step, gid, 4, 10, 2, group=4), exact.to(torch.bfloat16))
     assert "256" in readout.bin_spikes.__doc__
+
+
+def test_a_device_without_a_number():
+    for device in ("cuda", torch.device("cuda"), "cuda:0", torch.device("cuda", 0)):
+        r = make(device=device)
+        assert r.device == torch.device("cuda", torch.cuda.current_device())
+        r.read(counts(1, 5, 24))
