@@ -117,8 +117,8 @@ class Readout:
             o, end = linattn.forward(q.unflatten(0, (b, t)), k.unflatten(0, (b, t)), v.unflatten(0, (b, t)), self.log_decay,
                                      state=None if states is None else states[i], cu_seqlens=cu_seqlens)
             after.append(end)
-            return o.reshape(b * t, -1)
-        return self._through(counts.reshape(b * t, -1), attend, small).view(b, t, -1), after
+            return o.reshape(b * t, self.heads * self.dv)
+        return self._through(counts.reshape(b * t, self.features), attend, small).view(b, t, self.outputs), after
 
     def step(self, counts, states, slots=None, small=None):
         """Answers [batch, outputs] for one bin [batch, features] of each session; ``states`` are updated in place
@@ -130,6 +130,7 @@ class Readout:
         """(loss, gradients by the weights' names) of the mean squared error of ``read``'s answers."""
         check_rows(counts, "counts", torch.bfloat16, self.device, (*counts.shape[:2], self.features))
         b, t = counts.shape[:2]
+        require(b * t > 0, "counts: no bins, no mean over them")
         c = counts.reshape(b * t, -1)
         w = self.quantized().__getitem__
         x = scaled.product(scaled.quantize(c), w("embed"))

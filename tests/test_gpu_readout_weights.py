@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from libnrn_b200 import _native as N
+
 pytestmark = pytest.mark.gpu
 
 
@@ -76,3 +78,15 @@ def test_a_device_without_a_number():
         r = make(device=device)
         assert r.device == torch.device("cuda", torch.cuda.current_device())
         r.read(counts(1, 5, 24))
+
+
+def test_no_bins_and_no_sessions():
+    r = make()
+    answers, states = r.read(counts(2, 0, 24))
+    assert answers.shape == (2, 0, 16) and not states[0].any()
+    some = [s.normal_() for s in r.new_states(2)]
+    assert torch.equal(r.read(counts(2, 0, 24), states=some)[1][0], some[0])
+    assert r.read(counts(0, 7, 24))[0].shape == (0, 7, 16)
+    assert r.step(counts(0, 24), r.new_states(3)).shape == (0, 16)
+    with pytest.raises(N.NrnError):
+        r.gradients(counts(1, 0, 24), counts(1, 0, 16))
