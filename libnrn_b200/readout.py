@@ -131,6 +131,7 @@ class Readout:
         check_rows(counts, "counts", torch.bfloat16, self.device, (*counts.shape[:2], self.features))
         b, t = counts.shape[:2]
         require(b * t > 0, "counts: no bins, no mean over them")
+        require(targets.numel() == b * t * self.outputs, f"targets: must be {(b, t, self.outputs)}, are {tuple(targets.shape)}")
         c = counts.reshape(b * t, -1)
         w = self.quantized().__getitem__
         x = scaled.product(scaled.quantize(c), w("embed"))

@@ -90,3 +90,12 @@ def test_no_bins_and_no_sessions():
     assert r.step(counts(0, 24), r.new_states(3)).shape == (0, 16)
     with pytest.raises(N.NrnError):
         r.gradients(counts(1, 0, 24), counts(1, 0, 16))
+
+
+def test_targets_of_another_shape_are_refused():
+    """One target for all outputs would be taken for each of them."""
+    r, x = make(), counts(1, 7, 24)
+    r.gradients(x, x[..., :16])
+    for bad in (x[..., :1], x, x[:, :6, :16]):
+        with pytest.raises(N.NrnError, match="targets"):
+            r.gradients(x, bad)
