@@ -134,6 +134,8 @@ def on(device, stream=None):
     i = device.index
     if stream is None and _current_device() == i:
         return _Current(_raw_stream(i))
+    if stream is not None:
+        require(stream.device == device, f"stream: must be of {device}, is of {stream.device}")
     return _switched(device, stream)
 
 

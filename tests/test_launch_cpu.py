@@ -4,6 +4,9 @@ import re
 import subprocess
 
 import pytest
+import torch
+
+from libnrn_b200 import _native as N
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "libnrn_b200", "csrc")
@@ -92,3 +95,13 @@ def test_no_kernel_lets_the_next_in_before_it_has_its_tmem(name):
             # only where the block ends without any
             assert re.match(r"let_next\(\);\s*previous_done\(\);\s*return;", body[at:]), f"{name}: let_next before tcgen05.alloc"
         assert re.search(r"\blet_next\(\)", kernel[alloc:])
+
+
+def test_a_stream_of_another_device_is_refused():
+    from libnrn_b200._tensors import on
+
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 0
+    with pytest.raises(N.NrnError, match="stream"):
+        with on(torch.device("cuda", 0), Stream()):
+            pass
