@@ -61,6 +61,7 @@ def _describe(q, k, v, log_decay, scale, cu_seqlens, state, dstate, do, out):
         require(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and cu_seqlens.is_contiguous(),
                 "cu_seqlens: must be a contiguous vector of sequences + 1 starts")
         a.seqs, a.cu_seqlens = cu_seqlens.numel() - 1, cu_seqlens.data_ptr()
+        require(a.seqs > 0 or t == 0, f"cu_seqlens: no sequences for {t} tokens")
     shape = (a.seqs, h, dk, dv)
     for name, x in (("state", state), ("dstate", dstate)):
         if x is not None:

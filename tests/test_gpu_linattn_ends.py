@@ -66,3 +66,16 @@ def test_results_on_one_another_are_refused(monkeypatch):
     linattn.forward(q, k, v, g, out=torch.empty(2, 2, 10, 32, device="cuda", dtype=BF16).transpose(1, 2))
     linattn.forward(q, k, v, g, out=torch.empty(2, 10, 2, 96, device="cuda", dtype=BF16)[..., 32:64])
     linattn.forward(q, k, v, g, out=torch.empty(10, 2, 2, 32, device="cuda", dtype=BF16).transpose(0, 1))
+
+
+def test_tokens_without_a_sequence_are_refused():
+    from libnrn_b200 import linattn
+    q, k, v, _, do, _ = make(1, 10, 2, 2, 32, 32, BF16)
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(N.NrnError, match="cu_seqlens"):
+        linattn.forward(q, k, v, decays(2), cu_seqlens=none)
+    with pytest.raises(N.NrnError, match="cu_seqlens"):
+        linattn.backward(do, q, k, v, decays(2), cu_seqlens=none)
+    e = q[:, :0]
+    o, end = linattn.forward(e, e, e, decays(2), cu_seqlens=none)
+    assert o.shape == (1, 0, 2, 32) and end.shape == (0, 2, 32, 32)
