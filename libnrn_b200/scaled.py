@@ -121,7 +121,6 @@ def _describe_quantize(x, row_block, transpose):
     require(row_block in (1, BLOCK), f"row_block: must be 1 or {BLOCK}, is {row_block}")
     rows, cols = x.shape
     require(cols <= 1 or x.stride(1) == 1, f"x: the last dimension must have stride 1, has {x.stride(1)}")
-    require(rows <= 1 or x.stride(0) >= cols, "x: rows overlap")
     require(not transpose or row_block == 1, "transpose: only with a scale for each row")
     return DTYPE[x.dtype], rows, cols, x.stride(0) if rows > 1 else max(cols, 1)
 
@@ -130,7 +129,7 @@ _quantized = Layouts(_describe_quantize)
 
 
 def quantize(x: torch.Tensor, *, row_block: int = 1, transpose: bool = False, stream=None) -> Scaled:
-    """x (bf16, fp16 or fp32 [rows, cols], last stride 1) in 8 bits.  A block's scale is its largest magnitude / 448; an
+    """x (bf16, fp16 or fp32 [rows, cols], last stride 1, rows anywhere) in 8 bits.  A block's scale is its largest magnitude / 448; an
     infinity or NaN makes its whole block NaN.  ``transpose`` gives x^T with a scale for each of its rows (row_block 1)."""
     require(isinstance(x, torch.Tensor) and x.is_cuda, "x: a CUDA tensor is needed")
     dtype, rows, cols, stride = _quantized.get((layout(x), row_block, transpose), x, row_block, transpose)
@@ -249,7 +248,6 @@ def _describe_backward(dy, x, w, dx_dtype, dw_dtype):
         require(isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[1] == cols, f"{name}: must be [rows, {cols}]")
         check_tensor(t, name, dy.dtype, w.device)
         require(cols <= 1 or t.stride(1) == 1, f"{name}: the last dimension must have stride 1")
-        require(t.shape[0] <= 1 or t.stride(0) >= cols, f"{name}: rows overlap")
     rows = dy.shape[0]
     require(rows == x.shape[0], f"dy: has {rows} rows, x has {x.shape[0]}")
     for name, t in (("dy", dy.dtype), ("dx_dtype", dx_dtype), ("dw_dtype", dw_dtype)):
