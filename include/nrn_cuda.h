@@ -409,7 +409,7 @@ typedef struct {
     int64_t tokens;            /* of each sequence, or of all packed ones    */
     const int32_t* cu_seqlens; /* [seqs + 1], or NULL                        */
     const float* log_decay;    /* [heads]                                    */
-    float scale;               /* finite, not 0                              */
+    float scale;               /* finite, not 0; backward: 1 / scale too     */
     int32_t pad;
     const void* q;
     const void* k;

@@ -1771,6 +1771,7 @@ extern "C" nrn_status_t nrn_cuda_linattn_forward(const nrn_linattn_t* a, nrn_str
 extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const nrn_linattn_grad_t* g, nrn_stream_t stream) {
     NRN_TRY(check_common(a, "nrn_cuda_linattn_backward"));
     NRN_CHECK_ARG(g != nullptr, "nrn_cuda_linattn_backward: null gradients");
+    NRN_CHECK_ARG(std::isfinite(1.0f / a->scale), "nrn_cuda_linattn_backward: 1 / scale must be finite");   // the final states' gradient goes through it
     if (a->seqs == 0) return NRN_OK;
     NRN_CHECK_ARG(all_tokens(a) == 0 || (a->q && a->k && a->v && g->d_o && g->dq && g->dk && g->dv),
                   "nrn_cuda_linattn_backward: null array");

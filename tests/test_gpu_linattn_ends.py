@@ -79,3 +79,16 @@ def test_tokens_without_a_sequence_are_refused():
     e = q[:, :0]
     o, end = linattn.forward(e, e, e, decays(2), cu_seqlens=none)
     assert o.shape == (1, 0, 2, 32) and end.shape == (0, 2, 32, 32)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, -2.0 ** -100, 2.0 ** 100])
+def test_scales_far_from_one(scale):
+    """The gradient of the final state passes through 1 / scale: scales whose inverse is no number are refused."""
+    from libnrn_b200 import linattn
+    q, k, v, s0, do, ds = make(1, 40, 1, 1, 32, 32, FP32)
+    got = linattn.backward(do * 0, q, k, v, decays(1), scale=scale, state=s0, dstate=ds * scale)
+    ref = R.linattn_backward(do * 0, q, k, v, decays(1), scale, s0, ds * scale)
+    close(got[1] / scale, ref[1] / scale, TOL[FP32])
+    for x in (2.0 ** -140, -2.0 ** -130):
+        with pytest.raises(N.NrnError, match="scale"):
+            linattn.backward(do, q, k, v, decays(1), scale=x, dstate=ds)
