@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
 
 // ------------------------------------------------------- chunks of 64 tokens
 //
-// bf16 inputs, b.d <= 128.  For a chunk of tokens p with entering state X:
+// bf16 inputs with rows off 16-byte boundaries, b.d <= 128.  For a chunk of
+// tokens p with entering state X:
 //     o_p = lam^(p+off) X^T a_p + sum_{j<=p} lam^(p-j) (a_p . b_j) c_j
 //     X'  = lam^n X + sum_j lam^(n-off-j) b_j c_j^T
 // A block holds 64 columns (c) of one state, a warp 16 of them: X^T as
@@ -344,20 +345,14 @@ struct RowLoader {
         step = (p.reverse ? -m.tok : m.tok) * kRows;
         place = static_cast<uint32_t>((t * kPitch + c) * 2);
     }
-    // the next CH tokens, n of which there are
-    __device__ __forceinline__ void load(void* dst, const void* safe, int n, bool vec) {
-        const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst)) + place;
+    // the next CH tokens, n of which there are, element by element: rows on
+    // 16-byte boundaries go to the kernel below
+    __device__ __forceinline__ void load(void* dst, int n) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i, src += step) {
             const bool in = t + i * kRows < n && left > 0;
-            if (vec) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + i * kRows * kPitch * 2), "l"(in ? static_cast<const void*>(src) : safe),
-                             "r"(in ? 16 : 0)
-                             : "memory");
-            } else {
-                const Raw8<__nv_bfloat16> r = load8(src, in ? left : 0, false);
-                *reinterpret_cast<uint4*>(static_cast<char*>(dst) + place + i * kRows * kPitch * 2) = *reinterpret_cast<const uint4*>(&r);
-            }
+            const Raw8<__nv_bfloat16> r = load8(src, in ? left : 0, false);
+            *reinterpret_cast<uint4*>(static_cast<char*>(dst) + place + i * kRows * kPitch * 2) = *reinterpret_cast<const uint4*>(&r);
         }
     }
 };
@@ -407,24 +402,21 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
 
     RowLoader<CH, DK> la(p.a, p, u, head, 0), lb(p.b, p, u, head, 0);
     RowLoader<CH, kMmaCols> lc(p.c, p, u, head, col0);
-    const bool vec = p.vec != 0;
     // the results' place of this lane: token begin + lane / 2, eight of the warp's columns
     const int oj = wcol + 8 * (lane & 1);
     const int64_t ofirst = u.begin + (lane >> 1), ostep = p.reverse ? -p.o_tok : p.o_tok;
     int64_t oat = (u.row0 + (p.reverse ? u.len - 1 - ofirst : ofirst)) * p.o_tok + static_cast<int64_t>(u.seq) * p.o_seq + head * p.o_head + oj;
     auto fetch = [&](int64_t t0, int stage) {
         const int n = static_cast<int>(u.end - t0 < CH ? u.end - t0 : CH);
-        lb.load(&M.b[stage][0][0], p.b.p, n, vec);
-        lc.load(&M.c[stage][0][0], p.c.p, n, vec);
-        if (!STATE_ONLY) la.load(&M.a[stage][0][0], p.a.p, n, vec);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        lb.load(&M.b[stage][0][0], n);
+        lc.load(&M.c[stage][0][0], n);
+        if (!STATE_ONLY) la.load(&M.a[stage][0][0], n);
     };
     if (u.begin < u.end) fetch(u.begin, 0);
 
     int stage = 0;
     for (int64_t t0 = u.begin; t0 < u.end; t0 += CH, stage ^= 1) {
         const int n = static_cast<int>(u.end - t0 < CH ? u.end - t0 : CH);
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();                 // this chunk is here, and everybody is done with the last one
         if (t0 + CH < u.end) fetch(t0 + CH, stage ^ 1);
         const auto& A = M.a[stage];
