@@ -11,6 +11,8 @@ whose bracket loses a factor of at most 5 where gates keep 0.25 from its zero at
 import pytest
 import torch
 
+import operator_refs as R
+
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 TOL = {BF16: 2.0 ** -8 + 2.0 ** -16, FP16: 2.0 ** -11 + 2.0 ** -16, FP32: 2.0 ** -18}
@@ -58,3 +60,16 @@ def test_an_infinity_as_8_bits(bad, shape):
     want = scaled.quantize(plain)
     assert torch.equal(z.dequantize().isnan(), want.dequantize().isnan())
     assert bool(z.dequantize()[1, 128:256].isnan().all()) and torch.equal(z.scales.isnan(), want.scales.isnan())
+
+
+@pytest.mark.parametrize("dtype", [FP16, FP32], ids=str)
+def test_z_as_8_bits_from_other_types(dtype):
+    from libnrn_b200 import gatednorm
+    for rows, d in ((3, 200), (65, 2048), (2, 8200), (3, 16384)):
+        gen = torch.Generator(device="cuda").manual_seed(2)
+        r, h, gate = (torch.randn(rows, d, device="cuda", generator=gen).to(dtype) for _ in range(3))
+        _, z = gatednorm.forward(r, h, gate, scaled=True, eps=EPS)
+        _, ref = R.gatednorm(r.double(), h.double(), gate.double(), None, None, None, EPS)
+        v, s = R.quantized(ref)
+        assert R.rel(z.scales, s) <= 2.0 ** -19
+        assert float((z.values.float() != v.float()).float().mean()) <= 1e-3

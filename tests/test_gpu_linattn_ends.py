@@ -92,3 +92,63 @@ def test_scales_far_from_one(scale):
     for x in (2.0 ** -140, -2.0 ** -130):
         with pytest.raises(N.NrnError, match="scale"):
             linattn.backward(do, q, k, v, decays(1), scale=x, dstate=ds)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("which", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("kind", ["bf16", "bf16 off 16 bytes", "fp16", "fp32"])
+def test_a_bad_token_in_the_gradients(kind, which, bad):
+    """Keys and values before it see a token of q or do that is no number, queries after it one of k or v; nobody else does."""
+    from libnrn_b200 import linattn
+    dtype = {"fp16": FP16, "fp32": FP32}.get(kind, BF16)
+    at, h = 77, 1
+    q, k, v, _, do, _ = make(2, 200, 2, 2, 64, 64, dtype, seed=5)
+    if kind == "bf16 off 16 bytes":
+        q, k, v, do = (torch.cat([x[..., :1], x], -1)[..., 1:] for x in (q, k, v, do))
+    g = decays(2)
+    good = linattn.backward(do, q, k, v, g)
+    {"q": q, "k": k, "v": v, "do": do}[which][1, at, h, 3] = bad
+    got = linattn.backward(do, q, k, v, g)
+    for n, x, y in zip(("q", "k", "v"), got, good):
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1, :, 0], y[1, :, 0])
+        later, earlier = slice(at + 1, None), slice(None, at)
+        clean = {"q": {"q": [earlier, slice(at, None)], "k": [earlier], "v": [earlier], "do": [earlier, later]},
+                 "k": {"q": [later], "k": [earlier, slice(at, None)], "v": [earlier, later], "do": [later]},
+                 "v": {"q": [later], "k": [earlier, later], "v": [earlier, slice(at, None)], "do": [later]}}[n][which]
+        for part in clean:
+            z = x[1, part, h]
+            assert bool(torch.isfinite(z).all()), (n, part)
+            assert R.rel(z, y[1, part, h]) <= TOL[dtype]
+    assert torch.equal(got[3][0], good[3][0]) and torch.equal(got[3][1, 0], good[3][1, 0])
+
+
+@pytest.mark.parametrize("lens", [[0, 1, 64, 0, 65, 300, 2], [17, 16, 15, 1]], ids=str)
+def test_packed_fp16(lens):
+    from libnrn_b200 import linattn
+    n = len(lens)
+    q, k, v, _, do, _ = make(1, sum(lens), 4, 2, 64, 96, FP16, seed=1)
+    _, _, _, s0, _, ds = make(n, 0, 4, 2, 64, 96, FP16, seed=2)
+    g, cu = decays(4), torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    o, end = linattn.forward(q, k, v, g, state=s0, cu_seqlens=cu)
+    ro, rend = R.linattn(q, k, v, g, 0.125, s0, lens)
+    close(o, ro, TOL[FP16])
+    close(end, rend, STATE_TOL)
+    got = linattn.backward(do, q, k, v, g, state=s0, dstate=ds, cu_seqlens=cu)
+    for x, y, tol in zip(got, R.linattn_backward(do, q, k, v, g, 0.125, s0, ds, lens), [TOL[FP16]] * 3 + [STATE_TOL]):
+        close(x, y, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=str)
+def test_one_key_head_for_all(dtype):
+    """k and v expanded over the heads (a stride of 0), as a caller without shared heads would give them."""
+    from libnrn_b200 import linattn
+    q, k, v, s0, do, ds = make(2, 150, 4, 1, 64, 64, dtype, seed=6)
+    kx, vx, g = k.expand(2, 150, 4, 64), v.expand(2, 150, 4, 64), decays(4)
+    o, end = linattn.forward(q, kx, vx, g, state=s0)
+    ro, rend = R.linattn(q, k, v, g, 0.125, s0)
+    close(o, ro, TOL[dtype])
+    close(end, rend, STATE_TOL)
+    got = linattn.backward(do, q, kx, vx, g, state=s0, dstate=ds)
+    ref = R.linattn_backward(do, q, kx, vx, g, 0.125, s0, ds)
+    for x, y, tol in zip(got, ref, [TOL[dtype]] * 3 + [STATE_TOL]):
+        close(x, y, tol)

@@ -237,3 +237,43 @@ def test_sizes_are_asked_for_on_the_tensors_device(monkeypatch):
     scaled.product_backward(randn(37, 53, dtype=BF16), x, w)
     gatednorm.forward(x)
     assert sorted(n for n, _ in asked) == sorted(names) and all(s == 1 for _, s in asked), asked
+
+
+def replayed(call, change):
+    """The results of `call` captured and replayed after `change` of its inputs, and those of a call after it."""
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    change()
+    graph.replay()
+    return got, call()
+
+
+def test_steps_norms_and_gradients_in_graphs():
+    from libnrn_b200 import gatednorm, linattn, scaled
+    # two sequences that are split, shared heads: every kernel of the chain
+    q, k, v, do = (randn(2, 3000, h, 64, seed=i, dtype=BF16) for i, h in enumerate((4, 2, 2, 4)))
+    g = torch.full((4,), -0.01, device="cuda")
+    got, want = replayed(lambda: linattn.backward(do, q, k, v, g), lambda: do.copy_(do.flip(1)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x, dy, w = randn(300, 640, seed=5, dtype=BF16), randn(300, 256, seed=6, dtype=BF16), scaled.quantize(randn(256, 640, seed=7), row_block=128)
+    got, want = replayed(lambda: scaled.product_backward(dy, x, w), lambda: (dy.copy_(dy.flip(0)), x.copy_(x.flip(1))))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    p = torch.rand(640, device="cuda")
+    got, want = replayed(lambda: gatednorm.forward(x, x, x, w_post=p, scaled=True), lambda: x.copy_(x.flip(0)))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1].dequantize(), want[1].dequantize())
+    got, want = replayed(lambda: gatednorm.backward(x, x, x, x, x, w_post=p, w_pre=p), lambda: x.copy_(x.flip(0)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+    state = randn(5, 4, 64, 64, seed=8)
+    slots = torch.tensor([4, 0], device="cuda", dtype=torch.int32)
+    one = lambda s: linattn.step(q[:, 0], k[:, 0], v[:, 0], g, s, slots=slots)      # noqa: E731
+    graph, mine = torch.cuda.CUDAGraph(), state.clone()
+    one(mine)
+    with torch.cuda.graph(graph):
+        o = one(state)
+    state.copy_(mine)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(o, one(mine)) and torch.equal(state, mine)
+    linattn.check()
