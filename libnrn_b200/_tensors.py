@@ -139,6 +139,18 @@ def on(device, stream=None):
     return _switched(device, stream)
 
 
+def share(stream, device, inputs, results) -> None:
+    """After a call on a stream of the caller's choice: the memory of its inputs, should they be dropped, is not given out again
+    before that stream is past the call, nor that of its results before the current stream is past what it does with them."""
+    here = torch.cuda.current_stream(device)
+    if stream.cuda_stream == here.cuda_stream:
+        return
+    for of, tensors in ((stream, inputs), (here, results)):
+        for t in tensors:
+            if t is not None:
+                t.record_stream(of)
+
+
 class _Flag:
     """A device's word that kernels set when one of their bounded waits gives up, and the same as a tensor.  The library
     makes it: made here by the first call it could become part of a graph that is being captured, whose replays would clear

@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, Layouts, check_rows, check_vector, check_waits, error_flag, layout, number, on, ptr, require
+from ._tensors import DTYPE, Layouts, check_rows, check_vector, check_waits, error_flag, layout, number, on, ptr, require, share
 from .scaled import Scaled
 
 check = check_waits
@@ -99,6 +99,8 @@ def forward(residual, h=None, gate=None, *, alpha=None, w_post=None, w_pre=None,
             z = torch.empty_strided((rows, d), (d, 1), dtype=residual.dtype, device=dev)
             a.z, a.z_stride = z.data_ptr(), d
         N.check(N.lib().nrn_cuda_gatednorm_forward(C.byref(a), st), "nrn_cuda_gatednorm_forward")
+    if stream is not None:
+        share(stream, dev, (residual, h, gate, alpha, w_post, w_pre), (y, *z.memory()) if isinstance(z, Scaled) else (y, z))
     return y, z
 
 
@@ -122,4 +124,6 @@ def backward(dy, dz, residual, h=None, gate=None, *, alpha=None, w_post=None, w_
             w = torch.empty(need, dtype=torch.uint8, device=dev)
             g.workspace, g.workspace_bytes = w.data_ptr(), need
         N.check(N.lib().nrn_cuda_gatednorm_backward(C.byref(a), C.byref(g), st), "nrn_cuda_gatednorm_backward")
+    if stream is not None:
+        share(stream, dev, (dy, dz, residual, h, gate, alpha, w_post, w_pre), (*like, *sums))
     return Gradients(*like, *sums)

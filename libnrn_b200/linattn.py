@@ -24,7 +24,7 @@ import torch
 
 from . import _native as N
 from ._tensors import (DTYPE, Layouts, check_result, check_rows, check_state, check_tensor, check_vector, check_waits, error_flag, layout, number,
-                       on, ptr, require)
+                       on, ptr, require, share)
 
 check = check_waits
 
@@ -101,6 +101,7 @@ def forward(q, k, v, log_decay, *, scale=None, state=None, cu_seqlens=None, out=
     """(o, final states) of whole sequences that go on from ``state`` (default: zero states).
     o is like q with v's last dimension; ``scale`` defaults to dk ** -0.5."""
     _check_q(q)
+    given = out
     with on(q.device, stream) as st:
         a, need, shape = _call(q, k, v, log_decay, scale, cu_seqlens, state, None, None, out)
         if out is None:
@@ -111,6 +112,8 @@ def forward(q, k, v, log_decay, *, scale=None, state=None, cu_seqlens=None, out=
             w = torch.empty(need, dtype=torch.uint8, device=q.device)
             a.workspace, a.workspace_bytes = w.data_ptr(), need
         N.check(N.lib().nrn_cuda_linattn_forward(C.byref(a), st), "nrn_cuda_linattn_forward")
+    if stream is not None:
+        share(stream, q.device, (q, k, v, log_decay, cu_seqlens, state, given), (out, end))
     return out, end
 
 
@@ -132,6 +135,8 @@ def backward(do, q, k, v, log_decay, *, scale=None, state=None, dstate=None, cu_
             w = torch.empty(need, dtype=torch.uint8, device=q.device)
             a.workspace, a.workspace_bytes = w.data_ptr(), need
         N.check(N.lib().nrn_cuda_linattn_backward(C.byref(a), C.byref(g), st), "nrn_cuda_linattn_backward")
+    if stream is not None:
+        share(stream, q.device, (do, q, k, v, log_decay, cu_seqlens, state, dstate), (dq, dk, dv, ds))
     return dq, dk, dv, ds
 
 
@@ -177,10 +182,13 @@ def step(q, k, v, log_decay, state, *, scale=None, slots=None, out=None, stream=
     scale = number(scale)
     key = (layout(q), layout(k), layout(v), layout(log_decay), layout(state), scale, layout(slots), layout(out))
     block, shape, strides, stride, count = _steps.get(key, q, k, v, log_decay, state, scale, slots, out)
+    given = out
     with on(q.device, stream) as st:
         if out is None:
             out = torch.empty_strided(shape, strides, dtype=q.dtype, device=q.device)
         a = N.LinAttn.from_buffer_copy(block)
         a.q, a.k, a.v, a.o, a.log_decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr()
         N.check(N.lib().nrn_cuda_linattn_step(C.byref(a), state.data_ptr(), stride, count, ptr(slots), st), "nrn_cuda_linattn_step")
+    if stream is not None:
+        share(stream, q.device, (q, k, v, log_decay, state, slots, given), (out,))
     return out

@@ -21,7 +21,7 @@ import threading
 import torch
 
 from . import _native as N
-from ._tensors import DTYPE, Layouts, after_timeout, check_gradient, check_tensor, check_waits, error_flag, layout, on, require
+from ._tensors import DTYPE, Layouts, after_timeout, check_gradient, check_tensor, check_waits, error_flag, layout, on, require, share
 
 BLOCK = 128
 
@@ -71,7 +71,7 @@ class Scaled:
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, row_block: int = 1):
         require(isinstance(values, torch.Tensor) and values.is_cuda, "values: a CUDA matrix is needed")
         block = _matrices.get((layout(values), layout(scales), row_block), values, scales, row_block)
-        self._values, self._scales, self.row_block = values, scales, row_block
+        self._base, self._values, self._scales, self.row_block = None, values, scales, row_block
         self.shape, self.device = values.shape, values.device
         at = values.data_ptr()
         require(at % 16 == 0, "values: rows must start on 16-byte boundaries (Scaled.empty allocates them so)")
@@ -107,6 +107,10 @@ class Scaled:
             self._scales = self._base[self._at:self._at + 4 * rows * cols].view(torch.float32).view(cols, rows).t()
         return self._scales
 
+    def memory(self) -> tuple:
+        """The tensors that hold it."""
+        return (self._values, self._scales) if self._base is None else (self._base,)
+
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """What the matrix stands for, by torch operations (for checks and export)."""
         rows, cols = self.shape
@@ -138,6 +142,8 @@ def quantize(x: torch.Tensor, *, row_block: int = 1, transpose: bool = False, st
         out = Scaled.empty(cols, rows, dev) if transpose else Scaled.empty(rows, cols, dev, row_block)
         N.check(N.lib().nrn_cuda_scaled_quantize(x.data_ptr(), dtype, rows, cols, stride, int(transpose), C.byref(out.desc), st),
                 "nrn_cuda_scaled_quantize")
+    if stream is not None:
+        share(stream, dev, (x,), out.memory())
     return out
 
 
@@ -150,6 +156,8 @@ def transpose(w: Scaled, *, stream=None) -> Scaled:
         values = torch.empty(cols, pitch, dtype=torch.float8_e4m3fn, device=w.device)
         out = Scaled(values[:, :rows], w.scales.t(), BLOCK)
         N.check(N.lib().nrn_cuda_scaled_transpose(C.byref(w.desc), C.byref(out.desc), st), "nrn_cuda_scaled_transpose")
+    if stream is not None:
+        share(stream, w.device, w.memory(), (values,))
     return out
 
 
@@ -224,7 +232,7 @@ def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None
     """a @ b^T, [a rows, b rows], in ``dtype`` (bf16, fp16 or fp32)."""
     require(isinstance(a, Scaled) and isinstance(b, Scaled), "a, b: must be Scaled (scaled.quantize)")
     dev = a.device
-    key = (a.shape, b.shape, dev, b.device, dtype, layout(out))
+    key, given = (a.shape, b.shape, dev, b.device, dtype, layout(out)), out
     with on(dev, stream) as st:
         kind, stride, need = _products.get(key, a, b, dtype, out)
         if out is None:
@@ -238,6 +246,8 @@ def product(a: Scaled, b: Scaled, *, dtype=torch.bfloat16, out=None, stream=None
         else:
             s = N.lib().nrn_cuda_scaled_product(C.byref(a.desc), C.byref(b.desc), out.data_ptr(), kind, stride, None, 0, error_flag(dev), st)
         N.check(s, "nrn_cuda_scaled_product")
+    if stream is not None:
+        share(stream, dev, (*a.memory(), *b.memory(), given), (out,))
     return out
 
 
@@ -280,4 +290,6 @@ def product_backward(dy: torch.Tensor, x: torch.Tensor, w: Scaled, *, dx_dtype=N
             s = N.lib().nrn_cuda_scaled_backward(dy.data_ptr(), x.data_ptr(), kind, rows, dy_stride, x_stride, C.byref(w.desc), dx.data_ptr(),
                                                  dx_kind, dw.data_ptr(), dw_kind, work.data_ptr(), need, error_flag(dev), st)
         N.check(s, "nrn_cuda_scaled_backward")
+    if stream is not None:
+        share(stream, dev, (dy, x, *w.memory()), (dx, dw))
     return dx, dw

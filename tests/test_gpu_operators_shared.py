@@ -277,3 +277,60 @@ def test_steps_norms_and_gradients_in_graphs():
         graph.replay()
         assert torch.equal(o, one(mine)) and torch.equal(state, mine)
     linattn.check()
+
+
+# ------------------------------------------------------------ other streams
+
+def _on_side():
+    """Calls on a stream of the caller's choice, by name: (input made anew, call of it and the stream that gives its results)."""
+    from libnrn_b200 import gatednorm, linattn, scaled
+    n = 1 << 19
+    q, big = randn(1, n // 256, 4, 64, dtype=BF16), randn(n // 256, 256, dtype=BF16)
+    g, w = torch.full((4,), -0.1, device="cuda"), scaled.quantize(randn(512, 256, seed=1), row_block=128)
+    square = scaled.quantize(randn(256, 256, seed=2), row_block=128)
+    return {
+        "forward": (q.clone, lambda x, s: linattn.forward(x, x, x, g, stream=s)),
+        "backward": (q.clone, lambda x, s: linattn.backward(x, x, x, x, g, stream=s)),
+        "step": (q[0].clone, lambda x, s: [linattn.step(x, x, x, g, torch.zeros(n // 256, 4, 64, 64, device="cuda"), stream=s)]),
+        "quantize": (big.clone, lambda x, s: [scaled.quantize(x, stream=s).values]),
+        "transpose": (lambda: scaled.quantize(randn(2048, 1024), row_block=128), lambda x, s: [scaled.transpose(x, stream=s).values]),
+        "product": (lambda: scaled.quantize(randn(8192, 256)), lambda x, s: [scaled.product(x, w, stream=s)]),
+        "product_backward": (big.clone, lambda x, s: scaled.product_backward(x, x, square, stream=s)),
+        "norm": (big.clone, lambda x, s: gatednorm.forward(x, x, x, stream=s)),
+        "norm backward": (big.clone, lambda x, s: [t for t in gatednorm.backward(x, x, x, x, x, stream=s) if t is not None]),
+    }
+
+
+@pytest.mark.parametrize("name", ["forward", "backward", "step", "quantize", "transpose", "product", "product_backward", "norm", "norm backward"])
+def test_memory_is_not_given_out_while_another_stream_uses_it(name):
+    make, call = _on_side()[name]
+    side = torch.cuda.Stream()
+    call(make(), None)
+    torch.cuda.synchronize()
+
+    def busy(stream):
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(400_000_000)               # 0.2 s
+
+    def fresh(n):
+        """Addresses that the allocator gives the current stream for as much memory again."""
+        got = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        return [t.data_ptr() for t in got]
+    # an input that is dropped after the call, before the call has run
+    x = make()
+    side.wait_stream(torch.cuda.current_stream())
+    busy(side)
+    held = x if isinstance(x, torch.Tensor) else x.values
+    at, size = held.data_ptr(), held.numel() * held.element_size()
+    results = call(x, side)
+    del x, held
+    assert at not in fresh(size)
+    torch.cuda.synchronize()
+    # a result that is dropped while the current stream may still read it
+    busy(torch.cuda.current_stream())
+    held = [(t.data_ptr(), t.numel() * t.element_size()) for t in results if t.numel() * t.element_size() >= 1 << 20]
+    del results
+    with torch.cuda.stream(side):
+        for p, n in held:
+            assert p not in fresh(n)
+    torch.cuda.synchronize()
