@@ -1570,15 +1570,22 @@ cudaError_t launch_tc_any(const ScanArgs& p, const CUtensorMap* maps, bool state
     return whole ? launch_tc<DK, 3, false, false>(p, maps, after, s) : launch_tc<DK, 2, false, false>(p, maps, after, s);
 }
 
+// Which kernel a scan runs on.
+enum class Scan { kTensor, kMma, kSerial };
+Scan scan_of(int dtype, int bd, bool vec, int64_t tokens) {
+    if (dtype != NRN_BF16 || bd > 128) return Scan::kSerial;
+    return vec && tokens > 0 && tokens < (int64_t(1) << 31) - kChunk ? Scan::kTensor : Scan::kMma;
+}
+
 // after: a kernel of the same call comes before it
 cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, bool after, cudaStream_t s) {
-    if (dtype == NRN_BF16 && p.b.d <= 128 && p.vec && p.tokens > 0 && p.tokens < (int64_t(1) << 31) - kChunk) {
+    const Scan scan = scan_of(dtype, p.b.d, p.vec != 0, p.tokens);
+    if (scan == Scan::kTensor) {
         CUtensorMap maps[3];
         if (make_scan_map(p.a, p, &maps[0]) && make_scan_map(p.b, p, &maps[1]) && make_scan_map(p.c, p, &maps[2]))
             return p.b.d <= 64 ? launch_tc_any<64>(p, maps, state_only, after, s) : launch_tc_any<128>(p, maps, state_only, after, s);
     }
-    if (dtype == NRN_BF16 && p.b.d <= 64) return launch_mma_any<64>(p, state_only, s);
-    if (dtype == NRN_BF16 && p.b.d <= 128) return launch_mma_any<128>(p, state_only, s);
+    if (scan != Scan::kSerial) return p.b.d <= 64 ? launch_mma_any<64>(p, state_only, s) : launch_mma_any<128>(p, state_only, s);
     if (dtype == NRN_BF16) return launch_serial<__nv_bfloat16>(p, state_only, s);
     if (dtype == NRN_FP16) return launch_serial<__half>(p, state_only, s);
     return launch_serial<float>(p, state_only, s);
@@ -1586,15 +1593,17 @@ cudaError_t launch_scan(const ScanArgs& p, int dtype, bool state_only, bool afte
 
 int elem_size(int dtype) { return dtype == NRN_FP32 ? 4 : 2; }
 
-// Tokens of a segment.  A scan is serial in time and one block holds an SM, so
-// its parallelism is sequences x heads x 128-column tiles; where that leaves
-// SMs idle, or a last round of blocks nearly empty, the sequences are split.
-// Splitting costs a pass over b and c for the segments' states and the join,
-// so the least time is looked for, by a model of microseconds measured on
-// d 128: 2.0 a chunk and 5 a block, 0.9 and 4 for the states, 4 for the join
-// and its bytes.  Packed sequences' lengths are not known here: their segments
-// are counted as if half of them were cut short.
-int64_t segment_length(const nrn_linattn_t* a, int dc) {
+// Tokens of a segment.  A scan is serial in time, so its parallelism is
+// sequences x heads x tiles of columns; where that leaves SMs idle, or a last
+// round of blocks nearly empty, the sequences are split.  Splitting costs a
+// pass over b and c for the segments' states and the join, so the least time
+// is looked for, by a model of microseconds measured for each kernel.  Packed
+// sequences' lengths are not known here: their segments are counted as if half
+// of them were cut short, and whole ones as if the longest were twice the mean.
+//
+// scan_tc_kernel, one block an SM (d 128): 2.0 a chunk of 64 tokens and 5 a
+// block, 0.9 and 4 for the states, 4 for the join and its bytes.
+int64_t tensor_segment(const nrn_linattn_t* a, int dc) {
     const int64_t rows = static_cast<int64_t>(a->heads) * ((dc + kTcCols - 1) / kTcCols), sms = sm_count();
     const bool packed = a->cu_seqlens != nullptr;
     const int64_t chunks = (a->tokens + kChunk - 1) / kChunk;              // of each sequence, or of all packed ones
@@ -1624,6 +1633,50 @@ int64_t segment_length(const nrn_linattn_t* a, int dc) {
     return best * kChunk;
 }
 
+// The others have several blocks on an SM: the first costs `main` a chunk,
+// each further one `more`, and likewise for the states (fp32 and fp16 alike;
+// 64 sequences of 1,024 tokens of 16 heads against one of one head).  4 x 2,048
+// fp32 tokens of 16 heads of 128 take 1.67 ms whole and 1.96 to 2.94 split,
+// 65,536 fp16 ones of 8 heads of 64 32 ms whole, 3.4 in 18 segments, 2.2 in 64.
+struct ScanCost {
+    int cols;
+    double main, more, state, state_more;
+};
+ScanCost cost_of(Scan scan, int bd) {
+    if (scan == Scan::kMma) return bd <= 64 ? ScanCost{kMmaCols, 3.7, 2.8, 1.6, 1.4} : ScanCost{kMmaCols, 5.5, 3.9, 2.7, 2.7};
+    if (bd <= 64) return {kSerialCols, 24.0, 12.0, 14.0, 7.0};
+    return bd <= 128 ? ScanCost{kSerialCols, 33.0, 19.0, 22.0, 13.5} : ScanCost{kSerialCols, 56.0, 30.0, 41.0, 24.0};
+}
+
+// passes: of states to scans (in a backward pass two of three, the values' and
+// the keys' scan have one).
+int64_t segment_length(const nrn_linattn_t* a, int bd, int dc, Scan scan, double passes) {
+    if (scan == Scan::kTensor) return tensor_segment(a, dc);
+    const ScanCost c = cost_of(scan, bd);
+    const double rows = static_cast<double>(a->heads) * ((dc + c.cols - 1) / c.cols), sms = std::max(1, sm_count());
+    const bool packed = a->cu_seqlens != nullptr;
+    const int64_t chunks = (a->tokens + kChunk - 1) / kChunk;
+    if (chunks <= 1) return kChunk;
+    int64_t best = chunks;
+    double cost = 1e300;
+    for (int64_t k = 1; k <= chunks; k += k < 8 ? 1 : k / 4) {
+        const int64_t s = (chunks + k - 1) / k;
+        const double mean = packed && k == 1 ? static_cast<double>(chunks) / std::max(1, a->seqs) : static_cast<double>(s);
+        const double units = !packed ? static_cast<double>(a->seqs) * ((chunks + s - 1) / s)
+                                     : (k == 1 ? static_cast<double>(a->seqs) : static_cast<double>(chunks) / s + 0.5 * a->seqs);
+        const double further = std::max(0.0, units * rows / sms - 1.0);          // blocks an SM past the first
+        double t = mean * (c.main + c.more * further) + 5.0;
+        if (packed && k == 1) t = std::max(t, std::min<double>(static_cast<double>(chunks), 2.0 * mean) * c.main + 5.0);
+        if (k > 1) t += passes * (mean * (c.state + c.state_more * further) + 8.0 + units * a->heads * a->dk * a->dv * 8.0 / 3e6);
+        if (t < cost) {
+            cost = t;
+            best = s;
+        }
+        if (units * rows > 16.0 * sms) break;
+    }
+    return best * kChunk;
+}
+
 int64_t unit_count(const nrn_linattn_t* a, int64_t seg_len) {
     if (a->cu_seqlens) return a->tokens / seg_len + a->seqs;
     return a->seqs * std::max<int64_t>(1, (a->tokens + seg_len - 1) / seg_len);
@@ -1635,28 +1688,37 @@ bool is_split(const nrn_linattn_t* a, int64_t seg_len) {
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
-int64_t seg_bytes(const nrn_linattn_t* a) {
-    int64_t most = 0;
-    for (int dc : {a->dv, a->dk}) {
-        const int64_t l = segment_length(a, dc);
-        if (is_split(a, l)) most = std::max(most, unit_count(a, l));
-    }
-    return align256(most * a->heads * a->dk * a->dv * 4);
-}
-
 int64_t all_tokens(const nrn_linattn_t* a) { return a->cu_seqlens ? a->tokens : a->tokens * a->seqs; }
 
-int64_t workspace_need(const nrn_linattn_t* a, bool backward) {
-    int64_t n = seg_bytes(a);
-    if (backward && a->kv_heads != a->heads) n += align256(all_tokens(a) * a->heads * std::max(a->dk, a->dv) * 4);
-    return n;
+// Segments of the scans whose b has the keys' dimension (the forward one and
+// the values') and of those whose b has the values' (the queries' and keys').
+struct Segments {
+    int64_t by_k = 0, by_v = 0;        // tokens
+
+    Segments(const nrn_linattn_t* a, bool vec, bool backward) {
+        const Scan k = scan_of(a->dtype, a->dk, vec, a->tokens), v = scan_of(a->dtype, a->dv, vec, a->tokens);
+        const double passes = backward ? 2.0 / 3.0 : 1.0;
+        by_k = segment_length(a, a->dk, a->dv, k, passes);
+        by_v = !backward || (k == v && a->dk == a->dv) ? by_k : segment_length(a, a->dv, a->dk, v, passes);
+    }
+    // of the segments' states
+    int64_t bytes(const nrn_linattn_t* a) const {
+        int64_t most = 0;
+        for (int64_t l : {by_k, by_v})
+            if (is_split(a, l)) most = std::max(most, unit_count(a, l));
+        return align256(most * a->heads * a->dk * a->dv * 4);
+    }
+};
+
+// of the fp32 parts of shared heads
+int64_t part_bytes(const nrn_linattn_t* a) {
+    return a->kv_heads == a->heads ? 0 : align256(all_tokens(a) * a->heads * std::max(a->dk, a->dv) * 4);
 }
 
 nrn_status_t run_scan(ScanArgs p, const nrn_linattn_t* a, bool after, cudaStream_t s) {
     const int per16 = 16 / elem_size(a->dtype);
     p.o_vec = reinterpret_cast<uintptr_t>(p.o) % 16 == 0 && p.o_seq % per16 == 0 && p.o_tok % per16 == 0 && p.o_head % per16 == 0 && p.c.d % per16 == 0;
     if (p.cu) p.a.seq = p.b.seq = p.c.seq = p.o_seq = 0;      // packed: a token's row counts from the arrays' start
-    p.seg_len = segment_length(a, p.c.d);
     const int64_t units = unit_count(a, p.seg_len);
     NRN_CHECK_ARG(units * p.heads * ((p.c.d + 31) / 32) < (int64_t(1) << 31), "nrn_cuda_linattn: too many sequences, heads and segments for one launch");
     NRN_CHECK_ARG(static_cast<int64_t>(p.seqs) * p.heads < 65536 || !is_split(a, p.seg_len),
@@ -1737,7 +1799,8 @@ using namespace nrn;
 extern "C" nrn_status_t nrn_cuda_linattn_workspace(const nrn_linattn_t* a, int32_t backward, int64_t* bytes) {
     NRN_TRY(check_common(a, "nrn_cuda_linattn_workspace"));
     NRN_CHECK_ARG(bytes != nullptr, "nrn_cuda_linattn_workspace: null result");
-    *bytes = workspace_need(a, backward != 0);
+    // whatever the arrays' alignment turns out to be
+    *bytes = std::max(Segments(a, false, backward != 0).bytes(a), Segments(a, true, backward != 0).bytes(a)) + (backward ? part_bytes(a) : 0);
     return NRN_OK;
 }
 
@@ -1745,14 +1808,16 @@ extern "C" nrn_status_t nrn_cuda_linattn_forward(const nrn_linattn_t* a, nrn_str
     NRN_TRY(check_common(a, "nrn_cuda_linattn_forward"));
     if (a->seqs == 0) return NRN_OK;
     NRN_CHECK_ARG(all_tokens(a) == 0 || (a->q && a->k && a->v && a->o), "nrn_cuda_linattn_forward: null array");
-    const int64_t need = workspace_need(a, false);
-    NRN_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need), "nrn_cuda_linattn_forward: workspace too small");
     ScanArgs p = scan_args(a);
     const int share = a->heads / a->kv_heads;
     p.a = strided(a->q, a->q_stride, 1, a->dk);
     p.b = strided(a->k, a->k_stride, share, a->dk);
     p.c = strided(a->v, a->v_stride, share, a->dv);
     p.vec = rows_aligned(p.a, a->dtype) && rows_aligned(p.b, a->dtype) && rows_aligned(p.c, a->dtype);
+    const Segments segs(a, p.vec != 0, false);
+    const int64_t need = segs.bytes(a);
+    NRN_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need), "nrn_cuda_linattn_forward: workspace too small");
+    p.seg_len = segs.by_k;
     p.o = a->o;
     p.o_seq = a->o_stride[0], p.o_tok = a->o_stride[1], p.o_head = a->o_stride[2];
     p.s_in = a->state_in, p.s_out = a->state_out;
@@ -1767,16 +1832,18 @@ extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const 
     if (a->seqs == 0) return NRN_OK;
     NRN_CHECK_ARG(all_tokens(a) == 0 || (a->q && a->k && a->v && g->d_o && g->dq && g->dk && g->dv),
                   "nrn_cuda_linattn_backward: null array");
-    const int64_t need = workspace_need(a, true);
-    NRN_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need), "nrn_cuda_linattn_backward: workspace too small");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int share = a->heads / a->kv_heads;
     const Strided q = strided(a->q, a->q_stride, 1, a->dk), k = strided(a->k, a->k_stride, share, a->dk);
     const Strided v = strided(a->v, a->v_stride, share, a->dv), d = strided(g->d_o, g->d_o_stride, 1, a->dv);
     const int vec = rows_aligned(q, a->dtype) && rows_aligned(k, a->dtype) && rows_aligned(v, a->dtype) && rows_aligned(d, a->dtype);
 
+    const Segments segs(a, vec != 0, true);
+    const int64_t states = segs.bytes(a), need = states + part_bytes(a);
+    NRN_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need), "nrn_cuda_linattn_backward: workspace too small");
     ScanArgs p = scan_args(a);
     p.vec = vec;
+    p.seg_len = segs.by_v;
     p.a = d, p.b = v, p.c = k;
     p.o = g->dq;
     p.o_seq = g->dq_stride[0], p.o_tok = g->dq_stride[1], p.o_head = g->dq_stride[2];
@@ -1791,11 +1858,12 @@ extern "C" nrn_status_t nrn_cuda_linattn_backward(const nrn_linattn_t* a, const 
     p.in_mul = 1.0f / a->scale;
     p.end_mul = a->scale;
     p.s_in = g->dstate_out;
-    float* part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + seg_bytes(a));
+    float* part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + states);
     // both carry the state of q and do, one transposed: where their segments
     // are alike, the values' scan leaves the keys' its entering states
-    const bool alike = segment_length(a, a->dv) == segment_length(a, a->dk);
+    const bool alike = segs.by_k == segs.by_v;
     for (int which : {1, 0}) {
+        p.seg_len = which ? segs.by_k : segs.by_v;
         p.a = which ? k : v, p.b = which ? q : d, p.c = which ? d : q;
         p.seg_made = !which && alike;
         p.g_i = 1, p.g_j = a->dv;

@@ -1,4 +1,6 @@
 """Linear attention at its ends.  Tolerances as in test_gpu_linattn.py."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -151,4 +153,44 @@ def test_one_key_head_for_all(dtype):
     got = linattn.backward(do, q, kx, vx, g, state=s0, dstate=ds)
     ref = R.linattn_backward(do, q, kx, vx, g, 0.125, s0, ds)
     for x, y, tol in zip(got, ref, [TOL[dtype]] * 3 + [STATE_TOL]):
+        close(x, y, tol)
+
+
+def test_sequences_are_split_by_their_own_kernels_costs():
+    """Seen in the workspace of the segments' states: none where whole sequences are faster, many where they are long."""
+    def states(dtype, seqs, tokens, heads, d):
+        a, n = N.LinAttn(), C.c_int64()
+        a.dtype, a.seqs, a.heads, a.kv_heads, a.dk, a.dv, a.tokens, a.scale, a.log_decay = dtype, seqs, heads, heads, d, d, tokens, 1.0, 256
+        N.check(N.lib().nrn_cuda_linattn_workspace(C.byref(a), 0, C.byref(n)), "nrn_cuda_linattn_workspace")
+        return n.value // (heads * d * d * 4)
+    for dtype in (1, 2):                             # fp16, fp32: token by token
+        assert states(dtype, 4, 2048, 16, 128) == 0          # 1.67 ms whole, 1.96 and more split
+        assert states(dtype, 1, 65536, 8, 64) >= 32          # 18 segments 3.4 ms, 32 2.4, 64 2.2
+        assert states(dtype, 1, 8192, 16, 64) >= 16          # 8 segments 0.92 ms, 16 0.61, 32 0.58
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16 off 16 bytes", "bf16 wide"])
+def test_many_segments(kind):
+    """Long sequences, packed too, on the kernels that are not the tensor cores' (whose segments test_gpu_linattn.py has)."""
+    from libnrn_b200 import linattn
+    dtype, d = {"fp32": FP32, "fp16": FP16}.get(kind, BF16), 136 if kind == "bf16 wide" else 32
+    lens = [1201, 0, 700, 64, 1, 900]
+    q, k, v, _, do, _ = make(1, sum(lens), 2, 1, d, d, dtype, seed=7)
+    _, _, _, s0, _, ds = make(len(lens), 0, 2, 1, d, d, dtype, seed=8)
+    if kind == "bf16 off 16 bytes":
+        q, k, v, do = (torch.cat([x[..., :1], x], -1)[..., 1:] for x in (q, k, v, do))
+    g, cu = decays(2), torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    tols = [TOL[dtype]] * 3 + [STATE_TOL]
+    o, end = linattn.forward(q, k, v, g, state=s0, cu_seqlens=cu)
+    ro, rend = R.linattn(q, k, v, g, d ** -0.5, s0, lens)
+    close(o, ro, TOL[dtype])
+    close(end, rend, STATE_TOL)
+    for x, y, tol in zip(linattn.backward(do, q, k, v, g, state=s0, dstate=ds, cu_seqlens=cu), R.linattn_backward(do, q, k, v, g, d ** -0.5, s0, ds, lens), tols):
+        close(x, y, tol)
+    q, k, v, do = (x[:, :1201] for x in (q, k, v, do))
+    o, end = linattn.forward(q, k, v, g, state=s0[:1])
+    ro, rend = R.linattn(q, k, v, g, d ** -0.5, s0[:1])
+    close(o, ro, TOL[dtype])
+    close(end, rend, STATE_TOL)
+    for x, y, tol in zip(linattn.backward(do, q, k, v, g, state=s0[:1], dstate=ds[:1]), R.linattn_backward(do, q, k, v, g, d ** -0.5, s0[:1], ds[:1]), tols):
         close(x, y, tol)
