@@ -139,9 +139,10 @@ __device__ __forceinline__ const T* row_ptr(const Strided& m, const Unit& u, int
 // 3 * b.d / 8 operations and three shuffles; 16 tokens at a time are staged
 // in shared memory as fp32.  It does 3 b.d c.d operations a token and head on
 // the fp32 pipe, at about a sixth of the pipe's rate (256 x 64 fp32 tokens of
-// 16 heads of 128 x 128: 2.1 ms): every token is a chain of shared-memory
-// loads, products and shuffles that the next one waits for.  It serves fp16,
-// fp32 and b.d > 128; bf16 with b.d <= 128 has the kernels below.
+// 16 heads of 128 x 128: 2.1 ms, 13 times their bytes; bf16 of 200 x 200 5.8
+// ms): every token is a chain of shared-memory loads, products and shuffles
+// that the next one waits for.  It serves fp16, fp32 and b.d > 128; bf16 with
+// b.d <= 128 has the kernels below.
 //
 // lam in fp32 is off by up to 3e-8, which over a memory of thousands of
 // tokens would show; the error of its powers is taken out of the state after
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const __gri
     }
 }
 
-// ------------------------------------------------------- chunks of 64 tokens
+// ------------------------------------------------------- chunks of 32 tokens
 //
 // bf16 inputs with rows off 16-byte boundaries, b.d <= 128.  For a chunk of
 // tokens p with entering state X:
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(kMmaThreads, DK == 64 ? 4 : 3) scan_mma_kernel
 // What bounds it: neither HBM (9 x 4096 tokens of 16 heads of 128: 604 MB in
 // 142 us, 65% of the measured copy) nor the MMAs, but the chain P -> mask ->
 // intra -> results and U -> state -> inter, each through TMEM and registers.
-// With three stages of copies 137 us where two take 144.  64 tokens a chunk:
+// The third stage of copies brought 5%.  64 tokens a chunk:
 // 128 would halve the chain but double P's work and does not fit shared
 // memory; 128 columns a block: with 64 a and b are read and P is made twice.
 // With mma.sync (the kernel above) operands pass through every warp's
@@ -1633,11 +1634,12 @@ int64_t tensor_segment(const nrn_linattn_t* a, int dc) {
     return best * kChunk;
 }
 
-// The others have several blocks on an SM: the first costs `main` a chunk,
-// each further one `more`, and likewise for the states (fp32 and fp16 alike;
-// 64 sequences of 1,024 tokens of 16 heads against one of one head).  4 x 2,048
-// fp32 tokens of 16 heads of 128 take 1.67 ms whole and 1.96 to 2.94 split,
-// 65,536 fp16 ones of 8 heads of 64 32 ms whole, 3.4 in 18 segments, 2.2 in 64.
+// The others have several blocks on an SM: the first costs `main` a chunk of
+// 64 tokens, each further one `more`, and likewise for the states (one head's
+// 16,384 tokens, and 64 sequences of 1,024 tokens of 16 heads; fp32 and fp16
+// alike).  Whole and split: 4 x 2,048 fp32 tokens of 16 heads of 128 take 1.65
+// ms whole, 1.96 to 2.94 split; 65,536 fp16 tokens of 8 heads of 64 take 32 ms
+// whole, 3.4 in 18 segments, 2.2 in 64.
 struct ScanCost {
     int cols;
     double main, more, state, state_more;

@@ -13,7 +13,11 @@ sequences, [sequences + 1], on the device, from 0 to the number of tokens) the
 batch dimension is 1 and states have one entry for each sequence.  dk and dv
 are at most 256; ``log_decay`` (fp32 [heads]) is at most 0, -inf forgets
 everything at each token.  The decays are time constants, not learned: they
-have no gradient.  Results have no autograd graph: tensors that require
+have no gradient.  States are summed in fp32.  For bf16 inputs the scores
+q . k and the state as q reads it are rounded to bf16 on their way to the
+tensor cores, so a result is about 1.4 times as far from the exact one as its
+own rounding; a caller who wants every bit gives fp32 tensors (slower, one
+token at a time).  Results have no autograd graph: tensors that require
 gradients are refused where these are recorded, and ``backward`` gives them.
 """
 from __future__ import annotations

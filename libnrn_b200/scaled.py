@@ -10,8 +10,15 @@ products summed in fp32 within a block, scaled, and summed in fp32.
     y = scaled.product(scaled.quantize(x), w)            # x @ weights^T, bf16
     dx, dw = scaled.product_backward(dy, x, w)
 
+What 8 bits save is memory: weights take half of bf16's.  In time a product
+with its quantise is close to a bf16 one (8192 x 8192 over 4096 columns: 337 us
+against 349, run for a second 383 against 398; three rows of 4096 x 4096 15
+against 11), and both gradients are behind (4097 rows, 2048 x 4096: 170
+against 98): they quantise and transpose first.
+
 Results have no autograd graph: tensors that require gradients are refused
-where these are recorded.
+where these are recorded.  Calls on one stream share its workspace; threads
+take turns at it.
 """
 from __future__ import annotations
 
