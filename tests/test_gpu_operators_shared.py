@@ -334,3 +334,26 @@ def test_memory_is_not_given_out_while_another_stream_uses_it(name):
         for p, n in held:
             assert p not in fresh(n)
     torch.cuda.synchronize()
+
+
+def test_another_stream_inside_a_captured_graph():
+    from libnrn_b200 import gatednorm, linattn, scaled
+    q, x = randn(1, 700, 2, 64, dtype=BF16), randn(8, 4096, seed=1, dtype=BF16)
+    g, w = torch.full((2,), -0.1, device="cuda"), scaled.quantize(randn(2048, 4096, seed=2), row_block=128)
+    side = torch.cuda.Stream()
+
+    def calls(s):
+        return (*linattn.forward(q, q, q, g, stream=s), scaled.product(scaled.quantize(x, stream=s), w, stream=s), gatednorm.forward(x, x, x, stream=s)[1],
+                *scaled.product_backward(x[:, :2048], x, w, stream=s))
+    calls(None)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        got = calls(side)
+        torch.cuda.current_stream().wait_stream(side)
+    q.copy_(q.flip(1))
+    x.copy_(x.flip(0))
+    for _ in range(2):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, calls(None)))
+    scaled.check()
