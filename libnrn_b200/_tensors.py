@@ -79,7 +79,10 @@ def layout(t):
     """All of a tensor argument that its checks look at (None and anything else stand for themselves)."""
     if t is None:
         return None
-    return (t.shape, t.stride(), t.dtype, t.device, t.requires_grad and _recorded()) if isinstance(t, torch.Tensor) else type(t)
+    try:
+        return t.shape, t.stride(), t.dtype, t.device, t.requires_grad and _recorded()
+    except AttributeError:               # no tensor
+        return type(t)
 
 
 class Layouts:
@@ -178,7 +181,8 @@ def flag(index: int) -> _Flag:
 
 def error_flag(device) -> int:
     """Address of the device's flag."""
-    return flag(device.index).address
+    i = device.index
+    return (_flags.get(i) or flag(i)).address
 
 
 # Called with a device's index when a wait there gave up: what later calls would take over from the unfinished ones.

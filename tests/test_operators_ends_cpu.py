@@ -26,3 +26,10 @@ def test_steps_of_states_that_overlap():
     step = lambda stride, n: N.lib().nrn_cuda_linattn_step(C.byref(a), 256, stride, n, None, None)      # noqa: E731
     assert step(0, 2) == 1 and step(511, 2) == 1 and b"one another" in N.lib().nrn_last_error()
     assert step(512, 2) == 0 and step(0, 1) == 0
+
+
+def test_flag_of_no_device():
+    p = C.c_void_p()
+    for device in (-1, 64):
+        assert N.lib().nrn_cuda_wait_flag(device, C.byref(p)) == 1 and p.value is None
+    assert N.lib().nrn_cuda_wait_flag(0, None) == 1
